@@ -279,6 +279,108 @@ typedef struct tqb_store_args {
 
 int tqb_store(const tqb_store_args* args, cudaStream_t stream);
 
+/*
+ * Ranged decode (no reference counterpart): which tokens of its sequence a
+ * query attends to.  With L = min(seq_lens[b], max_seq_len):
+ *   - the tokens [lo, L), lo = max(L - window, prefix_len, 0) (window 0: no
+ *     limit), shared equally by the splits first_tokens > 0 ? 1 : 0 .. S - 1;
+ *   - the tokens [0, min(first_tokens, lo)), which stay visible before the
+ *     window, as split 0 on their own (first_tokens > 0 needs S >= 2 and
+ *     prefix_len 0).
+ * Tokens [0, prefix_len) are left out: another call supplies their partials
+ * (tqb_prefix).  Splits without a token are left unwritten.
+ */
+typedef struct tqb_range {
+    int32_t window;        /* 0: every token */
+    int32_t first_tokens;
+    int32_t prefix_len;
+    int32_t max_seq_len;   /* at most max_blocks_per_seq * 16; > 0 */
+} tqb_range;
+
+/*
+ * Stage1 over a range; s1->num_splits_per_seq must be NULL.  rot may be NULL
+ * (s1->q_rot holds the queries); otherwise as in tqb_stage1_rotated, with its
+ * restriction: such calls on one device must not overlap in time.
+ */
+int tqb_stage1_range(const tqb_stage1_args* s1, const tqb_rotate_args* rot, const tqb_range* range,
+                     cudaStream_t stream);
+
+/*
+ * Stage2 for tqb_stage1_range's partials: args->num_splits counts `lead`
+ * splits that are always written (a shared prefix's; LSE -inf where empty, O
+ * finite) and then the ranged call's splits.  sinks (optional, [Hq] fp32)
+ * adds one token of logit sinks[h] and value 0 to every sequence with
+ * seq_len > 0.  output is written in out_dtype as by tqb_stage2_typed.
+ */
+int tqb_stage2_range(const tqb_stage2_args* args, const tqb_range* range, int32_t lead, const float* sinks,
+                     int out_dtype, void* output, cudaStream_t stream);
+
+/*
+ * Append (reference/soa_store.py:381-524 with its host part, after the model's
+ * own rotary step): new tokens from the projections' raw keys and values into
+ * their slots.  Per token n and KV head, x = rope(key, positions[n]):
+ *   codes of x R / (|x| + 1e-8) against the midpoints, `>=` going right, as
+ *   in exact arithmetic (borders are resolved in 64 bits); stored norm
+ *   fp16(|x| / sqrt(sum c^2 + 1e-16)) for SoA with norm_correction, else
+ *   fp16(|x|); FP8-key layouts store x as e4m3 (saturating); values as
+ *   tqb_store, bit for bit.
+ * q_rot[n, h] = rope(query) R (FP8-key layouts: rope(query)) when query is
+ * given.  Rotary rule: cos_sin[p] = [cos of rotary_dim / 2 angles | their
+ * sines]; pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved;
+ * dims from rotary_dim on are not turned.  positions NULL: no rotary step.
+ * rotation is orthogonal.  A token with a negative or out-of-range slot is
+ * not stored; nor is one whose position is outside [0, max_pos), and its
+ * q_rot rows are NaN.  Slots must be distinct: a slot named twice holds a
+ * mixture of its tokens.  key, value and query have unit inner stride and any
+ * other strides and alignment their type allows.
+ */
+typedef struct tqb_append_args {
+    const void *key, *value;           /* [N, Hk, D] */
+    const void* query;                 /* [N, Hq, D], may be NULL */
+    int32_t dtype;                     /* tqb_dtype of the three */
+    int64_t k_stride_n, k_stride_h, v_stride_n, v_stride_h, q_stride_n, q_stride_h; /* elements */
+    const void* positions;             /* [N] int32 or int64, may be NULL */
+    int32_t positions_are_64;
+    const float* cos_sin;              /* [max_pos, rotary_dim] */
+    int64_t cos_sin_stride;            /* elements between rows */
+    int32_t max_pos, rotary_dim;       /* rotary_dim even, <= D */
+    int32_t interleaved;
+    const float* rotation;             /* [D, D] row-major, 16-byte aligned (unused for FP8 keys) */
+    const float* midpoints;            /* [n_centroids - 1] */
+    const float* centroids;            /* [n_centroids] */
+    const int32_t* slot_mapping;       /* [N] */
+    uint8_t* kv_cache;
+    int32_t layout;                    /* tqb_layout */
+    int64_t cache_stride_block, cache_stride_pos, cache_stride_head; /* bytes */
+    int64_t num_blocks;                /* 0: skip the range check */
+    float* q_rot;                      /* [N, Hq, D] fp32 */
+    int64_t q_rot_stride_n, q_rot_stride_h;
+    int32_t num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, n_centroids, norm_correction;
+} tqb_append_args;
+
+int tqb_append(const tqb_append_args* args, cudaStream_t stream);
+
+/*
+ * Gather (reference/soa_decode_v1.py:322-454, _tq_full_dequant_kv): the keys
+ * and values that the cache holds in slot_mapping's slots, in out_dtype, one
+ * rounding each.  Keys stay in the rotated basis.  Rows of a negative or
+ * out-of-range slot are zeros.
+ */
+typedef struct tqb_gather_args {
+    const uint8_t* kv_cache;
+    int32_t layout;                    /* tqb_layout */
+    int64_t cache_stride_block, cache_stride_pos, cache_stride_head; /* bytes */
+    int64_t num_blocks;                /* 0: skip the range check */
+    const int32_t* slot_mapping;       /* [N] */
+    const float* centroids;            /* [n_centroids] (unused for FP8 keys) */
+    void *key, *value;                 /* [N, Hk, D] of out_dtype, unit inner stride */
+    int32_t out_dtype;                 /* tqb_dtype */
+    int64_t k_stride_n, k_stride_h, v_stride_n, v_stride_h; /* elements */
+    int32_t num_tokens, num_kv_heads, head_dim, block_size, n_centroids;
+} tqb_gather_args;
+
+int tqb_gather(const tqb_gather_args* args, cudaStream_t stream);
+
 const char* tqb_strerror(int status);
 const char* tqb_last_error_detail(void);
 int tqb_version(void);

@@ -1,0 +1,371 @@
+"""Append, gather, windowed and shared-prefix decode on the GPU against their float64 forms.
+
+Bars, derived before the first run.  Bytes of an append: equal (the codes are those of exact arithmetic, the values'
+steps are the store's).  Rotated queries: 128 fp32 products, each partial sum off by at most 2^-24 of |x| (Cauchy-Schwarz
+on a unit column), 2^-17 |x| in all.  Gather: the output type's half step, and 2^-20 for the fp32 product (AoS: the fp32
+length of the centroids).  Decode: the repository's 1e-4 + 2e-3 |ref|, and the output type's half step."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import serving_oracle as SO
+import tqb
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+@pytest.fixture(autouse=True)
+def no_wait_timeouts(cuda_device):
+    tqb.wait_timeouts(reset=True)
+    yield
+    torch.cuda.synchronize()
+    assert tqb.wait_timeouts(reset=True) == 0, "a bounded device wait gave up"
+
+
+def half_step(dtype) -> float:
+    return torch.finfo(dtype).eps / 2
+
+
+def book(layout):
+    kb = SO.LAYOUTS[layout][0]
+    if kb == 8:
+        return None, None, None
+    c = tqb.get_centroids(128, kb)
+    R = np.linalg.qr(np.random.default_rng(7).standard_normal((128, 128)))[0].astype(np.float32)
+    return c, tqb.get_midpoints(c), torch.from_numpy(R)
+
+
+def cuda(x):
+    return None if x is None else x.cuda()
+
+
+def npy(x):
+    return None if x is None else x.detach().float().cpu().numpy()
+
+
+def cos_sin_table(n, r):
+    a = np.arange(n)[:, None] * 10000.0 ** (-np.arange(0, r, 2) / r)
+    return np.concatenate([np.cos(a), np.sin(a)], 1).astype(np.float32)
+
+
+def projections(rng, n, hq, hk, dtype, pad=0):
+    """Query, key and value as slices of one [n, heads * 128 (+ pad)] projection."""
+    x = torch.from_numpy(rng.standard_normal((n, (hq + 2 * hk) * 128 + pad)).astype(np.float32)).to(dtype).cuda()
+    part = lambda a, b: x[:, a * 128:b * 128].unflatten(-1, (b - a, 128))  # noqa: E731
+    return part(0, hq), part(hq, hq + hk), part(hq + hk, hq + 2 * hk)
+
+
+def run_append(layout, dtype, n, hq, hk, rotary, interleaved, *, seed=0, pad=0, pos64=True, pad_slots=0, norm_correction=True,
+               scale=1.0):
+    rng = np.random.default_rng(seed)
+    c, m, R = book(layout)
+    nb = -(-n // 16) + 2
+    cache0 = rng.integers(0, 256, (nb, 16, hk, SO.LAYOUTS[layout][2]), dtype=np.uint8)
+    slots = rng.permutation(nb * 16)[:n].astype(np.int32)
+    slots[rng.permutation(n)[:pad_slots]] = -1
+    q, k, v = projections(rng, n, hq, hk, dtype, pad)
+    if scale != 1.0:
+        k, v = k * scale, v * scale
+    table = cos_sin_table(500, rotary) if rotary else None
+    pos = rng.integers(0, 500, n) if rotary else None
+    cache = torch.from_numpy(cache0).cuda()
+    got_q = tqb.rope_append(
+        k, v, cache, torch.from_numpy(slots).cuda(),
+        None if pos is None else torch.from_numpy(pos.astype(np.int64 if pos64 else np.int32)).cuda(),
+        None if table is None else torch.from_numpy(table).cuda(), cuda(R), cuda(m), cuda(c), layout=layout,
+        interleaved=interleaved, query=q if hq else None, norm_correction=norm_correction)
+    want = SO.append(cache0, layout, npy(k), npy(v), slots, pos, table, npy(R), npy(m), npy(c), interleaved=interleaved,
+                     norm_correction=norm_correction)
+    got = cache.cpu().numpy()
+    assert np.array_equal(got, want), f"{(got != want).sum()} of {got.size} bytes differ"
+    if hq:
+        x = npy(q).astype(np.float64)
+        if rotary:
+            x = SO.rope(x, table[pos], interleaved)
+        ref = x if R is None else x @ npy(R).astype(np.float64)
+        tol = (2.0 ** -17 if R is not None else 2.0 ** -24) * np.linalg.norm(x, axis=-1, keepdims=True)
+        assert (np.abs(npy(got_q) - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_append_writes_the_definitions_bytes(layout, dtype):
+    run_append(layout, DT[dtype], 45, 8, 2, 128, False, seed=1, pad_slots=4)
+
+
+@pytest.mark.parametrize("n,hq,hk,rotary,interleaved,pad,pos64", [
+    (1, 32, 8, 128, False, 0, True), (1, 1, 1, 64, True, 0, False), (17, 0, 8, 96, False, 8, True),
+    (129, 5, 1, 2, True, 3, True), (300, 16, 2, 34, False, 1, False), (64, 4, 4, 0, False, 0, True),
+    (200, 24, 3, 126, False, 0, True), (520, 8, 8, 128, True, 0, True)])
+def test_append_shapes(n, hq, hk, rotary, interleaved, pad, pos64):
+    """Single tokens, odd heads, partial rotary dims of every alignment, no rotary step, odd row strides."""
+    for layout in ("soa", "aos_k3v3", "soa_k8"):
+        run_append(layout, torch.bfloat16, n, hq, hk, rotary, interleaved, seed=n, pad=pad, pos64=pos64)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-6, 3000.0])
+def test_append_extreme_norms(scale):
+    """All-zero keys sit on the codebook's middle border; large norms near the end of fp16."""
+    run_append("soa", torch.float32, 37, 0, 2, 64, False, seed=3, scale=scale)
+    run_append("aos_k3", torch.float32, 37, 0, 2, 64, False, seed=3, scale=scale)
+
+
+def test_append_without_norm_correction():
+    run_append("soa_k3", torch.bfloat16, 33, 0, 2, 128, False, seed=4, norm_correction=False)
+
+
+def test_append_large_batch_bytes():
+    """Enough coordinates (2 M) that some lie next to every border."""
+    run_append("soa", torch.bfloat16, 2048, 0, 8, 128, False, seed=5)
+
+
+def test_append_skips_what_has_no_place():
+    """Out-of-range slots and positions: nothing stored, and NaN queries for the positions."""
+    rng = np.random.default_rng(9)
+    c, m, R = book("soa")
+    cache = torch.from_numpy(rng.integers(0, 256, (3, 16, 2, 134), dtype=np.uint8)).cuda()
+    before = cache.clone()
+    q, k, v = projections(rng, 4, 4, 2, torch.bfloat16)
+    out = tqb.rope_append(k, v, cache, torch.tensor([48, -7, 5, 6], dtype=torch.int32).cuda(),
+                          torch.tensor([1, 2, 500, -1]).cuda(), torch.from_numpy(cos_sin_table(500, 128)).cuda(), cuda(R),
+                          cuda(m), cuda(c), query=q)
+    assert torch.equal(cache, before)
+    assert torch.isfinite(out[:2]).all() and torch.isnan(out[2:]).all()
+
+
+def test_append_empty():
+    c, m, R = book("soa")
+    cache = torch.zeros(2, 16, 2, 134, dtype=torch.uint8, device="cuda")
+    e = torch.empty(0, 2, 128, device="cuda")
+    out = tqb.rope_append(e, e, cache, torch.empty(0, dtype=torch.int32, device="cuda"), None, None, cuda(R), cuda(m),
+                          cuda(c), query=e)
+    assert out.shape == (0, 2, 128)
+
+
+@pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n,hk", [(1, 1), (53, 3), (131, 8)])
+def test_gather(layout, dtype, n, hk):
+    rng = np.random.default_rng(n)
+    c, _, _ = book(layout)
+    cache = random_cache(rng, 12, hk, layout)
+    slots = rng.integers(0, 12 * 16, n).astype(np.int32)  # repeated slots may be read
+    slots[n // 2:n // 2 + 1] = rng.choice([-1, 12 * 16, slots[0]])
+    k, v = tqb.gather_kv(torch.from_numpy(cache).cuda(), torch.from_numpy(slots).cuda(), cuda(c), layout=layout,
+                         dtype=DT[dtype])
+    assert k.dtype == DT[dtype]
+    rk, rv = SO.read(cache, layout, slots, npy(c))
+    tol = half_step(DT[dtype]) + 2.0 ** -20
+    for got, ref in ((k, rk), (v, rv)):
+        assert (np.abs(got.double().cpu().numpy() - ref) <= tol * np.abs(ref) + 2.0 ** -25).all()
+
+
+def test_gather_into_strided_outputs():
+    rng = np.random.default_rng(2)
+    c, _, _ = book("soa")
+    cache = torch.from_numpy(random_cache(rng, 4, 2, "soa")).cuda()
+    slots = torch.arange(40, dtype=torch.int32, device="cuda")
+    k, v = tqb.gather_kv(cache, slots, cuda(c))
+    buf = torch.zeros(40, 2, 2 * 128 + 3, dtype=torch.bfloat16, device="cuda")
+    tqb.gather_kv(cache, slots, cuda(c), key=buf[..., :128], value=buf[..., 129:257])
+    assert torch.equal(buf[..., :128], k) and torch.equal(buf[..., 129:257], v)
+    assert (buf[..., 128] == 0).all() and (buf[..., 257:] == 0).all()
+
+
+def random_cache(rng, nb, hk, layout):
+    """Every byte a valid code, norms, scales and zeros of ordinary size."""
+    kb, vb, slot = SO.LAYOUTS[layout]
+    cache = rng.integers(0, 256, (nb, 16, hk, slot), dtype=np.uint8)
+    flat = cache.reshape(nb, -1)
+    for t in range(16):
+        for h in range(hk):
+            ka, va, norm, scale, zero = SO.places(layout, hk, t, h)
+            if kb == 8:
+                e = torch.from_numpy(rng.standard_normal((nb, 128)).astype(np.float32)).to(torch.float8_e4m3fn)
+                flat[:, ka:ka + 128] = e.view(torch.uint8).numpy()
+            put = lambda at, v: flat.__setitem__((slice(None), slice(at, at + 2)),  # noqa: E731
+                                                 v.astype(np.float16)[:, None].view(np.uint8))
+            if norm is not None:
+                put(norm, 11.3 * np.exp(0.2 * rng.standard_normal(nb)))
+            put(scale, 0.3 * np.exp(0.2 * rng.standard_normal(nb)))
+            put(zero, -2 + 0.3 * rng.standard_normal(nb))
+    return cache
+
+
+def batch(rng, lens, hk, layout, shared=0):
+    """Cache, block table and lengths; the first ``shared`` pages are everyone's."""
+    pages = [max(0, -(-n // 16) - shared) for n in lens]
+    nb = shared + sum(pages) + 2
+    order = rng.permutation(nb).astype(np.int32)
+    table = np.zeros((len(lens), max(1, shared + max(pages))), np.int32)
+    table[:, :shared] = order[:shared]
+    at = shared
+    for b, n in enumerate(pages):
+        table[b, shared:shared + n] = order[at:at + n]
+        at += n
+    return random_cache(rng, nb, hk, layout), table, np.asarray(lens, np.int32)
+
+
+def check_decode(got, lse, ref, ref_lse, dtype):
+    got, lse = got.double().cpu().numpy(), lse.double().cpu().numpy()
+    dead = np.isnan(ref)
+    assert np.array_equal(np.isnan(got), dead)
+    assert (np.abs(got - ref)[~dead] <= 1e-4 + (2e-3 + half_step(dtype)) * np.abs(ref[~dead])).all()
+    assert np.array_equal(np.isneginf(lse), np.isneginf(ref_lse))
+    live = np.isfinite(ref_lse)
+    assert (np.abs(lse - ref_lse)[live] <= 1e-4 + 2e-3 * np.abs(ref_lse[live])).all()
+
+
+def run_window(layout, dtype, lens, hq, hk, window, first, *, seed=0, sinks=False, raw=True, **kw):
+    rng = np.random.default_rng(seed)
+    c, _, R = book(layout)
+    cache, table, lens = batch(rng, lens, hk, layout)
+    q = torch.from_numpy(rng.standard_normal((len(lens), hq, 128)).astype(np.float32) * 1.5).to(dtype).cuda()
+    raw = raw and R is not None
+    s = torch.from_numpy(rng.standard_normal(hq).astype(np.float32) * 2).cuda() if sinks else None
+    lse = torch.empty(len(lens), hq, device="cuda")
+    got = tqb.window_attention(q, torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(),
+                               torch.from_numpy(lens).cuda(), cuda(R) if raw else None, cuda(c), window=window,
+                               first_tokens=first, layout=layout, sinks=s, lse=lse, **kw)
+    x = npy(q).astype(np.float64)
+    x = x @ npy(R).astype(np.float64) if raw else x
+    ref, ref_lse = SO.attention(x, cache, layout, table, lens, npy(c), lambda t, L: (t < first) | (t >= L - window),
+                                scale=kw.get("scale"), sinks=npy(s))
+    assert got.dtype == kw.get("out_dtype", dtype)
+    check_decode(got, lse, ref, ref_lse, got.dtype)
+
+
+RAGGED = [1, 0, 15, 16, 17, 40, 99, 100, 101, 104, 105, 160, 333]
+
+
+@pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
+@pytest.mark.parametrize("window,first", [(100, 4), (37, 0), (1, 1)])
+def test_window_layouts(layout, window, first):
+    run_window(layout, torch.bfloat16, RAGGED, 8, 2, window, first, seed=window)
+
+
+@pytest.mark.parametrize("hq,hk", [(32, 8), (64, 8), (5, 1), (6, 3), (10, 10), (40, 5)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_window_heads_and_types(hq, hk, dtype):
+    run_window("soa", DT[dtype], [1, 70, 200, 129], hq, hk, 64, 17, seed=hq, sinks=True)
+
+
+@pytest.mark.parametrize("window,first,num_splits", [(1, 0, 1), (1, 0, 7), (16, 16, 3), (333, 0, 5), (1000, 50, 2),
+                                                     (5, 400, 4), (320, 13, 64), (2 ** 30, 2 ** 30, None)])
+def test_window_splits(window, first, num_splits):
+    """More splits than tokens, windows and first tokens beyond the sequence, first tokens that meet the window."""
+    run_window("soa", torch.float32, RAGGED, 4, 1, window, first, seed=1, num_splits=num_splits, sinks=True)
+
+
+def test_window_register_kernel(monkeypatch):
+    monkeypatch.setenv("TQB_STAGE1_KERNEL", "regs")
+    for layout in ("soa", "aos", "soa_k8"):
+        run_window(layout, torch.bfloat16, RAGGED, 8, 2, 50, 5, seed=2)
+
+
+def test_window_in_the_caches_basis_and_other_arguments():
+    run_window("soa", torch.float32, RAGGED, 8, 2, 50, 3, seed=3, raw=False, scale=0.05, out_dtype=torch.float16)
+
+
+def test_window_many_sequences():
+    """More items than one round of the grid, ragged lengths: the weight cut with a split of first tokens."""
+    rng = np.random.default_rng(4)
+    run_window("soa", torch.bfloat16, list(rng.integers(1, 300, 90)), 8, 8, 128, 4, seed=5, num_splits=6)
+
+
+def test_window_covering_everything_equals_the_decode_call():
+    rng = np.random.default_rng(8)
+    c, _, R = book("soa")
+    cache, table, lens = batch(rng, [5, 300, 77], 2, "soa")
+    q = torch.from_numpy(rng.standard_normal((3, 8, 128)).astype(np.float32)).cuda()
+    args = (torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda())
+    a = tqb.window_attention(q, *args, cuda(R), cuda(c), window=10 ** 6, num_splits=32)
+    b = tqb.triton_turboquant_decode_attention(q, *args, cuda(R).T.contiguous(), cuda(c), 128 ** -0.5, 4, 66, 4)
+    assert torch.equal(a, b)
+
+
+def run_prefix(layout, dtype, own, prefix, hq, hk, *, seed=0, sinks=False, raw=True, short=(), scale_q=1.5, **kw):
+    rng = np.random.default_rng(seed)
+    c, _, R = book(layout)
+    cache, table, lens = batch(rng, [prefix + n for n in own], hk, layout, prefix // 16)
+    for b, n in short:
+        lens[b] = n
+    q = torch.from_numpy(rng.standard_normal((len(lens), hq, 128)).astype(np.float32) * scale_q).to(dtype).cuda()
+    raw = raw and R is not None
+    s = torch.from_numpy(rng.standard_normal(hq).astype(np.float32) * 2).cuda() if sinks else None
+    lse = torch.empty(len(lens), hq, device="cuda")
+    got = tqb.prefix_attention(q, torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(),
+                               torch.from_numpy(lens).cuda(), cuda(R) if raw else None, cuda(c), prefix_len=prefix,
+                               layout=layout, sinks=s, lse=lse, **kw)
+    x = npy(q).astype(np.float64)
+    x = x @ npy(R).astype(np.float64) if raw else x
+    ref, ref_lse = SO.attention(x, cache, layout, table, lens, npy(c), lambda t, L: t >= 0, scale=kw.get("scale"),
+                                sinks=npy(s))
+    check_decode(got, lse, ref, ref_lse, got.dtype)
+
+
+@pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
+def test_prefix_layouts(layout):
+    run_prefix(layout, torch.bfloat16, [1, 0, 20, 63], 400, 8, 2, seed=1)
+
+
+@pytest.mark.parametrize("hq,hk", [(32, 8), (16, 2), (5, 1), (6, 3)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_prefix_heads_and_types(hq, hk, dtype):
+    run_prefix("soa", DT[dtype], [3, 40, 17], 160, hq, hk, seed=hq, sinks=True)
+
+
+@pytest.mark.parametrize("prefix", [0, 16, 112, 128, 144, 640])
+@pytest.mark.parametrize("batch_size", [1, 2, 37, 70])
+def test_prefix_lengths_and_batches(prefix, batch_size):
+    rng = np.random.default_rng(prefix + batch_size)
+    run_prefix("soa", torch.bfloat16, list(rng.integers(1, 50, batch_size)), prefix, 4, 1, seed=prefix)
+
+
+def test_prefix_rows_shorter_than_the_prefix():
+    """Padded rows of a batch (length 0) and rows that end inside the prefix, at a page's and a tile's edges."""
+    run_prefix("soa", torch.bfloat16, [9] * 8, 320, 4, 1, seed=2, short=[(0, 0), (2, 1), (3, 128), (4, 129), (5, 320), (6, 255)])
+
+
+def test_step_append_then_attend_on_a_side_stream_and_in_a_graph():
+    """Append, then both decode calls, as a step runs them: on a side stream, captured and replayed on new inputs."""
+    rng = np.random.default_rng(11)
+    c, m, R = (cuda(x) for x in book("soa"))
+    cache_np, table, lens = batch(rng, [64 + n for n in (5, 30, 17)], 2, "soa", 4)
+    cache, table, lens = (torch.from_numpy(x).cuda() for x in (cache_np, table, lens))
+    cs = torch.from_numpy(cos_sin_table(500, 128)).cuda()
+    q, k, v = projections(rng, 3, 8, 2, torch.bfloat16)
+    slots = (table.gather(1, (lens[:, None].long() - 1) // 16) * 16 + (lens[:, None] - 1) % 16).flatten().int()
+    pos = lens.long() - 1
+
+    def step():
+        qr = tqb.rope_append(k, v, cache, slots, pos, cs, R, m, c, query=q)
+        w = tqb.window_attention(qr, cache, table, lens, None, c, window=40, first_tokens=4, out_dtype=q.dtype)
+        return w, tqb.prefix_attention(qr, cache, table, lens, None, c, prefix_len=64, out_dtype=q.dtype)
+
+    def ref():
+        x = SO.rope(npy(q).astype(np.float64), npy(cs)[pos.cpu().numpy()], False) @ npy(R).astype(np.float64)
+        t, l, ca = table.cpu().numpy(), lens.cpu().numpy(), cache.cpu().numpy()
+        return [SO.attention(x, ca, "soa", t, l, npy(c), f)[0] for f in (lambda t, L: (t < 4) | (t >= L - 40), lambda t, L: t >= 0)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    for a, b in zip(got, ref()):
+        assert (np.abs(npy(a) - b) <= 1e-4 + (2e-3 + half_step(q.dtype)) * np.abs(b)).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    q.copy_(torch.randn_like(q))
+    k.copy_(torch.randn_like(k))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs, ref()):
+        assert (np.abs(npy(a) - b) <= 1e-4 + (2e-3 + half_step(q.dtype)) * np.abs(b)).all()

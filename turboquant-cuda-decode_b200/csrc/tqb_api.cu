@@ -112,6 +112,31 @@ const char* tqb_strerror(int status) {
 
 const char* tqb_last_error_detail(void) { return g_detail; }
 
+// Cache pointer, block stride and AoS strides of the store, append and gather
+// calls.
+static int cache_check(const uint8_t* cache, int layout, int64_t block, int64_t ps, int64_t hs, int64_t hk) {
+    TQB_REQUIRE(aligned(cache, 2) && block % 2 == 0, TQB_ERR_ALIGNMENT, "kv_cache and its block stride must be even");
+    if (layout == TQB_LAYOUT_SOA_K8) {
+        TQB_REQUIRE(block >= tqb::kBlockSize * hk * tqb::kSlotBytesK8 && block % 4 == 0, TQB_ERR_INVALID_ARG,
+                    "FP8-key block stride must be >= 16*Hk*196 bytes and a multiple of 4");
+        TQB_REQUIRE(aligned(cache, 4), TQB_ERR_ALIGNMENT, "FP8-key kv_cache must be 4-byte aligned");
+    } else if (layout == TQB_LAYOUT_SOA_K3 || layout == TQB_LAYOUT_SOA_K3V3) {
+        TQB_REQUIRE(block >= tqb::kBlockSize * hk *
+                                 (layout == TQB_LAYOUT_SOA_K3V3 ? tqb::kSlotBytesK3V3 : tqb::kSlotBytesK3),
+                    TQB_ERR_INVALID_ARG,
+                    "3-bit-key block stride must be >= 16*Hk*slot bytes (118, or 102 with 3-bit values)");
+    } else if (layout == TQB_LAYOUT_SOA) {
+        TQB_REQUIRE(block >= tqb::kBlockSize * hk * tqb::kSlotBytes, TQB_ERR_INVALID_ARG,
+                    "SoA block stride must be >= 16*Hk*134 bytes");
+    } else {
+        TQB_REQUIRE(ps % 2 == 0 && hs % 2 == 0, TQB_ERR_ALIGNMENT, "AoS strides must be even");
+        TQB_REQUIRE(aos_strides_ok(block, ps, hs, hk, tqb::aos_slot_bytes(layout)), TQB_ERR_INVALID_ARG,
+                    "AoS strides must describe [blocks, 16, Hk, >= slot] slots (slot 134, 196, 118 or 102 bytes "
+                    "by layout), token- or head-major");
+    }
+    return TQB_OK;
+}
+
 // Validates Stage1 arguments and fills p (for batch > 0).
 static int stage1_check(const tqb_stage1_args* a, tqb::Stage1Params& p) {
     TQB_REQUIRE(a != nullptr, TQB_ERR_INVALID_ARG, "args is NULL");
@@ -212,9 +237,8 @@ int tqb_stage1(const tqb_stage1_args* a, cudaStream_t stream) {
     return tqb::launch_stage1(p, stream, nsm);
 }
 
-int tqb_stage1_rotated(const tqb_rotate_args* r, const tqb_stage1_args* a, cudaStream_t stream) {
-    g_detail[0] = '\0';
-    TQB_REQUIRE(r != nullptr && a != nullptr, TQB_ERR_INVALID_ARG, "args is NULL");
+// The rotation's arguments of a call whose Stage1 arguments are `a`.
+static int rotated_check(const tqb_rotate_args* r, const tqb_stage1_args* a) {
     TQB_REQUIRE(r->q_rot == a->q_rot && r->out_stride_b == a->q_stride_b && r->out_stride_h == a->q_stride_h &&
                     r->batch == a->batch && r->num_q_heads == a->num_q_heads && r->head_dim == a->head_dim,
                 TQB_ERR_INVALID_ARG,
@@ -222,28 +246,43 @@ int tqb_stage1_rotated(const tqb_rotate_args* r, const tqb_stage1_args* a, cudaS
     TQB_REQUIRE(r->query_dtype == TQB_DTYPE_F32 || r->query_dtype == TQB_DTYPE_F16 ||
                     r->query_dtype == TQB_DTYPE_BF16,
                 TQB_ERR_INVALID_ARG, "query_dtype must be TQB_DTYPE_F32, TQB_DTYPE_F16 or TQB_DTYPE_BF16");
-    tqb::Stage1Params p{};
-    int rc = stage1_check(a, p);
-    if (rc != TQB_OK || a->batch == 0) return rc;
+    if (a->batch == 0) return TQB_OK;
     TQB_REQUIRE(r->query && r->rotation, TQB_ERR_INVALID_ARG, "query or rotation is NULL");
     TQB_REQUIRE(aligned(r->query, r->query_dtype == TQB_DTYPE_F32 ? 4 : 2) && aligned(r->rotation, 16),
                 TQB_ERR_ALIGNMENT, "query must be aligned to its element size, rotation to 16 bytes");
+    return TQB_OK;
+}
+// One kernel where the page ring runs with a group of at most 4 query
+// heads per KV head (its rotation prologue stages the 64 KB rotation in
+// a ring it has not started yet); otherwise the rotation kernel, then
+// Stage1.
+static bool rotation_fuses(const tqb::Stage1Params& p) {
+    return p.G <= 4 && !tqb::stage1_register_kernel_forced() && tqb::stage1_ring_supported(p);
+}
+static void fuse_rotation(tqb::Stage1Params& p, const tqb_rotate_args* r) {
+    p.rq = r->query;
+    p.rq_dtype = r->query_dtype;
+    p.rqsb = r->q_stride_b;
+    p.rqsh = r->q_stride_h;
+    p.rot = r->rotation;
+    p.q_out = r->q_rot;
+}
+
+int tqb_stage1_rotated(const tqb_rotate_args* r, const tqb_stage1_args* a, cudaStream_t stream) {
+    g_detail[0] = '\0';
+    TQB_REQUIRE(r != nullptr && a != nullptr, TQB_ERR_INVALID_ARG, "args is NULL");
+    int rc = rotated_check(r, a);
+    if (rc != TQB_OK) return rc;
+    tqb::Stage1Params p{};
+    rc = stage1_check(a, p);
+    if (rc != TQB_OK || a->batch == 0) return rc;
     DeviceGuard guard(a->mid_o);
     TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning mid_o");
     const int nsm = sm_count();
     TQB_REQUIRE(nsm > 0, TQB_ERR_CUDA, "cannot query the current CUDA device");
-    // One kernel where the page ring runs with a group of at most 4 query
-    // heads per KV head (its rotation prologue stages the 64 KB rotation in
-    // a ring it has not started yet); otherwise the rotation kernel, then
-    // Stage1.
-    if (p.G <= 4 && !tqb::stage1_register_kernel_forced() && tqb::stage1_ring_supported(p)) {
+    if (rotation_fuses(p)) {
         tqb::Stage1Params pr = p;
-        pr.rq = r->query;
-        pr.rq_dtype = r->query_dtype;
-        pr.rqsb = r->q_stride_b;
-        pr.rqsh = r->q_stride_h;
-        pr.rot = r->rotation;
-        pr.q_out = r->q_rot;
+        fuse_rotation(pr, r);
         rc = tqb::launch_stage1_ring(pr, stream, nsm);
         if (rc != TQB_ERR_UNSUPPORTED) return rc;
         g_detail[0] = '\0';
@@ -253,8 +292,9 @@ int tqb_stage1_rotated(const tqb_rotate_args* r, const tqb_stage1_args* a, cudaS
     return tqb::launch_stage1(p, stream, nsm);
 }
 
-// Stage2 with the output written as `dtype` to `out` (a->output ignored).
-static int stage2_impl(const tqb_stage2_args* a, void* out, int dtype, cudaStream_t stream) {
+// Validates Stage2 arguments and fills p (for batch > 0); the output is
+// written as `dtype` to `out` (a->output ignored).
+static int stage2_check(const tqb_stage2_args* a, void* out, int dtype, tqb::Stage2Params& p) {
     g_detail[0] = '\0';
     TQB_REQUIRE(a != nullptr, TQB_ERR_INVALID_ARG, "args is NULL");
     TQB_REQUIRE(dtype == TQB_DTYPE_F32 || dtype == TQB_DTYPE_F16 || dtype == TQB_DTYPE_BF16, TQB_ERR_INVALID_ARG,
@@ -268,9 +308,6 @@ static int stage2_impl(const tqb_stage2_args* a, void* out, int dtype, cudaStrea
     TQB_REQUIRE(a->mid_o && a->seq_lens && out && a->lse, TQB_ERR_INVALID_ARG, "a required pointer is NULL");
     TQB_REQUIRE(aligned(a->mid_o, 4) && aligned(out, dtype == TQB_DTYPE_F32 ? 4 : 2) && aligned(a->lse, 4),
                 TQB_ERR_ALIGNMENT, "buffers must be aligned to their element size");
-    DeviceGuard guard(out);
-    TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning output");
-    tqb::Stage2Params p{};
     p.mid = a->mid_o;
     p.msb = a->mid_stride_b;
     p.msh = a->mid_stride_h;
@@ -286,6 +323,15 @@ static int stage2_impl(const tqb_stage2_args* a, void* out, int dtype, cudaStrea
     p.B = a->batch;
     p.Hq = a->num_q_heads;
     p.S = a->num_splits;
+    return TQB_OK;
+}
+
+static int stage2_impl(const tqb_stage2_args* a, void* out, int dtype, cudaStream_t stream) {
+    tqb::Stage2Params p{};
+    const int rc = stage2_check(a, out, dtype, p);
+    if (rc != TQB_OK || a->batch == 0) return rc;
+    DeviceGuard guard(out);
+    TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning output");
     return tqb::launch_stage2(p, stream);
 }
 
@@ -526,8 +572,6 @@ int tqb_store(const tqb_store_args* a, cudaStream_t stream) {
     TQB_REQUIRE(a->head_dim == tqb::kHeadDim, TQB_ERR_UNSUPPORTED, "head_dim must be 128");
     TQB_REQUIRE(a->block_size == tqb::kBlockSize, TQB_ERR_UNSUPPORTED, "block_size must be 16");
     TQB_REQUIRE(tqb::layout_valid(a->layout), TQB_ERR_INVALID_ARG, "layout must be a tqb_layout value");
-    const bool k8 = a->layout == TQB_LAYOUT_SOA_K8, v3 = a->layout == TQB_LAYOUT_SOA_K3V3;
-    const bool k3 = a->layout == TQB_LAYOUT_SOA_K3 || v3;
     const bool fp8 = tqb::layout_fp8_keys(a->layout);
     TQB_REQUIRE(fp8 || a->n_centroids == (tqb::layout_3bit_keys(a->layout) ? 8 : tqb::kNumCentroids),
                 TQB_ERR_UNSUPPORTED, "n_centroids must be 16, or 8 for 3-bit keys");
@@ -542,29 +586,9 @@ int tqb_store(const tqb_store_args* a, cudaStream_t stream) {
                 "norm_correction requires centroids");
     TQB_REQUIRE(aligned(a->y, 16) && aligned(a->value, 16), TQB_ERR_ALIGNMENT,
                 "y and value must be 16-byte aligned");
-    TQB_REQUIRE(aligned(a->kv_cache, 2) && a->cache_stride_block % 2 == 0, TQB_ERR_ALIGNMENT,
-                "kv_cache and its block stride must be even");
-    const int64_t hk = a->num_kv_heads;
-    if (k8) {
-        TQB_REQUIRE(a->cache_stride_block >= tqb::kBlockSize * hk * tqb::kSlotBytesK8 &&
-                        a->cache_stride_block % 4 == 0,
-                    TQB_ERR_INVALID_ARG, "FP8-key block stride must be >= 16*Hk*196 bytes and a multiple of 4");
-        TQB_REQUIRE(aligned(a->kv_cache, 4), TQB_ERR_ALIGNMENT, "FP8-key kv_cache must be 4-byte aligned");
-    } else if (k3) {
-        TQB_REQUIRE(a->cache_stride_block >= tqb::kBlockSize * hk * (v3 ? tqb::kSlotBytesK3V3 : tqb::kSlotBytesK3),
-                    TQB_ERR_INVALID_ARG, "3-bit-key block stride must be >= 16*Hk*slot bytes (118, or 102 with 3-bit values)");
-    } else if (a->layout == TQB_LAYOUT_SOA) {
-        TQB_REQUIRE(a->cache_stride_block >= tqb::kBlockSize * hk * tqb::kSlotBytes,
-                    TQB_ERR_INVALID_ARG, "SoA block stride must be >= 16*Hk*134 bytes");
-    } else {
-        TQB_REQUIRE(a->cache_stride_pos % 2 == 0 && a->cache_stride_head % 2 == 0, TQB_ERR_ALIGNMENT,
-                    "AoS strides must be even");
-        TQB_REQUIRE(aos_strides_ok(a->cache_stride_block, a->cache_stride_pos, a->cache_stride_head, hk,
-                                   tqb::aos_slot_bytes(a->layout)),
-                    TQB_ERR_INVALID_ARG,
-                    "AoS strides must describe [blocks, 16, Hk, >= slot] slots (slot 134, 196, 118 or 102 bytes "
-                    "by layout), token- or head-major");
-    }
+    const int rc0 = cache_check(a->kv_cache, a->layout, a->cache_stride_block, a->cache_stride_pos,
+                                a->cache_stride_head, a->num_kv_heads);
+    if (rc0 != TQB_OK) return rc0;
     DeviceGuard guard(a->kv_cache);
     TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning kv_cache");
     tqb::StoreParams p{};
@@ -585,6 +609,197 @@ int tqb_store(const tqb_store_args* a, cudaStream_t stream) {
     const int rc = tqb::launch_store(p, stream);
     if (rc != TQB_OK) return rc;
     return TQB_OK;
+}
+
+// ---- ranged decode, append, gather -----------------------------------------
+
+static bool dtype_ok(int d) { return d == TQB_DTYPE_F32 || d == TQB_DTYPE_F16 || d == TQB_DTYPE_BF16; }
+
+static int range_check(const tqb_range* r, int num_splits, tqb::KeyRange& k) {
+    TQB_REQUIRE(r != nullptr, TQB_ERR_INVALID_ARG, "range is NULL");
+    TQB_REQUIRE(r->window >= 0 && r->first_tokens >= 0 && r->prefix_len >= 0 && r->max_seq_len > 0,
+                TQB_ERR_INVALID_ARG, "window, first_tokens, prefix_len must be >= 0 and max_seq_len > 0");
+    TQB_REQUIRE(r->first_tokens == 0 || (r->prefix_len == 0 && num_splits >= 2), TQB_ERR_INVALID_ARG,
+                "first_tokens needs prefix_len 0 and a split of its own (two splits or more)");
+    k.window = r->window;
+    k.first = r->first_tokens;
+    k.prefix = r->prefix_len;
+    k.max_len = r->max_seq_len;
+    return TQB_OK;
+}
+
+int tqb_stage1_range(const tqb_stage1_args* a, const tqb_rotate_args* r, const tqb_range* range, cudaStream_t stream) {
+    g_detail[0] = '\0';
+    tqb::Stage1Params p{};
+    int rc = stage1_check(a, p);
+    if (rc != TQB_OK) return rc;
+    rc = range_check(range, a->num_splits, p.range);
+    if (rc != TQB_OK) return rc;
+    TQB_REQUIRE(a->num_splits_per_seq == nullptr, TQB_ERR_INVALID_ARG, "a ranged call has one split count");
+    if (r != nullptr) {
+        rc = rotated_check(r, a);
+        if (rc != TQB_OK) return rc;
+    }
+    if (a->batch == 0) return TQB_OK;
+    TQB_REQUIRE(range->max_seq_len <= (int64_t)a->max_blocks_per_seq * tqb::kBlockSize, TQB_ERR_INVALID_ARG,
+                "max_seq_len must be at most max_blocks_per_seq * 16");
+    DeviceGuard guard(a->mid_o);
+    TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning mid_o");
+    const int nsm = sm_count();
+    TQB_REQUIRE(nsm > 0, TQB_ERR_CUDA, "cannot query the current CUDA device");
+    if (r != nullptr) {
+        // One kernel where the page ring serves the cache, as in
+        // tqb_stage1_rotated.
+        if (rotation_fuses(p)) {
+            tqb::Stage1Params pr = p;
+            fuse_rotation(pr, r);
+            rc = tqb::launch_stage1_ring_range(pr, stream, nsm);
+            if (rc != TQB_ERR_UNSUPPORTED) return rc;
+            g_detail[0] = '\0';
+        }
+        rc = tqb_rotate_query(r, stream);
+        if (rc != TQB_OK) return rc;
+    }
+    return tqb::launch_stage1_range(p, stream, nsm);
+}
+
+int tqb_stage2_range(const tqb_stage2_args* a, const tqb_range* range, int32_t lead, const float* sinks, int out_dtype,
+                     void* out, cudaStream_t stream) {
+    tqb::Stage2Params p{};
+    int rc = stage2_check(a, out, out_dtype, p);
+    if (rc != TQB_OK) return rc;
+    TQB_REQUIRE(lead >= 0 && lead < a->num_splits, TQB_ERR_INVALID_ARG, "lead must be in [0, num_splits)");
+    rc = range_check(range, a->num_splits - lead, p.range);
+    if (rc != TQB_OK || a->batch == 0) return rc;
+    TQB_REQUIRE(a->num_splits_per_seq == nullptr, TQB_ERR_INVALID_ARG, "a ranged call has one split count");
+    TQB_REQUIRE(aligned(sinks, 4), TQB_ERR_ALIGNMENT, "sinks must be 4-byte aligned");
+    p.lead = lead;
+    p.sinks = sinks;
+    DeviceGuard guard(out);
+    TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning output");
+    return tqb::launch_stage2_range(p, stream);
+}
+
+int tqb_append(const tqb_append_args* a, cudaStream_t stream) {
+    g_detail[0] = '\0';
+    TQB_REQUIRE(a != nullptr, TQB_ERR_INVALID_ARG, "args is NULL");
+    TQB_REQUIRE(a->num_tokens >= 0 && a->num_kv_heads > 0, TQB_ERR_INVALID_ARG,
+                "num_tokens must be >= 0 and num_kv_heads > 0");
+    TQB_REQUIRE(a->head_dim == tqb::kHeadDim, TQB_ERR_UNSUPPORTED, "head_dim must be 128");
+    TQB_REQUIRE(a->block_size == tqb::kBlockSize, TQB_ERR_UNSUPPORTED, "block_size must be 16");
+    TQB_REQUIRE(tqb::layout_valid(a->layout), TQB_ERR_INVALID_ARG, "layout must be a tqb_layout value");
+    TQB_REQUIRE(dtype_ok(a->dtype), TQB_ERR_INVALID_ARG, "dtype must be a tqb_dtype value");
+    const bool fp8 = tqb::layout_fp8_keys(a->layout);
+    TQB_REQUIRE(fp8 || a->n_centroids == (tqb::layout_3bit_keys(a->layout) ? 8 : tqb::kNumCentroids),
+                TQB_ERR_UNSUPPORTED, "n_centroids must be 16, or 8 for 3-bit keys");
+    TQB_REQUIRE(!(fp8 && a->norm_correction), TQB_ERR_INVALID_ARG, "the FP8-key layouts have no norm correction");
+    TQB_REQUIRE(a->positions == nullptr ||
+                    (a->rotary_dim > 0 && a->rotary_dim % 2 == 0 && a->rotary_dim <= tqb::kHeadDim && a->max_pos > 0 &&
+                     a->cos_sin_stride >= a->rotary_dim),
+                TQB_ERR_INVALID_ARG, "rotary_dim must be even, 2 .. 128, and cos_sin [max_pos > 0, rotary_dim]");
+    TQB_REQUIRE(a->query == nullptr || a->num_q_heads > 0, TQB_ERR_INVALID_ARG, "num_q_heads must be positive");
+    if (a->num_tokens == 0) return TQB_OK;
+    const int64_t most = a->query && a->num_q_heads > a->num_kv_heads ? a->num_q_heads : a->num_kv_heads;
+    TQB_REQUIRE(a->num_tokens * most < ((int64_t)1 << 31), TQB_ERR_UNSUPPORTED, "num_tokens x heads must be below 2^31");
+    TQB_REQUIRE(a->key && a->value && a->slot_mapping && a->kv_cache &&
+                    (fp8 || (a->rotation && a->midpoints && a->centroids)) && (!a->positions || a->cos_sin) &&
+                    (!a->query || a->q_rot),
+                TQB_ERR_INVALID_ARG, "a required pointer is NULL");
+    const uintptr_t es = a->dtype == TQB_DTYPE_F32 ? 4 : 2;
+    TQB_REQUIRE(aligned(a->key, es) && aligned(a->value, es) && aligned(a->query, es) && aligned(a->rotation, 16) &&
+                    aligned(a->midpoints, 4) && aligned(a->centroids, 4) && aligned(a->cos_sin, 4) &&
+                    aligned(a->q_rot, 4) && aligned(a->slot_mapping, 4) &&
+                    aligned(a->positions, a->positions_are_64 ? 8 : 4),
+                TQB_ERR_ALIGNMENT, "buffers must be aligned to their element size, rotation to 16 bytes");
+    const int rc = cache_check(a->kv_cache, a->layout, a->cache_stride_block, a->cache_stride_pos, a->cache_stride_head,
+                               a->num_kv_heads);
+    if (rc != TQB_OK) return rc;
+    DeviceGuard guard(a->kv_cache);
+    TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning kv_cache");
+    const int nsm = sm_count();
+    TQB_REQUIRE(nsm > 0, TQB_ERR_CUDA, "cannot query the current CUDA device");
+    tqb::AppendParams p{};
+    p.key = a->key;
+    p.value = a->value;
+    p.query = a->query;
+    p.dtype = a->dtype;
+    p.ksn = a->k_stride_n;
+    p.ksh = a->k_stride_h;
+    p.vsn = a->v_stride_n;
+    p.vsh = a->v_stride_h;
+    p.qsn = a->q_stride_n;
+    p.qsh = a->q_stride_h;
+    p.pos = a->positions;
+    p.pos_is_64 = a->positions_are_64;
+    p.cos_sin = a->cos_sin;
+    p.cs_stride = a->cos_sin_stride;
+    p.max_pos = a->max_pos;
+    p.rotary = a->positions ? a->rotary_dim : 0;
+    p.interleaved = a->interleaved;
+    p.rot = a->rotation;
+    p.mids = a->midpoints;
+    p.cents = a->centroids;
+    p.slots = a->slot_mapping;
+    p.cache = a->kv_cache;
+    p.layout = a->layout;
+    p.block_bytes = a->cache_stride_block;
+    p.pos_stride = a->cache_stride_pos;
+    p.head_stride = a->cache_stride_head;
+    p.num_blocks = a->num_blocks;
+    p.q_rot = a->q_rot;
+    p.osn = a->q_rot_stride_n;
+    p.osh = a->q_rot_stride_h;
+    p.N = a->num_tokens;
+    p.Hq = a->query ? a->num_q_heads : 0;
+    p.Hk = a->num_kv_heads;
+    p.norm_correction = a->norm_correction;
+    return tqb::launch_append(p, stream, nsm);
+}
+
+int tqb_gather(const tqb_gather_args* a, cudaStream_t stream) {
+    g_detail[0] = '\0';
+    TQB_REQUIRE(a != nullptr, TQB_ERR_INVALID_ARG, "args is NULL");
+    TQB_REQUIRE(a->num_tokens >= 0 && a->num_kv_heads > 0, TQB_ERR_INVALID_ARG,
+                "num_tokens must be >= 0 and num_kv_heads > 0");
+    TQB_REQUIRE(a->head_dim == tqb::kHeadDim, TQB_ERR_UNSUPPORTED, "head_dim must be 128");
+    TQB_REQUIRE(a->block_size == tqb::kBlockSize, TQB_ERR_UNSUPPORTED, "block_size must be 16");
+    TQB_REQUIRE(tqb::layout_valid(a->layout), TQB_ERR_INVALID_ARG, "layout must be a tqb_layout value");
+    TQB_REQUIRE(dtype_ok(a->out_dtype), TQB_ERR_INVALID_ARG, "out_dtype must be a tqb_dtype value");
+    const bool fp8 = tqb::layout_fp8_keys(a->layout);
+    TQB_REQUIRE(fp8 || a->n_centroids == (tqb::layout_3bit_keys(a->layout) ? 8 : tqb::kNumCentroids),
+                TQB_ERR_UNSUPPORTED, "n_centroids must be 16, or 8 for 3-bit keys");
+    if (a->num_tokens == 0) return TQB_OK;
+    TQB_REQUIRE((int64_t)a->num_tokens * a->num_kv_heads < ((int64_t)1 << 31), TQB_ERR_UNSUPPORTED,
+                "num_tokens x num_kv_heads must be below 2^31");
+    TQB_REQUIRE(a->kv_cache && a->slot_mapping && a->key && a->value && (fp8 || a->centroids), TQB_ERR_INVALID_ARG,
+                "a required pointer is NULL");
+    const uintptr_t es = a->out_dtype == TQB_DTYPE_F32 ? 4 : 2;
+    TQB_REQUIRE(aligned(a->key, es) && aligned(a->value, es) && aligned(a->slot_mapping, 4) && aligned(a->centroids, 4),
+                TQB_ERR_ALIGNMENT, "buffers must be aligned to their element size");
+    const int rc = cache_check(a->kv_cache, a->layout, a->cache_stride_block, a->cache_stride_pos, a->cache_stride_head,
+                               a->num_kv_heads);
+    if (rc != TQB_OK) return rc;
+    DeviceGuard guard(a->key);
+    TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning key");
+    tqb::GatherParams p{};
+    p.cache = a->kv_cache;
+    p.layout = a->layout;
+    p.block_bytes = a->cache_stride_block;
+    p.pos_stride = a->cache_stride_pos;
+    p.head_stride = a->cache_stride_head;
+    p.num_blocks = a->num_blocks;
+    p.slots = a->slot_mapping;
+    p.cents = a->centroids;
+    p.key = a->key;
+    p.value = a->value;
+    p.dtype = a->out_dtype;
+    p.ksn = a->k_stride_n;
+    p.ksh = a->k_stride_h;
+    p.vsn = a->v_stride_n;
+    p.vsh = a->v_stride_h;
+    p.N = a->num_tokens;
+    p.Hk = a->num_kv_heads;
+    return tqb::launch_gather(p, stream);
 }
 
 }  // extern "C"

@@ -58,6 +58,24 @@ struct FastDiv {
 #endif
 };
 
+// The tokens of a sequence that a ranged Stage1 attends to (tqb_range): the
+// last `window` of them (0: all) from `prefix` on, and the first `first` ones
+// before the window, which are split 0 on their own; splits `off` .. S - 1
+// then share the tokens [lo, L) equally.
+struct KeyRange {
+    int first, window, prefix;
+    int max_len;  // longer sequences are cut there (Stage1 and Stage2 alike)
+#ifdef __CUDACC__
+    __device__ __forceinline__ int len(int L) const { return min(L, max_len); }
+    __device__ __forceinline__ int off() const { return first > 0 ? 1 : 0; }  // splits before the window's
+    __device__ __forceinline__ int lo(int L) const {
+        const int w = window > 0 ? max(L - window, 0) : 0;
+        return min(max(w, prefix), max(L, 0));
+    }
+    __device__ __forceinline__ int firsts(int lo_) const { return min(first, lo_); }
+#endif
+};
+
 struct Stage1Params {
     const float* q;
     int64_t qsb, qsh;
@@ -77,6 +95,7 @@ struct Stage1Params {
     float attn_scale;
     int64_t num_items;  // B * S * Hk work items, KV head fastest (< 2^31)
     FastDiv div_hk, div_s;
+    KeyRange range;  // the tokens attended to (kernel instances with RG set)
     // Fused query rotation (the page-ring kernel only; rot == nullptr: off):
     // q_out[b, h, :] = float(rq[b, h, :]) @ rot, written by the kernel's
     // prologue before its producers load the rows from q (== q_out).
@@ -98,6 +117,11 @@ struct Stage2Params {
     float* lse;
     int64_t lsb;
     int B, Hq, S;
+    // Ranged merge (kernel instances with RG set): the first `lead` splits are
+    // always written, the others follow `range`; sinks is optional.
+    KeyRange range;
+    int lead;
+    const float* sinks;  // [Hq]
 };
 
 // Attention sinks folded into split 0 of mid_o (tqb_stage2.cu).
@@ -161,6 +185,40 @@ struct StoreParams {
     int norm_correction;
 };
 
+// RoPE, rotation, quantised store and query rotation of new tokens
+// (tqb_append.cu).
+struct AppendParams {
+    const void *key, *value, *query;  // query may be null
+    int dtype;                        // TQB_DTYPE_* of the three
+    int64_t ksn, ksh, vsn, vsh, qsn, qsh;
+    const void* pos;  // null: no rotary positions
+    int pos_is_64;
+    const float* cos_sin;
+    int64_t cs_stride;
+    int max_pos, rotary, interleaved;
+    const float *rot, *mids, *cents;
+    const int32_t* slots;
+    uint8_t* cache;
+    int layout;
+    int64_t block_bytes, pos_stride, head_stride, num_blocks;
+    float* q_rot;
+    int64_t osn, osh;
+    int N, Hq, Hk, norm_correction;
+};
+
+// Cached keys and values of chosen slots (tqb_gather.cu).
+struct GatherParams {
+    const uint8_t* cache;
+    int layout;
+    int64_t block_bytes, pos_stride, head_stride, num_blocks;
+    const int32_t* slots;
+    const float* cents;
+    void *key, *value;
+    int dtype;
+    int64_t ksn, ksh, vsn, vsh;
+    int N, Hk;
+};
+
 // Records the CUDA error text for tqb_last_error_detail(); returns
 // TQB_OK or TQB_ERR_LAUNCH.
 int report_launch(cudaError_t e);
@@ -187,5 +245,11 @@ int launch_sp_exchange(const SpExchangeParams& p, cudaStream_t stream);
 int launch_sp_merge(const SpMergeParams& p, cudaStream_t stream);
 int read_p2p_timeouts(unsigned int* count, bool reset);
 int launch_store(const StoreParams& p, cudaStream_t stream);
+// Stage1 and Stage2 over p.range (tqb_range).
+int launch_stage1_range(const Stage1Params& p, cudaStream_t stream, int num_sms);
+int launch_stage1_ring_range(const Stage1Params& p, cudaStream_t stream, int num_sms);
+int launch_stage2_range(const Stage2Params& p, cudaStream_t stream);
+int launch_append(const AppendParams& p, cudaStream_t stream, int num_sms);
+int launch_gather(const GatherParams& p, cudaStream_t stream);
 
 }  // namespace tqb

@@ -21,7 +21,9 @@ namespace tqb {
 
 constexpr int kSplitsPerPass = 4;  // splits whose loads a warp keeps in flight at once
 
-template <int kParts = kHeadDim / 32>
+// RG: the splits of a ranged call (Stage2Params::range, lead), and the sink
+// logit of the head as one more weight.
+template <int kParts = kHeadDim / 32, bool RG = false>
 __device__ __forceinline__ void merge_row(const Stage2Params& P, int b, int h, float* o, float* lse_out) {
     static_assert(kParts * 32 >= kHeadDim, "one thread per output dim");
     __shared__ float s_acc[kParts][kHeadDim];
@@ -31,7 +33,19 @@ __device__ __forceinline__ void merge_row(const Stage2Params& P, int b, int h, f
     const int L = __ldg(P.seq_lens + b);
     const int split_len = nsp > 0 ? (L + nsp - 1) / nsp : 0;
     // split s is non-empty iff split_len * s < L (its end is min(.., L))
-    const int nvalid = split_len > 0 ? min(nsp, (L + split_len - 1) / split_len) : 0;
+    int nvalid = split_len > 0 ? min(nsp, (L + split_len - 1) / split_len) : 0;
+    // ranged: valid split i is split i, or i + skip from the lead splits on
+    // (the split of the first tokens is empty unless the window starts after
+    // token 0)
+    int skip = 0;
+    if constexpr (RG) {
+        const int Lr = P.range.len(L);
+        const int lo = P.range.lo(Lr), off = P.range.off(), n = Lr - lo, per = P.S - P.lead - off;
+        const int sl = (n + per - 1) / per;
+        const int has_first = P.range.firsts(lo) > 0 ? 1 : 0;
+        nvalid = L > 0 ? P.lead + has_first + (sl > 0 ? (n + sl - 1) / sl : 0) : 0;
+        skip = off - has_first;
+    }
     const float* row0 = P.mid + (int64_t)b * P.msb + (int64_t)h * P.msh;
 
     float m = -INFINITY, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -40,7 +54,7 @@ __device__ __forceinline__ void merge_row(const Stage2Params& P, int b, int h, f
 #pragma unroll
         for (int k = 0; k < kSplitsPerPass; k++) {
             const int s = s0 + kParts * k;
-            const float* row = row0 + (int64_t)s * P.mss;
+            const float* row = row0 + (int64_t)(RG && s >= P.lead ? s + skip : s) * P.mss;
             ls[k] = s < nvalid ? __ldg(row + kHeadDim) : -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; j++) os[k][j] = s < nvalid ? __ldg(row + lane + 32 * j) : 0.0f;
@@ -73,6 +87,13 @@ __device__ __forceinline__ void merge_row(const Stage2Params& P, int b, int h, f
 #pragma unroll
     for (int p = 0; p < kParts; p++) gmax = fmaxf(gmax, s_max[p]);
     float acc_d = 0.0f, wsum = 0.0f;
+    if constexpr (RG) {
+        if (P.sinks != nullptr && nvalid > 0) {
+            const float sink = __ldg(P.sinks + h);
+            gmax = fmaxf(gmax, sink);
+            wsum = sink == -INFINITY ? 0.0f : ex2_approx((sink - gmax) * kLog2e);
+        }
+    }
 #pragma unroll
     for (int p = 0; p < kParts; p++) {
         const float w = s_max[p] == -INFINITY ? 0.0f : ex2_approx((s_max[p] - gmax) * kLog2e);

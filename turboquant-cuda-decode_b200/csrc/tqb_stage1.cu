@@ -480,7 +480,7 @@ __device__ __forceinline__ void process_page(ItemState<NT>& st, const PageRegs& 
     }
 }
 
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
     stage1_kernel(const Stage1Params P) {
     // Shared memory: the K table (256 entries x 256 bytes: SoA keeps 32 lane
@@ -543,6 +543,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
         const uint32_t bq = P.div_s.div(rest);
         r.s = (int)(rest - bq * (uint32_t)P.S);
         r.b = (int)bq;
+        if constexpr (RG) {
+            const int L = P.range.len(__ldg(P.seq_lens + r.b));
+            const int lo = P.range.lo(L), off = P.range.off();
+            r.start = 0;
+            if (r.s < off) {  // the first tokens
+                r.end = P.range.firsts(lo);
+            } else {
+                const int split_len = (L - lo + P.S - off - 1) / (P.S - off);
+                r.start = lo + split_len * (r.s - off);
+                r.end = min(r.start + split_len, L);
+            }
+            return r.start < r.end;
+        }
         const int nsp = P.nsplits ? min(__ldg(P.nsplits + r.b), P.S) : P.S;
         if (r.s >= nsp) return false;
         // Tokens past the block-table row are outside the sequence's pages.
@@ -711,10 +724,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
     }
 }
 
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG>
 int launch_t(const Stage1Params& P, cudaStream_t stream, int num_sms) {
     const size_t smem = kLutBytes + (size_t)kWarps * NT * 4 * (kHeadDim + 1) * sizeof(float);
-    auto kern = stage1_kernel<NT, LAYOUT>;
+    auto kern = stage1_kernel<NT, LAYOUT, RG>;
     static thread_local int configured_dev = -1;  // per template instance
     int dev = 0;
     cudaGetDevice(&dev);
@@ -741,38 +754,46 @@ bool stage1_register_kernel_forced() {
     return v != nullptr && strcmp(v, "regs") == 0;
 }
 
-int launch_stage1(const Stage1Params& P, cudaStream_t stream, int num_sms) {
+template <bool RG>
+static int launch_stage1_rg(const Stage1Params& P, cudaStream_t stream, int num_sms) {
     if (stage1_ring_supported(P) && !stage1_register_kernel_forced()) {
-        const int rc = launch_stage1_ring(P, stream, num_sms);
+        const int rc = RG ? launch_stage1_ring_range(P, stream, num_sms) : launch_stage1_ring(P, stream, num_sms);
         if (rc != TQB_ERR_UNSUPPORTED) return rc;  // else: tensor maps refused, use the register kernel
     }
     switch (P.layout) {
         case TQB_LAYOUT_AOS_K8:
-            return P.G <= 4 ? launch_t<1, TQB_LAYOUT_AOS_K8>(P, stream, num_sms)
-                            : launch_t<2, TQB_LAYOUT_AOS_K8>(P, stream, num_sms);
+            return P.G <= 4 ? launch_t<1, TQB_LAYOUT_AOS_K8, RG>(P, stream, num_sms)
+                            : launch_t<2, TQB_LAYOUT_AOS_K8, RG>(P, stream, num_sms);
         case TQB_LAYOUT_AOS_K3:
-            return P.G <= 4 ? launch_t<1, TQB_LAYOUT_AOS_K3>(P, stream, num_sms)
-                            : launch_t<2, TQB_LAYOUT_AOS_K3>(P, stream, num_sms);
+            return P.G <= 4 ? launch_t<1, TQB_LAYOUT_AOS_K3, RG>(P, stream, num_sms)
+                            : launch_t<2, TQB_LAYOUT_AOS_K3, RG>(P, stream, num_sms);
         case TQB_LAYOUT_AOS_K3V3:
-            return P.G <= 4 ? launch_t<1, TQB_LAYOUT_AOS_K3V3>(P, stream, num_sms)
-                            : launch_t<2, TQB_LAYOUT_AOS_K3V3>(P, stream, num_sms);
+            return P.G <= 4 ? launch_t<1, TQB_LAYOUT_AOS_K3V3, RG>(P, stream, num_sms)
+                            : launch_t<2, TQB_LAYOUT_AOS_K3V3, RG>(P, stream, num_sms);
         default:
             break;
     }
     if (P.layout == TQB_LAYOUT_SOA_K8)
-        return P.G <= 4 ? launch_t<1, TQB_LAYOUT_SOA_K8>(P, stream, num_sms)
-                        : launch_t<2, TQB_LAYOUT_SOA_K8>(P, stream, num_sms);
+        return P.G <= 4 ? launch_t<1, TQB_LAYOUT_SOA_K8, RG>(P, stream, num_sms)
+                        : launch_t<2, TQB_LAYOUT_SOA_K8, RG>(P, stream, num_sms);
     if (P.layout == TQB_LAYOUT_SOA_K3)
-        return P.G <= 4 ? launch_t<1, TQB_LAYOUT_SOA_K3>(P, stream, num_sms)
-                        : launch_t<2, TQB_LAYOUT_SOA_K3>(P, stream, num_sms);
+        return P.G <= 4 ? launch_t<1, TQB_LAYOUT_SOA_K3, RG>(P, stream, num_sms)
+                        : launch_t<2, TQB_LAYOUT_SOA_K3, RG>(P, stream, num_sms);
     if (P.layout == TQB_LAYOUT_SOA_K3V3)
-        return P.G <= 4 ? launch_t<1, TQB_LAYOUT_SOA_K3V3>(P, stream, num_sms)
-                        : launch_t<2, TQB_LAYOUT_SOA_K3V3>(P, stream, num_sms);
+        return P.G <= 4 ? launch_t<1, TQB_LAYOUT_SOA_K3V3, RG>(P, stream, num_sms)
+                        : launch_t<2, TQB_LAYOUT_SOA_K3V3, RG>(P, stream, num_sms);
     const bool soa = P.layout == TQB_LAYOUT_SOA;
-    if (P.G <= 4) return soa ? launch_t<1, TQB_LAYOUT_SOA>(P, stream, num_sms)
-                             : launch_t<1, TQB_LAYOUT_AOS>(P, stream, num_sms);
-    return soa ? launch_t<2, TQB_LAYOUT_SOA>(P, stream, num_sms)
-               : launch_t<2, TQB_LAYOUT_AOS>(P, stream, num_sms);
+    if (P.G <= 4) return soa ? launch_t<1, TQB_LAYOUT_SOA, RG>(P, stream, num_sms)
+                             : launch_t<1, TQB_LAYOUT_AOS, RG>(P, stream, num_sms);
+    return soa ? launch_t<2, TQB_LAYOUT_SOA, RG>(P, stream, num_sms)
+               : launch_t<2, TQB_LAYOUT_AOS, RG>(P, stream, num_sms);
+}
+
+int launch_stage1(const Stage1Params& P, cudaStream_t stream, int num_sms) {
+    return launch_stage1_rg<false>(P, stream, num_sms);
+}
+int launch_stage1_range(const Stage1Params& P, cudaStream_t stream, int num_sms) {
+    return launch_stage1_rg<true>(P, stream, num_sms);
 }
 
 }  // namespace tqb

@@ -309,6 +309,7 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
 struct ItemInfo {
     int b, s, kvh, start, end;
 };
+template <bool RG>
 __device__ __forceinline__ bool decode_item(const Stage1Params& P, uint32_t item, ItemInfo& r) {
     r.b = r.s = r.kvh = r.start = r.end = 0;
     if (item >= (uint32_t)P.num_items) return false;
@@ -317,6 +318,18 @@ __device__ __forceinline__ bool decode_item(const Stage1Params& P, uint32_t item
     const uint32_t bq = P.div_s.div(rest);
     r.s = (int)(rest - bq * (uint32_t)P.S);
     r.b = (int)bq;
+    if constexpr (RG) {
+        const int L = P.range.len(__ldg(P.seq_lens + r.b));
+        const int lo = P.range.lo(L), off = P.range.off();
+        if (r.s < off) {  // the first tokens
+            r.end = P.range.firsts(lo);
+        } else {
+            const int split_len = (L - lo + P.S - off - 1) / (P.S - off);
+            r.start = lo + split_len * (r.s - off);
+            r.end = min(r.start + split_len, L);
+        }
+        return r.start < r.end;
+    }
     const int nsp = P.nsplits ? min(__ldg(P.nsplits + r.b), P.S) : P.S;
     if (r.s >= nsp) return false;
     const int L = min(__ldg(P.seq_lens + r.b), P.max_blocks * kBlockSize);
@@ -330,9 +343,10 @@ __device__ __forceinline__ bool decode_item(const Stage1Params& P, uint32_t item
 // Lanes 0-7 decode the 8 items of tile t (lane l: item 8t + l); returns the
 // lane's page count (0 for lanes >= 8 and empty items) in `np` and the
 // tile's page count (max over its items) as the result.
+template <bool RG>
 __device__ __forceinline__ int tile_items(const Stage1Params& P, uint32_t t, int lane, ItemInfo& ir, int& np) {
     np = 0;
-    if (lane < kGroupWarps && decode_item(P, t * kGroupWarps + lane, ir))
+    if (lane < kGroupWarps && decode_item<RG>(P, t * kGroupWarps + lane, ir))
         np = (ir.end - 1) / kBlockSize - ir.start / kBlockSize + 1;
     else
         ir.b = ir.s = ir.kvh = ir.start = ir.end = 0;
@@ -355,24 +369,41 @@ __device__ __forceinline__ int tile_items(const Stage1Params& P, uint32_t t, int
 // splits weigh nothing either way.  Every CTA derives the same cut from
 // seq_lens (and nsplits), so no state is shared between CTAs or launches.
 // ---------------------------------------------------------------------------
+// A ranged call adds the split of the first tokens in front: nf tokens, and
+// `base` the index of the first of the ne splits after it.
 struct SeqSplit {
     int L, sl, ne;  // clamped length, split length, non-empty splits
+    int nf, base;
 };
+template <bool RG>
 __device__ __forceinline__ SeqSplit seq_split_of(const Stage1Params& P, int len, int nsplit) {
-    SeqSplit r{0, 1, 0};
-    const int nsp = min(nsplit, P.S);
-    const int L = min(len, P.max_blocks * kBlockSize);
+    SeqSplit r{0, 1, 0, 0, 0};
+    int nsp = min(nsplit, P.S);
+    int L = min(len, P.max_blocks * kBlockSize);
+    if constexpr (RG) {
+        L = P.range.len(len);
+        const int lo = P.range.lo(L);
+        r.base = P.range.off();
+        r.nf = P.range.firsts(lo);
+        nsp = P.S - r.base;
+        L -= lo;
+    }
     if (nsp <= 0 || L <= 0) return r;
     r.L = L;
     r.sl = (L + nsp - 1) / nsp;  // ceil(L / nsp), the split rule of decode_item
     r.ne = (L + r.sl - 1) / r.sl;
     return r;
 }
+template <bool RG>
 __device__ __forceinline__ SeqSplit seq_split(const Stage1Params& P, int b) {
-    return seq_split_of(P, __ldg(P.seq_lens + b), P.nsplits ? __ldg(P.nsplits + b) : P.S);
+    return seq_split_of<RG>(P, __ldg(P.seq_lens + b), P.nsplits ? __ldg(P.nsplits + b) : P.S);
 }
 __device__ __forceinline__ long long seq_weight(const Stage1Params& P, const SeqSplit& q, bool by_count) {
     return by_count ? (long long)P.Hk * q.ne : (long long)P.Hk * ((long long)q.L + (long long)kSplitCost * q.ne);
+}
+// Weight of the split of the first tokens, per KV head (0: none).
+__device__ __forceinline__ long long first_weight(const SeqSplit& q, bool by_count) {
+    return q.nf <= 0 ? 0 : by_count ? 1 : (long long)(q.nf + kSplitCost);
 }
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
 #pragma unroll
@@ -382,15 +413,24 @@ __device__ __forceinline__ long long warp_sum_ll(long long v) {
 // Tile of the first item of sequence b whose start weight reaches r (>= 1,
 // at most the sequence's weight): split s* = the last split starting below
 // r, then the KV head in it.
+template <bool RG>
 __device__ __forceinline__ uint32_t cut_tile(const Stage1Params& P, const SeqSplit& q, int b, long long r,
                                              uint32_t num_tiles, bool by_count) {
+    if constexpr (RG) {
+        const long long fw = first_weight(q, by_count);
+        if (r <= fw * P.Hk) {
+            const long long item = (long long)b * P.S * P.Hk + (r + fw - 1) / fw;
+            return (uint32_t)min((long long)num_tiles, (item + kGroupWarps - 1) / kGroupWarps);
+        }
+        r -= fw * P.Hk;
+    }
     const long long unit = by_count ? (long long)P.Hk : (long long)P.Hk * (q.sl + kSplitCost);
     const long long ss = min((long long)(q.ne - 1), (r - 1) / unit);
     const long long a = unit * ss;
     const long long per =
         by_count ? 1 : (long long)(min((int)(ss + 1) * q.sl, q.L) - (int)ss * q.sl) + kSplitCost;
     const long long kv = (r - a + per - 1) / per;  // in [1, Hk]
-    const long long item = ((long long)b * P.S + ss) * P.Hk + kv;
+    const long long item = ((long long)b * P.S + ss + (RG ? q.base : 0)) * P.Hk + kv;
     return (uint32_t)min((long long)num_tiles, (item + kGroupWarps - 1) / kGroupWarps);
 }
 // Tile walk of group gi of this CTA: tiles first, first + stride, ... below
@@ -400,6 +440,7 @@ __device__ __forceinline__ uint32_t cut_tile(const Stage1Params& P, const SeqSpl
 // warps keep their query fragments across them); any other batch takes the
 // contiguous ranges of the weight cut.  One warp (compact loops:
 // this code runs once, cold, ahead of every other warp's first tile).
+template <bool RG>
 __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uint32_t num_tiles, uint32_t (&res)[3],
                           int lane) {
     const uint32_t cuts = gridDim.x * (uint32_t)groups_per_cta;
@@ -411,9 +452,13 @@ __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uin
         const int b = b0 + lane;
         if (b < P.B) {
             const int len = __ldg(P.seq_lens + b), nsp = P.nsplits ? __ldg(P.nsplits + b) : P.S;
-            const SeqSplit q = seq_split_of(P, len, nsp);
+            const SeqSplit q = seq_split_of<RG>(P, len, nsp);
             tot += seq_weight(P, q, false);
             cnt += seq_weight(P, q, true);
+            if constexpr (RG) {
+                tot += P.Hk * first_weight(q, false);
+                cnt += P.Hk * first_weight(q, true);
+            }
             lmin = min(lmin, len);
             lmax = max(lmax, len);
             nmin = min(nmin, nsp);
@@ -422,7 +467,8 @@ __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uin
     }
     tot = warp_sum_ll(tot);
     cnt = warp_sum_ll(cnt);
-    if (__reduce_min_sync(0xffffffffu, lmin) == __reduce_max_sync(0xffffffffu, lmax) &&
+    // (a ranged call with first tokens has splits of two lengths: weight cut)
+    if ((!RG || P.range.first == 0) && __reduce_min_sync(0xffffffffu, lmin) == __reduce_max_sync(0xffffffffu, lmax) &&
         __reduce_min_sync(0xffffffffu, nmin) == __reduce_max_sync(0xffffffffu, nmax)) {
         // contiguous ranges: consecutive tiles of a group are consecutive
         // splits of one sequence, so its warps keep their query fragments
@@ -449,9 +495,9 @@ __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uin
 #pragma unroll 1
             for (int b0 = 0; b0 < P.B; b0 += 32) {
                 const int b = b0 + lane;
-                SeqSplit q{0, 1, 0};
-                if (b < P.B) q = seq_split(P, b);
-                const long long w = seq_weight(P, q, by_count);
+                SeqSplit q{0, 1, 0, 0, 0};
+                if (b < P.B) q = seq_split<RG>(P, b);
+                const long long w = seq_weight(P, q, by_count) + (RG ? P.Hk * first_weight(q, by_count) : 0);
                 long long incl = w;
 #pragma unroll 1
                 for (int o = 1; o < 32; o <<= 1) {
@@ -462,7 +508,7 @@ __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uin
                 const bool here = w > 0 && excl < tgt && tgt <= base + incl;
                 const uint32_t m = __ballot_sync(0xffffffffu, here);
                 if (m) {
-                    const uint32_t tl = here ? cut_tile(P, q, b, tgt - excl, num_tiles, by_count) : 0u;
+                    const uint32_t tl = here ? cut_tile<RG>(P, q, b, tgt - excl, num_tiles, by_count) : 0u;
                     t = __shfl_sync(0xffffffffu, tl, __ffs(m) - 1);
                     break;
                 }
@@ -580,7 +626,7 @@ __device__ __forceinline__ bool rot_barrier_wait(uint32_t seen, int lane) {
 // Runs at kProducerRegs registers, so run parameters live one run per lane
 // and block ids are fetched one stage ahead into a single register.
 // ---------------------------------------------------------------------------
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG>
 __device__ __forceinline__ void produce(const Stage1Params& P, const RingMaps& M, const GroupSmem& gs, int gi,
                                         int lane, int pj, int npj) {
     using C = Cfg<NT, LAYOUT>;
@@ -626,7 +672,7 @@ __device__ __forceinline__ void produce(const Stage1Params& P, const RingMaps& M
     // Next tile of this group with at least one page (or t >= t_end).
     auto next_tile = [&](uint32_t t, ItemInfo& x, int& npx, int& np_tile) {
         for (; t < t_end; t += t_stride)
-            if ((np_tile = tile_items(P, t, lane, x, npx)) > 0) return t;
+            if ((np_tile = tile_items<RG>(P, t, lane, x, npx)) > 0) return t;
         return t;
     };
 
@@ -1143,7 +1189,7 @@ __device__ __forceinline__ bool page_step(ItemState<NT>& st, const GroupSmem& gs
     return true;
 }
 
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG>
 __device__ __forceinline__ void consume(const Stage1Params& P, const GroupSmem& gs, int gi, int w, int lane,
                                         int ec) {
     using C = Cfg<NT, LAYOUT>;
@@ -1232,7 +1278,7 @@ __device__ __forceinline__ void consume(const Stage1Params& P, const GroupSmem& 
     for (uint32_t t = t_first; t < t_end; t += t_stride) {
         ItemInfo ir;
         int np;
-        const int np_tile = tile_items(P, t, lane, ir, np);
+        const int np_tile = tile_items<RG>(P, t, lane, ir, np);
         if (np_tile == 0) continue;
         const int b = __shfl_sync(0xffffffffu, ir.b, w);
         const int s = __shfl_sync(0xffffffffu, ir.s, w);
@@ -1323,7 +1369,7 @@ __device__ __forceinline__ void consume(const Stage1Params& P, const GroupSmem& 
     }
 }
 
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG>
 __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     stage1_ring_kernel(const Stage1Params P, const __grid_constant__ RingMaps M) {
     using C = Cfg<NT, LAYOUT>;
@@ -1348,7 +1394,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     const int planner = warp - (C::kWarps - C::kGroups);  // group planned by this warp, if >= 0
     uint32_t walk[3] = {0u, 0u, 0u};
     if (planner >= 0)
-        tile_walk(P, planner, C::kGroups, num_tiles, walk, lane);
+        tile_walk<RG>(P, planner, C::kGroups, num_tiles, walk, lane);
     else if (C::kTable)
         for (int e = tid; e < 256 * kLutCopies; e += C::kThreads - 32 * C::kGroups) {
         const int byte = e / kLutCopies;
@@ -1414,23 +1460,23 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     if (producer) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(C::kProducerRegs));
         const int pj = (warp - C::kComputeWarps) / C::kGroups;
-        if (pj < kProducersPerGroup) produce<NT, LAYOUT>(P, M, gs, gi, lane, pj, kProducersPerGroup);
+        if (pj < kProducersPerGroup) produce<NT, LAYOUT, RG>(P, M, gs, gi, lane, pj, kProducersPerGroup);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(C::kComputeRegs));
-        consume<NT, LAYOUT>(P, gs, gi, warp % kGroupWarps, lane, ec);
+        consume<NT, LAYOUT, RG>(P, gs, gi, warp % kGroupWarps, lane, ec);
     }
 }
 
 // True when the compiled kernel launches with enough registers per thread
 // for its setmaxnreg split (otherwise a setmaxnreg.inc could wait forever,
 // so the ring kernel is not used).
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG = false>
 bool ring_registers_ok() {
     using C = Cfg<NT, LAYOUT>;
     static int ok = -1;
     if (ok < 0) {
         cudaFuncAttributes a{};
-        ok = cudaFuncGetAttributes(&a, stage1_ring_kernel<NT, LAYOUT>) == cudaSuccess &&
+        ok = cudaFuncGetAttributes(&a, stage1_ring_kernel<NT, LAYOUT, RG>) == cudaSuccess &&
              (int64_t)a.numRegs * C::kThreads >=
                  (int64_t)C::kComputeWarps * 32 * C::kComputeRegs + 128 * C::kProducerRegs &&
              a.maxThreadsPerBlock >= C::kThreads;
@@ -1489,10 +1535,11 @@ bool encode_maps(const Stage1Params& P, RingMaps& M) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG>
 int launch_ring_t(const Stage1Params& P, const RingMaps& M, cudaStream_t stream, int num_sms) {
     using C = Cfg<NT, LAYOUT>;
-    auto kern = stage1_ring_kernel<NT, LAYOUT>;
+    if (RG && !ring_registers_ok<NT, LAYOUT, RG>()) return TQB_ERR_UNSUPPORTED;
+    auto kern = stage1_ring_kernel<NT, LAYOUT, RG>;
     static thread_local int configured_dev = -1;
     int dev = 0;
     cudaGetDevice(&dev);
@@ -1568,36 +1615,44 @@ bool stage1_ring_supported(const Stage1Params& P) {
            P.qsb >= P.qsh && (P.qsb & 3) == 0 && encoder() != nullptr;
 }
 
-int launch_stage1_ring(const Stage1Params& P, cudaStream_t stream, int num_sms) {
+template <bool RG>
+static int launch_stage1_ring_rg(const Stage1Params& P, cudaStream_t stream, int num_sms) {
     RingMaps M;
     if (!encode_maps(P, M)) return TQB_ERR_UNSUPPORTED;
     if (P.layout == TQB_LAYOUT_SOA)
-        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_SOA>(P, M, stream, num_sms)
-                        : launch_ring_t<2, TQB_LAYOUT_SOA>(P, M, stream, num_sms);
+        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_SOA, RG>(P, M, stream, num_sms)
+                        : launch_ring_t<2, TQB_LAYOUT_SOA, RG>(P, M, stream, num_sms);
     if (P.layout == TQB_LAYOUT_SOA_K8) {
         if (P.rot != nullptr) return TQB_ERR_UNSUPPORTED;  // no rotation prologue in this instance
-        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_SOA_K8>(P, M, stream, num_sms)
-                        : launch_ring_t<2, TQB_LAYOUT_SOA_K8>(P, M, stream, num_sms);
+        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_SOA_K8, RG>(P, M, stream, num_sms)
+                        : launch_ring_t<2, TQB_LAYOUT_SOA_K8, RG>(P, M, stream, num_sms);
     }
     if (P.layout == TQB_LAYOUT_AOS_K8) {
         if (P.rot != nullptr) return TQB_ERR_UNSUPPORTED;  // no rotation prologue in this instance
-        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_AOS_K8>(P, M, stream, num_sms)
-                        : launch_ring_t<2, TQB_LAYOUT_AOS_K8>(P, M, stream, num_sms);
+        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_AOS_K8, RG>(P, M, stream, num_sms)
+                        : launch_ring_t<2, TQB_LAYOUT_AOS_K8, RG>(P, M, stream, num_sms);
     }
     if (P.layout == TQB_LAYOUT_AOS_K3)
-        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_AOS_K3>(P, M, stream, num_sms)
-                        : launch_ring_t<2, TQB_LAYOUT_AOS_K3>(P, M, stream, num_sms);
+        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_AOS_K3, RG>(P, M, stream, num_sms)
+                        : launch_ring_t<2, TQB_LAYOUT_AOS_K3, RG>(P, M, stream, num_sms);
     if (P.layout == TQB_LAYOUT_AOS_K3V3)
-        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_AOS_K3V3>(P, M, stream, num_sms)
-                        : launch_ring_t<2, TQB_LAYOUT_AOS_K3V3>(P, M, stream, num_sms);
+        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_AOS_K3V3, RG>(P, M, stream, num_sms)
+                        : launch_ring_t<2, TQB_LAYOUT_AOS_K3V3, RG>(P, M, stream, num_sms);
     if (P.layout == TQB_LAYOUT_SOA_K3)
-        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_SOA_K3>(P, M, stream, num_sms)
-                        : launch_ring_t<2, TQB_LAYOUT_SOA_K3>(P, M, stream, num_sms);
+        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_SOA_K3, RG>(P, M, stream, num_sms)
+                        : launch_ring_t<2, TQB_LAYOUT_SOA_K3, RG>(P, M, stream, num_sms);
     if (P.layout == TQB_LAYOUT_SOA_K3V3)
-        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_SOA_K3V3>(P, M, stream, num_sms)
-                        : launch_ring_t<2, TQB_LAYOUT_SOA_K3V3>(P, M, stream, num_sms);
-    return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_AOS>(P, M, stream, num_sms)
-                    : launch_ring_t<2, TQB_LAYOUT_AOS>(P, M, stream, num_sms);
+        return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_SOA_K3V3, RG>(P, M, stream, num_sms)
+                        : launch_ring_t<2, TQB_LAYOUT_SOA_K3V3, RG>(P, M, stream, num_sms);
+    return P.G <= 4 ? launch_ring_t<1, TQB_LAYOUT_AOS, RG>(P, M, stream, num_sms)
+                    : launch_ring_t<2, TQB_LAYOUT_AOS, RG>(P, M, stream, num_sms);
+}
+
+int launch_stage1_ring(const Stage1Params& P, cudaStream_t stream, int num_sms) {
+    return launch_stage1_ring_rg<false>(P, stream, num_sms);
+}
+int launch_stage1_ring_range(const Stage1Params& P, cudaStream_t stream, int num_sms) {
+    return launch_stage1_ring_rg<true>(P, stream, num_sms);
 }
 
 int read_wait_timeouts(unsigned int* count, bool reset) {

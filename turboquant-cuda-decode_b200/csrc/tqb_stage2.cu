@@ -32,14 +32,14 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 
 // One CTA of 4 warps per (b, h): merge_row (tqb_merge_row.cuh) merges the
 // row's non-empty splits; thread d writes output dim d, thread 0 the LSE.
-template <typename OutT>
+template <typename OutT, bool RG>
 __global__ void __launch_bounds__(kHeadDim, 8) stage2_kernel(const Stage2Params P) {
     pdl_trigger();
     pdl_wait();  // Stage1's partials, when it ran just before on the stream
     const int64_t item = blockIdx.x;  // b * Hq + h
     const int b = (int)(item / P.Hq), h = (int)(item % P.Hq);
     float o, lse;
-    merge_row(P, b, h, &o, &lse);
+    merge_row<kHeadDim / 32, RG>(P, b, h, &o, &lse);
     OutT* out = static_cast<OutT*>(P.out) + (int64_t)b * P.osb + (int64_t)h * P.osh;
     out[threadIdx.x] = from_f32<OutT>(o);
     if (threadIdx.x == 0) P.lse[(int64_t)b * P.lsb + h] = lse;
@@ -102,17 +102,22 @@ __global__ void __launch_bounds__(kWarpsPerCta * 32) sink_fold_kernel(const Sink
 
 }  // namespace
 
-int launch_stage2(const Stage2Params& P, cudaStream_t stream) {
+template <bool RG>
+static int launch_stage2_rg(const Stage2Params& P, cudaStream_t stream) {
     const int64_t items = (int64_t)P.B * P.Hq;
     if (items == 0) return TQB_OK;
+    const dim3 grid((unsigned)items), block(kHeadDim);
     switch (P.out_dtype) {
-        case TQB_DTYPE_F32: return report_launch(launch_pdl(stage2_kernel<float>, dim3((unsigned)items), dim3(kHeadDim), 0, stream, P));
-        case TQB_DTYPE_F16: return report_launch(launch_pdl(stage2_kernel<__half>, dim3((unsigned)items), dim3(kHeadDim), 0, stream, P));
+        case TQB_DTYPE_F32: return report_launch(launch_pdl(stage2_kernel<float, RG>, grid, block, 0, stream, P));
+        case TQB_DTYPE_F16: return report_launch(launch_pdl(stage2_kernel<__half, RG>, grid, block, 0, stream, P));
         case TQB_DTYPE_BF16:
-            return report_launch(launch_pdl(stage2_kernel<__nv_bfloat16>, dim3((unsigned)items), dim3(kHeadDim), 0, stream, P));
+            return report_launch(launch_pdl(stage2_kernel<__nv_bfloat16, RG>, grid, block, 0, stream, P));
         default: return TQB_ERR_INVALID_ARG;
     }
 }
+
+int launch_stage2(const Stage2Params& P, cudaStream_t stream) { return launch_stage2_rg<false>(P, stream); }
+int launch_stage2_range(const Stage2Params& P, cudaStream_t stream) { return launch_stage2_rg<true>(P, stream); }
 
 int launch_merge(const MergeParams& P, cudaStream_t stream) {
     const int64_t items = (int64_t)P.B * P.Hq;

@@ -12,6 +12,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -20,8 +22,8 @@ INCLUDE = PKG_DIR.parent.parent / "include"
 LIB_PATH = PKG_DIR / "libtqb.so"
 
 SOURCES = ["tqb_api.cu", "tqb_stage1.cu", "tqb_stage1_ring.cu", "tqb_stage2.cu", "tqb_store.cu", "tqb_noalloc.cu",
-           "tqb_rotate.cu", "tqb_p2p.cu"]
-HEADERS = ["tqb_common.cuh", "tqb_internal.h", "tqb_merge_row.cuh"]
+           "tqb_rotate.cu", "tqb_p2p.cu", "tqb_append.cu", "tqb_gather.cu"]
+HEADERS = ["tqb_common.cuh", "tqb_internal.h", "tqb_merge_row.cuh", "tqb_quant_row.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -52,16 +54,22 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
     if not force and not _stale():
         return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [nvcc_path(), *ARCH_FLAGS, *NVCC_FLAGS, *(extra_flags or []),
-           f"-I{INCLUDE}", "-shared", "-o", str(tmp),
-           *[str(CSRC / s) for s in SOURCES]]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    if verbose and (res.stdout or res.stderr):
-        print(res.stdout + res.stderr, flush=True)
+    nvcc, flags = nvcc_path(), [*ARCH_FLAGS, *NVCC_FLAGS, *(extra_flags or []), f"-I{INCLUDE}"]
+    with tempfile.TemporaryDirectory() as objs:
+        def run(cmd: list[str]) -> None:
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            res = subprocess.run(cmd, capture_output=True, text=True)
+            if res.returncode != 0:
+                raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+            if verbose and (res.stdout or res.stderr):
+                print(res.stdout + res.stderr, flush=True)
+
+        # one compiler process per source, at most one per core
+        obj = {s: str(Path(objs) / f"{s}.o") for s in SOURCES}
+        with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            list(pool.map(lambda s: run([nvcc, *flags, "-c", str(CSRC / s), "-o", obj[s]]), SOURCES))
+        run([nvcc, *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", str(tmp), *obj.values()])
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

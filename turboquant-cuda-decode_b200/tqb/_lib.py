@@ -27,6 +27,9 @@ TQB_LAYOUT_AOS = 1
 TQB_LAYOUT_SOA_K8 = 2
 TQB_LAYOUT_SOA_K3 = 3
 TQB_LAYOUT_SOA_K3V3 = 4
+TQB_LAYOUT_AOS_K8 = 5
+TQB_LAYOUT_AOS_K3 = 6
+TQB_LAYOUT_AOS_K3V3 = 7
 
 TQB_P2P_MAX_RANKS = 8
 TQB_IPC_HANDLE_BYTES = 64
@@ -58,6 +61,10 @@ EXPORTED_SYMBOLS = (
     "tqb_ipc_close",
     "tqb_sp_exchange",
     "tqb_sp_merge",
+    "tqb_stage1_range",
+    "tqb_stage2_range",
+    "tqb_append",
+    "tqb_gather",
 )
 
 
@@ -171,6 +178,38 @@ class StoreArgs(ctypes.Structure):
     ]
 
 
+class RangeArgs(ctypes.Structure):
+    """``tqb_range``: which tokens of its sequence a query attends to."""
+
+    _fields_ = [("window", _i32), ("first_tokens", _i32), ("prefix_len", _i32), ("max_seq_len", _i32)]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("key", _vp), ("value", _vp), ("query", _vp), ("dtype", _i32),
+        ("k_stride_n", _i64), ("k_stride_h", _i64), ("v_stride_n", _i64), ("v_stride_h", _i64),
+        ("q_stride_n", _i64), ("q_stride_h", _i64),
+        ("positions", _vp), ("positions_are_64", _i32), ("cos_sin", _vp), ("cos_sin_stride", _i64),
+        ("max_pos", _i32), ("rotary_dim", _i32), ("interleaved", _i32),
+        ("rotation", _vp), ("midpoints", _vp), ("centroids", _vp), ("slot_mapping", _vp),
+        ("kv_cache", _vp), ("layout", _i32),
+        ("cache_stride_block", _i64), ("cache_stride_pos", _i64), ("cache_stride_head", _i64),
+        ("num_blocks", _i64), ("q_rot", _vp), ("q_rot_stride_n", _i64), ("q_rot_stride_h", _i64),
+        ("num_tokens", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("block_size", _i32), ("n_centroids", _i32), ("norm_correction", _i32),
+    ]
+
+
+class GatherArgs(ctypes.Structure):
+    _fields_ = [
+        ("kv_cache", _vp), ("layout", _i32),
+        ("cache_stride_block", _i64), ("cache_stride_pos", _i64), ("cache_stride_head", _i64),
+        ("num_blocks", _i64), ("slot_mapping", _vp), ("centroids", _vp), ("key", _vp), ("value", _vp),
+        ("out_dtype", _i32), ("k_stride_n", _i64), ("k_stride_h", _i64), ("v_stride_n", _i64), ("v_stride_h", _i64),
+        ("num_tokens", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("block_size", _i32), ("n_centroids", _i32),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -223,6 +262,14 @@ def load() -> ctypes.CDLL:
             lib.tqb_sp_merge.argtypes = [ctypes.POINTER(SpMergeArgs), _vp]
             for f in (lib.tqb_p2p_alloc, lib.tqb_p2p_free, lib.tqb_ipc_export, lib.tqb_ipc_import,
                       lib.tqb_ipc_close, lib.tqb_sp_exchange, lib.tqb_sp_merge):
+                f.restype = ctypes.c_int
+            lib.tqb_stage1_range.argtypes = [ctypes.POINTER(Stage1Args), ctypes.POINTER(RotateArgs),
+                                             ctypes.POINTER(RangeArgs), _vp]
+            lib.tqb_stage2_range.argtypes = [ctypes.POINTER(Stage2Args), ctypes.POINTER(RangeArgs), _i32, _vp, _i32,
+                                             _vp, _vp]
+            lib.tqb_append.argtypes = [ctypes.POINTER(AppendArgs), _vp]
+            lib.tqb_gather.argtypes = [ctypes.POINTER(GatherArgs), _vp]
+            for f in (lib.tqb_stage1_range, lib.tqb_stage2_range, lib.tqb_append, lib.tqb_gather):
                 f.restype = ctypes.c_int
             _lib = lib
     return _lib
