@@ -61,9 +61,27 @@ def _block_dense(kv_cache: torch.Tensor) -> bool:
     return True
 
 
-def _stage1_args(q_rot, kv_cache, block_table, seq_lens, centroids, mid_o, *, layout, num_splits_per_seq=None,
-                 pair_lut=None, attn_scale=None, query=None, rotation=None):
-    """Checked ``Stage1Args``, and the ``RotateArgs`` of ``query`` and ``rotation`` when they are given (or None)."""
+def stage1(q_rot: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
+           seq_lens: torch.Tensor, centroids: torch.Tensor, mid_o: torch.Tensor, *,
+           layout="soa", num_splits_per_seq: Optional[torch.Tensor] = None,
+           pair_lut: Optional[torch.Tensor] = None, attn_scale: Optional[float] = None,
+           sinks: Optional[torch.Tensor] = None, query: Optional[torch.Tensor] = None,
+           rotation: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
+    """Decode Stage1 into ``mid_o [B, Hq, S, D+1]`` (S = ``mid_o.shape[2]``).
+
+    With ``query`` and ``rotation`` given, ``q_rot`` is an output: Stage1
+    first computes ``q_rot = float(query) @ rotation`` (:func:`rotate_query`)
+    and decodes with it; ``tqb_stage1_rotated`` does both in one kernel where
+    the page ring serves the cache and the GQA group is at most 4.
+
+    ``kv_cache`` is the ``[num_blocks, 16, Hk, 134]`` uint8 cache (a view
+    with a non-unit block stride is accepted; SoA needs the inner three dims
+    contiguous).  ``num_splits_per_seq`` (int32 ``[B]``, each <= S) switches
+    from the uniform split count S to per-sequence counts.  ``sinks``
+    (float32 ``[Hq]`` logits) adds the reference's attention sinks
+    (``USE_SINKS``, reference/soa_decode_v1.py:134-145) to split 0, through
+    :func:`fold_sinks` on the same stream.
+    """
     lay = layout_id(layout)
     _cuda(q_rot, "q_rot", torch.float32)
     _cuda(kv_cache, "kv_cache", torch.uint8)
@@ -93,6 +111,10 @@ def _stage1_args(q_rot, kv_cache, block_table, seq_lens, centroids, mid_o, *, la
         _require(num_splits_per_seq.shape == (B,) and num_splits_per_seq.is_contiguous(),
                  "num_splits_per_seq must be a contiguous [B] tensor")
         nsp = num_splits_per_seq
+    if sinks is not None:
+        _cuda(sinks, "sinks", torch.float32)
+        _require(sinks.shape == (Hq,) and sinks.is_contiguous() and sinks.device == mid_o.device,
+                 "sinks must be a contiguous [Hq] float32 tensor on mid_o's device")
     r = None
     if query is not None or rotation is not None:
         _require(query is not None and rotation is not None, "query and rotation go together")
@@ -118,37 +140,6 @@ def _stage1_args(q_rot, kv_cache, block_table, seq_lens, centroids, mid_o, *, la
     a.batch, a.num_q_heads, a.num_kv_heads, a.head_dim = B, Hq, Hk, D
     a.block_size, a.num_splits = bs, mid_o.shape[2]
     a.attn_scale = float(attn_scale) if attn_scale is not None else 1.0 / math.sqrt(D)
-    return a, r
-
-
-def stage1(q_rot: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
-           seq_lens: torch.Tensor, centroids: torch.Tensor, mid_o: torch.Tensor, *,
-           layout="soa", num_splits_per_seq: Optional[torch.Tensor] = None,
-           pair_lut: Optional[torch.Tensor] = None, attn_scale: Optional[float] = None,
-           sinks: Optional[torch.Tensor] = None, query: Optional[torch.Tensor] = None,
-           rotation: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
-    """Decode Stage1 into ``mid_o [B, Hq, S, D+1]`` (S = ``mid_o.shape[2]``).
-
-    With ``query`` and ``rotation`` given, ``q_rot`` is an output: Stage1
-    first computes ``q_rot = float(query) @ rotation`` (:func:`rotate_query`)
-    and decodes with it; ``tqb_stage1_rotated`` does both in one kernel where
-    the page ring serves the cache and the GQA group is at most 4.
-
-    ``kv_cache`` is the ``[num_blocks, 16, Hk, 134]`` uint8 cache (a view
-    with a non-unit block stride is accepted; SoA needs the inner three dims
-    contiguous).  ``num_splits_per_seq`` (int32 ``[B]``, each <= S) switches
-    from the uniform split count S to per-sequence counts.  ``sinks``
-    (float32 ``[Hq]`` logits) adds the reference's attention sinks
-    (``USE_SINKS``, reference/soa_decode_v1.py:134-145) to split 0, through
-    :func:`fold_sinks` on the same stream.
-    """
-    a, r = _stage1_args(q_rot, kv_cache, block_table, seq_lens, centroids, mid_o, layout=layout,
-                        num_splits_per_seq=num_splits_per_seq, pair_lut=pair_lut, attn_scale=attn_scale, query=query,
-                        rotation=rotation)
-    if sinks is not None:
-        _cuda(sinks, "sinks", torch.float32)
-        _require(sinks.shape == (q_rot.shape[1],) and sinks.is_contiguous() and sinks.device == mid_o.device,
-                 "sinks must be a contiguous [Hq] float32 tensor on mid_o's device")
     with torch.cuda.device(mid_o.device):
         st = stream if stream is not None else _stream(mid_o.device)
         if r is None:
@@ -186,7 +177,13 @@ def fold_sinks(mid_o: torch.Tensor, seq_lens: torch.Tensor, sinks: torch.Tensor,
     return mid_o
 
 
-def _stage2_args(mid_o, seq_lens, output, lse, *, num_splits_per_seq=None) -> Stage2Args:
+def stage2(mid_o: torch.Tensor, seq_lens: torch.Tensor, output: torch.Tensor, lse: torch.Tensor, *,
+           num_splits_per_seq: Optional[torch.Tensor] = None, stream: Optional[int] = None):
+    """Merge the non-empty splits of ``mid_o`` into ``output [B, Hq, D]`` and
+    ``lse [B, Hq]``.  ``output`` may be float32, float16 or bfloat16: a
+    16-bit output receives the fp32 result rounded to nearest even (the
+    launcher's ``output.to(query.dtype)``, reference/soa_decode_v1.py:643,
+    without the extra pass)."""
     _cuda(mid_o, "mid_o", torch.float32)
     _cuda(seq_lens, "seq_lens", torch.int32)
     _require(isinstance(output, torch.Tensor) and output.is_cuda and output.dtype in _DTYPE_ID,
@@ -209,17 +206,6 @@ def _stage2_args(mid_o, seq_lens, output, lse, *, num_splits_per_seq=None) -> St
     a.lse = lse.data_ptr()
     a.lse_stride_b = lse.stride(0)
     a.batch, a.num_q_heads, a.head_dim, a.num_splits = B, Hq, D1 - 1, S
-    return a
-
-
-def stage2(mid_o: torch.Tensor, seq_lens: torch.Tensor, output: torch.Tensor, lse: torch.Tensor, *,
-           num_splits_per_seq: Optional[torch.Tensor] = None, stream: Optional[int] = None):
-    """Merge the non-empty splits of ``mid_o`` into ``output [B, Hq, D]`` and
-    ``lse [B, Hq]``.  ``output`` may be float32, float16 or bfloat16: a
-    16-bit output receives the fp32 result rounded to nearest even (the
-    launcher's ``output.to(query.dtype)``, reference/soa_decode_v1.py:643,
-    without the extra pass)."""
-    a = _stage2_args(mid_o, seq_lens, output, lse, num_splits_per_seq=num_splits_per_seq)
     with torch.cuda.device(mid_o.device):
         st = stream if stream is not None else _stream(mid_o.device)
         if output.dtype == torch.float32:

@@ -14,48 +14,114 @@ nothing: calls that may overlap need one each.  Errors raise ``TqbError``.
 
 from __future__ import annotations
 
+import ctypes
+import math
+import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
-from ._lib import AppendArgs, GatherArgs, RangeArgs
-from .layout import BLOCK_SIZE, FP8_KEY_LAYOUTS, HEAD_DIM, KEY3_LAYOUTS, SLOT_BYTES, layout_id
-from .ops import (_DTYPE_ID, _SOA_FAMILY, _block_dense, _cuda, _require, _stage1_args, _stage2_args, _stream)
+from ._lib import AppendArgs, GatherArgs, RangeArgs, RotateArgs, Stage1Args, Stage2Args, TqbError
+from .layout import (BLOCK_SIZE, FP8_KEY_LAYOUTS, HEAD_DIM, KEY3_LAYOUTS, LAYOUT_SOA, LAYOUT_SOA_K3, LAYOUT_SOA_K3V3,
+                     SLOT_BYTES, layout_id)
+from .ops import _DTYPE_ID, _SOA_FAMILY, _block_dense
 
+_F32, _U8, _I32, _I64 = torch.float32, torch.uint8, torch.int32, torch.int64
+_FOLDED = (LAYOUT_SOA, LAYOUT_SOA_K3, LAYOUT_SOA_K3V3)  # the stored norm may hold the norm correction
 _SPLIT_TOKENS = 64    # shortest split worth its partial rows (516 bytes written and read per query head)
 _SPLIT_ITEMS = 2368   # (sequence, KV head, split) items of one round of the Stage1 grid: 148 CTAs x 2 groups x 8 warps
 
 
-def _same_device(**tensors) -> torch.device:
-    devs = {t.device for t in tensors.values() if t is not None}
-    _require(len(devs) == 1, f"all tensors must be on one device, got {sorted(map(str, devs))}")
-    return devs.pop()
+# The step's calls are launches of a few microseconds, so their arguments are packed into the C structs' bytes at once
+# (a third of the time that setting the fields of a ctypes structure takes) and every check reads a property once.
+def packer(cls):
+    """``struct.Struct.pack`` of a flat C argument struct, in the native layout with its tail padding."""
+    code = {ctypes.c_void_p: "P", ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f"}
+    fields = [t for _, t in cls._fields_]
+    return struct.Struct("@" + "".join(code[t] for t in fields) + "0" + code[max(fields, key=ctypes.sizeof)])
 
 
-def _check_cache(kv_cache: torch.Tensor, lay: int) -> None:
-    _cuda(kv_cache, "kv_cache", torch.uint8)
-    _require(kv_cache.dim() == 4 and kv_cache.shape[1] == BLOCK_SIZE and kv_cache.stride(3) == 1,
-             "kv_cache must be [num_blocks, 16, Hk, slot] bytes")
-    _require(kv_cache.shape[3] >= SLOT_BYTES[lay], f"this layout has slots of {SLOT_BYTES[lay]} bytes, "
-             f"kv_cache has {kv_cache.shape[3]}")
-    if lay in _SOA_FAMILY:
-        _require(_block_dense(kv_cache), "SoA cache needs each block's bytes contiguous")
+_APPEND, _GATHER, _STAGE1, _STAGE2, _ROTATE, _RANGE = map(
+    packer, (AppendArgs, GatherArgs, Stage1Args, Stage2Args, RotateArgs, RangeArgs))
+_calls = {}
 
 
-def _check_centroids(centroids: Optional[torch.Tensor], lay: int) -> int:
-    n = 8 if lay in KEY3_LAYOUTS else 16
-    if lay not in FP8_KEY_LAYOUTS:
-        _cuda(centroids, "centroids", torch.float32)
-        _require(centroids.shape == (n,) and centroids.is_contiguous(), f"centroids must be a contiguous [{n}] tensor")
-    return n
+def _call(name: str, *args) -> None:
+    """A library call whose structs are given as bytes (None: NULL)."""
+    f = _calls.get(name)
+    if f is None:
+        f = _lib.load()[name]  # a function object of its own, apart from _lib's
+        f.argtypes = {"tqb_append": [ctypes.c_char_p, ctypes.c_void_p],
+                      "tqb_gather": [ctypes.c_char_p, ctypes.c_void_p],
+                      "tqb_stage1_range": [ctypes.c_char_p] * 3 + [ctypes.c_void_p],
+                      "tqb_stage2_range": [ctypes.c_char_p] * 2 + [ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+                                                                   ctypes.c_void_p, ctypes.c_void_p]}[name]
+        f.restype = ctypes.c_int
+        _calls[name] = f
+    status = f(*args)
+    if status:
+        _lib.check(status)
 
 
-def _rows(t: torch.Tensor, name: str, n: int) -> None:
-    _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPE_ID,
-             f"{name} must be a float32/float16/bfloat16 CUDA tensor")
-    _require(t.dim() == 3 and t.shape[0] == n and t.shape[2] == HEAD_DIM and (t.stride(2) == 1 or t.numel() == 0),
-             f"{name} must be [{n}, heads, 128] with unit stride over the last dim")
+def _no(msg: str):
+    raise TqbError(_lib.TQB_ERR_INVALID_ARG, msg)
+
+
+def _on(t, name: str, dtype, dev: int = -1) -> int:
+    """The CUDA device of tensor ``t`` of ``dtype``: device ``dev`` if that is given."""
+    if not isinstance(t, torch.Tensor):
+        _no(f"{name} must be a torch.Tensor")
+    d = t.get_device()
+    if d < 0:
+        _no(f"{name} must be a CUDA tensor")
+    if t.dtype is not dtype:
+        _no(f"{name} must be {dtype}, got {t.dtype}")
+    if dev >= 0 and d != dev:
+        _no(f"all tensors must be on one device: {name} is on cuda:{d}, others on cuda:{dev}")
+    return d
+
+
+def _vector(t, name: str, n: int, dtype, dev: int) -> int:
+    """Address of a contiguous [n] tensor."""
+    _on(t, name, dtype, dev)
+    if t.shape != (n,) or not t.is_contiguous():
+        _no(f"{name} must be a contiguous [{n}] tensor")
+    return t.data_ptr()
+
+
+def _float_rows(t, name: str, dev: int = -1):
+    """(device, dtype id, shape, strides) of a [N, heads, 128] tensor of float32, float16 or bfloat16."""
+    d = t.get_device() if isinstance(t, torch.Tensor) else -1
+    kind = _DTYPE_ID.get(t.dtype) if d >= 0 else None
+    if kind is None:
+        _no(f"{name} must be a float32/float16/bfloat16 CUDA tensor")
+    if dev >= 0 and d != dev:
+        _no(f"all tensors must be on one device: {name} is on cuda:{d}, others on cuda:{dev}")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM:
+        _no(f"{name} must be [N, heads, 128], got {tuple(shape)}")
+    stride = t.stride()
+    if stride[2] != 1 and shape[0] and shape[1]:
+        _no(f"{name} must have unit stride over the last dim")
+    return d, kind, shape, stride
+
+
+def _cache(kv_cache, lay: int, dev: int = -1):
+    """(device, shape, strides in bytes) of the paged cache."""
+    d = _on(kv_cache, "kv_cache", _U8, dev)
+    shape, stride = kv_cache.shape, kv_cache.stride()
+    if len(shape) != 4 or shape[1] != BLOCK_SIZE or shape[2] < 1 or stride[3] != 1:
+        _no("kv_cache must be [num_blocks, 16, Hk, slot] bytes")
+    if shape[3] < SLOT_BYTES[lay]:
+        _no(f"this layout has slots of {SLOT_BYTES[lay]} bytes, kv_cache has {shape[3]}")
+    if lay in _SOA_FAMILY and not (stride[1] == shape[2] * shape[3] and stride[2] == shape[3]) and not _block_dense(kv_cache):
+        _no("SoA cache needs each block's bytes contiguous")
+    return d, shape, stride
+
+
+def _stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def rope_append(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
@@ -80,61 +146,54 @@ def rope_append(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, 
     ``q_rot`` rows are NaN).  Slots must be distinct."""
     lay = layout_id(layout)
     k8 = lay in FP8_KEY_LAYOUTS
-    _check_cache(kv_cache, lay)
-    _cuda(slot_mapping, "slot_mapping", torch.int32)
-    _require(slot_mapping.dim() == 1 and slot_mapping.is_contiguous(), "slot_mapping must be a contiguous [N] tensor")
-    N, Hk = slot_mapping.shape[0], kv_cache.shape[2]
-    _rows(key, "key", N)
-    _rows(value, "value", N)
-    _require(key.shape[1] == Hk and value.shape[1] == Hk, f"key and value must have the cache's {Hk} heads")
-    _require(value.dtype == key.dtype, "key and value must have one dtype")
-    n = _check_centroids(centroids, lay)
+    dev, kind, kshape, ks = _float_rows(key, "key")
+    _, vkind, vshape, vs = _float_rows(value, "value", dev)
+    _, cshape, cs = _cache(kv_cache, lay, dev)
+    N, Hk, _ = kshape
+    if vshape != kshape or Hk != cshape[2] or vkind != kind:
+        _no(f"key and value must be [N, {cshape[2]}, 128] tensors of one shape and dtype")
+    slots = _vector(slot_mapping, "slot_mapping", N, _I32, dev)
+    n = 8 if lay in KEY3_LAYOUTS else 16
+    rot = mids = cents = 0
     if not k8:
-        _cuda(midpoints, "midpoints", torch.float32)
-        _require(midpoints.shape == (n - 1,) and midpoints.is_contiguous(),
-                 f"midpoints must be a contiguous [{n - 1}] tensor")
-        _cuda(rotation, "rotation", torch.float32)
-        _require(tuple(rotation.shape) == (HEAD_DIM, HEAD_DIM) and rotation.is_contiguous(),
-                 "rotation must be a contiguous [128, 128] matrix")
-    a = AppendArgs()
+        cents = _vector(centroids, "centroids", n, _F32, dev)
+        mids = _vector(midpoints, "midpoints", n - 1, _F32, dev)
+        _on(rotation, "rotation", _F32, dev)
+        if rotation.shape != (HEAD_DIM, HEAD_DIM) or not rotation.is_contiguous():
+            _no("rotation must be a contiguous [128, 128] matrix")
+        rot = rotation.data_ptr()
+    pos = pos64 = table = table_stride = max_pos = rotary = 0
     if positions is not None:
-        _require(isinstance(positions, torch.Tensor) and positions.is_cuda and
-                 positions.dtype in (torch.int32, torch.int64), "positions must be an int32 or int64 CUDA tensor")
-        _require(positions.shape == (N,) and positions.is_contiguous(), "positions must be a contiguous [N] tensor")
-        _cuda(cos_sin, "cos_sin", torch.float32)
-        _require(cos_sin.dim() == 2 and cos_sin.stride(1) == 1, "cos_sin must be [max_pos, rotary_dim] row-major")
-        a.positions, a.positions_are_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-        a.cos_sin, a.cos_sin_stride = cos_sin.data_ptr(), max(cos_sin.stride(0), cos_sin.shape[1])
-        a.max_pos, a.rotary_dim = cos_sin.shape
-        _require(cos_sin.shape[0] <= 1 or cos_sin.stride(0) >= cos_sin.shape[1], "cos_sin rows must not overlap")
-    a.interleaved = int(bool(interleaved))
+        pos64 = isinstance(positions, torch.Tensor) and positions.dtype is _I64
+        pos = _vector(positions, "positions", N, _I64 if pos64 else _I32, dev)
+        _on(cos_sin, "cos_sin", _F32, dev)
+        if cos_sin.dim() != 2 or cos_sin.stride(1) != 1:
+            _no("cos_sin must be [max_pos, rotary_dim] row-major")
+        (max_pos, rotary), table_stride, table = cos_sin.shape, cos_sin.stride(0), cos_sin.data_ptr()
+        if max_pos == 1:
+            table_stride = rotary
+    q = out = Hq = 0
+    qs = os = (0, 0, 1)
     if query is not None:
-        _rows(query, "query", N)
-        _require(query.dtype == key.dtype, "query must have the key's dtype")
+        _, qkind, qshape, qs = _float_rows(query, "query", dev)
+        if qshape[0] != N or qkind != kind:
+            _no(f"query must be [{N}, Hq, 128] in the key's dtype")
         if q_rot is None:
-            q_rot = torch.empty(query.shape, dtype=torch.float32, device=query.device)
-        _cuda(q_rot, "q_rot", torch.float32)
-        _require(q_rot.shape == query.shape and q_rot.stride(2) == 1, "q_rot must have the query's shape")
-        a.query, a.q_stride_n, a.q_stride_h = query.data_ptr(), query.stride(0), query.stride(1)
-        a.q_rot, a.q_rot_stride_n, a.q_rot_stride_h = q_rot.data_ptr(), q_rot.stride(0), q_rot.stride(1)
-        a.num_q_heads = query.shape[1]
-    else:
-        _require(q_rot is None, "q_rot is the output of query")
-    dev = _same_device(key=key, value=value, kv_cache=kv_cache, slot_mapping=slot_mapping, positions=positions,
-                       cos_sin=cos_sin, rotation=rotation, midpoints=midpoints, centroids=centroids, query=query,
-                       q_rot=q_rot)
-    a.key, a.value, a.dtype = key.data_ptr(), value.data_ptr(), _DTYPE_ID[key.dtype]
-    a.k_stride_n, a.k_stride_h = key.stride(0), key.stride(1)
-    a.v_stride_n, a.v_stride_h = value.stride(0), value.stride(1)
-    if not k8:
-        a.rotation, a.midpoints, a.centroids = rotation.data_ptr(), midpoints.data_ptr(), centroids.data_ptr()
-    a.slot_mapping, a.kv_cache, a.layout = slot_mapping.data_ptr(), kv_cache.data_ptr(), lay
-    a.cache_stride_block, a.cache_stride_pos, a.cache_stride_head = kv_cache.stride()[:3]
-    a.num_blocks, a.block_size = kv_cache.shape[0], kv_cache.shape[1]
-    a.num_tokens, a.num_kv_heads, a.head_dim, a.n_centroids = N, Hk, HEAD_DIM, n
-    a.norm_correction = int(bool(norm_correction) and lay in _SOA_FAMILY and not k8)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().tqb_append(a, stream if stream is not None else _stream(dev)))
+            q_rot = torch.empty(qshape, dtype=_F32, device=query.device)
+            os = (qshape[1] * HEAD_DIM, HEAD_DIM)
+        else:
+            _on(q_rot, "q_rot", _F32, dev)
+            os = q_rot.stride()
+            if q_rot.shape != qshape or os[2] != 1:
+                _no("q_rot must have the query's shape and unit stride over the last dim")
+        q, out, Hq = query.data_ptr(), q_rot.data_ptr(), qshape[1]
+    elif q_rot is not None:
+        _no("q_rot is the output of query")
+    _call("tqb_append", _APPEND.pack(
+        key.data_ptr(), value.data_ptr(), q, kind, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], pos, bool(pos64), table,
+        table_stride, max_pos, rotary, bool(interleaved), rot, mids, cents, slots, kv_cache.data_ptr(), lay, cs[0], cs[1],
+        cs[2], cshape[0], out, os[0], os[1], N, Hq, Hk, HEAD_DIM, BLOCK_SIZE, n, bool(norm_correction) and lay in _FOLDED),
+        _stream(dev) if stream is None else stream)
     return q_rot
 
 
@@ -146,32 +205,28 @@ def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, centroids: Opt
     (reference/soa_decode_v1.py:322-454).  Lloyd-Max keys stay in the rotated basis, where the chunk's queries are taken
     too (:func:`rotate_query`).  Rows of negative or out-of-range slots are zeros."""
     lay = layout_id(layout)
-    _check_cache(kv_cache, lay)
-    _cuda(slot_mapping, "slot_mapping", torch.int32)
-    _require(slot_mapping.dim() == 1 and slot_mapping.is_contiguous(), "slot_mapping must be a contiguous [N] tensor")
-    n = _check_centroids(centroids, lay)
-    N, Hk = slot_mapping.shape[0], kv_cache.shape[2]
-    _require((key is None) == (value is None), "key and value go together")
-    if key is None:
-        _require(dtype in _DTYPE_ID, "dtype must be float32, float16 or bfloat16")
-        key, value = (torch.empty(N, Hk, HEAD_DIM, dtype=dtype, device=kv_cache.device) for _ in range(2))
-    _rows(key, "key", N)
-    _rows(value, "value", N)
-    _require(key.shape[1] == Hk and value.shape[1] == Hk and key.dtype == value.dtype,
-             f"key and value must be [{N}, {Hk}, 128] tensors of one dtype")
-    dev = _same_device(kv_cache=kv_cache, slot_mapping=slot_mapping, centroids=centroids, key=key, value=value)
-    a = GatherArgs()
-    a.kv_cache, a.layout = kv_cache.data_ptr(), lay
-    a.cache_stride_block, a.cache_stride_pos, a.cache_stride_head = kv_cache.stride()[:3]
-    a.num_blocks, a.block_size = kv_cache.shape[0], kv_cache.shape[1]
-    a.slot_mapping = slot_mapping.data_ptr()
-    a.centroids = centroids.data_ptr() if lay not in FP8_KEY_LAYOUTS else None
-    a.key, a.value, a.out_dtype = key.data_ptr(), value.data_ptr(), _DTYPE_ID[key.dtype]
-    a.k_stride_n, a.k_stride_h = key.stride(0), key.stride(1)
-    a.v_stride_n, a.v_stride_h = value.stride(0), value.stride(1)
-    a.num_tokens, a.num_kv_heads, a.head_dim, a.n_centroids = N, Hk, HEAD_DIM, n
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().tqb_gather(a, stream if stream is not None else _stream(dev)))
+    dev, cshape, cs = _cache(kv_cache, lay)
+    if not isinstance(slot_mapping, torch.Tensor):
+        _no("slot_mapping must be a torch.Tensor")
+    N, Hk = slot_mapping.numel(), cshape[2]
+    slots = _vector(slot_mapping, "slot_mapping", N, _I32, dev)
+    n = 8 if lay in KEY3_LAYOUTS else 16
+    cents = 0 if lay in FP8_KEY_LAYOUTS else _vector(centroids, "centroids", n, _F32, dev)
+    if key is None and value is None:
+        kind = _DTYPE_ID.get(dtype)
+        if kind is None:
+            _no("dtype must be float32, float16 or bfloat16")
+        key = torch.empty((N, Hk, HEAD_DIM), dtype=dtype, device=kv_cache.device)
+        value = torch.empty((N, Hk, HEAD_DIM), dtype=dtype, device=kv_cache.device)
+        ks = vs = (Hk * HEAD_DIM, HEAD_DIM)
+    else:
+        _, kind, kshape, ks = _float_rows(key, "key", dev)
+        _, vkind, vshape, vs = _float_rows(value, "value", dev)
+        if kshape != (N, Hk, HEAD_DIM) or vshape != kshape or kind != vkind:
+            _no(f"key and value must be [{N}, {Hk}, 128] tensors of one dtype")
+    _call("tqb_gather", _GATHER.pack(
+        kv_cache.data_ptr(), lay, cs[0], cs[1], cs[2], cshape[0], slots, cents, key.data_ptr(), value.data_ptr(), kind,
+        ks[0], ks[1], vs[0], vs[1], N, Hk, HEAD_DIM, BLOCK_SIZE, n), _stream(dev) if stream is None else stream)
     return key, value
 
 
@@ -181,42 +236,107 @@ def _splits(items: int, tokens: int) -> int:
     return max(1, min(-(-_SPLIT_ITEMS // max(items, 1)), -(-tokens // _SPLIT_TOKENS)))
 
 
-def _decode_args(query, kv_cache, block_table, seq_lens, rotation, centroids, lay, sinks, output, lse, out_dtype, mid_o):
-    """What both decode calls check and allocate: the rows that Stage1 reads, the raw query when it rotates them, and
-    the outputs."""
-    _require(isinstance(query, torch.Tensor) and query.is_cuda and query.dim() == 3 and query.shape[2] == HEAD_DIM and
-             query.dtype in _DTYPE_ID, "query must be a [B, Hq, 128] float32/float16/bfloat16 CUDA tensor")
-    _check_cache(kv_cache, lay)
-    _require(rotation is None or lay not in FP8_KEY_LAYOUTS, "FP8 keys are not rotated: rotation must be None")
-    _require(isinstance(block_table, torch.Tensor) and block_table.dim() == 2 and block_table.shape[1] > 0,
-             "block_table must be [B, max_blocks]")
-    B, Hq, D = query.shape
-    _require(Hq > 0 and Hq % kv_cache.shape[2] == 0, "query heads must be a multiple of the cache's")
-    raw = None
-    if rotation is not None:
-        raw = query if query.stride(2) == 1 else query.contiguous()
-        rows = torch.empty(B, Hq, D, dtype=torch.float32, device=query.device)
-    else:
-        rows = query.float().contiguous()
-    if output is None:
-        output = torch.empty(B, Hq, D, dtype=out_dtype or query.dtype, device=query.device)
-    if lse is None:
-        lse = torch.empty(B, Hq, dtype=torch.float32, device=query.device)
-    if sinks is not None:
-        _cuda(sinks, "sinks", torch.float32)
-        _require(sinks.shape == (Hq,) and sinks.is_contiguous(), "sinks must be a contiguous [Hq] tensor")
-    _same_device(query=query, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, rotation=rotation,
-                 centroids=centroids, sinks=sinks, output=output, lse=lse, mid_o=mid_o)
-    return rows, raw, output, lse
+class _Step:
+    """One decode call: its checked arguments, its workspace (rotated queries, split partials, LSE where the caller gives
+    none, in one allocation) and its outputs."""
 
+    def __init__(self, query, kv_cache, block_table, seq_lens, rotation, centroids, layout, scale, sinks, output, out_dtype,
+                 lse, mid_o):
+        self.lay = lay = layout_id(layout)
+        dev, self.kind, (self.B, self.Hq, _), self.qs = _float_rows(query, "query")
+        self.dev, self.query = dev, query
+        _, self.cshape, self.cs = _cache(kv_cache, lay, dev)
+        self.cache, self.Hk = kv_cache.data_ptr(), self.cshape[2]
+        if self.Hq < 1 or self.Hq % self.Hk:
+            _no(f"query heads must be a multiple of the cache's {self.Hk}")
+        self.seq_lens = _vector(seq_lens, "seq_lens", self.B, _I32, dev)
+        _on(block_table, "block_table", _I32, dev)
+        tshape, tstride = block_table.shape, block_table.stride()
+        if len(tshape) != 2 or tshape[0] != self.B or tshape[1] < 1 or tstride[1] != 1:
+            _no(f"block_table must be [{self.B}, max_blocks] row-major")
+        self.table, self.blocks = block_table.data_ptr(), tshape[1]
+        self.table_stride = tstride[0] if self.B > 1 else max(tstride[0], tshape[1])
+        self.n = 8 if lay in KEY3_LAYOUTS else 16
+        self.cents = 0 if lay in FP8_KEY_LAYOUTS else _vector(centroids, "centroids", self.n, _F32, dev)
+        self.rot = 0
+        if rotation is not None:
+            if lay in FP8_KEY_LAYOUTS:
+                _no("FP8 keys are not rotated: rotation must be None")
+            _on(rotation, "rotation", _F32, dev)
+            if rotation.shape != (HEAD_DIM, HEAD_DIM) or not rotation.is_contiguous():
+                _no("rotation must be a contiguous [128, 128] matrix")
+            self.rot = rotation.data_ptr()
+        self.sinks = None if sinks is None else _vector(sinks, "sinks", self.Hq, _F32, dev)
+        self.scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+        if not self.scale > 0:
+            _no("scale must be positive")
+        if output is None:
+            output = torch.empty((self.B, self.Hq, HEAD_DIM), dtype=out_dtype or query.dtype, device=query.device)
+            self.os = (self.Hq * HEAD_DIM, HEAD_DIM)
+            self.out_kind = _DTYPE_ID.get(output.dtype)
+            if self.out_kind is None:
+                _no("out_dtype must be float32, float16 or bfloat16")
+        else:
+            _, self.out_kind, oshape, self.os = _float_rows(output, "output", dev)
+            if oshape != query.shape:
+                _no("output must have the query's shape")
+        self.output = output
+        self.lse, self.lse_stride = 0, self.Hq
+        if lse is not None:
+            _on(lse, "lse", _F32, dev)
+            if lse.shape != (self.B, self.Hq) or lse.stride(1) != 1:
+                _no(f"lse must be [{self.B}, {self.Hq}] with unit stride over the heads")
+            self.lse, self.lse_stride = lse.data_ptr(), lse.stride(0)
+        self.mid_o = mid_o
+        if mid_o is not None:
+            _on(mid_o, "mid_o", _F32, dev)
 
-def _partials(mid_o, B, Hq, S, device) -> torch.Tensor:
-    if mid_o is None:
-        return torch.empty(B, Hq, S, HEAD_DIM + 1, dtype=torch.float32, device=device)
-    _cuda(mid_o, "mid_o", torch.float32)
-    _require(mid_o.dim() == 4 and mid_o.shape[0] >= B and mid_o.shape[1] >= Hq and mid_o.shape[2] >= S and
-             mid_o.shape[3] == HEAD_DIM + 1, f"mid_o must hold [{B}, {Hq}, {S}, 129] partials")
-    return mid_o[:B, :Hq, :S]
+    def workspace(self, S: int) -> None:
+        """Room for S splits; the query rows that Stage1 reads."""
+        rows = self.B * self.Hq
+        need = 0 if self.mid_o is not None else rows * S * (HEAD_DIM + 1)
+        lse_at, need = need, need + (0 if self.lse else rows)
+        q_at = need = (need + 31) // 32 * 32
+        # queries that need no rotation are read as they are where Stage1 can (fp32, 16-byte aligned rows)
+        q, qs = self.query, self.qs
+        direct = not self.rot and q.dtype is _F32 and not (q.data_ptr() | qs[0] * 4 | qs[1] * 4) & 15 and qs[0] >= 0 <= qs[1]
+        if not direct and self.rot:
+            need += rows * HEAD_DIM
+        self.keep = ws = torch.empty(max(need, 1), dtype=_F32, device=q.device)
+        base = ws.data_ptr()
+        if self.mid_o is None:
+            self.mid, self.ms = base, (self.Hq * S * (HEAD_DIM + 1), S * (HEAD_DIM + 1), HEAD_DIM + 1)
+        else:
+            m = self.mid_o
+            if m.dim() != 4 or m.shape[0] < self.B or m.shape[1] < self.Hq or m.shape[2] < S or \
+                    m.shape[3] != HEAD_DIM + 1 or m.stride(3) != 1:
+                _no(f"mid_o must hold [{self.B}, {self.Hq}, {S}, 129] partials with unit inner stride")
+            self.mid, self.ms = m.data_ptr(), m.stride()
+        if not self.lse:
+            self.lse = base + 4 * lse_at
+        if direct:
+            self.rows, self.rs = q.data_ptr(), qs
+        elif self.rot:
+            self.rows, self.rs = base + 4 * q_at, (self.Hq * HEAD_DIM, HEAD_DIM)
+        else:
+            self.query = q = q.to(_F32).contiguous()
+            self.rows, self.rs = q.data_ptr(), q.stride()
+
+    def launch(self, rng: bytes, lead: int, S: int, stream) -> torch.Tensor:
+        """Stage1 of the range into the splits from ``lead`` on, and the merge of all S."""
+        st = _stream(self.dev) if stream is None else stream
+        ms, rs, cs = self.ms, self.rs, self.cs
+        _call("tqb_stage1_range", _STAGE1.pack(
+            self.rows, rs[0], rs[1], self.cache, self.lay, cs[0], cs[1], cs[2], self.cshape[0], self.table,
+            self.table_stride, self.blocks, self.seq_lens, self.cents, self.n, 0, 0, self.mid + 4 * ms[2] * lead, ms[0],
+            ms[1], ms[2], self.B, self.Hq, self.Hk, HEAD_DIM, BLOCK_SIZE, S - lead, self.scale),
+            None if not self.rot else _ROTATE.pack(self.query.data_ptr(), self.kind, self.qs[0], self.qs[1], self.rot,
+                                                   self.rows, rs[0], rs[1], self.B, self.Hq, HEAD_DIM), rng, st)
+        out = self.output.data_ptr()
+        _call("tqb_stage2_range", _STAGE2.pack(
+            self.mid, ms[0], ms[1], ms[2], self.seq_lens, 0, out, self.os[0], self.os[1], self.lse, self.lse_stride,
+            self.B, self.Hq, HEAD_DIM, S), rng, lead, self.sinks, self.out_kind, out, st)
+        return self.output
 
 
 def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -239,38 +359,21 @@ def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     ``mid_o`` may hold the partials: float32 ``[>= B, >= Hq, >= splits, 129]``, with one split more than ``num_splits``
     when ``first_tokens > 0``.  Calls with a ``rotation`` must not overlap in time on one device (``tqb_stage1_rotated``'s
     rule); with ``rotation=None`` they may."""
-    lay = layout_id(layout)
-    _require(isinstance(window, int) and window >= 1, "window must be at least 1")
-    _require(isinstance(first_tokens, int) and first_tokens >= 0, "first_tokens must not be negative")
-    _require(num_splits is None or num_splits >= 1, "num_splits must be positive")
-    rows, raw, output, lse = _decode_args(query, kv_cache, block_table, seq_lens, rotation, centroids, lay, sinks, output,
-                                          lse, out_dtype, mid_o)
-    B, Hq, _ = query.shape
-    if B == 0:
-        return output
-    most = block_table.shape[1] * BLOCK_SIZE
+    if not isinstance(window, int) or window < 1:
+        _no("window must be at least 1")
+    if not isinstance(first_tokens, int) or first_tokens < 0:
+        _no("first_tokens must not be negative")
+    if num_splits is not None and num_splits < 1:
+        _no("num_splits must be positive")
+    s = _Step(query, kv_cache, block_table, seq_lens, rotation, centroids, layout, scale, sinks, output, out_dtype, lse,
+              mid_o)
+    if s.B == 0:
+        return s.output
+    most = s.blocks * BLOCK_SIZE
     window, first_tokens = min(window, most), min(first_tokens, most)
-    S = (num_splits or _splits(B * kv_cache.shape[2], window)) + (1 if first_tokens else 0)
-    mid = _partials(mid_o, B, Hq, S, query.device)
-    rng = RangeArgs(window, first_tokens, 0, most)
-    _ranged(rows, raw, kv_cache, block_table, seq_lens, rotation, centroids, mid, mid, rng, 0, scale, lay, sinks, output,
-            lse, stream)
-    return output
-
-
-def _ranged(rows, raw, kv_cache, block_table, seq_lens, rotation, centroids, mid, mid_stage1, rng, lead, scale, lay, sinks,
-            output, lse, stream):
-    """Stage1 of ``rng`` into ``mid_stage1`` (the splits of ``mid`` from ``lead`` on) and the merge of all of ``mid``."""
-    _require(seq_lens.dim() == 1 and seq_lens.shape[0] == rows.shape[0], "seq_lens must be a contiguous [B] tensor")
-    a, r = _stage1_args(rows, kv_cache, block_table, seq_lens, centroids, mid_stage1, layout=lay, attn_scale=scale,
-                        query=raw, rotation=rotation)
-    b = _stage2_args(mid, seq_lens, output, lse)
-    lib = _lib.load()
-    with torch.cuda.device(output.device):
-        st = stream if stream is not None else _stream(output.device)
-        _lib.check(lib.tqb_stage1_range(a, r, rng, st))
-        _lib.check(lib.tqb_stage2_range(b, rng, lead, sinks.data_ptr() if sinks is not None else None,
-                                        _DTYPE_ID[output.dtype], output.data_ptr(), st))
+    S = (num_splits or _splits(s.B * s.Hk, window)) + (1 if first_tokens else 0)
+    s.workspace(S)
+    return s.launch(_RANGE.pack(window, first_tokens, 0, most), 0, S, stream)
 
 
 def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -283,20 +386,17 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     multiple of 16: the first ``prefix_len / 16`` entries of every row of ``block_table`` are the same pages.
     ``seq_lens`` and ``block_table`` describe whole sequences, prefix included; a sequence shorter than the prefix sees
     its own tokens only.  The other arguments are :func:`window_attention`'s."""
-    lay = layout_id(layout)
-    _require(isinstance(prefix_len, int) and prefix_len >= 0 and prefix_len % BLOCK_SIZE == 0,
-             "prefix_len must be a multiple of 16")
-    _require(num_splits is None or num_splits >= 1, "num_splits must be positive")
-    rows, raw, output, lse = _decode_args(query, kv_cache, block_table, seq_lens, rotation, centroids, lay, sinks, output,
-                                          lse, out_dtype, mid_o)
-    B, Hq, _ = query.shape
-    _require(prefix_len <= block_table.shape[1] * BLOCK_SIZE, "the block table's rows do not hold the prefix")
-    if B == 0:
-        return output
-    most = block_table.shape[1] * BLOCK_SIZE
-    S = num_splits or _splits(B * kv_cache.shape[2], most)
-    mid = _partials(mid_o, B, Hq, S, query.device)
-    rng = RangeArgs(0, 0, 0, most)
-    _ranged(rows, raw, kv_cache, block_table, seq_lens, rotation, centroids, mid, mid, rng, 0, scale, lay, sinks, output,
-            lse, stream)
-    return output
+    if not isinstance(prefix_len, int) or prefix_len < 0 or prefix_len % BLOCK_SIZE:
+        _no("prefix_len must be a multiple of 16")
+    if num_splits is not None and num_splits < 1:
+        _no("num_splits must be positive")
+    s = _Step(query, kv_cache, block_table, seq_lens, rotation, centroids, layout, scale, sinks, output, out_dtype, lse,
+              mid_o)
+    most = s.blocks * BLOCK_SIZE
+    if prefix_len > most:
+        _no("the block table's rows do not hold the prefix")
+    if s.B == 0:
+        return s.output
+    S = num_splits or _splits(s.B * s.Hk, most)
+    s.workspace(S)
+    return s.launch(_RANGE.pack(0, 0, 0, most), 0, S, stream)
