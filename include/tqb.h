@@ -316,6 +316,22 @@ int tqb_stage2_range(const tqb_stage2_args* args, const tqb_range* range, int32_
                      int out_dtype, void* output, cudaStream_t stream);
 
 /*
+ * Shared prefix: partials of the tokens [0, prefix_len), whose pages are the
+ * first row of block_table and the same for the whole batch, for every
+ * query: mid_o[b, h, s] for s < num_splits, always written (O 0 and LSE -inf
+ * where sequence b, of seq_lens[b] tokens, sees none of them).  args are
+ * tqb_stage1's; prefix_len is a positive multiple of 16.  Each page is
+ * dequantised once for up to 256 queries of a KV head, and the products run
+ * on the tensor cores with fp16 operands and fp32 accumulators: the partials
+ * are good for 16-bit outputs (about 3e-4 relative), not for fp32 ones.
+ * num_splits is at most ceil(prefix_len / 128); with batch * (Hq / Hk) <= 128
+ * an even num_splits may be twice that.  tqb_stage1_range with the same
+ * prefix_len adds each sequence's own tokens as further splits, and
+ * tqb_stage2_range with lead = num_splits merges both.
+ */
+int tqb_prefix(const tqb_stage1_args* args, int32_t prefix_len, cudaStream_t stream);
+
+/*
  * Append (reference/soa_store.py:381-524 with its host part, after the model's
  * own rotary step): new tokens from the projections' raw keys and values into
  * their slots.  Per token n and KV head, x = rope(key, positions[n]):

@@ -130,13 +130,13 @@ def append(cache, layout, key, value, slots, positions, cos_sin, R, mids, cents,
 
 
 def attention(q, cache, layout, table, lens, cents, visible, *, scale=None, sinks=None):
-    """(output [B, Hq, 128], lse [B, Hq]) in float64; visible(t, L) says which tokens t < L each query sees.  q is in the
-    cache's basis.  A row with nothing to see: NaN and -inf."""
+    """(output [B, Hq, 128], lse [B, Hq], mean |v| under the weights [B, Hq, 128]) in float64; visible(t, L) says which
+    tokens t < L each query sees.  q is in the cache's basis.  A row with nothing to see: NaN and -inf."""
     B, Hq, _ = q.shape
     hk = cache.shape[2]
     g = Hq // hk
     scale = 1 / np.sqrt(D) if scale is None else scale
-    out, lse = np.full((B, Hq, D), np.nan), np.full((B, Hq), -np.inf)
+    out, lse, size = np.full((B, Hq, D), np.nan), np.full((B, Hq), -np.inf), np.zeros((B, Hq, D))
     for b in range(B):
         L = min(int(lens[b]), table.shape[1] * BLOCK)
         t = np.arange(max(L, 0))
@@ -155,5 +155,6 @@ def attention(q, cache, layout, table, lens, cents, visible, *, scale=None, sink
             top = s.max()
             w = np.exp(s - top)
             out[b, h] = w @ vv / w.sum()
+            size[b, h] = w @ np.abs(vv) / w.sum()
             lse[b, h] = top + np.log(w.sum())
-    return out, lse
+    return out, lse, size

@@ -3,7 +3,13 @@
 Bars, derived before the first run.  Bytes of an append: equal (the codes are those of exact arithmetic, the values'
 steps are the store's).  Rotated queries: 128 fp32 products, each partial sum off by at most 2^-24 of |x| (Cauchy-Schwarz
 on a unit column), 2^-17 |x| in all.  Gather: the output type's half step, and 2^-20 for the fp32 product (AoS: the fp32
-length of the centroids).  Decode: the repository's 1e-4 + 2e-3 |ref|, and the output type's half step."""
+length of the centroids).  Decode: the repository's 1e-4 + 2e-3 |ref|, and the output type's half step.
+
+The shared pass over a prefix (16-bit outputs) rounds its operands to fp16, 2^-11 at most each, so its errors go by the
+mean A = sum p |v| of what is summed and not by |ref|, which may cancel.  V and P: 2 * 2^-11 A.  Scores: q_i k_i carries
+three roundings (q, c, c norm) of rms at most 2^-11 / sqrt(3), 2^-11 together; over 128 products that is sigma = 2^-11
+scale sqrt(sum q_i^2 k_i^2) = 2^-11 * 1.5 = 7.3e-4 for the rows here (|q| = 1.5 sqrt(128), |k| = sqrt(128)), and a score's
+error moves the output by at most that times A; 4 sigma A = 3e-3 A.  Together 4e-3 A in place of 2e-3 |ref|."""
 
 from __future__ import annotations
 
@@ -211,11 +217,13 @@ def batch(rng, lens, hk, layout, shared=0):
     return random_cache(rng, nb, hk, layout), table, np.asarray(lens, np.int32)
 
 
-def check_decode(got, lse, ref, ref_lse, dtype):
+def check_decode(got, lse, ref, ref_lse, dtype, size=None):
+    """``size``: the mean |v| that the shared pass's bar goes by."""
     got, lse = got.double().cpu().numpy(), lse.double().cpu().numpy()
     dead = np.isnan(ref)
     assert np.array_equal(np.isnan(got), dead)
-    assert (np.abs(got - ref)[~dead] <= 1e-4 + (2e-3 + half_step(dtype)) * np.abs(ref[~dead])).all()
+    bar = 1e-4 + half_step(dtype) * np.abs(ref) + (2e-3 * np.abs(ref) if size is None else 4e-3 * size)
+    assert (np.abs(got - ref)[~dead] <= bar[~dead]).all()
     assert np.array_equal(np.isneginf(lse), np.isneginf(ref_lse))
     live = np.isfinite(ref_lse)
     assert (np.abs(lse - ref_lse)[live] <= 1e-4 + 2e-3 * np.abs(ref_lse[live])).all()
@@ -234,7 +242,7 @@ def run_window(layout, dtype, lens, hq, hk, window, first, *, seed=0, sinks=Fals
                                first_tokens=first, layout=layout, sinks=s, lse=lse, **kw)
     x = npy(q).astype(np.float64)
     x = x @ npy(R).astype(np.float64) if raw else x
-    ref, ref_lse = SO.attention(x, cache, layout, table, lens, npy(c), lambda t, L: (t < first) | (t >= L - window),
+    ref, ref_lse, _ = SO.attention(x, cache, layout, table, lens, npy(c), lambda t, L: (t < first) | (t >= L - window),
                                 scale=kw.get("scale"), sinks=npy(s))
     assert got.dtype == kw.get("out_dtype", dtype)
     check_decode(got, lse, ref, ref_lse, got.dtype)
@@ -304,9 +312,9 @@ def run_prefix(layout, dtype, own, prefix, hq, hk, *, seed=0, sinks=False, raw=T
                                layout=layout, sinks=s, lse=lse, **kw)
     x = npy(q).astype(np.float64)
     x = x @ npy(R).astype(np.float64) if raw else x
-    ref, ref_lse = SO.attention(x, cache, layout, table, lens, npy(c), lambda t, L: t >= 0, scale=kw.get("scale"),
-                                sinks=npy(s))
-    check_decode(got, lse, ref, ref_lse, got.dtype)
+    ref, ref_lse, size = SO.attention(x, cache, layout, table, lens, npy(c), lambda t, L: t >= 0, scale=kw.get("scale"),
+                                      sinks=npy(s))
+    check_decode(got, lse, ref, ref_lse, got.dtype, size if got.dtype != torch.float32 and prefix >= 128 else None)
 
 
 @pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))

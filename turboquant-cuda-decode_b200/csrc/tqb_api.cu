@@ -91,10 +91,11 @@ int tqb_version(void) { return TQB_VERSION; }
 int tqb_wait_timeouts(unsigned int* count, int reset) {
     g_detail[0] = '\0';
     TQB_REQUIRE(count != nullptr, TQB_ERR_INVALID_ARG, "count is NULL");
-    unsigned int ring = 0, p2p = 0;
+    unsigned int ring = 0, p2p = 0, prefix = 0;
     if (tqb::read_wait_timeouts(&ring, reset != 0) != TQB_OK) return TQB_ERR_CUDA;
     if (tqb::read_p2p_timeouts(&p2p, reset != 0) != TQB_OK) return TQB_ERR_CUDA;
-    *count = ring + p2p;
+    if (tqb::read_prefix_timeouts(&prefix, reset != 0) != TQB_OK) return TQB_ERR_CUDA;
+    *count = ring + p2p + prefix;
     return TQB_OK;
 }
 
@@ -678,6 +679,52 @@ int tqb_stage2_range(const tqb_stage2_args* a, const tqb_range* range, int32_t l
     DeviceGuard guard(out);
     TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning output");
     return tqb::launch_stage2_range(p, stream);
+}
+
+int tqb_prefix(const tqb_stage1_args* a, int32_t prefix_len, cudaStream_t stream) {
+    g_detail[0] = '\0';
+    tqb::Stage1Params s{};
+    const int rc = stage1_check(a, s);
+    if (rc != TQB_OK) return rc;
+    TQB_REQUIRE(prefix_len > 0 && prefix_len % tqb::kBlockSize == 0, TQB_ERR_INVALID_ARG,
+                "prefix_len must be a positive multiple of 16");
+    TQB_REQUIRE(a->num_splits_per_seq == nullptr, TQB_ERR_INVALID_ARG, "a shared prefix has one split count");
+    if (a->batch == 0) return TQB_OK;
+    TQB_REQUIRE(prefix_len <= (int64_t)a->max_blocks_per_seq * tqb::kBlockSize, TQB_ERR_INVALID_ARG,
+                "the block table's first row does not hold the prefix");
+    const int64_t rows = (int64_t)a->batch * s.G;
+    TQB_REQUIRE(rows <= int64_t(1) << 22 && a->num_kv_heads <= 65535, TQB_ERR_UNSUPPORTED,
+                "batch * (num_q_heads / num_kv_heads) must be at most 2^22, num_kv_heads 65535");
+    tqb::PrefixParams p{};
+    p.split = rows <= 128 && a->num_splits % 2 == 0;
+    p.chunks = p.split ? a->num_splits / 2 : a->num_splits;
+    TQB_REQUIRE(p.chunks <= (prefix_len + 127) / 128, TQB_ERR_INVALID_ARG,
+                "num_splits must leave each CTA a tile of 128 tokens: at most ceil(prefix_len / 128), twice that (even) "
+                "for 128 rows or fewer");
+    DeviceGuard guard(a->mid_o);
+    TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning mid_o");
+    p.q = s.q;
+    p.qsb = s.qsb;
+    p.qsh = s.qsh;
+    p.cache = s.cache;
+    p.layout = s.layout;
+    p.block_bytes = s.block_bytes;
+    p.pos_stride = s.pos_stride;
+    p.head_stride = s.head_stride;
+    p.num_blocks = s.num_blocks;
+    p.pages = s.bt;
+    p.n_pages = prefix_len / tqb::kBlockSize;
+    p.seq_lens = s.seq_lens;
+    p.cents = s.cents;
+    p.mid = s.mid;
+    p.msb = s.msb;
+    p.msh = s.msh;
+    p.mss = s.mss;
+    p.B = s.B;
+    p.Hk = s.Hk;
+    p.G = s.G;
+    p.scale = s.attn_scale;
+    return tqb::launch_prefix(p, stream);
 }
 
 int tqb_append(const tqb_append_args* a, cudaStream_t stream) {

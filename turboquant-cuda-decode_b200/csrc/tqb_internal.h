@@ -219,6 +219,25 @@ struct GatherParams {
     int N, Hk;
 };
 
+// A prefix shared by the whole batch (tqb_prefix.cu).
+struct PrefixParams {
+    const float* q;
+    int64_t qsb, qsh;
+    const uint8_t* cache;
+    int layout;
+    int64_t block_bytes, pos_stride, head_stride, num_blocks;
+    const int32_t* pages;  // [n_pages]
+    int n_pages;
+    const int32_t* seq_lens;
+    const float* cents;
+    float* mid;
+    int64_t msb, msh, mss;
+    int B, Hk, G;
+    int chunks;  // of the prefix's 128-token tiles, a CTA each per KV head and 256 rows
+    int split;   // two streams of the same <= 128 rows, a partial split each
+    float scale;
+};
+
 // Records the CUDA error text for tqb_last_error_detail(); returns
 // TQB_OK or TQB_ERR_LAUNCH.
 int report_launch(cudaError_t e);
@@ -250,6 +269,8 @@ int launch_stage1_range(const Stage1Params& p, cudaStream_t stream, int num_sms)
 int launch_stage1_ring_range(const Stage1Params& p, cudaStream_t stream, int num_sms);
 int launch_stage2_range(const Stage2Params& p, cudaStream_t stream);
 int launch_append(const AppendParams& p, cudaStream_t stream, int num_sms);
+int launch_prefix(const PrefixParams& p, cudaStream_t stream);
+int read_prefix_timeouts(unsigned int* count, bool reset);
 int launch_gather(const GatherParams& p, cudaStream_t stream);
 
 }  // namespace tqb

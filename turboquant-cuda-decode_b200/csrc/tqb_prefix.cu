@@ -1,0 +1,604 @@
+// tqb_prefix.cu — decode attention over a prefix that every sequence of the
+// batch shares, computed once for all of them on the 5th-generation tensor
+// cores.
+//
+// For KV head h the rows are the queries of its G heads in all B sequences
+// (R = B G of them), and for a chunk of the prefix's tokens T
+//     S = Q K^T,  P = exp2(S kfac - m),  l = sum P,  O = P V / l,
+// the softmax-normalised partial output and natural-log LSE of the chunk, in
+// Stage1's mid_o form; Stage2 merges the chunks with each sequence's own
+// tokens.  Per-sequence Stage1 dequantises the prefix B times; here a CTA
+// dequantises a 128-token tile once for up to 256 rows.
+//
+// One CTA per SM, one (chunk, KV head, block of 256 rows); warps:
+//   0-3, 4-7   softmax of streams 0 and 1: thread = row (= TMEM lane).  A
+//              stream is 128 rows over every tile, or with at most 128 rows
+//              the same rows over the even or the odd tiles, so that two
+//              tiles are always in flight;
+//   8-11       dequantise K and V tiles (fp16, 128-byte swizzle) into two
+//              stages of shared memory, the next tile's codes in registers;
+//   12         issues the MMAs (13-15 idle): S = Q K^T (operands in shared memory), then
+//              O += P V with P in TMEM where S was.
+// TMEM holds S0 S1 O0 O1 (128 columns each): all 512.
+//
+// Precision: Q (scaled per row by a power of two), K = c norm, V = code scale
+// + zero and P are rounded to fp16, each product accumulated in fp32; m, l, O
+// and the LSE are fp32.  Four roundings of relative size 2^-12 rms/sqrt(3) on
+// terms whose errors average out: about 3e-4 of the output, a third of a
+// bf16 output's own rounding, which is why only 16-bit outputs come here.
+//
+// m is a lazy reference: it moves (and l and O are rescaled) only when a
+// score exceeds it by more than 2^8, so p <= 2^8 in fp16 and l stays in fp32.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "tqb_common.cuh"
+#include "tqb_internal.h"
+#include "tqb_umma.cuh"
+
+namespace tqb {
+
+// Kernels that gave up a wait (read by tqb_wait_timeouts).
+__device__ unsigned int g_prefix_timeouts = 0;
+
+namespace {
+
+constexpr int kTile = 128;                       // tokens of a tile, rows of a stream
+constexpr int kTilePages = kTile / kBlockSize;   // 8
+constexpr int kOperand = kTile * kHeadDim * 2;   // 32 KB: one fp16 operand tile
+constexpr int kHalf = kOperand / 2;              // 16 KB: its 64-element half
+constexpr int kQOff = 0, kKOff = 2 * kOperand, kVOff = 4 * kOperand, kLutOff = 6 * kOperand;
+constexpr int kAuxOff = kLutOff + 256 * 32 * 4;  // the K table: 256 entries, a copy per lane
+constexpr int kBarOff = kAuxOff + 2 * kTile * 4;
+constexpr int kPrefixSmem = kBarOff + 192;
+static_assert(kPrefixSmem <= 232448, "shared memory per CTA");
+constexpr int kSoftmaxWarps = 8, kProducerWarps = 4;
+constexpr int kPrefixThreads = (kSoftmaxWarps + kProducerWarps + 4) * 32;  // whole warpgroups
+// Registers per thread: 128 at the launch, moved between the warpgroups by
+// setmaxnreg (the shares add up to the launch's).
+constexpr int kPrefixRegs = 128, kSoftmaxRegs = 168, kProducerRegs = 112, kIssueRegs = 64;
+static_assert(2 * kSoftmaxRegs + kProducerRegs + kIssueRegs <= 4 * kPrefixRegs && kPrefixRegs * kPrefixThreads <= 65536,
+              "register split");
+constexpr float kSlack = 8.0f;
+
+// Barriers (8 bytes each) at kBarOff, then words.
+enum : uint32_t { kKFull = 0, kVFull = 16, kKEmpty = 32, kVEmpty = 48, kSFull = 64, kPFull = 80, kOFull = 96, kDone = 112,
+                  kMasks = 128, kTmem = 144, kAbort = 148 };
+
+__device__ __forceinline__ uint32_t dup16(uint32_t h) { return __byte_perm(h, 0u, 0x1010); }
+__device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) { return h2_as_u32(__hmul2(u32_as_h2(a), u32_as_h2(b))); }
+__device__ __forceinline__ uint32_t g16(const uint8_t* p) { return __ldg(reinterpret_cast<const unsigned short*>(p)); }
+__device__ __forceinline__ uint32_t g32(const uint8_t* p) { return __ldg(reinterpret_cast<const unsigned int*>(p)); }
+__device__ __forceinline__ uint4 g128(const uint8_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ uint32_t g2x16(const uint8_t* p) { return g16(p) | (g16(p + 2) << 16); }
+template <bool A2>  // four bytes, 2-byte aligned (A2) or 4-byte aligned
+__device__ __forceinline__ uint32_t gw(const uint8_t* p) { return A2 ? g2x16(p) : g32(p); }
+
+// Codes and metadata of one token's 32 dims [32c, 32c + 32).
+template <int L>
+struct Raw {
+    uint32_t k[layout_fp8_keys(L) ? 8 : 4], v[4], kn, vs, vz;
+};
+template <int L>
+__device__ __forceinline__ void load_raw(Raw<L>& r, const PrefixParams& P, int id, uint32_t off, uint32_t h, uint32_t c) {
+    constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), v3 = layout_3bit_values(L), aos = layout_is_aos(L);
+    constexpr int kKey = aos_key_bytes(L), kRow = kKey + val_code_bytes(L);
+    if (id < 0) {  // no such page: zeros, and the mask hides its scores
+#pragma unroll
+        for (int i = 0; i < (k8 ? 8 : 4); i++) r.k[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.v[i] = 0u;
+        r.kn = r.vs = r.vz = 0u;
+        return;
+    }
+    const uint8_t* base = P.cache + (size_t)(uint32_t)id * (size_t)P.block_bytes;
+    const uint8_t* kp;
+    const uint8_t* vp;
+    if constexpr (aos) {
+        const uint8_t* sp = base + (size_t)off * P.pos_stride + (size_t)h * P.head_stride;
+        kp = sp + (k8 ? 32 : k3 ? 12 : 16) * c;
+        vp = sp + aos_val_off(L) + (v3 ? 12 : 16) * c;
+        r.kn = k8 ? 0u : g16(sp + aos_norm_off(L));
+        r.vs = g16(sp + aos_scale_off(L));
+        r.vz = g16(sp + aos_scale_off(L) + 2);
+    } else {
+        const uint8_t* row = base + off * ((uint32_t)P.Hk * kRow) + h * (uint32_t)kRow;
+        kp = row + (k8 ? 32 : k3 ? 12 : 16) * c;
+        vp = row + kKey + (v3 ? 12 : 16) * c;
+        constexpr uint32_t kFields = k8 ? 2 : 3;
+        const uint8_t* meta = base + (uint32_t)kBlockSize * P.Hk * kRow + (h * kFields * kBlockSize + off) * 2;
+        r.kn = k8 ? 0u : g16(meta);
+        r.vs = g16(meta + (kFields - 2) * kBlockSize * 2);
+        r.vz = g16(meta + (kFields - 1) * kBlockSize * 2);
+    }
+    if constexpr (!aos && !k3) {
+        const uint4 a = g128(kp);
+        r.k[0] = a.x; r.k[1] = a.y; r.k[2] = a.z; r.k[3] = a.w;
+        if constexpr (k8) {
+            const uint4 b = g128(kp + 16);
+            r.k[4] = b.x; r.k[5] = b.y; r.k[6] = b.z; r.k[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < (k8 ? 8 : k3 ? 3 : 4); i++) r.k[i] = gw<aos>(kp + 4 * i);
+    }
+    if constexpr (!aos && !v3) {
+        const uint4 a = g128(vp);
+        r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < (v3 ? 3 : 4); i++) r.v[i] = gw<aos>(vp + 4 * i);
+    }
+}
+// 3-bit codes 8i .. 8i + 7 (24 bits) of a 12-byte run.
+__device__ __forceinline__ uint32_t bits24(const uint32_t* w, int i) {
+    return i == 0 ? w[0] & 0xFFFFFFu
+         : i == 1 ? __funnelshift_r(w[0], w[1], 24) & 0xFFFFFFu
+         : i == 2 ? __funnelshift_r(w[1], w[2], 16) & 0xFFFFFFu
+                  : w[2] >> 8;
+}
+
+// 32 dims of a token into the K tile: 4 16-byte chunks of its row.
+template <int L>
+__device__ __forceinline__ void put_k(uint8_t* smem, uint32_t tile, const Raw<L>& r, uint32_t tok, uint32_t c, int lane) {
+    constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), aos = layout_is_aos(L);
+    uint32_t f[16];
+    if constexpr (k8) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) f[i] = fp8x2_to_h2((r.k[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+    } else {
+        const uint8_t* lut = smem + kLutOff + 4 * lane;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            uint32_t at;  // entry (two codes) * 128 bytes
+            const int j = i & 3;
+            if constexpr (k3) {
+                const uint32_t x = bits24(r.k, i >> 2);
+                at = (j == 0 ? x << 7 : j == 1 ? x << 1 : j == 2 ? x >> 5 : x >> 11) & 0x1F80u;
+            } else {
+                const uint32_t x = r.k[i >> 2];
+                at = (j == 0 ? x << 7 : j == 1 ? x >> 1 : j == 2 ? x >> 9 : x >> 17) & 0x7F80u;
+            }
+            f[i] = *reinterpret_cast<const uint32_t*>(lut + at);
+        }
+        uint32_t norm = r.kn;
+        if constexpr (aos) {
+            // AoS stores the raw |k|: divide by the centroids' length (the
+            // token's four quarters sit 8 lanes apart)
+            float q = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float2 x = __half22float2(u32_as_h2(f[i]));
+                q = fmaf(x.x, x.x, fmaf(x.y, x.y, q));
+            }
+            q += __shfl_xor_sync(0xffffffffu, q, 8);
+            q += __shfl_xor_sync(0xffffffffu, q, 16);
+            norm = __half_as_ushort(__float2half_rn(half_bits_to_float(norm) * rsqrtf(q + 1e-16f)));
+        }
+        const uint32_t n2 = dup16(norm);
+#pragma unroll
+        for (int i = 0; i < 16; i++) f[i] = hmul2u(f[i], n2);
+    }
+    uint8_t* row = smem + tile + (c >> 1) * kHalf + tok * 128;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        *reinterpret_cast<uint4*>(row + ((((c & 1) * 4 + i) ^ (tok & 7)) << 4)) =
+            make_uint4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+}
+
+// 32 dims of a token into the V tile, each group of 8 in the order 0 4 1 5 2
+// 6 3 7 (the nibble pairs that one mask of a word yields): the columns of O
+// come out in that order and are put right when they are written.
+template <int L>
+__device__ __forceinline__ void put_v(uint8_t* smem, uint32_t tile, const Raw<L>& r, uint32_t tok, uint32_t c) {
+    constexpr bool v3 = layout_3bit_values(L);
+    // a nibble in the mantissa of 1024 (bits 0-3) or of 64 (bits 4-7) adds its
+    // own value to it, exactly
+    const __half2 k1024 = u32_as_h2(0x64006400u), k64 = u32_as_h2(0x54005400u);
+    const __half2 s2 = u32_as_h2(dup16(r.vs)), z2 = u32_as_h2(dup16(r.vz));
+    uint8_t* row = smem + tile + (c >> 1) * kHalf + tok * 128;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = v3 ? spread3to4(bits24(r.v, i)) : r.v[i];
+        const uint32_t w8 = w >> 8;
+        uint4 o;
+        o.x = h2_as_u32(__hfma2(__hsub2(u32_as_h2(and_or(w, 0x000F000Fu, 0x64006400u)), k1024), s2, z2));
+        o.y = h2_as_u32(__hfma2(__hsub2(u32_as_h2(and_or(w, 0x00F000F0u, 0x54005400u)), k64), s2, z2));
+        o.z = h2_as_u32(__hfma2(__hsub2(u32_as_h2(and_or(w8, 0x000F000Fu, 0x64006400u)), k1024), s2, z2));
+        o.w = h2_as_u32(__hfma2(__hsub2(u32_as_h2(and_or(w8, 0x00F000F0u, 0x54005400u)), k64), s2, z2));
+        *reinterpret_cast<uint4*>(row + ((((c & 1) * 4 + i) ^ (tok & 7)) << 4)) = o;
+    }
+}
+
+// Where a CTA works: its tiles [t0, t1) and rows [row0, row0 + rows), and the
+// tiles of a stream (every tile, or with `split` every other one).
+struct Place {
+    int h, t0, n, row0, rows;
+    bool split;
+    __device__ __forceinline__ int tiles(int m) const { return split ? (n + 1 - m) / 2 : (m == 0 || rows > kTile ? n : 0); }
+    __device__ __forceinline__ int tile(int m, int i) const { return split ? 2 * i + m : i; }  // from t0 on
+};
+
+template <int L>
+__device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W, uint8_t* smem, uint32_t bars, volatile uint32_t* abort,
+                           int pw, int lane) {
+    const uint32_t t8 = lane & 7, c = lane >> 3;
+    const uint32_t off = (pw & 1) * 8 + t8;  // token in its page
+    const int nblocks = P.num_blocks > 0 && P.num_blocks < 0x7fffffff ? (int)P.num_blocks : 0x7fffffff;
+    // Task i of a tile: token 32i + 8 pw + t8, in page 2i + pw / 2.
+    auto page_id = [&](int tile, int i) {
+        const int pg = (W.t0 + tile) * kTilePages + 2 * i + (pw >> 1);
+        if (tile >= W.n || pg >= P.n_pages) return -1;
+        const int id = __ldg(P.pages + pg);
+        return id >= 0 && id < nblocks ? id : -1;
+    };
+    Raw<L> raw[4];
+    int ids[4], next[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) ids[i] = page_id(0, i);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        load_raw<L>(raw[i], P, ids[i], off, W.h, c);
+        next[i] = page_id(1, i);
+    }
+    for (int j = 0; j < W.n; j++) {
+        const int s = j & 1;
+        const uint32_t phase = ((j >> 1) & 1) ^ 1;
+        if (!__all_sync(0xffffffffu, bar_wait(bars + kKEmpty + 8 * s, phase, abort))) return;
+#pragma unroll
+        for (int i = 0; i < 4; i++) put_k<L>(smem, kKOff + s * kOperand, raw[i], 32 * i + 8 * pw + t8, c, lane);
+        // pages of this tile that exist, a bit each (warps 0 and 2 own four)
+        if ((pw & 1) == 0 && lane == 0) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) m |= ids[i] >= 0 ? 1u << (2 * i + (pw >> 1)) : 0u;
+            smem[kBarOff + kMasks + 4 * (j & 3) + (pw >> 1)] = (uint8_t)m;
+        }
+        fence_async_smem();
+        bar_arrive(bars + kKFull + 8 * s);
+        if (!__all_sync(0xffffffffu, bar_wait(bars + kVEmpty + 8 * s, phase, abort))) return;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            put_v<L>(smem, kVOff + s * kOperand, raw[i], 32 * i + 8 * pw + t8, c);
+            ids[i] = next[i];
+            load_raw<L>(raw[i], P, ids[i], off, W.h, c);
+            next[i] = page_id(j + 2, i);
+        }
+        fence_async_smem();
+        bar_arrive(bars + kVFull + 8 * s);
+    }
+}
+
+// The MMA thread.  All its MMAs execute in the order of issue, so S_m of the
+// next tile may follow P_m V of this one on the same columns, and the commit
+// that announces S_m also says that the stream's earlier products are done.
+__device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t bars, uint32_t tmem, volatile uint32_t* abort) {
+    constexpr uint32_t kQK = umma_idesc(kTile, kTile, false), kPV = umma_idesc(kTile, kHeadDim, true);
+    const int last = W.split || W.rows <= kTile ? -1 : 1;  // the stream that releases a shared stage (-1: each its own)
+    auto qk = [&](int m, int tile) {
+        const int s = tile & 1;
+        if (!bar_wait(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
+        tc_fence_after();
+        const uint32_t q = smem + kQOff + (W.split ? 0 : m * kOperand), k = smem + kKOff + s * kOperand;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t at = (e >> 2) * kHalf + (e & 3) * 32;
+            umma_ss(tmem + m * kTile, umma_desc(q + at, 16, 1024), umma_desc(k + at, 16, 1024), kQK, e != 0);
+        }
+        umma_commit(bars + kSFull + 8 * m);
+        if (last < 0 || m == last) umma_commit(bars + kKEmpty + 8 * s);
+        return true;
+    };
+    bool ok = true;
+    for (int m = 0; m < 2 && ok; m++)
+        if (W.tiles(m) > 0) ok = qk(m, W.tile(m, 0));
+    for (int i = 0; ok && i < W.tiles(0); i++) {
+        for (int m = 0; m < 2 && ok; m++) {
+            if (i >= W.tiles(m)) continue;
+            const int tile = W.tile(m, i), s = tile & 1;
+            ok = bar_wait(bars + kPFull + 8 * m, i & 1, abort) && bar_wait(bars + kVFull + 8 * s, (tile >> 1) & 1, abort);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t v = smem + kVOff + s * kOperand;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + 8 * e, umma_desc(v + e * 2048, kHalf, 1024),
+                        kPV, i != 0 || e != 0);
+            if (last < 0 || m == last) umma_commit(bars + kVEmpty + 8 * s);
+            if (i + 1 < W.tiles(m))
+                ok = qk(m, W.tile(m, i + 1));
+            else
+                umma_commit(bars + kOFull + 8 * m);
+        }
+    }
+    // every product has ended before the CTA frees its TMEM
+    umma_commit(bars + kDone);
+    bar_wait(bars + kDone, 0, abort);
+}
+
+// One pass over a tile's scores of this thread's row: p = exp2(s kfac - ref)
+// as fp16 pairs, their sum, and the largest exponent.
+template <bool MASK>
+__device__ __forceinline__ void weigh(uint32_t tmem_s, float kfac, float ref, int lim, uint32_t pages, uint32_t (&p)[64],
+                                      float& sum, float& top) {
+    const uint64_t k2 = pack2(kfac, kfac), r2 = pack2(-ref, -ref);
+    uint64_t acc = pack2(0.0f, 0.0f);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        uint32_t s[32];
+        tmem_ld32(s, tmem_s + 32 * q);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const uint64_t x = fma2((uint64_t)s[2 * j] | ((uint64_t)s[2 * j + 1] << 32), k2, r2);
+            float a = lo2(x), b = hi2(x);
+            if constexpr (MASK) {
+                const int t = 32 * q + 2 * j;
+                a = t < lim && (pages >> (t >> 4)) & 1u ? a : -INFINITY;
+                b = t + 1 < lim && (pages >> (t >> 4)) & 1u ? b : -INFINITY;
+            }
+            mx = fmaxf(mx, fmaxf(a, b));
+            a = ex2_approx(a);
+            b = ex2_approx(b);
+            acc = add2(acc, pack2(a, b));
+            p[16 * q + j] = h2_as_u32(__floats2half2_rn(a, b));
+        }
+    }
+    sum = lo2(acc) + hi2(acc);
+    top = mx;
+}
+// The largest score of the row (before kfac).
+template <bool MASK>
+__device__ __forceinline__ float largest(uint32_t tmem_s, int lim, uint32_t pages) {
+    float mx = -INFINITY;
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        uint32_t s[32];
+        tmem_ld32(s, tmem_s + 32 * q);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const int t = 32 * q + j;
+            const float x = __uint_as_float(s[j]);
+            mx = fmaxf(mx, !MASK || (t < lim && (pages >> (t >> 4)) & 1u) ? x : -INFINITY);
+        }
+    }
+    return mx;
+}
+
+__device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, uint8_t* smem, uint32_t bars, uint32_t tmem,
+                        volatile uint32_t* abort, int m, int warp, int lane) {
+    const int wq = warp & 3;
+    const uint32_t lanes = (uint32_t)(32 * wq) << 16;
+    const uint32_t ts = tmem + lanes + m * kTile, to = tmem + lanes + 2 * kTile + m * kHeadDim;
+    const int local = (W.split ? 0 : m * kTile) + 32 * wq + lane;  // row of the CTA
+    const bool live = local < W.rows;
+    const int row = W.row0 + min(local, W.rows - 1);
+    const int b = (int)((uint32_t)row / (uint32_t)P.G), g = row - b * P.G;
+    const float kfac = *reinterpret_cast<const float*>(smem + kAuxOff + 4 * ((W.split ? 0 : m * kTile) + 32 * wq + lane));
+    // tokens of the chunk this row sees, from the chunk's start
+    const int lim = min(__ldg(P.seq_lens + b), P.n_pages * kBlockSize) - W.t0 * kTile;
+    const bool any_row = __any_sync(0xffffffffu, live);
+    float ref = -INFINITY, l = 0.0f;
+    const int n = W.tiles(m);
+    for (int i = 0; i < n; i++) {
+        const int tile = W.tile(m, i);
+        if (!__all_sync(0xffffffffu, bar_wait(bars + kSFull + 8 * m, i & 1, abort))) return;
+        tc_fence_after();
+        if (any_row) {
+            const uint32_t pages = smem[kBarOff + kMasks + 4 * (tile & 3)] | smem[kBarOff + kMasks + 4 * (tile & 3) + 1];
+            const int left = lim - tile * kTile;
+            const bool mask = __any_sync(0xffffffffu, left < kTile || pages != 0xFFu);
+            uint32_t p[64];
+            float sum, top;
+            if (__any_sync(0xffffffffu, ref == -INFINITY)) {  // the first tile with a visible token
+                const float mx = mask ? largest<true>(ts, left, pages) : largest<false>(ts, left, pages);
+                if (ref == -INFINITY) ref = mx * kfac;
+            }
+            for (;;) {
+                const float r = ref == -INFINITY ? 0.0f : ref;
+                if (mask)
+                    weigh<true>(ts, kfac, r, left, pages, p, sum, top);
+                else
+                    weigh<false>(ts, kfac, r, left, pages, p, sum, top);
+                const bool over = top > kSlack && top < INFINITY;
+                if (!__any_sync(0xffffffffu, over)) break;
+                // move the reference of the rows that need it, and what they
+                // have summed so far
+                const float f = over ? ex2_approx(-top) : 1.0f;
+                ref = over ? ref + top : ref;
+                l *= f;
+                if (i > 0) {
+#pragma unroll 1
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t o[32];
+                        tmem_ld32(o, to + 32 * q);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tmem_st32(to + 32 * q, o);
+                    }
+                    tmem_wait_st();
+                }
+            }
+            l += sum;
+            tmem_st32(ts, p);
+            tmem_st32(ts + 32, p + 32);
+            tmem_wait_st();
+        }
+        tc_fence_before();
+        bar_arrive(bars + kPFull + 8 * m);
+    }
+    // ---- the partial rows ----
+    if (n > 0) {
+        if (!__all_sync(0xffffffffu, bar_wait(bars + kOFull + 8 * m, 0, abort))) return;
+        tc_fence_after();
+    }
+    if (!any_row) return;
+    const int sp = W.split ? 2 * (int)blockIdx.x + m : (int)blockIdx.x;
+    const bool seen = l > 0.0f || l != l;
+    const float inv = seen ? rcp_approx(l) : 0.0f;
+    float* dst = P.mid + (int64_t)b * P.msb + (int64_t)(W.h * P.G + g) * P.msh + (int64_t)sp * P.mss;
+    if (live) dst[kHeadDim] = seen ? (ref + lg2_approx(l)) * kLn2 : -INFINITY;
+    // 32 x 32 blocks turn through shared memory (this stream's query tile, or
+    // the unused second one), so that rows are written in runs of 128 bytes
+    float* turn = reinterpret_cast<float*>(smem + kQOff + (W.split ? kOperand + m * kHalf : m * kOperand) + wq * 4096);
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        uint32_t o[32];
+        if (n > 0) {
+            tmem_ld32(o, to + 32 * q);
+            tmem_wait_ld();
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const int d = (j & ~7) | ((j & 1) << 2) | ((j & 7) >> 1);  // column j of O is dim d
+            turn[32 * lane + (d ^ lane)] = seen ? __uint_as_float(o[j]) * inv : 0.0f;
+        }
+        __syncwarp();
+        for (int r = 0; r < 32; r++) {
+            float* to_row = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+            if (__shfl_sync(0xffffffffu, (int)live, r)) to_row[32 * q + lane] = turn[32 * r + (lane ^ r)];
+        }
+        __syncwarp();
+    }
+}
+
+template <int L>
+__global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixParams P) {
+    constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L);
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = smem_addr(smem), bars = base + kBarOff;
+    volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kAbort);
+    pdl_trigger();
+
+    Place W;
+    const int R = P.B * P.G, n_tiles = (P.n_pages + kTilePages - 1) / kTilePages;
+    W.h = blockIdx.y;
+    W.t0 = (int)((int64_t)n_tiles * blockIdx.x / gridDim.x);
+    W.n = (int)((int64_t)n_tiles * (blockIdx.x + 1) / gridDim.x) - W.t0;
+    W.row0 = blockIdx.z * 2 * kTile;
+    W.rows = min(R - W.row0, 2 * kTile);
+    W.split = P.split != 0;
+
+    if (tid == 0) {
+        for (int s = 0; s < 2; s++) {
+            bar_init(bars + kKFull + 8 * s, kProducerWarps * 32);
+            bar_init(bars + kVFull + 8 * s, kProducerWarps * 32);
+            bar_init(bars + kKEmpty + 8 * s, 1);
+            bar_init(bars + kVEmpty + 8 * s, 1);
+            bar_init(bars + kSFull + 8 * s, 1);
+            bar_init(bars + kPFull + 8 * s, 128);
+            bar_init(bars + kOFull + 8 * s, 1);
+        }
+        bar_init(bars + kDone, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == kSoftmaxWarps + kProducerWarps) tmem_alloc<512>(bars + kTmem);
+    pdl_wait();  // the rotated queries, and the kernel before that reads mid_o
+
+    // ---- K table: entry = two codes, {c[low], c[high]} in fp16, a copy per lane
+    if constexpr (!k8) {
+        constexpr int kPairs = k3 ? 64 : 256, kBits = k3 ? 3 : 4, kMask = k3 ? 7 : 15;
+        for (int e = tid; e < kPairs * 32; e += kPrefixThreads) {
+            const int pair = e >> 5;
+            reinterpret_cast<uint32_t*>(smem + kLutOff)[e] =
+                h2_as_u32(__floats2half2_rn(__ldg(P.cents + (pair & kMask)), __ldg(P.cents + (pair >> kBits))));
+        }
+    }
+    // ---- queries: fp16, scaled per row into [2^14, 2^15), 128-byte swizzle
+    const int slots = W.split || W.rows <= kTile ? kTile : 2 * kTile;
+    for (int r = warp; r < slots; r += kPrefixThreads / 32) {
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < W.rows) {
+            const int row = W.row0 + r, b = row / P.G, g = row - b * P.G;
+            x = __ldg(reinterpret_cast<const float4*>(P.q + (int64_t)b * P.qsb + (int64_t)(W.h * P.G + g) * P.qsh) + lane);
+        }
+        const float amax = warp_max_xor(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), 1, 16);
+        const int e = fp16_scale_exp(amax);
+        const float f = exp2i(e);
+        if (lane == 0) reinterpret_cast<float*>(smem + kAuxOff)[r] = P.scale * kLog2e * exp2i(-e);
+        // dims 4 lane .. 4 lane + 3: half lane / 16, chunk (lane % 16) / 2
+        uint8_t* at = smem + kQOff + (r >> 7) * kOperand + (lane >> 4) * kHalf + (r & 127) * 128 +
+                      ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+        *reinterpret_cast<uint2*>(at) = make_uint2(h2_as_u32(__floats2half2_rn(x.x * f, x.y * f)),
+                                                   h2_as_u32(__floats2half2_rn(x.z * f, x.w * f)));
+    }
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kTmem);
+
+    if (warp < kSoftmaxWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
+        softmax(P, W, smem, bars, tmem, abort, warp >> 2, warp, lane);
+    } else if (warp < kSoftmaxWarps + kProducerWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kProducerRegs));
+        dequantise<L>(P, W, smem, bars, abort, warp - kSoftmaxWarps, lane);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegs));
+        if (warp == kSoftmaxWarps + kProducerWarps && lane == 0) issue(W, base, bars, tmem, abort);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kSoftmaxWarps + kProducerWarps) tmem_free<512>(tmem);
+    if (tid == 0 && *abort != 0) atomicAdd(&g_prefix_timeouts, 1u);
+}
+
+template <int L>
+int launch_prefix_t(const PrefixParams& P, cudaStream_t stream) {
+    auto kern = prefix_kernel<L>;
+    static thread_local int configured_dev = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (configured_dev != dev) {
+        // the register split draws on what the kernel was launched with
+        cudaFuncAttributes a{};
+        if (cudaFuncGetAttributes(&a, kern) != cudaSuccess) return report_launch(cudaGetLastError());
+        if (a.numRegs < kPrefixRegs) {
+            set_error_detail("the shared-prefix kernel was built with fewer registers than its split needs");
+            return TQB_ERR_UNSUPPORTED;
+        }
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrefixSmem) != cudaSuccess)
+            return report_launch(cudaGetLastError());
+        configured_dev = dev;
+    }
+    const unsigned blocks = (unsigned)(((int64_t)P.B * P.G + 2 * kTile - 1) / (2 * kTile));
+    return report_launch(launch_pdl(kern, dim3((unsigned)P.chunks, (unsigned)P.Hk, blocks), dim3(kPrefixThreads), kPrefixSmem,
+                                    stream, P));
+}
+
+}  // namespace
+
+int launch_prefix(const PrefixParams& P, cudaStream_t stream) {
+    switch (P.layout) {
+        case TQB_LAYOUT_SOA: return launch_prefix_t<TQB_LAYOUT_SOA>(P, stream);
+        case TQB_LAYOUT_SOA_K8: return launch_prefix_t<TQB_LAYOUT_SOA_K8>(P, stream);
+        case TQB_LAYOUT_SOA_K3: return launch_prefix_t<TQB_LAYOUT_SOA_K3>(P, stream);
+        case TQB_LAYOUT_SOA_K3V3: return launch_prefix_t<TQB_LAYOUT_SOA_K3V3>(P, stream);
+        case TQB_LAYOUT_AOS: return launch_prefix_t<TQB_LAYOUT_AOS>(P, stream);
+        case TQB_LAYOUT_AOS_K8: return launch_prefix_t<TQB_LAYOUT_AOS_K8>(P, stream);
+        case TQB_LAYOUT_AOS_K3: return launch_prefix_t<TQB_LAYOUT_AOS_K3>(P, stream);
+        case TQB_LAYOUT_AOS_K3V3: return launch_prefix_t<TQB_LAYOUT_AOS_K3V3>(P, stream);
+        default: return TQB_ERR_INVALID_ARG;
+    }
+}
+
+int read_prefix_timeouts(unsigned int* count, bool reset) {
+    cudaError_t e = cudaMemcpyFromSymbol(count, g_prefix_timeouts, sizeof(unsigned int));
+    if (e == cudaSuccess && reset) {
+        const unsigned int zero = 0;
+        e = cudaMemcpyToSymbol(g_prefix_timeouts, &zero, sizeof(unsigned int));
+    }
+    return e == cudaSuccess ? TQB_OK : report_launch(e);
+}
+
+}  // namespace tqb

@@ -65,6 +65,7 @@ EXPORTED_SYMBOLS = (
     "tqb_stage2_range",
     "tqb_append",
     "tqb_gather",
+    "tqb_prefix",
 )
 
 
@@ -269,6 +270,8 @@ def load() -> ctypes.CDLL:
                                              _vp, _vp]
             lib.tqb_append.argtypes = [ctypes.POINTER(AppendArgs), _vp]
             lib.tqb_gather.argtypes = [ctypes.POINTER(GatherArgs), _vp]
+            lib.tqb_prefix.argtypes = [ctypes.POINTER(Stage1Args), _i32, _vp]
+            lib.tqb_prefix.restype = ctypes.c_int
             for f in (lib.tqb_stage1_range, lib.tqb_stage2_range, lib.tqb_append, lib.tqb_gather):
                 f.restype = ctypes.c_int
             _lib = lib

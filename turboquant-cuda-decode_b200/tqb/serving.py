@@ -55,6 +55,7 @@ def _call(name: str, *args) -> None:
         f.argtypes = {"tqb_append": [ctypes.c_char_p, ctypes.c_void_p],
                       "tqb_gather": [ctypes.c_char_p, ctypes.c_void_p],
                       "tqb_stage1_range": [ctypes.c_char_p] * 3 + [ctypes.c_void_p],
+                      "tqb_prefix": [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p],
                       "tqb_stage2_range": [ctypes.c_char_p] * 2 + [ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
                                                                    ctypes.c_void_p, ctypes.c_void_p]}[name]
         f.restype = ctypes.c_int
@@ -322,21 +323,41 @@ class _Step:
             self.query = q = q.to(_F32).contiguous()
             self.rows, self.rs = q.data_ptr(), q.stride()
 
-    def launch(self, rng: bytes, lead: int, S: int, stream) -> torch.Tensor:
-        """Stage1 of the range into the splits from ``lead`` on, and the merge of all S."""
-        st = _stream(self.dev) if stream is None else stream
+    def stage1(self, at: int, S: int) -> bytes:
+        """Stage1 arguments for S splits from split ``at`` on."""
         ms, rs, cs = self.ms, self.rs, self.cs
-        _call("tqb_stage1_range", _STAGE1.pack(
+        return _STAGE1.pack(
             self.rows, rs[0], rs[1], self.cache, self.lay, cs[0], cs[1], cs[2], self.cshape[0], self.table,
-            self.table_stride, self.blocks, self.seq_lens, self.cents, self.n, 0, 0, self.mid + 4 * ms[2] * lead, ms[0],
-            ms[1], ms[2], self.B, self.Hq, self.Hk, HEAD_DIM, BLOCK_SIZE, S - lead, self.scale),
-            None if not self.rot else _ROTATE.pack(self.query.data_ptr(), self.kind, self.qs[0], self.qs[1], self.rot,
-                                                   self.rows, rs[0], rs[1], self.B, self.Hq, HEAD_DIM), rng, st)
+            self.table_stride, self.blocks, self.seq_lens, self.cents, self.n, 0, 0, self.mid + 4 * ms[2] * at, ms[0],
+            ms[1], ms[2], self.B, self.Hq, self.Hk, HEAD_DIM, BLOCK_SIZE, S, self.scale)
+
+    def launch(self, rng: bytes, lead: int, S: int, stream, prefix_len: int = 0) -> torch.Tensor:
+        """Stage1 of the range into the splits from ``lead`` on, the shared prefix into those before, the merge of all
+        S."""
+        st = _stream(self.dev) if stream is None else stream
+        ms, rs = self.ms, self.rs
+        _call("tqb_stage1_range", self.stage1(lead, S - lead),
+              None if not self.rot else _ROTATE.pack(self.query.data_ptr(), self.kind, self.qs[0], self.qs[1], self.rot,
+                                                     self.rows, rs[0], rs[1], self.B, self.Hq, HEAD_DIM), rng, st)
+        if lead:  # after Stage1, which rotates the queries
+            _call("tqb_prefix", self.stage1(0, lead), prefix_len, st)
         out = self.output.data_ptr()
         _call("tqb_stage2_range", _STAGE2.pack(
             self.mid, ms[0], ms[1], ms[2], self.seq_lens, 0, out, self.os[0], self.os[1], self.lse, self.lse_stride,
             self.B, self.Hq, HEAD_DIM, S), rng, lead, self.sinks, self.out_kind, out, st)
         return self.output
+
+
+def _prefix_splits(rows: int, heads: int, prefix_len: int) -> int:
+    """Splits of the shared prefix for ``rows`` queries of each of ``heads`` KV heads: chunks of 128-token tiles that
+    fill the 148 SMs in as few rounds as pay (a CTA starts and ends in about the time of three tiles)."""
+    tiles, units = -(-prefix_len // 128), heads * -(-rows // 256)
+    best = (float("inf"), 1)
+    for rounds in (1, 2, 3):
+        chunks = min(tiles, 148 * rounds // units)
+        if chunks:
+            best = min(best, (rounds * (-(-tiles // chunks) + 3), chunks))
+    return best[1] * (2 if rows <= 128 else 1)
 
 
 def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -397,6 +418,12 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
         _no("the block table's rows do not hold the prefix")
     if s.B == 0:
         return s.output
-    S = num_splits or _splits(s.B * s.Hk, most)
+    # Each sequence on its own: fp32 outputs, and prefixes too short for the shared pass.
+    lead = 0
+    if s.out_kind != _lib.TQB_DTYPE_F32 and s.B > 1 and prefix_len >= 128:
+        lead = _prefix_splits(s.B * (s.Hq // s.Hk), s.Hk, prefix_len)
+    else:
+        prefix_len = 0
+    S = (num_splits or _splits(s.B * s.Hk, max(1, most - prefix_len))) + lead
     s.workspace(S)
-    return s.launch(_RANGE.pack(0, 0, 0, most), 0, S, stream)
+    return s.launch(_RANGE.pack(0, 0, prefix_len, most), lead, S, stream, prefix_len)
