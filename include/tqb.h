@@ -281,14 +281,14 @@ int tqb_store(const tqb_store_args* args, cudaStream_t stream);
 
 /*
  * Ranged decode (no reference counterpart): which tokens of its sequence a
- * query attends to.  With L = min(seq_lens[b], max_seq_len):
- *   - the tokens [lo, L), lo = max(L - window, prefix_len, 0) (window 0: no
- *     limit), shared equally by the splits first_tokens > 0 ? 1 : 0 .. S - 1;
- *   - the tokens [0, min(first_tokens, lo)), which stay visible before the
- *     window, as split 0 on their own (first_tokens > 0 needs S >= 2 and
- *     prefix_len 0).
- * Tokens [0, prefix_len) are left out: another call supplies their partials
- * (tqb_prefix).  Splits without a token are left unwritten.
+ * query attends to.  With L = min(seq_lens[b], max_seq_len) these are the
+ * tokens [lo, L), lo = max(L - window, prefix_len, 0) (window 0: no limit),
+ * and the tokens [0, min(first_tokens, lo)), which stay visible before the
+ * window (first_tokens > 0 needs prefix_len 0).  Tokens [0, prefix_len), a
+ * multiple of 16, are left out: another call supplies their partials
+ * (tqb_prefix).  The splits share the pages that hold these tokens equally;
+ * pages without any are not read, and splits without a page are left
+ * unwritten.
  */
 typedef struct tqb_range {
     int32_t window;        /* 0: every token */
@@ -299,8 +299,9 @@ typedef struct tqb_range {
 
 /*
  * Stage1 over a range; s1->num_splits_per_seq must be NULL.  rot may be NULL
- * (s1->q_rot holds the queries); otherwise as in tqb_stage1_rotated, with its
- * restriction: such calls on one device must not overlap in time.
+ * (s1->q_rot holds the queries); otherwise it is as in tqb_stage1_rotated, the
+ * rotation runs as a kernel of its own beside Stage1's prologue, and q_rot
+ * agrees with tqb_rotate_query's to fp32 rounding (another order of sums).
  */
 int tqb_stage1_range(const tqb_stage1_args* s1, const tqb_rotate_args* rot, const tqb_range* range,
                      cudaStream_t stream);

@@ -19,6 +19,7 @@ import torch
 
 import serving_oracle as SO
 import tqb
+from tqb import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -292,9 +293,39 @@ def test_window_covering_everything_equals_the_decode_call():
     cache, table, lens = batch(rng, [5, 300, 77], 2, "soa")
     q = torch.from_numpy(rng.standard_normal((3, 8, 128)).astype(np.float32)).cuda()
     args = (torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda())
-    a = tqb.window_attention(q, *args, cuda(R), cuda(c), window=10 ** 6, num_splits=32)
+    a = tqb.window_attention(tqb.rotate_query(q, cuda(R)), *args, None, cuda(c), window=10 ** 6, num_splits=32)
     b = tqb.triton_turboquant_decode_attention(q, *args, cuda(R).T.contiguous(), cuda(c), 128 ** -0.5, 4, 66, 4)
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows", [1, 15, 16, 17, 50])
+def test_rotation_beside_stage1(dtype, rows):
+    """The queries that a ranged call rotates on the way: 2^-17 |q| for the fp32 sums, as in the append, for rows of
+    every size that their type holds (the split into parts keeps the range)."""
+    rng = np.random.default_rng(rows)
+    c, _, R = book("soa")
+    cache, table, lens = batch(rng, [3] * rows, 1, "soa")
+    q = torch.from_numpy(rng.standard_normal((rows, 1, 128)).astype(np.float32) * np.exp2(rng.integers(-9, 12, (rows, 1, 1))))
+    q = q.to(DT[dtype]).cuda()
+    a, r = _lib.Stage1Args(), _lib.RotateArgs()
+    out = torch.full((rows, 1, 128), np.nan, device="cuda")
+    mid = torch.empty(rows, 1, 1, 129, device="cuda")
+    dev = [torch.from_numpy(x).cuda() for x in (cache, table, lens)] + [cuda(c), cuda(R)]
+    a.q_rot = r.q_rot = out.data_ptr()
+    a.q_stride_b = a.q_stride_h = r.out_stride_b = r.out_stride_h = 128
+    a.kv_cache, a.block_table, a.seq_lens, a.centroids, r.rotation = (x.data_ptr() for x in dev)
+    a.cache_stride_block, a.num_blocks = dev[0].stride(0), dev[0].shape[0]
+    a.block_table_stride = a.max_blocks_per_seq = table.shape[1]
+    a.n_centroids, a.mid_o, a.mid_stride_b, a.mid_stride_h, a.mid_stride_s = 16, mid.data_ptr(), 129, 129, 129
+    a.batch, a.num_q_heads, a.num_kv_heads, a.head_dim, a.block_size, a.num_splits = rows, 1, 1, 128, 16, 1
+    r.query, r.q_stride_b, r.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
+    r.query_dtype = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[q.dtype]
+    r.batch, r.num_q_heads, r.head_dim = rows, 1, 128
+    _lib.check(_lib.load().tqb_stage1_range(a, r, _lib.RangeArgs(0, 0, 0, 16), torch.cuda.current_stream().cuda_stream))
+    x = q.double().cpu().numpy()
+    tol = 2.0 ** -17 * np.linalg.norm(x, axis=-1, keepdims=True)
+    assert (np.abs(out.cpu().numpy() - x @ npy(R).astype(np.float64)) <= tol).all()
 
 
 def run_prefix(layout, dtype, own, prefix, hq, hk, *, seed=0, sinks=False, raw=True, short=(), scale_q=1.5, **kw):

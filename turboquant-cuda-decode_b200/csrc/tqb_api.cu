@@ -253,6 +253,18 @@ static int rotated_check(const tqb_rotate_args* r, const tqb_stage1_args* a) {
                 TQB_ERR_ALIGNMENT, "query must be aligned to its element size, rotation to 16 bytes");
     return TQB_OK;
 }
+static void rotate_params(const tqb_rotate_args* a, tqb::RotateParams& p) {
+    p.q = a->query;
+    p.dtype = a->query_dtype;
+    p.qsb = a->q_stride_b;
+    p.qsh = a->q_stride_h;
+    p.rot = a->rotation;
+    p.out = a->q_rot;
+    p.osb = a->out_stride_b;
+    p.osh = a->out_stride_h;
+    p.B = a->batch;
+    p.Hq = a->num_q_heads;
+}
 // One kernel where the page ring runs with a group of at most 4 query
 // heads per KV head (its rotation prologue stages the 64 KB rotation in
 // a ring it has not started yet); otherwise the rotation kernel, then
@@ -528,16 +540,7 @@ int tqb_rotate_query(const tqb_rotate_args* a, cudaStream_t stream) {
     DeviceGuard guard(a->q_rot);
     TQB_REQUIRE(guard.ok, TQB_ERR_CUDA, "cannot select the device owning q_rot");
     tqb::RotateParams p{};
-    p.q = a->query;
-    p.dtype = a->query_dtype;
-    p.qsb = a->q_stride_b;
-    p.qsh = a->q_stride_h;
-    p.rot = a->rotation;
-    p.out = a->q_rot;
-    p.osb = a->out_stride_b;
-    p.osh = a->out_stride_h;
-    p.B = a->batch;
-    p.Hq = a->num_q_heads;
+    rotate_params(a, p);
     return tqb::launch_rotate(p, stream);
 }
 
@@ -620,8 +623,11 @@ static int range_check(const tqb_range* r, int num_splits, tqb::KeyRange& k) {
     TQB_REQUIRE(r != nullptr, TQB_ERR_INVALID_ARG, "range is NULL");
     TQB_REQUIRE(r->window >= 0 && r->first_tokens >= 0 && r->prefix_len >= 0 && r->max_seq_len > 0,
                 TQB_ERR_INVALID_ARG, "window, first_tokens, prefix_len must be >= 0 and max_seq_len > 0");
-    TQB_REQUIRE(r->first_tokens == 0 || (r->prefix_len == 0 && num_splits >= 2), TQB_ERR_INVALID_ARG,
-                "first_tokens needs prefix_len 0 and a split of its own (two splits or more)");
+    TQB_REQUIRE(r->first_tokens == 0 || r->prefix_len == 0, TQB_ERR_INVALID_ARG, "first_tokens needs prefix_len 0");
+    TQB_REQUIRE(r->prefix_len % tqb::kBlockSize == 0, TQB_ERR_INVALID_ARG, "prefix_len must be a multiple of 16");
+    // the split rule adds the split count to a run of at most max_seq_len + 16 tokens
+    TQB_REQUIRE((int64_t)r->max_seq_len + 16 + num_splits < (int64_t(1) << 31), TQB_ERR_UNSUPPORTED,
+                "max_seq_len plus the split count must be below 2^31");
     k.window = r->window;
     k.first = r->first_tokens;
     k.prefix = r->prefix_len;
@@ -649,17 +655,11 @@ int tqb_stage1_range(const tqb_stage1_args* a, const tqb_rotate_args* r, const t
     const int nsm = sm_count();
     TQB_REQUIRE(nsm > 0, TQB_ERR_CUDA, "cannot query the current CUDA device");
     if (r != nullptr) {
-        // One kernel where the page ring serves the cache, as in
-        // tqb_stage1_rotated.
-        if (rotation_fuses(p)) {
-            tqb::Stage1Params pr = p;
-            fuse_rotation(pr, r);
-            rc = tqb::launch_stage1_ring_range(pr, stream, nsm);
-            if (rc != TQB_ERR_UNSUPPORTED) return rc;
-            g_detail[0] = '\0';
-        }
-        rc = tqb_rotate_query(r, stream);
+        tqb::RotateParams rp{};
+        rotate_params(r, rp);
+        rc = tqb::launch_rotate_beside(rp, stream);
         if (rc != TQB_OK) return rc;
+        p.after_rotation = 1;
     }
     return tqb::launch_stage1_range(p, stream, nsm);
 }

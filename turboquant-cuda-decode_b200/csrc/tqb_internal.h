@@ -58,21 +58,43 @@ struct FastDiv {
 #endif
 };
 
-// The tokens of a sequence that a ranged Stage1 attends to (tqb_range): the
-// last `window` of them (0: all) from `prefix` on, and the first `first` ones
-// before the window, which are split 0 on their own; splits `off` .. S - 1
-// then share the tokens [lo, L) equally.
+// The tokens of a sequence that a ranged call attends to (tqb_range): the last
+// `window` of them (0: all) from `prefix` on, and the first `first` ones.
+// Stage1 and Stage2 see them as one run of tokens: the first tokens' pages,
+// then the window's pages, each whole.  Run token v is token v + 16 * (v / 16
+// >= fp ? shift : 0) of the sequence, and the tokens in [hole0, hole1) of the
+// run (behind the first ones in their last page, before the window in its
+// first) are masked.
+struct KeyRun {
+    int len;           // tokens of the run, masked ones included
+    int hole0, hole1;
+    int fp, shift;     // pages
+};
 struct KeyRange {
     int first, window, prefix;
     int max_len;  // longer sequences are cut there (Stage1 and Stage2 alike)
 #ifdef __CUDACC__
-    __device__ __forceinline__ int len(int L) const { return min(L, max_len); }
-    __device__ __forceinline__ int off() const { return first > 0 ? 1 : 0; }  // splits before the window's
-    __device__ __forceinline__ int lo(int L) const {
-        const int w = window > 0 ? max(L - window, 0) : 0;
-        return min(max(w, prefix), max(L, 0));
+    __device__ __forceinline__ KeyRun run(int seq_len) const {
+        const int L = max(min(seq_len, max_len), 0);
+        const int lo = min(max(window > 0 ? L - window : 0, prefix), L);
+        int nf = min(first, lo);
+        const int start = nf < lo ? lo : 0;  // nothing hidden: the whole sequence
+        nf = nf < lo ? nf : 0;
+        const int lo16 = start & ~15, nf16 = (nf + 15) & ~15;
+        KeyRun r;
+        r.hole0 = nf;
+        if (nf16 > lo16) {  // one page holds the last first token and the window's first
+            r.fp = r.shift = 0;
+            r.hole1 = start;
+            r.len = L;
+        } else {
+            r.fp = nf16 >> 4;
+            r.shift = (lo16 - nf16) >> 4;
+            r.hole1 = nf16 + start - lo16;
+            r.len = nf16 + L - lo16;
+        }
+        return r;
     }
-    __device__ __forceinline__ int firsts(int lo_) const { return min(first, lo_); }
 #endif
 };
 
@@ -104,6 +126,9 @@ struct Stage1Params {
     int64_t rqsb, rqsh;
     const float* rot;  // [D, D] row-major
     float* q_out;
+    // The kernel before on the stream is this library's rotation (launched
+    // after everything before it had ended): only q_rot needs to be waited for.
+    int after_rotation;
 };
 
 struct Stage2Params {
@@ -259,6 +284,9 @@ int launch_stage2(const Stage2Params& p, cudaStream_t stream);
 int launch_merge(const MergeParams& p, cudaStream_t stream);
 int launch_fold_sinks(const SinkParams& p, cudaStream_t stream);
 int launch_rotate(const RotateParams& p, cudaStream_t stream);
+// The same product (fp32 accuracy) from a kernel without shared memory, which
+// lets the next launch_pdl kernel start beside it.
+int launch_rotate_beside(const RotateParams& p, cudaStream_t stream);
 int64_t p2p_buffer_bytes(int world, int64_t cap_rows);
 int launch_sp_exchange(const SpExchangeParams& p, cudaStream_t stream);
 int launch_sp_merge(const SpMergeParams& p, cudaStream_t stream);

@@ -29,23 +29,16 @@ __device__ __forceinline__ void merge_row(const Stage2Params& P, int b, int h, f
     __shared__ float s_acc[kParts][kHeadDim];
     __shared__ float s_max[kParts], s_sum[kParts];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nsp = P.nsplits ? min(__ldg(P.nsplits + b), P.S) : P.S;
-    const int L = __ldg(P.seq_lens + b);
+    // ranged: the splits after the lead ones share the run's tokens, and the
+    // lead ones count as valid
+    const int lead = RG ? P.lead : 0;
+    const int nsp = RG ? P.S - lead : P.nsplits ? min(__ldg(P.nsplits + b), P.S) : P.S;
+    const int seq_len = __ldg(P.seq_lens + b);
+    const int L = RG ? P.range.run(seq_len).len : seq_len;
     const int split_len = nsp > 0 ? (L + nsp - 1) / nsp : 0;
     // split s is non-empty iff split_len * s < L (its end is min(.., L))
     int nvalid = split_len > 0 ? min(nsp, (L + split_len - 1) / split_len) : 0;
-    // ranged: valid split i is split i, or i + skip from the lead splits on
-    // (the split of the first tokens is empty unless the window starts after
-    // token 0)
-    int skip = 0;
-    if constexpr (RG) {
-        const int Lr = P.range.len(L);
-        const int lo = P.range.lo(Lr), off = P.range.off(), n = Lr - lo, per = P.S - P.lead - off;
-        const int sl = (n + per - 1) / per;
-        const int has_first = P.range.firsts(lo) > 0 ? 1 : 0;
-        nvalid = L > 0 ? P.lead + has_first + (sl > 0 ? (n + sl - 1) / sl : 0) : 0;
-        skip = off - has_first;
-    }
+    if (RG) nvalid = seq_len > 0 ? nvalid + lead : 0;
     const float* row0 = P.mid + (int64_t)b * P.msb + (int64_t)h * P.msh;
 
     float m = -INFINITY, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -54,7 +47,7 @@ __device__ __forceinline__ void merge_row(const Stage2Params& P, int b, int h, f
 #pragma unroll
         for (int k = 0; k < kSplitsPerPass; k++) {
             const int s = s0 + kParts * k;
-            const float* row = row0 + (int64_t)(RG && s >= P.lead ? s + skip : s) * P.mss;
+            const float* row = row0 + (int64_t)s * P.mss;
             ls[k] = s < nvalid ? __ldg(row + kHeadDim) : -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; j++) os[k][j] = s < nvalid ? __ldg(row + lane + 32 * j) : 0.0f;

@@ -86,6 +86,79 @@ __global__ void __launch_bounds__(kRotThreads) rotate_kernel(const RotateParams 
     }
 }
 
+// The same product on the tensor cores from registers alone (no shared
+// memory), so that a kernel that needs a whole SM's can start beside it.  A
+// warp takes 16 rows and 32 output dims; every operand is split into bf16
+// parts of 8 bits (R into three, the rows into as many as their type holds),
+// which keep fp32's range, and the products that matter are summed in fp32:
+// dropped terms are 2^-24 of the row and column lengths.  2048 rows are 512
+// warps; R's fragments are read from L2, 16 loads in flight each step.
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Part p of a pair of numbers, which keep the rest.
+__device__ __forceinline__ uint32_t take_bf16(float& x, float& y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    x -= __low2float(h);
+    y -= __high2float(h);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kHeadDim) rotate_beside_kernel(const RotateParams P) {
+    constexpr int kParts = sizeof(T) == 4 ? 3 : __is_same(T, __half) ? 2 : 1;  // 24, 11 and 8 bits
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, n0 = 32 * (threadIdx.x >> 5);
+    const int64_t rows = (int64_t)P.B * P.Hq, r0 = (int64_t)blockIdx.x * 16;
+    const T* x[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int64_t r = min(r0 + g + 8 * i, rows - 1), b = r / P.Hq, h = r - b * P.Hq;
+        x[i] = static_cast<const T*>(P.q) + b * P.qsb + h * P.qsh + 2 * c;
+    }
+    const float* R = P.rot + 2 * c * kHeadDim + n0 + g;
+    float acc[4][4] = {};
+#pragma unroll
+    for (int k = 0; k < kHeadDim; k += 16) {
+        float bv[4][4], av[8];
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                bv[n][i] = __ldg(R + (k + (i & 1) + 8 * (i >> 1)) * kHeadDim + 8 * n);
+#pragma unroll
+        for (int i = 0; i < 8; i++) av[i] = to_f32<T>(x[(i >> 1) & 1][k + (i & 1) + 8 * (i >> 2)]);
+        uint32_t a[kParts][4];
+#pragma unroll
+        for (int p = 0; p < kParts; p++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[p][i] = take_bf16(av[2 * i], av[2 * i + 1]);
+#pragma unroll
+        for (int q = 0; q < 3; q++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const uint32_t b0 = take_bf16(bv[n][0], bv[n][1]), b1 = take_bf16(bv[n][2], bv[n][3]);
+#pragma unroll
+                for (int p = 0; p < kParts; p++)
+                    if (p + q < 3 || kParts == 2) mma_bf16(acc[n], a[p], b0, b1);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if (r0 + g + 8 * i >= rows) continue;
+        const int64_t r = r0 + g + 8 * i, b = r / P.Hq, h = r - b * P.Hq;
+        float* out = P.out + b * P.osb + h * P.osh + n0 + 2 * c;
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            out[8 * n] = acc[n][2 * i];
+            out[8 * n + 1] = acc[n][2 * i + 1];
+        }
+    }
+}
+
 }  // namespace
 
 template <typename T>
@@ -112,6 +185,23 @@ int launch_rotate(const RotateParams& P, cudaStream_t stream) {
         case TQB_DTYPE_F32: return launch_rotate_t<float>(P, grid, stream);
         case TQB_DTYPE_F16: return launch_rotate_t<__half>(P, grid, stream);
         case TQB_DTYPE_BF16: return launch_rotate_t<__nv_bfloat16>(P, grid, stream);
+        default: return TQB_ERR_INVALID_ARG;
+    }
+}
+
+template <typename T>
+static int launch_rotate_beside_t(const RotateParams& P, cudaStream_t stream) {
+    const int64_t rows = (int64_t)P.B * P.Hq;
+    rotate_beside_kernel<T><<<(unsigned)((rows + 15) / 16), kHeadDim, 0, stream>>>(P);
+    return report_launch(cudaGetLastError());
+}
+
+int launch_rotate_beside(const RotateParams& P, cudaStream_t stream) {
+    if (P.B == 0) return TQB_OK;
+    switch (P.dtype) {
+        case TQB_DTYPE_F32: return launch_rotate_beside_t<float>(P, stream);
+        case TQB_DTYPE_F16: return launch_rotate_beside_t<__half>(P, stream);
+        case TQB_DTYPE_BF16: return launch_rotate_beside_t<__nv_bfloat16>(P, stream);
         default: return TQB_ERR_INVALID_ARG;
     }
 }

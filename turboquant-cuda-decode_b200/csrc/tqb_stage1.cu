@@ -295,12 +295,12 @@ __device__ __forceinline__ uint2 lut_v2(const uint8_t* lut, uint32_t off) {
 }
 
 // One 16-token page of one work item.
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG>
 __device__ __forceinline__ void process_page(ItemState<NT>& st, const PageRegs& cur, bool page_ok,
-                                             int tok0, int start, int end, const uint8_t* lut,
+                                             int tok0, int start, int end, int hole0, uint32_t hole, const uint8_t* lut,
                                              uint32_t lut_base, uint32_t lut_sel_src, int g, int c) {
-    const bool va = page_ok && tok0 >= start && tok0 < end;
-    const bool vb = page_ok && tok0 + 1 >= start && tok0 + 1 < end;
+    const bool va = page_ok && tok0 >= start && tok0 < end && (!RG || (uint32_t)(tok0 - hole0) >= hole);
+    const bool vb = page_ok && tok0 + 1 >= start && tok0 + 1 < end && (!RG || (uint32_t)(tok0 + 1 - hole0) >= hole);
 
     // -- Q.K on the tensor cores --
     // Two M tiles per page: tile 0 = tokens 2g (even), tile 1 = tokens 2g+1.
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
     float* stage = stage_all + warp * (NT * 4 * (kHeadDim + 1));
 
     // Work item -> (b, s, kvh) and its token range; false for an empty split.
-    struct ItemRange { int b, s, kvh, start, end; };
+    struct ItemRange { int b, s, kvh, start, end; KeyRun run; };
     auto decode_item = [&](uint32_t item, ItemRange& r) {
         const uint32_t rest = P.div_hk.div(item);
         r.kvh = (int)(item - rest * (uint32_t)P.Hk);
@@ -544,16 +544,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
         r.s = (int)(rest - bq * (uint32_t)P.S);
         r.b = (int)bq;
         if constexpr (RG) {
-            const int L = P.range.len(__ldg(P.seq_lens + r.b));
-            const int lo = P.range.lo(L), off = P.range.off();
-            r.start = 0;
-            if (r.s < off) {  // the first tokens
-                r.end = P.range.firsts(lo);
-            } else {
-                const int split_len = (L - lo + P.S - off - 1) / (P.S - off);
-                r.start = lo + split_len * (r.s - off);
-                r.end = min(r.start + split_len, L);
-            }
+            r.run = P.range.run(__ldg(P.seq_lens + r.b));
+            const int per = (int)P.div_s.div((uint32_t)(r.run.len + P.S - 1));
+            r.start = per * r.s;
+            r.end = min(r.start + per, r.run.len);
             return r.start < r.end;
         }
         const int nsp = P.nsplits ? min(__ldg(P.nsplits + r.b), P.S) : P.S;
@@ -572,6 +566,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
         ItemRange ir;
         if (!decode_item(item, ir)) continue;  // empty split: left unwritten
         const int b = ir.b, s = ir.s, kvh = ir.kvh, start = ir.start, end = ir.end;
+        const int hole0 = RG ? ir.run.hole0 : 0;  // ranged: the run's masked tokens
+        const uint32_t hole = RG ? (uint32_t)(ir.run.hole1 - ir.run.hole0) : 0u;
+        // ranged: page p of the run is page p (+ shift from fp on)
+        auto entry = [&](int p) { return RG ? p + (p >= ir.run.fp ? ir.run.shift : 0) : p; };
         // Ask L2 for the first two pages of this warp's next item now, so
         // the item boundary does not stall on DRAM.
         {
@@ -580,7 +578,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
             if (nitem < (uint32_t)P.num_items && decode_item(nitem, nx)) {
                 const int np0 = nx.start / kBlockSize, np1 = min(np0 + 1, (nx.end - 1) / kBlockSize);
                 const int32_t* nrow = P.bt + (int64_t)nx.b * P.bt_stride;
-                const int id0 = __ldg(nrow + np0), id1 = __ldg(nrow + np1);
+                auto nentry = [&](int p) { return RG ? p + (p >= nx.run.fp ? nx.run.shift : 0) : p; };
+                const int id0 = __ldg(nrow + nentry(np0)), id1 = __ldg(nrow + nentry(np1));
                 const uint32_t bb = (uint32_t)P.block_bytes;
                 const bool nlead = lane == 0 && nx.kvh == 0 &&
                                    ((reinterpret_cast<uintptr_t>(P.cache) | bb) & 15) == 0;
@@ -604,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
         // Block ids of pages [w0, w0 + 32), one per lane; an id outside
         // [0, num_blocks) masks its page, whose loads then read block 0.
         int w0 = p_first;
-        int blk_reg = (p_first + lane <= p_last) ? __ldg(bt_row + p_first + lane) : 0;
+        int blk_reg = (p_first + lane <= p_last) ? __ldg(bt_row + entry(p_first + lane)) : 0;
         auto valid_blk = [&](int id) { return (uint32_t)id < nblocks; };
         auto blk_of = [&](int pp) { return __shfl_sync(0xffffffffu, blk_reg, pp - w0); };
         auto block_ptr = [&](int id) {
@@ -674,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
         auto stage_page = [&](PageRegs& r, bool& ok, int pp) {
             if (pp + kPrefetchPages - w0 >= 32) {  // refill the block-id window
                 w0 = pp;
-                blk_reg = (pp + lane <= p_last) ? __ldg(bt_row + pp + lane) : 0;
+                blk_reg = (pp + lane <= p_last) ? __ldg(bt_row + entry(pp + lane)) : 0;
             }
             const int id = blk_of(pp);
             ok = valid_blk(id);
@@ -684,11 +683,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kMinBlocksNT1 : 1)
         };
         for (int p = p_first; p <= p_last; p += 2) {
             if (p + 1 <= p_last) stage_page(rb, ok_b, p + 1);
-            process_page<NT, LAYOUT>(st, ra, ok_a, p * kBlockSize + 2 * g, start, end, smem, lut_base,
+            process_page<NT, LAYOUT, RG>(st, ra, ok_a, p * kBlockSize + 2 * g, start, end, hole0, hole, smem, lut_base,
                                      lut_sel_src, g, c);
             if (p + 1 > p_last) break;
             if (p + 2 <= p_last) stage_page(ra, ok_a, p + 2);
-            process_page<NT, LAYOUT>(st, rb, ok_b, (p + 1) * kBlockSize + 2 * g, start, end, smem, lut_base,
+            process_page<NT, LAYOUT, RG>(st, rb, ok_b, (p + 1) * kBlockSize + 2 * g, start, end, hole0, hole, smem, lut_base,
                                      lut_sel_src, g, c);
         }
 

@@ -308,10 +308,11 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
 // the item does not exist or its split is empty (left unwritten).
 struct ItemInfo {
     int b, s, kvh, start, end;
+    KeyRun run;  // ranged calls: start and end count the run's tokens
 };
 template <bool RG>
 __device__ __forceinline__ bool decode_item(const Stage1Params& P, uint32_t item, ItemInfo& r) {
-    r.b = r.s = r.kvh = r.start = r.end = 0;
+    r = ItemInfo{};
     if (item >= (uint32_t)P.num_items) return false;
     const uint32_t rest = P.div_hk.div(item);
     r.kvh = (int)(item - rest * (uint32_t)P.Hk);
@@ -319,15 +320,10 @@ __device__ __forceinline__ bool decode_item(const Stage1Params& P, uint32_t item
     r.s = (int)(rest - bq * (uint32_t)P.S);
     r.b = (int)bq;
     if constexpr (RG) {
-        const int L = P.range.len(__ldg(P.seq_lens + r.b));
-        const int lo = P.range.lo(L), off = P.range.off();
-        if (r.s < off) {  // the first tokens
-            r.end = P.range.firsts(lo);
-        } else {
-            const int split_len = (L - lo + P.S - off - 1) / (P.S - off);
-            r.start = lo + split_len * (r.s - off);
-            r.end = min(r.start + split_len, L);
-        }
+        r.run = P.range.run(__ldg(P.seq_lens + r.b));
+        const int per = (int)P.div_s.div((uint32_t)(r.run.len + P.S - 1));
+        r.start = per * r.s;
+        r.end = min(r.start + per, r.run.len);
         return r.start < r.end;
     }
     const int nsp = P.nsplits ? min(__ldg(P.nsplits + r.b), P.S) : P.S;
@@ -349,7 +345,7 @@ __device__ __forceinline__ int tile_items(const Stage1Params& P, uint32_t t, int
     if (lane < kGroupWarps && decode_item<RG>(P, t * kGroupWarps + lane, ir))
         np = (ir.end - 1) / kBlockSize - ir.start / kBlockSize + 1;
     else
-        ir.b = ir.s = ir.kvh = ir.start = ir.end = 0;
+        ir = ItemInfo{};
     int m = np;
 #pragma unroll
     for (int o = 1; o < kGroupWarps; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -369,25 +365,14 @@ __device__ __forceinline__ int tile_items(const Stage1Params& P, uint32_t t, int
 // splits weigh nothing either way.  Every CTA derives the same cut from
 // seq_lens (and nsplits), so no state is shared between CTAs or launches.
 // ---------------------------------------------------------------------------
-// A ranged call adds the split of the first tokens in front: nf tokens, and
-// `base` the index of the first of the ne splits after it.
 struct SeqSplit {
     int L, sl, ne;  // clamped length, split length, non-empty splits
-    int nf, base;
 };
 template <bool RG>
 __device__ __forceinline__ SeqSplit seq_split_of(const Stage1Params& P, int len, int nsplit) {
-    SeqSplit r{0, 1, 0, 0, 0};
-    int nsp = min(nsplit, P.S);
-    int L = min(len, P.max_blocks * kBlockSize);
-    if constexpr (RG) {
-        L = P.range.len(len);
-        const int lo = P.range.lo(L);
-        r.base = P.range.off();
-        r.nf = P.range.firsts(lo);
-        nsp = P.S - r.base;
-        L -= lo;
-    }
+    SeqSplit r{0, 1, 0};
+    const int nsp = min(nsplit, P.S);
+    const int L = RG ? P.range.run(len).len : min(len, P.max_blocks * kBlockSize);
     if (nsp <= 0 || L <= 0) return r;
     r.L = L;
     r.sl = (L + nsp - 1) / nsp;  // ceil(L / nsp), the split rule of decode_item
@@ -401,10 +386,6 @@ __device__ __forceinline__ SeqSplit seq_split(const Stage1Params& P, int b) {
 __device__ __forceinline__ long long seq_weight(const Stage1Params& P, const SeqSplit& q, bool by_count) {
     return by_count ? (long long)P.Hk * q.ne : (long long)P.Hk * ((long long)q.L + (long long)kSplitCost * q.ne);
 }
-// Weight of the split of the first tokens, per KV head (0: none).
-__device__ __forceinline__ long long first_weight(const SeqSplit& q, bool by_count) {
-    return q.nf <= 0 ? 0 : by_count ? 1 : (long long)(q.nf + kSplitCost);
-}
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -413,24 +394,15 @@ __device__ __forceinline__ long long warp_sum_ll(long long v) {
 // Tile of the first item of sequence b whose start weight reaches r (>= 1,
 // at most the sequence's weight): split s* = the last split starting below
 // r, then the KV head in it.
-template <bool RG>
 __device__ __forceinline__ uint32_t cut_tile(const Stage1Params& P, const SeqSplit& q, int b, long long r,
                                              uint32_t num_tiles, bool by_count) {
-    if constexpr (RG) {
-        const long long fw = first_weight(q, by_count);
-        if (r <= fw * P.Hk) {
-            const long long item = (long long)b * P.S * P.Hk + (r + fw - 1) / fw;
-            return (uint32_t)min((long long)num_tiles, (item + kGroupWarps - 1) / kGroupWarps);
-        }
-        r -= fw * P.Hk;
-    }
     const long long unit = by_count ? (long long)P.Hk : (long long)P.Hk * (q.sl + kSplitCost);
     const long long ss = min((long long)(q.ne - 1), (r - 1) / unit);
     const long long a = unit * ss;
     const long long per =
         by_count ? 1 : (long long)(min((int)(ss + 1) * q.sl, q.L) - (int)ss * q.sl) + kSplitCost;
     const long long kv = (r - a + per - 1) / per;  // in [1, Hk]
-    const long long item = ((long long)b * P.S + ss + (RG ? q.base : 0)) * P.Hk + kv;
+    const long long item = ((long long)b * P.S + ss) * P.Hk + kv;
     return (uint32_t)min((long long)num_tiles, (item + kGroupWarps - 1) / kGroupWarps);
 }
 // Tile walk of group gi of this CTA: tiles first, first + stride, ... below
@@ -455,10 +427,6 @@ __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uin
             const SeqSplit q = seq_split_of<RG>(P, len, nsp);
             tot += seq_weight(P, q, false);
             cnt += seq_weight(P, q, true);
-            if constexpr (RG) {
-                tot += P.Hk * first_weight(q, false);
-                cnt += P.Hk * first_weight(q, true);
-            }
             lmin = min(lmin, len);
             lmax = max(lmax, len);
             nmin = min(nmin, nsp);
@@ -467,8 +435,7 @@ __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uin
     }
     tot = warp_sum_ll(tot);
     cnt = warp_sum_ll(cnt);
-    // (a ranged call with first tokens has splits of two lengths: weight cut)
-    if ((!RG || P.range.first == 0) && __reduce_min_sync(0xffffffffu, lmin) == __reduce_max_sync(0xffffffffu, lmax) &&
+    if (__reduce_min_sync(0xffffffffu, lmin) == __reduce_max_sync(0xffffffffu, lmax) &&
         __reduce_min_sync(0xffffffffu, nmin) == __reduce_max_sync(0xffffffffu, nmax)) {
         // contiguous ranges: consecutive tiles of a group are consecutive
         // splits of one sequence, so its warps keep their query fragments
@@ -495,9 +462,9 @@ __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uin
 #pragma unroll 1
             for (int b0 = 0; b0 < P.B; b0 += 32) {
                 const int b = b0 + lane;
-                SeqSplit q{0, 1, 0, 0, 0};
+                SeqSplit q{0, 1, 0};
                 if (b < P.B) q = seq_split<RG>(P, b);
-                const long long w = seq_weight(P, q, by_count) + (RG ? P.Hk * first_weight(q, by_count) : 0);
+                const long long w = seq_weight(P, q, by_count);
                 long long incl = w;
 #pragma unroll 1
                 for (int o = 1; o < 32; o <<= 1) {
@@ -508,7 +475,7 @@ __device__ void tile_walk(const Stage1Params& P, int gi, int groups_per_cta, uin
                 const bool here = w > 0 && excl < tgt && tgt <= base + incl;
                 const uint32_t m = __ballot_sync(0xffffffffu, here);
                 if (m) {
-                    const uint32_t tl = here ? cut_tile<RG>(P, q, b, tgt - excl, num_tiles, by_count) : 0u;
+                    const uint32_t tl = here ? cut_tile(P, q, b, tgt - excl, num_tiles, by_count) : 0u;
                     t = __shfl_sync(0xffffffffu, tl, __ffs(m) - 1);
                     break;
                 }
@@ -679,7 +646,7 @@ __device__ __forceinline__ void produce(const Stage1Params& P, const RingMaps& M
     ItemInfo ir;
     int np = 0, np_tile = 0;
     uint32_t t = next_tile(lds32(gs.tiles()), ir, np, np_tile);
-    if (P.rot != nullptr && pj == 0 && t < t_end) {
+    if (!RG && P.rot != nullptr && pj == 0 && t < t_end) {
         // fused rotation: the query rows are written by every CTA's prologue
         const uint32_t base = gs.bars - (uint32_t)gi * kBarStride - C::kBarOff;
         if (!rot_barrier_wait(lds32(base + C::kBarOff + 112u), lane)) abort = true;
@@ -717,15 +684,22 @@ __device__ __forceinline__ void produce(const Stage1Params& P, const RingMaps& M
         const int r_pf = __shfl_sync(0xffffffffu, ir.start, col) / kBlockSize;
         const int r_kvh = __shfl_sync(0xffffffffu, ir.kvh, col);
         const int r_nw = lane < nruns ? __ffs(emask >> col) : 0;
-        const int32_t* r_bt = P.bt + (int64_t)r_b * P.bt_stride + r_pf;
+        const int32_t* r_bt = P.bt + (int64_t)r_b * P.bt_stride + (RG ? 0 : r_pf);
+        // ranged: the run's page r_pf + k is page (.. + shift from fp on)
+        int fp = 0, shift = 0;
+        if constexpr (RG) {
+            fp = __shfl_sync(0xffffffffu, ir.run.fp, col);
+            shift = __shfl_sync(0xffffffffu, ir.run.shift, col);
+        }
+        auto entry = [&](int k) { return RG ? r_pf + k + (r_pf + k >= fp ? shift : 0) : k; };
         const int np_r = lane < nruns ? r_np : 0;
-        int next_id = np_r > 0 ? __ldg(r_bt) : 0;
+        int next_id = np_r > 0 ? __ldg(r_bt + entry(0)) : 0;
 
         // ---- pages ---------------------------------------------------------
         int slot = 0;
         for (int k = 0; k < np_tile; k++) {
             const int id = next_id;
-            next_id = k + 1 < np_r ? __ldg(r_bt + k + 1) : 0;  // lands while we wait
+            next_id = k + 1 < np_r ? __ldg(r_bt + entry(k + 1)) : 0;  // lands while we wait
             const bool here = k < np_r;
             const bool ok = (uint32_t)id < nblocks;
             const uint32_t bytes =
@@ -836,9 +810,9 @@ struct LaneSmem {
     uint32_t row;     // AoS: bytes between consecutive tokens of a page
 };
 
-template <int NT, int LAYOUT>
+template <int NT, int LAYOUT, bool RG>
 __device__ __forceinline__ void page_math(ItemState<NT>& st, const uint32_t sb, const LaneSmem& o, bool page_ok,
-                                          int tok0, int start, int end, uint32_t lut_sel_src, int g,
+                                          int tok0, int start, int end, int hole0, uint32_t hole, uint32_t lut_sel_src, int g,
                                           int c, int src_a, uint32_t release_bar, float csq_unscale) {
     // Every ring byte this lane uses is read first and the slot released, so
     // its next page is fetched while this one is computed.  The arrive has
@@ -919,8 +893,8 @@ __device__ __forceinline__ void page_math(ItemState<NT>& st, const uint32_t sb, 
         v[3] = lds64(sb + o.v1 + 8u * kDataBytes);
     }
     if constexpr (LAYOUT == TQB_LAYOUT_SOA) mbar_arrive(release_bar);
-    const bool va = page_ok && tok0 >= start && tok0 < end;
-    const bool vb = page_ok && tok0 + 1 >= start && tok0 + 1 < end;
+    const bool va = page_ok && tok0 >= start && tok0 < end && (!RG || (uint32_t)(tok0 - hole0) >= hole);
+    const bool vb = page_ok && tok0 + 1 >= start && tok0 + 1 < end && (!RG || (uint32_t)(tok0 + 1 - hole0) >= hole);
 
     // -- Q.K: M tile 0 = token tau(g) (rows g: C_hi, g+8: C_lo), tile 1 = tau(g)+1
     float dq[NT][2][4];
@@ -1171,18 +1145,18 @@ __device__ __forceinline__ void epilogue(const Stage1Params& P, const ItemState<
 
 // One page from ring slot S (a compile-time constant, so every shared and
 // barrier address below is a register plus an immediate).
-template <int NT, int LAYOUT, int S>
+template <int NT, int LAYOUT, bool RG, int S>
 __device__ __forceinline__ bool page_step(ItemState<NT>& st, const GroupSmem& gs, const LaneSmem& o, uint32_t& cbits,
                                           int k, int my_np, int w, int tok_first, int start, int end,
-                                          uint32_t lut_sel_src, int g, int c, int src_a, float csq_unscale) {
+                                          int hole0, uint32_t hole, uint32_t lut_sel_src, int g, int c, int src_a, float csq_unscale) {
     constexpr int NS = Cfg<NT, LAYOUT>::kStages;
     if (!mbar_wait(gs.full(S), (cbits >> S) & 1u)) return false;
     cbits ^= 1u << S;
     // all 32 lanes arrive on the slot's release barrier (no branch on the lane)
     if (k < my_np) {
         const bool page_ok = (lds32(gs.vmask<NS>(S)) >> w) & 1u;
-        page_math<NT, LAYOUT>(st, (uint32_t)(S * stage_bytes(LAYOUT)), o, page_ok, tok_first + k * kBlockSize, start, end,
-                      lut_sel_src, g, c, src_a, gs.empty<NS>(S), csq_unscale);
+        page_math<NT, LAYOUT, RG>(st, (uint32_t)(S * stage_bytes(LAYOUT)), o, page_ok, tok_first + k * kBlockSize, start,
+                                  end, hole0, hole, lut_sel_src, g, c, src_a, gs.empty<NS>(S), csq_unscale);
     } else {
         mbar_arrive(gs.empty<NS>(S));
     }
@@ -1286,6 +1260,12 @@ __device__ __forceinline__ void consume(const Stage1Params& P, const GroupSmem& 
         const int start = __shfl_sync(0xffffffffu, ir.start, w);
         const int end = __shfl_sync(0xffffffffu, ir.end, w);
         const int my_np = __shfl_sync(0xffffffffu, np, w);
+        int hole0 = 0;  // ranged: the run's masked tokens
+        uint32_t hole = 0;
+        if constexpr (RG) {
+            hole0 = __shfl_sync(0xffffffffu, ir.run.hole0, w);
+            hole = (uint32_t)(__shfl_sync(0xffffffffu, ir.run.hole1, w) - hole0);
+        }
 
         // ---- query fragments from the tile's query rows ---------------------
         // Every item keeps its sequence and KV head: the producer copied no
@@ -1356,12 +1336,13 @@ __device__ __forceinline__ void consume(const Stage1Params& P, const GroupSmem& 
         // ---- pages: slot S of the ring holds pages k = S (mod NS) ------------
         const int tok_first = (start / kBlockSize) * kBlockSize + tau;
         for (int k = 0; k < np_tile; k += NS) {
-            if (!page_step<NT, LAYOUT, 0>(st, gs, o, cbits, k, my_np, w, tok_first, start, end, lut_sel_src, g, c, src_a, csq_unscale))
-                return;
-            if (k + 1 < np_tile && !page_step<NT, LAYOUT, 1>(st, gs, o, cbits, k + 1, my_np, w, tok_first, start, end,
+            if (!page_step<NT, LAYOUT, RG, 0>(st, gs, o, cbits, k, my_np, w, tok_first, start, end, hole0, hole,
                                                      lut_sel_src, g, c, src_a, csq_unscale))
                 return;
-            if (k + 2 < np_tile && !page_step<NT, LAYOUT, 2>(st, gs, o, cbits, k + 2, my_np, w, tok_first, start, end,
+            if (k + 1 < np_tile && !page_step<NT, LAYOUT, RG, 1>(st, gs, o, cbits, k + 1, my_np, w, tok_first, start, end, hole0, hole,
+                                                     lut_sel_src, g, c, src_a, csq_unscale))
+                return;
+            if (k + 2 < np_tile && !page_step<NT, LAYOUT, RG, 2>(st, gs, o, cbits, k + 2, my_np, w, tok_first, start, end, hole0, hole,
                                                      lut_sel_src, g, c, src_a, csq_unscale))
                 return;
         }
@@ -1376,7 +1357,9 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_trigger();
-    pdl_wait();  // the kernel before on the stream (e.g. the previous step's Stage2 reading mid_o)
+    // the kernel before on the stream (e.g. the previous step's Stage2 reading
+    // mid_o); behind the rotation, the table and the tile walk are made first
+    if (!RG || !P.after_rotation) pdl_wait();
 
     // ---- K table: 256 entries x 32 lane copies of {C_hi pair, C_lo pair} ----
     // (FP8 keys: no table, no centroids, no scale; 3-bit keys: 8 centroids,
@@ -1405,6 +1388,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
         *reinterpret_cast<uint2*>(smem + C::kLutOff + (size_t)e * 8) = make_uint2(h2_as_u32(h), h2_as_u32(l));
         }
 
+    if (RG && P.after_rotation) pdl_wait();
     const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
     if (base != (uint32_t)kDynBase) {  // the table address above assumes this window layout
         if (tid == 0) atomicAdd(&g_wait_timeouts, 1u);
@@ -1440,7 +1424,7 @@ __global__ void __launch_bounds__(Cfg<NT>::kThreads, 1)
     }
     __syncthreads();
 
-    if constexpr (NT == 1 && C::kTable) {  // the fused rotation (not for FP8 keys)
+    if constexpr (NT == 1 && C::kTable && !RG) {  // the fused rotation (not for FP8 keys)
         if (P.rot != nullptr) {
             rotate_share<NT>(P, smem, tid);
             // generic writes to the ring and query areas, before the tensor

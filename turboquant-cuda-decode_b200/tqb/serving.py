@@ -232,9 +232,18 @@ def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, centroids: Opt
 
 
 def _splits(items: int, tokens: int) -> int:
-    """Splits of ``tokens`` for ``items`` (sequence, KV head) pairs: enough items for one round of the Stage1 grid, none
-    under ``_SPLIT_TOKENS`` tokens."""
-    return max(1, min(-(-_SPLIT_ITEMS // max(items, 1)), -(-tokens // _SPLIT_TOKENS)))
+    """Splits of ``tokens`` for ``items`` (sequence, KV head) pairs.  Stage1 walks tiles of 8 items with 296 groups of
+    warps, so a split count that just exceeds a whole round of the groups costs another round: of the counts that fill
+    one to four rounds, the one with the least time, a round taking its split's tokens and the start and end of a tile
+    (about 48 tokens' time); splits stay above ``_SPLIT_TOKENS`` tokens."""
+    most = max(1, -(-tokens // _SPLIT_TOKENS))
+    best = (float("inf"), 1)
+    for rounds in (1, 2, 3, 4):
+        s = min(most, _SPLIT_ITEMS * rounds // items)
+        if s:
+            used = -(-items * s // _SPLIT_ITEMS)
+            best = min(best, (used * (-(-tokens // s) + 48), s))
+    return best[1]
 
 
 class _Step:
@@ -376,10 +385,8 @@ def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     visible tokens are read.  A sequence of length 0 gets NaN and an LSE of -inf, as in ``stage2``.  Sequences longer
     than the block table's rows are cut there.
 
-    The first tokens are a split of their own and the window is shared by the others; ``num_splits`` counts the latter.
-    ``mid_o`` may hold the partials: float32 ``[>= B, >= Hq, >= splits, 129]``, with one split more than ``num_splits``
-    when ``first_tokens > 0``.  Calls with a ``rotation`` must not overlap in time on one device (``tqb_stage1_rotated``'s
-    rule); with ``rotation=None`` they may."""
+    ``num_splits`` splits share the pages of a sequence's visible tokens; ``mid_o`` may hold their partials: float32
+    ``[>= B, >= Hq, >= num_splits, 129]``."""
     if not isinstance(window, int) or window < 1:
         _no("window must be at least 1")
     if not isinstance(first_tokens, int) or first_tokens < 0:
@@ -392,7 +399,7 @@ def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
         return s.output
     most = s.blocks * BLOCK_SIZE
     window, first_tokens = min(window, most), min(first_tokens, most)
-    S = (num_splits or _splits(s.B * s.Hk, window)) + (1 if first_tokens else 0)
+    S = num_splits or _splits(s.B * s.Hk, min(window + first_tokens, most))
     s.workspace(S)
     return s.launch(_RANGE.pack(window, first_tokens, 0, most), 0, S, stream)
 
