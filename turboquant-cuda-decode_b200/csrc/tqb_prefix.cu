@@ -78,59 +78,79 @@ __device__ __forceinline__ uint32_t gw(const uint8_t* p) { return A2 ? g2x16(p) 
 
 // Codes and metadata of one token's 32 dims [32c, 32c + 32).
 template <int L>
-struct Raw {
-    uint32_t k[layout_fp8_keys(L) ? 8 : 4], v[4], kn, vs, vz;
+struct RawK {
+    uint32_t k[layout_fp8_keys(L) ? 8 : 4], norm;
 };
+struct RawV {
+    uint32_t v[4], scale, zero;
+};
+// Addresses of a token-head's key codes, value codes and metadata.
 template <int L>
-__device__ __forceinline__ void load_raw(Raw<L>& r, const PrefixParams& P, int id, uint32_t off, uint32_t h, uint32_t c) {
-    constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), v3 = layout_3bit_values(L), aos = layout_is_aos(L);
-    constexpr int kKey = aos_key_bytes(L), kRow = kKey + val_code_bytes(L);
-    if (id < 0) {  // no such page: zeros, and the mask hides its scores
+struct Where {
+    const uint8_t *k, *v, *norm, *scale, *zero;
+    __device__ __forceinline__ Where(const PrefixParams& P, int id, uint32_t off, uint32_t h) {
+        constexpr bool k8 = layout_fp8_keys(L);
+        constexpr int kKey = aos_key_bytes(L), kRow = kKey + val_code_bytes(L);
+        const uint8_t* base = P.cache + (size_t)(uint32_t)id * (size_t)P.block_bytes;
+        if constexpr (layout_is_aos(L)) {
+            k = base + (size_t)off * P.pos_stride + (size_t)h * P.head_stride;
+            v = k + aos_val_off(L);
+            norm = k + aos_norm_off(L);
+            scale = k + aos_scale_off(L);
+            zero = scale + 2;
+        } else {
+            constexpr uint32_t kFields = k8 ? 2 : 3;
+            k = base + off * ((uint32_t)P.Hk * kRow) + h * (uint32_t)kRow;
+            v = k + kKey;
+            norm = base + (uint32_t)kBlockSize * P.Hk * kRow + (h * kFields * kBlockSize + off) * 2;
+            scale = norm + (kFields - 2) * kBlockSize * 2;
+            zero = scale + kBlockSize * 2;
+        }
+    }
+};
+// A page that does not exist (id < 0) reads as zeros; the mask hides its scores.
+template <int L>
+__device__ __forceinline__ void load_k(RawK<L>& r, const PrefixParams& P, int id, uint32_t off, uint32_t h, uint32_t c) {
+    constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), aos = layout_is_aos(L);
+    constexpr int kWords = k8 ? 8 : k3 ? 3 : 4;
+    if (id < 0) {
 #pragma unroll
-        for (int i = 0; i < (k8 ? 8 : 4); i++) r.k[i] = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; i++) r.v[i] = 0u;
-        r.kn = r.vs = r.vz = 0u;
+        for (int i = 0; i < kWords; i++) r.k[i] = 0u;
+        r.norm = 0u;
         return;
     }
-    const uint8_t* base = P.cache + (size_t)(uint32_t)id * (size_t)P.block_bytes;
-    const uint8_t* kp;
-    const uint8_t* vp;
-    if constexpr (aos) {
-        const uint8_t* sp = base + (size_t)off * P.pos_stride + (size_t)h * P.head_stride;
-        kp = sp + (k8 ? 32 : k3 ? 12 : 16) * c;
-        vp = sp + aos_val_off(L) + (v3 ? 12 : 16) * c;
-        r.kn = k8 ? 0u : g16(sp + aos_norm_off(L));
-        r.vs = g16(sp + aos_scale_off(L));
-        r.vz = g16(sp + aos_scale_off(L) + 2);
-    } else {
-        const uint8_t* row = base + off * ((uint32_t)P.Hk * kRow) + h * (uint32_t)kRow;
-        kp = row + (k8 ? 32 : k3 ? 12 : 16) * c;
-        vp = row + kKey + (v3 ? 12 : 16) * c;
-        constexpr uint32_t kFields = k8 ? 2 : 3;
-        const uint8_t* meta = base + (uint32_t)kBlockSize * P.Hk * kRow + (h * kFields * kBlockSize + off) * 2;
-        r.kn = k8 ? 0u : g16(meta);
-        r.vs = g16(meta + (kFields - 2) * kBlockSize * 2);
-        r.vz = g16(meta + (kFields - 1) * kBlockSize * 2);
-    }
+    const Where<L> w(P, id, off, h);
+    const uint8_t* p = w.k + 4 * kWords * c;
     if constexpr (!aos && !k3) {
-        const uint4 a = g128(kp);
-        r.k[0] = a.x; r.k[1] = a.y; r.k[2] = a.z; r.k[3] = a.w;
-        if constexpr (k8) {
-            const uint4 b = g128(kp + 16);
-            r.k[4] = b.x; r.k[5] = b.y; r.k[6] = b.z; r.k[7] = b.w;
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4) {
+            const uint4 a = g128(p + 4 * i);
+            r.k[i] = a.x; r.k[i + 1] = a.y; r.k[i + 2] = a.z; r.k[i + 3] = a.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < (k8 ? 8 : k3 ? 3 : 4); i++) r.k[i] = gw<aos>(kp + 4 * i);
+        for (int i = 0; i < kWords; i++) r.k[i] = gw<aos>(p + 4 * i);
     }
+    r.norm = k8 ? 0u : g16(w.norm);
+}
+template <int L>
+__device__ __forceinline__ void load_v(RawV& r, const PrefixParams& P, int id, uint32_t off, uint32_t h, uint32_t c) {
+    constexpr bool v3 = layout_3bit_values(L), aos = layout_is_aos(L);
+    if (id < 0) {
+        r.v[0] = r.v[1] = r.v[2] = r.v[3] = r.scale = r.zero = 0u;
+        return;
+    }
+    const Where<L> w(P, id, off, h);
+    const uint8_t* p = w.v + (v3 ? 12 : 16) * c;
     if constexpr (!aos && !v3) {
-        const uint4 a = g128(vp);
+        const uint4 a = g128(p);
         r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < (v3 ? 3 : 4); i++) r.v[i] = gw<aos>(vp + 4 * i);
+        for (int i = 0; i < (v3 ? 3 : 4); i++) r.v[i] = gw<aos>(p + 4 * i);
     }
+    r.scale = g16(w.scale);
+    r.zero = g16(w.zero);
 }
 // 3-bit codes 8i .. 8i + 7 (24 bits) of a 12-byte run.
 __device__ __forceinline__ uint32_t bits24(const uint32_t* w, int i) {
@@ -142,7 +162,7 @@ __device__ __forceinline__ uint32_t bits24(const uint32_t* w, int i) {
 
 // 32 dims of a token into the K tile: 4 16-byte chunks of its row.
 template <int L>
-__device__ __forceinline__ void put_k(uint8_t* smem, uint32_t tile, const Raw<L>& r, uint32_t tok, uint32_t c, int lane) {
+__device__ __forceinline__ void put_k(uint8_t* smem, uint32_t tile, const RawK<L>& r, uint32_t tok, uint32_t c, int lane) {
     constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), aos = layout_is_aos(L);
     uint32_t f[16];
     if constexpr (k8) {
@@ -163,7 +183,7 @@ __device__ __forceinline__ void put_k(uint8_t* smem, uint32_t tile, const Raw<L>
             }
             f[i] = *reinterpret_cast<const uint32_t*>(lut + at);
         }
-        uint32_t norm = r.kn;
+        uint32_t norm = r.norm;
         if constexpr (aos) {
             // AoS stores the raw |k|: divide by the centroids' length (the
             // token's four quarters sit 8 lanes apart)
@@ -192,12 +212,12 @@ __device__ __forceinline__ void put_k(uint8_t* smem, uint32_t tile, const Raw<L>
 // 6 3 7 (the nibble pairs that one mask of a word yields): the columns of O
 // come out in that order and are put right when they are written.
 template <int L>
-__device__ __forceinline__ void put_v(uint8_t* smem, uint32_t tile, const Raw<L>& r, uint32_t tok, uint32_t c) {
+__device__ __forceinline__ void put_v(uint8_t* smem, uint32_t tile, const RawV& r, uint32_t tok, uint32_t c) {
     constexpr bool v3 = layout_3bit_values(L);
     // a nibble in the mantissa of 1024 (bits 0-3) or of 64 (bits 4-7) adds its
     // own value to it, exactly
     const __half2 k1024 = u32_as_h2(0x64006400u), k64 = u32_as_h2(0x54005400u);
-    const __half2 s2 = u32_as_h2(dup16(r.vs)), z2 = u32_as_h2(dup16(r.vz));
+    const __half2 s2 = u32_as_h2(dup16(r.scale)), z2 = u32_as_h2(dup16(r.zero));
     uint8_t* row = smem + tile + (c >> 1) * kHalf + tok * 128;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -234,21 +254,28 @@ __device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W
         const int id = __ldg(P.pages + pg);
         return id >= 0 && id < nblocks ? id : -1;
     };
-    Raw<L> raw[4];
+    // The codes of the next tile are in flight while this one is unpacked.
+    RawK<L> rk[4];
+    RawV rv[4];
     int ids[4], next[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) ids[i] = page_id(0, i);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        load_raw<L>(raw[i], P, ids[i], off, W.h, c);
+        load_k<L>(rk[i], P, ids[i], off, W.h, c);
         next[i] = page_id(1, i);
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) load_v<L>(rv[i], P, ids[i], off, W.h, c);
     for (int j = 0; j < W.n; j++) {
         const int s = j & 1;
         const uint32_t phase = ((j >> 1) & 1) ^ 1;
         if (!__all_sync(0xffffffffu, bar_wait(bars + kKEmpty + 8 * s, phase, abort))) return;
 #pragma unroll
-        for (int i = 0; i < 4; i++) put_k<L>(smem, kKOff + s * kOperand, raw[i], 32 * i + 8 * pw + t8, c, lane);
+        for (int i = 0; i < 4; i++) {
+            put_k<L>(smem, kKOff + s * kOperand, rk[i], 32 * i + 8 * pw + t8, c, lane);
+            load_k<L>(rk[i], P, next[i], off, W.h, c);
+        }
         // pages of this tile that exist, a bit each (warps 0 and 2 own four)
         if ((pw & 1) == 0 && lane == 0) {
             uint32_t m = 0;
@@ -261,9 +288,9 @@ __device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W
         if (!__all_sync(0xffffffffu, bar_wait(bars + kVEmpty + 8 * s, phase, abort))) return;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            put_v<L>(smem, kVOff + s * kOperand, raw[i], 32 * i + 8 * pw + t8, c);
+            put_v<L>(smem, kVOff + s * kOperand, rv[i], 32 * i + 8 * pw + t8, c);
             ids[i] = next[i];
-            load_raw<L>(raw[i], P, ids[i], off, W.h, c);
+            load_v<L>(rv[i], P, ids[i], off, W.h, c);
             next[i] = page_id(j + 2, i);
         }
         fence_async_smem();
@@ -318,55 +345,89 @@ __device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t ba
     bar_wait(bars + kDone, 0, abort);
 }
 
-// One pass over a tile's scores of this thread's row: p = exp2(s kfac - ref)
-// as fp16 pairs, their sum, and the largest exponent.
+// Running reference, sum and products of a row.
+struct RowState {
+    float ref, l;
+};
+
+// Moves the reference of the rows whose exponents exceed it by more than
+// kSlack (or that see their first token), and scales what they have summed so
+// far: l, O, and the weights of this tile's first q quarters.  Rare.
+__device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32_t ts, uint32_t to, int q, bool has_o) {
+    const float f = over && st.ref != -INFINITY ? ex2_approx(-top) : 1.0f;
+    if (over) st.ref = (st.ref == -INFINITY ? 0.0f : st.ref) + top;
+    st.l *= f;
+    const __half2 f2 = __float2half2_rn(f);
+    for (int i = 0; i < q; i++) {
+        uint32_t p[16];
+        tmem_ld16(p, ts + 16 * i);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; j++) p[j] = h2_as_u32(__hmul2(u32_as_h2(p[j]), f2));
+        tmem_st16(ts + 16 * i, p);
+    }
+    if (has_o) {
+        for (int i = 0; i < kHeadDim; i += 16) {
+            uint32_t o[16];
+            tmem_ld16(o, to + i);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            tmem_st16(to + i, o);
+        }
+    }
+    tmem_wait_st();
+    return st;
+}
+
+// The weights of a tile's tokens for this thread's row: p = exp2(s kfac - ref)
+// in place of the scores (columns 0 .. 63, two fp16 each), a quarter of the
+// tile at a time; the next quarter's scores are loaded under the
+// exponentials.
 template <bool MASK>
-__device__ __forceinline__ void weigh(uint32_t tmem_s, float kfac, float ref, int lim, uint32_t pages, uint32_t (&p)[64],
-                                      float& sum, float& top) {
-    const uint64_t k2 = pack2(kfac, kfac), r2 = pack2(-ref, -ref);
+__device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, bool has_o, float kfac, int lim,
+                                      uint32_t pages) {
+    const uint64_t k2 = pack2(kfac, kfac);
     uint64_t acc = pack2(0.0f, 0.0f);
-    float mx = -INFINITY;
+    uint32_t s[2][32];
+    tmem_ld32(s[0], ts);
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-        uint32_t s[32];
-        tmem_ld32(s, tmem_s + 32 * q);
         tmem_wait_ld();
+        const float r = st.ref == -INFINITY ? 0.0f : st.ref;
+        uint64_t r2 = pack2(-r, -r), x[16];
+        float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            const uint64_t x = fma2((uint64_t)s[2 * j] | ((uint64_t)s[2 * j + 1] << 32), k2, r2);
-            float a = lo2(x), b = hi2(x);
+            x[j] = fma2((uint64_t)s[q & 1][2 * j] | ((uint64_t)s[q & 1][2 * j + 1] << 32), k2, r2);
             if constexpr (MASK) {
                 const int t = 32 * q + 2 * j;
-                a = t < lim && (pages >> (t >> 4)) & 1u ? a : -INFINITY;
-                b = t + 1 < lim && (pages >> (t >> 4)) & 1u ? b : -INFINITY;
+                const bool page = (pages >> (t >> 4)) & 1u;
+                x[j] = pack2(page && t < lim ? lo2(x[j]) : -INFINITY, page && t + 1 < lim ? hi2(x[j]) : -INFINITY);
             }
-            mx = fmaxf(mx, fmaxf(a, b));
-            a = ex2_approx(a);
-            b = ex2_approx(b);
-            acc = add2(acc, pack2(a, b));
-            p[16 * q + j] = h2_as_u32(__floats2half2_rn(a, b));
+            top = fmaxf(top, fmaxf(lo2(x[j]), hi2(x[j])));
         }
-    }
-    sum = lo2(acc) + hi2(acc);
-    top = mx;
-}
-// The largest score of the row (before kfac).
-template <bool MASK>
-__device__ __forceinline__ float largest(uint32_t tmem_s, int lim, uint32_t pages) {
-    float mx = -INFINITY;
-#pragma unroll 1
-    for (int q = 0; q < 4; q++) {
-        uint32_t s[32];
-        tmem_ld32(s, tmem_s + 32 * q);
-        tmem_wait_ld();
+        const bool over = top < INFINITY && (top > kSlack || (st.ref == -INFINITY && top > -INFINITY));
+        if (__any_sync(0xffffffffu, over)) {
+            st.l += lo2(acc) + hi2(acc);
+            acc = pack2(0.0f, 0.0f);
+            st = raise(st, top, over, ts, to, q, has_o);
+            r2 = over ? pack2(-top, -top) : acc;
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const int t = 32 * q + j;
-            const float x = __uint_as_float(s[j]);
-            mx = fmaxf(mx, !MASK || (t < lim && (pages >> (t >> 4)) & 1u) ? x : -INFINITY);
+            for (int j = 0; j < 16; j++) x[j] = add2(x[j], r2);
         }
+        if (q < 3) tmem_ld32(s[(q + 1) & 1], ts + 32 * (q + 1));
+        uint32_t p[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float a = ex2_approx(lo2(x[j])), b = ex2_approx(hi2(x[j]));
+            acc = add2(acc, pack2(a, b));
+            p[j] = h2_as_u32(__floats2half2_rn(a, b));
+        }
+        tmem_st16(ts + 16 * q, p);
     }
-    return mx;
+    st.l += lo2(acc) + hi2(acc);
+    tmem_wait_st();
 }
 
 __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, uint8_t* smem, uint32_t bars, uint32_t tmem,
@@ -382,7 +443,7 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     // tokens of the chunk this row sees, from the chunk's start
     const int lim = min(__ldg(P.seq_lens + b), P.n_pages * kBlockSize) - W.t0 * kTile;
     const bool any_row = __any_sync(0xffffffffu, live);
-    float ref = -INFINITY, l = 0.0f;
+    RowState st{-INFINITY, 0.0f};
     const int n = W.tiles(m);
     for (int i = 0; i < n; i++) {
         const int tile = W.tile(m, i);
@@ -391,43 +452,10 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
         if (any_row) {
             const uint32_t pages = smem[kBarOff + kMasks + 4 * (tile & 3)] | smem[kBarOff + kMasks + 4 * (tile & 3) + 1];
             const int left = lim - tile * kTile;
-            const bool mask = __any_sync(0xffffffffu, left < kTile || pages != 0xFFu);
-            uint32_t p[64];
-            float sum, top;
-            if (__any_sync(0xffffffffu, ref == -INFINITY)) {  // the first tile with a visible token
-                const float mx = mask ? largest<true>(ts, left, pages) : largest<false>(ts, left, pages);
-                if (ref == -INFINITY) ref = mx * kfac;
-            }
-            for (;;) {
-                const float r = ref == -INFINITY ? 0.0f : ref;
-                if (mask)
-                    weigh<true>(ts, kfac, r, left, pages, p, sum, top);
-                else
-                    weigh<false>(ts, kfac, r, left, pages, p, sum, top);
-                const bool over = top > kSlack && top < INFINITY;
-                if (!__any_sync(0xffffffffu, over)) break;
-                // move the reference of the rows that need it, and what they
-                // have summed so far
-                const float f = over ? ex2_approx(-top) : 1.0f;
-                ref = over ? ref + top : ref;
-                l *= f;
-                if (i > 0) {
-#pragma unroll 1
-                    for (int q = 0; q < 4; q++) {
-                        uint32_t o[32];
-                        tmem_ld32(o, to + 32 * q);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                        tmem_st32(to + 32 * q, o);
-                    }
-                    tmem_wait_st();
-                }
-            }
-            l += sum;
-            tmem_st32(ts, p);
-            tmem_st32(ts + 32, p + 32);
-            tmem_wait_st();
+            if (__any_sync(0xffffffffu, left < kTile || pages != 0xFFu))
+                weigh<true>(st, ts, to, i > 0, kfac, left, pages);
+            else
+                weigh<false>(st, ts, to, i > 0, kfac, left, pages);
         }
         tc_fence_before();
         bar_arrive(bars + kPFull + 8 * m);
@@ -439,10 +467,11 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     }
     if (!any_row) return;
     const int sp = W.split ? 2 * (int)blockIdx.x + m : (int)blockIdx.x;
-    const bool seen = l > 0.0f || l != l;
-    const float inv = seen ? rcp_approx(l) : 0.0f;
+    const bool seen = st.l > 0.0f || st.l != st.l;
+    const float inv = seen ? rcp_approx(st.l) : 0.0f;
     float* dst = P.mid + (int64_t)b * P.msb + (int64_t)(W.h * P.G + g) * P.msh + (int64_t)sp * P.mss;
-    if (live) dst[kHeadDim] = seen ? (ref + lg2_approx(l)) * kLn2 : -INFINITY;
+    const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+    if (live) dst[kHeadDim] = seen ? (st.ref + lg2_approx(st.l)) * kLn2 : -INFINITY;
     // 32 x 32 blocks turn through shared memory (this stream's query tile, or
     // the unused second one), so that rows are written in runs of 128 bytes
     float* turn = reinterpret_cast<float*>(smem + kQOff + (W.split ? kOperand + m * kHalf : m * kOperand) + wq * 4096);
@@ -459,9 +488,11 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
             turn[32 * lane + (d ^ lane)] = seen ? __uint_as_float(o[j]) * inv : 0.0f;
         }
         __syncwarp();
+#pragma unroll 8
         for (int r = 0; r < 32; r++) {
             float* to_row = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
-            if (__shfl_sync(0xffffffffu, (int)live, r)) to_row[32 * q + lane] = turn[32 * r + (lane ^ r)];
+            const float v = turn[32 * r + (lane ^ r)];
+            if ((live_rows >> r) & 1u) to_row[32 * q + lane] = v;
         }
         __syncwarp();
     }
@@ -504,30 +535,44 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
 
     // ---- K table: entry = two codes, {c[low], c[high]} in fp16, a copy per lane
     if constexpr (!k8) {
+        // a warp makes 16 entries, a lane each, and spreads them over the copies
         constexpr int kPairs = k3 ? 64 : 256, kBits = k3 ? 3 : 4, kMask = k3 ? 7 : 15;
-        for (int e = tid; e < kPairs * 32; e += kPrefixThreads) {
-            const int pair = e >> 5;
-            reinterpret_cast<uint32_t*>(smem + kLutOff)[e] =
-                h2_as_u32(__floats2half2_rn(__ldg(P.cents + (pair & kMask)), __ldg(P.cents + (pair >> kBits))));
+        static_assert(kPrefixThreads / 32 * 16 >= kPairs, "one round of the warps");
+        if (warp < kPairs / 16) {
+            const int pair = 16 * warp + (lane & 15);
+            const uint32_t v = h2_as_u32(__floats2half2_rn(__ldg(P.cents + (pair & kMask)), __ldg(P.cents + (pair >> kBits))));
+            uint32_t* lut = reinterpret_cast<uint32_t*>(smem + kLutOff) + 16 * warp * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 16; i++) lut[32 * i] = __shfl_sync(0xffffffffu, v, i);
         }
     }
-    // ---- queries: fp16, scaled per row into [2^14, 2^15), 128-byte swizzle
+    // ---- queries: fp16, scaled per row into [2^14, 2^15), 128-byte swizzle;
+    // a warp takes rows warp, warp + 16, ..., eight of them in flight
     const int slots = W.split || W.rows <= kTile ? kTile : 2 * kTile;
-    for (int r = warp; r < slots; r += kPrefixThreads / 32) {
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (r < W.rows) {
-            const int row = W.row0 + r, b = row / P.G, g = row - b * P.G;
-            x = __ldg(reinterpret_cast<const float4*>(P.q + (int64_t)b * P.qsb + (int64_t)(W.h * P.G + g) * P.qsh) + lane);
+    for (int r0 = warp; r0 < slots; r0 += 8 * (kPrefixThreads / 32)) {
+        float4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = r0 + i * (kPrefixThreads / 32);
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r < W.rows) {
+                const int row = W.row0 + r, b = (int)((uint32_t)row / (uint32_t)P.G), g = row - b * P.G;
+                x[i] = __ldg(reinterpret_cast<const float4*>(P.q + (int64_t)b * P.qsb + (int64_t)(W.h * P.G + g) * P.qsh) + lane);
+            }
         }
-        const float amax = warp_max_xor(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), 1, 16);
-        const int e = fp16_scale_exp(amax);
-        const float f = exp2i(e);
-        if (lane == 0) reinterpret_cast<float*>(smem + kAuxOff)[r] = P.scale * kLog2e * exp2i(-e);
-        // dims 4 lane .. 4 lane + 3: half lane / 16, chunk (lane % 16) / 2
-        uint8_t* at = smem + kQOff + (r >> 7) * kOperand + (lane >> 4) * kHalf + (r & 127) * 128 +
-                      ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
-        *reinterpret_cast<uint2*>(at) = make_uint2(h2_as_u32(__floats2half2_rn(x.x * f, x.y * f)),
-                                                   h2_as_u32(__floats2half2_rn(x.z * f, x.w * f)));
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = r0 + i * (kPrefixThreads / 32);
+            const float amax = warp_max_xor(fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))), 1, 16);
+            const int e = fp16_scale_exp(amax);
+            const float f = exp2i(e);
+            if (lane == 0) reinterpret_cast<float*>(smem + kAuxOff)[r] = P.scale * kLog2e * exp2i(-e);
+            // dims 4 lane .. 4 lane + 3: half lane / 16, chunk (lane % 16) / 2
+            uint8_t* at = smem + kQOff + (r >> 7) * kOperand + (lane >> 4) * kHalf + (r & 127) * 128 +
+                          ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+            *reinterpret_cast<uint2*>(at) = make_uint2(h2_as_u32(__floats2half2_rn(x[i].x * f, x[i].y * f)),
+                                                       h2_as_u32(__floats2half2_rn(x[i].z * f, x[i].w * f)));
+        }
     }
     fence_async_smem();
     tc_fence_before();
