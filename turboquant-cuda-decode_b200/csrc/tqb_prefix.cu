@@ -270,7 +270,7 @@ __device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W
     for (int j = 0; j < W.n; j++) {
         const int s = j & 1;
         const uint32_t phase = ((j >> 1) & 1) ^ 1;
-        if (!__all_sync(0xffffffffu, bar_wait(bars + kKEmpty + 8 * s, phase, abort))) return;
+        if (!bar_wait_warp(bars + kKEmpty + 8 * s, phase, abort)) return;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             put_k<L>(smem, kKOff + s * kOperand, rk[i], 32 * i + 8 * pw + t8, c, lane);
@@ -285,7 +285,7 @@ __device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W
         }
         fence_async_smem();
         bar_arrive(bars + kKFull + 8 * s);
-        if (!__all_sync(0xffffffffu, bar_wait(bars + kVEmpty + 8 * s, phase, abort))) return;
+        if (!bar_wait_warp(bars + kVEmpty + 8 * s, phase, abort)) return;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             put_v<L>(smem, kVOff + s * kOperand, rv[i], 32 * i + 8 * pw + t8, c);
@@ -298,24 +298,27 @@ __device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W
     }
 }
 
-// The MMA thread.  All its MMAs execute in the order of issue, so S_m of the
-// next tile may follow P_m V of this one on the same columns, and the commit
-// that announces S_m also says that the stream's earlier products are done.
-__device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t bars, uint32_t tmem, volatile uint32_t* abort) {
+// The MMA warp (lane 0 issues).  All its MMAs execute in the order of issue,
+// so S_m of the next tile may follow P_m V of this one on the same columns,
+// and the commit that announces S_m also says that the stream's earlier
+// products are done.
+__device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t bars, uint32_t tmem, volatile uint32_t* abort,
+                                      uint32_t one) {
     constexpr uint32_t kQK = umma_idesc(kTile, kTile, false), kPV = umma_idesc(kTile, kHeadDim, true);
     const int last = W.split || W.rows <= kTile ? -1 : 1;  // the stream that releases a shared stage (-1: each its own)
     auto qk = [&](int m, int tile) {
         const int s = tile & 1;
-        if (!bar_wait(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
+        if (!bar_wait_warp(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
         tc_fence_after();
-        const uint32_t q = smem + kQOff + (W.split ? 0 : m * kOperand), k = smem + kKOff + s * kOperand;
+        const uint64_t q = umma_desc(smem + kQOff + (W.split ? 0 : m * kOperand), 16, 1024);
+        const uint64_t k = umma_desc(smem + kKOff + s * kOperand, 16, 1024);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint32_t at = (e >> 2) * kHalf + (e & 3) * 32;
-            umma_ss(tmem + m * kTile, umma_desc(q + at, 16, 1024), umma_desc(k + at, 16, 1024), kQK, e != 0);
+        for (int e = 0; e < 8; e++) {  // 16 dims: 32 bytes of a swizzled row, the upper 64 dims a half further
+            const uint64_t at = ((e >> 2) * kHalf + (e & 3) * 32) >> 4;
+            umma_ss(tmem + m * kTile, q + at, k + at, kQK, e != 0, one);
         }
-        umma_commit(bars + kSFull + 8 * m);
-        if (last < 0 || m == last) umma_commit(bars + kKEmpty + 8 * s);
+        umma_commit(bars + kSFull + 8 * m, one);
+        if (last < 0 || m == last) umma_commit(bars + kKEmpty + 8 * s, one);
         return true;
     };
     bool ok = true;
@@ -325,24 +328,25 @@ __device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t ba
         for (int m = 0; m < 2 && ok; m++) {
             if (i >= W.tiles(m)) continue;
             const int tile = W.tile(m, i), s = tile & 1;
-            ok = bar_wait(bars + kPFull + 8 * m, i & 1, abort) && bar_wait(bars + kVFull + 8 * s, (tile >> 1) & 1, abort);
+            ok = bar_wait_warp(bars + kVFull + 8 * s, (tile >> 1) & 1, abort) &&
+                 bar_wait_warp(bars + kPFull + 8 * m, i & 1, abort);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t v = smem + kVOff + s * kOperand;
+            const uint64_t v = umma_desc(smem + kVOff + s * kOperand, kHalf, 1024);
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + 8 * e, umma_desc(v + e * 2048, kHalf, 1024),
-                        kPV, i != 0 || e != 0);
-            if (last < 0 || m == last) umma_commit(bars + kVEmpty + 8 * s);
+            for (int e = 0; e < 8; e++)  // 16 tokens: two 8-row groups
+                umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + 8 * e, v + e * (2048 >> 4), kPV, i != 0 || e != 0,
+                        one);
+            if (last < 0 || m == last) umma_commit(bars + kVEmpty + 8 * s, one);
             if (i + 1 < W.tiles(m))
                 ok = qk(m, W.tile(m, i + 1));
             else
-                umma_commit(bars + kOFull + 8 * m);
+                umma_commit(bars + kOFull + 8 * m, one);
         }
     }
     // every product has ended before the CTA frees its TMEM
-    umma_commit(bars + kDone);
-    bar_wait(bars + kDone, 0, abort);
+    umma_commit(bars + kDone, one);
+    bar_wait_warp(bars + kDone, 0, abort);
 }
 
 // Running reference, sum and products of a row.
@@ -447,7 +451,7 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     const int n = W.tiles(m);
     for (int i = 0; i < n; i++) {
         const int tile = W.tile(m, i);
-        if (!__all_sync(0xffffffffu, bar_wait(bars + kSFull + 8 * m, i & 1, abort))) return;
+        if (!bar_wait_warp(bars + kSFull + 8 * m, i & 1, abort)) return;
         tc_fence_after();
         if (any_row) {
             const uint32_t pages = smem[kBarOff + kMasks + 4 * (tile & 3)] | smem[kBarOff + kMasks + 4 * (tile & 3) + 1];
@@ -462,7 +466,7 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     }
     // ---- the partial rows ----
     if (n > 0) {
-        if (!__all_sync(0xffffffffu, bar_wait(bars + kOFull + 8 * m, 0, abort))) return;
+        if (!bar_wait_warp(bars + kOFull + 8 * m, 0, abort)) return;
         tc_fence_after();
     }
     if (!any_row) return;
@@ -502,7 +506,7 @@ template <int L>
 __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixParams P) {
     constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L);
     extern __shared__ __align__(1024) uint8_t smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t base = smem_addr(smem), bars = base + kBarOff;
     volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kAbort);
     pdl_trigger();
@@ -578,7 +582,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kTmem);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kTmem), 0);
 
     if (warp < kSoftmaxWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
@@ -588,7 +592,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
         dequantise<L>(P, W, smem, bars, abort, warp - kSoftmaxWarps, lane);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegs));
-        if (warp == kSoftmaxWarps + kProducerWarps && lane == 0) issue(W, base, bars, tmem, abort);
+        if (warp == kSoftmaxWarps + kProducerWarps) issue(W, base, bars, tmem, abort, lane == 0 ? 1u : 0u);
     }
     __syncwarp();
     tc_fence_before();

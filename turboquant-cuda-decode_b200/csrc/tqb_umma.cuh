@@ -28,15 +28,15 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Waits for the phase of `bar` with the given parity, for each thread on its
-// own.  False when about a second passes first, or when another thread of the
-// CTA has given up (`abort`, in shared memory, which this sets too).
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort) {
-    if (bar_try(bar, parity)) return true;
+// Waits, as a converged warp, for the phase of `bar` with the given parity.
+// False when about a second passes first, or when another warp of the CTA has
+// given up (`abort`, in shared memory, which this sets too).
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort) {
+    if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
     const long long t0 = clock64();
     for (uint32_t i = 1;; i++) {
-        if (bar_try(bar, parity)) return true;
-        if ((i & 15u) == 0 && (*abort != 0 || clock64() - t0 > kUmmaWaitCycles)) {
+        if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
+        if ((i & 15u) == 0 && __any_sync(0xffffffffu, *abort != 0 || clock64() - t0 > kUmmaWaitCycles)) {
             *abort = 1;
             return false;
         }
@@ -116,25 +116,34 @@ constexpr uint32_t umma_idesc(int m, int n, bool b_mn_major) {
     return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// D (TMEM) (+)= A B, one issuing thread.
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// Issued by the lane with `one` set while the whole warp runs the code around
+// it: with operands that the compiler can see to be uniform, an MMA costs its
+// issue and nothing else (from a branch that one lane takes, forming the
+// operands took 140 cycles of the 64 that a 128 x 128 x 16 product takes).
+
+// D (TMEM) (+)= A B.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t one) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(one)
         : "memory");
 }
 // A from TMEM (two f16 per column).
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t one) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(one)
         : "memory");
 }
-// `bar` completes one arrival when every MMA issued so far by this thread has.
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+// `bar` completes one arrival when every MMA issued so far by this lane has.
+__device__ __forceinline__ void umma_commit(uint32_t bar, uint32_t one) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+        "r"(one)
+        : "memory");
 }
 
 // ---- packed fp32 -----------------------------------------------------------
