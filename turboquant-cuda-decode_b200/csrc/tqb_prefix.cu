@@ -17,9 +17,12 @@
 //              tiles are always in flight;
 //   8-11       dequantise K and V tiles (fp16, 128-byte swizzle) into two
 //              stages of shared memory, the next tile's codes in registers;
-//   12         issues the MMAs (13-15 idle): S = Q K^T (operands in shared memory), then
-//              O += P V with P in TMEM where S was.
-// TMEM holds S0 S1 O0 O1 (128 columns each): all 512.
+//   12         issues the MMAs (13-15 idle): S = Q K^T (operands in shared
+//              memory), then O += P V with P in TMEM where S was.
+// A stream goes by half tiles of 64 tokens with two S buffers, so the next
+// half's scores are there when the softmax of this one ends (with one S per
+// stream of 128 tokens, softmax and MMAs took turns: 5300 cycles a tile for
+// 2800 of softmax).  TMEM: 2 x 2 S of 64 columns, 2 O of 128: all 512.
 //
 // Precision: Q (scaled per row by a power of two), K = c norm, V = code scale
 // + zero and P are rounded to fp16, each product accumulated in fp32; m, l, O
@@ -64,8 +67,12 @@ static_assert(2 * kSoftmaxRegs + kProducerRegs + kIssueRegs <= 4 * kPrefixRegs &
 constexpr float kSlack = 8.0f;
 
 // Barriers (8 bytes each) at kBarOff, then words.
-enum : uint32_t { kKFull = 0, kVFull = 16, kKEmpty = 32, kVEmpty = 48, kSFull = 64, kPFull = 80, kOFull = 96, kDone = 112,
-                  kMasks = 128, kTmem = 144, kAbort = 148 };
+// Two of each: stages of K and V, S and P per stream m and buffer b (at 16 m +
+// 8 b), products of O per stream.
+enum : uint32_t { kKFull = 0, kVFull = 16, kKEmpty = 32, kVEmpty = 48, kSFull = 64, kPFull = 96, kODone = 128, kDone = 144,
+                  kMasks = 152, kTmem = 168, kAbort = 172 };
+constexpr int kHalfTile = kTile / 2;  // tokens of a softmax step
+
 
 __device__ __forceinline__ uint32_t dup16(uint32_t h) { return __byte_perm(h, 0u, 0x1010); }
 __device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) { return h2_as_u32(__hmul2(u32_as_h2(a), u32_as_h2(b))); }
@@ -232,13 +239,19 @@ __device__ __forceinline__ void put_v(uint8_t* smem, uint32_t tile, const RawV& 
     }
 }
 
-// Where a CTA works: its tiles [t0, t1) and rows [row0, row0 + rows), and the
-// tiles of a stream (every tile, or with `split` every other one).
+// Where a CTA works: its n tiles from t0 on (`tokens` of them tokens of the
+// prefix) and rows [row0, row0 + rows), and the half tiles of a stream (of
+// every tile, or with `split` of every other one).
 struct Place {
-    int h, t0, n, row0, rows;
+    int h, t0, n, tokens, row0, rows;
     bool split;
     __device__ __forceinline__ int tiles(int m) const { return split ? (n + 1 - m) / 2 : (m == 0 || rows > kTile ? n : 0); }
-    __device__ __forceinline__ int tile(int m, int i) const { return split ? 2 * i + m : i; }  // from t0 on
+    // half step u of stream m: tile (from t0 on), then the number of steps
+    __device__ __forceinline__ int tile(int m, int u) const { return split ? 2 * (u >> 1) + m : u >> 1; }
+    __device__ __forceinline__ int steps(int m) const {
+        const int t = tiles(m);  // the chunk's last tile may have one half only
+        return 2 * t - (t > 0 && tile(m, 2 * t - 2) == n - 1 && tokens <= (n - 1) * kTile + kHalfTile ? 1 : 0);
+    }
 };
 
 template <int L>
@@ -298,54 +311,56 @@ __device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W
     }
 }
 
-// The MMA warp (lane 0 issues).  All its MMAs execute in the order of issue,
-// so S_m of the next tile may follow P_m V of this one on the same columns,
-// and the commit that announces S_m also says that the stream's earlier
-// products are done.
-__device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t bars, uint32_t tmem, volatile uint32_t* abort,
-                                      uint32_t one) {
-    constexpr uint32_t kQK = umma_idesc(kTile, kTile, false), kPV = umma_idesc(kTile, kHeadDim, true);
+// The MMA warp.  All its MMAs execute in the order of issue,
+// so the scores of step u + 2 may follow P V of step u on the same columns.
+__device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t bars, uint32_t tmem, volatile uint32_t* abort) {
+    constexpr uint32_t kQK = umma_idesc(kTile, kHalfTile, false), kPV = umma_idesc(kTile, kHeadDim, true);
     const int last = W.split || W.rows <= kTile ? -1 : 1;  // the stream that releases a shared stage (-1: each its own)
-    auto qk = [&](int m, int tile) {
-        const int s = tile & 1;
+    const int steps[2] = {W.steps(0), W.steps(1)};
+    // the stream's last step on this step's tile, by the stream that releases it
+    auto releases = [&](int m, int u) { return (last < 0 || m == last) && ((u & 1) || u + 1 == steps[m]); };
+    auto qk = [&](int m, int u) {
+        const int tile = W.tile(m, u), s = tile & 1;
         if (!bar_wait_warp(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
         tc_fence_after();
         const uint64_t q = umma_desc(smem + kQOff + (W.split ? 0 : m * kOperand), 16, 1024);
-        const uint64_t k = umma_desc(smem + kKOff + s * kOperand, 16, 1024);
+        const uint64_t k = umma_desc(smem + kKOff + s * kOperand + (u & 1) * (kHalfTile * 128), 16, 1024);
 #pragma unroll
         for (int e = 0; e < 8; e++) {  // 16 dims: 32 bytes of a swizzled row, the upper 64 dims a half further
             const uint64_t at = ((e >> 2) * kHalf + (e & 3) * 32) >> 4;
-            umma_ss(tmem + m * kTile, q + at, k + at, kQK, e != 0, one);
+            umma_ss(tmem + m * kTile + (u & 1) * kHalfTile, q + at, k + at, kQK, e != 0);
         }
-        umma_commit(bars + kSFull + 8 * m, one);
-        if (last < 0 || m == last) umma_commit(bars + kKEmpty + 8 * s, one);
+        umma_commit(bars + kSFull + 16 * m + 8 * (u & 1));
+        if (releases(m, u)) umma_commit(bars + kKEmpty + 8 * s);
         return true;
     };
     bool ok = true;
-    for (int m = 0; m < 2 && ok; m++)
-        if (W.tiles(m) > 0) ok = qk(m, W.tile(m, 0));
-    for (int i = 0; ok && i < W.tiles(0); i++) {
-        for (int m = 0; m < 2 && ok; m++) {
-            if (i >= W.tiles(m)) continue;
-            const int tile = W.tile(m, i), s = tile & 1;
-            ok = bar_wait_warp(bars + kVFull + 8 * s, (tile >> 1) & 1, abort) &&
-                 bar_wait_warp(bars + kPFull + 8 * m, i & 1, abort);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t v = umma_desc(smem + kVOff + s * kOperand, kHalf, 1024);
 #pragma unroll
-            for (int e = 0; e < 8; e++)  // 16 tokens: two 8-row groups
-                umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + 8 * e, v + e * (2048 >> 4), kPV, i != 0 || e != 0,
-                        one);
-            if (last < 0 || m == last) umma_commit(bars + kVEmpty + 8 * s, one);
-            if (i + 1 < W.tiles(m))
-                ok = qk(m, W.tile(m, i + 1));
-            else
-                umma_commit(bars + kOFull + 8 * m, one);
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+            if (ok && u < steps[m]) ok = qk(m, u);
+    for (int u = 0; ok && u < steps[0]; u++) {
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            if (!ok || u >= steps[m]) continue;
+            const int tile = W.tile(m, u), s = tile & 1;
+            ok = bar_wait_warp(bars + kVFull + 8 * s, (tile >> 1) & 1, abort) &&
+                 bar_wait_warp(bars + kPFull + 16 * m + 8 * (u & 1), (u >> 1) & 1, abort);
+            if (!ok) continue;
+            tc_fence_after();
+            const uint64_t v = umma_desc(smem + kVOff + s * kOperand + (u & 1) * (kHalfTile * 128), kHalf, 1024);
+#pragma unroll
+            for (int e = 0; e < 4; e++)  // 16 tokens: two 8-row groups
+                umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + (u & 1) * kHalfTile + 8 * e, v + e * (2048 >> 4), kPV,
+                        u != 0 || e != 0);
+            umma_commit(bars + kODone + 8 * m);
+            if (releases(m, u)) umma_commit(bars + kVEmpty + 8 * s);
+            if (u + 2 < steps[m]) ok = qk(m, u + 2);
         }
     }
     // every product has ended before the CTA frees its TMEM
-    umma_commit(bars + kDone, one);
+    umma_commit(bars + kDone);
     bar_wait_warp(bars + kDone, 0, abort);
 }
 
@@ -356,21 +371,26 @@ struct RowState {
 
 // Moves the reference of the rows whose exponents exceed it by more than
 // kSlack (or that see their first token), and scales what they have summed so
-// far: l, O, and the weights of this tile's first q quarters.  Rare.
-__device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32_t ts, uint32_t to, int q, bool has_o) {
+// far: l, O (once the products before this step are in it: phase u - 1 of
+// `o_done`, phase u - 2 being over since these scores were announced), and the first 32 weights of this step if they are written.
+// Rare.
+__device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32_t ts, uint32_t to, bool second, int u,
+                                       uint32_t o_done, volatile uint32_t* abort) {
     const float f = over && st.ref != -INFINITY ? ex2_approx(-top) : 1.0f;
     if (over) st.ref = (st.ref == -INFINITY ? 0.0f : st.ref) + top;
     st.l *= f;
-    const __half2 f2 = __float2half2_rn(f);
-    for (int i = 0; i < q; i++) {
+    if (second) {
+        tmem_wait_st();  // the weights just written
+        const __half2 f2 = __float2half2_rn(f);
         uint32_t p[16];
-        tmem_ld16(p, ts + 16 * i);
+        tmem_ld16(p, ts);
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; j++) p[j] = h2_as_u32(__hmul2(u32_as_h2(p[j]), f2));
-        tmem_st16(ts + 16 * i, p);
+        tmem_st16(ts, p);
     }
-    if (has_o) {
+    if (u > 0 && bar_wait_warp(o_done, (u - 1) & 1, abort)) {
+        tc_fence_after();
         for (int i = 0; i < kHeadDim; i += 16) {
             uint32_t o[16];
             tmem_ld16(o, to + i);
@@ -384,26 +404,25 @@ __device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32
     return st;
 }
 
-// The weights of a tile's tokens for this thread's row: p = exp2(s kfac - ref)
-// in place of the scores (columns 0 .. 63, two fp16 each), a quarter of the
-// tile at a time; the next quarter's scores are loaded under the
-// exponentials.
+// The weights of a step's 64 tokens for this thread's row: p = exp2(s kfac -
+// ref) in place of the scores (columns 0 .. 31, two fp16 each), 32 tokens at a
+// time; the second 32 scores are loaded under the first exponentials.
 template <bool MASK>
-__device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, bool has_o, float kfac, int lim,
-                                      uint32_t pages) {
+__device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, float kfac, int lim, uint32_t pages, int u,
+                                      uint32_t o_done, volatile uint32_t* abort) {
     const uint64_t k2 = pack2(kfac, kfac);
     uint64_t acc = pack2(0.0f, 0.0f);
     uint32_t s[2][32];
     tmem_ld32(s[0], ts);
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
+    for (int q = 0; q < 2; q++) {
         tmem_wait_ld();
         const float r = st.ref == -INFINITY ? 0.0f : st.ref;
         uint64_t r2 = pack2(-r, -r), x[16];
         float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            x[j] = fma2((uint64_t)s[q & 1][2 * j] | ((uint64_t)s[q & 1][2 * j + 1] << 32), k2, r2);
+            x[j] = fma2((uint64_t)s[q][2 * j] | ((uint64_t)s[q][2 * j + 1] << 32), k2, r2);
             if constexpr (MASK) {
                 const int t = 32 * q + 2 * j;
                 const bool page = (pages >> (t >> 4)) & 1u;
@@ -415,12 +434,12 @@ __device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, bo
         if (__any_sync(0xffffffffu, over)) {
             st.l += lo2(acc) + hi2(acc);
             acc = pack2(0.0f, 0.0f);
-            st = raise(st, top, over, ts, to, q, has_o);
+            st = raise(st, top, over, ts, to, q > 0, u, o_done, abort);
             r2 = over ? pack2(-top, -top) : acc;
 #pragma unroll
             for (int j = 0; j < 16; j++) x[j] = add2(x[j], r2);
         }
-        if (q < 3) tmem_ld32(s[(q + 1) & 1], ts + 32 * (q + 1));
+        if (q == 0) tmem_ld32(s[1], ts + 32);
         uint32_t p[16];
 #pragma unroll
         for (int j = 0; j < 16; j++) {
@@ -448,25 +467,30 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     const int lim = min(__ldg(P.seq_lens + b), P.n_pages * kBlockSize) - W.t0 * kTile;
     const bool any_row = __any_sync(0xffffffffu, live);
     RowState st{-INFINITY, 0.0f};
-    const int n = W.tiles(m);
-    for (int i = 0; i < n; i++) {
-        const int tile = W.tile(m, i);
-        if (!bar_wait_warp(bars + kSFull + 8 * m, i & 1, abort)) return;
+    const int n = W.steps(m);
+    for (int u = 0; u < n; u++) {
+        const int tile = W.tile(m, u), half = u & 1;
+        if (!bar_wait_warp(bars + kSFull + 16 * m + 8 * half, (u >> 1) & 1, abort)) return;
         tc_fence_after();
         if (any_row) {
-            const uint32_t pages = smem[kBarOff + kMasks + 4 * (tile & 3)] | smem[kBarOff + kMasks + 4 * (tile & 3) + 1];
-            const int left = lim - tile * kTile;
-            if (__any_sync(0xffffffffu, left < kTile || pages != 0xFFu))
-                weigh<true>(st, ts, to, i > 0, kfac, left, pages);
+            const uint32_t pages = (smem[kBarOff + kMasks + 4 * (tile & 3)] | smem[kBarOff + kMasks + 4 * (tile & 3) + 1]) >>
+                                   (kTilePages / 2 * half) & 0xFu;
+            const int left = lim - tile * kTile - half * kHalfTile;
+            const uint32_t at = ts + half * kHalfTile;
+            if (__any_sync(0xffffffffu, left < kHalfTile || pages != 0xFu))
+                weigh<true>(st, at, to, kfac, left, pages, u, bars + kODone + 8 * m, abort);
             else
-                weigh<false>(st, ts, to, i > 0, kfac, left, pages);
+                weigh<false>(st, at, to, kfac, left, pages, u, bars + kODone + 8 * m, abort);
         }
         tc_fence_before();
-        bar_arrive(bars + kPFull + 8 * m);
+        bar_arrive(bars + kPFull + 16 * m + 8 * half);
     }
     // ---- the partial rows ----
+    // (the last scores say that the products up to step n - 3 are done: the
+    // two phases after it are waited for one by one)
     if (n > 0) {
-        if (!bar_wait_warp(bars + kOFull + 8 * m, 0, abort)) return;
+        if (n > 1 && !bar_wait_warp(bars + kODone + 8 * m, (n - 2) & 1, abort)) return;
+        if (!bar_wait_warp(bars + kODone + 8 * m, (n - 1) & 1, abort)) return;
         tc_fence_after();
     }
     if (!any_row) return;
@@ -516,6 +540,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
     W.h = blockIdx.y;
     W.t0 = (int)((int64_t)n_tiles * blockIdx.x / gridDim.x);
     W.n = (int)((int64_t)n_tiles * (blockIdx.x + 1) / gridDim.x) - W.t0;
+    W.tokens = min(P.n_pages * kBlockSize - W.t0 * kTile, W.n * kTile);
     W.row0 = blockIdx.z * 2 * kTile;
     W.rows = min(R - W.row0, 2 * kTile);
     W.split = P.split != 0;
@@ -526,9 +551,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
             bar_init(bars + kVFull + 8 * s, kProducerWarps * 32);
             bar_init(bars + kKEmpty + 8 * s, 1);
             bar_init(bars + kVEmpty + 8 * s, 1);
-            bar_init(bars + kSFull + 8 * s, 1);
-            bar_init(bars + kPFull + 8 * s, 128);
-            bar_init(bars + kOFull + 8 * s, 1);
+            for (int b = 0; b < 16; b += 8) {
+                bar_init(bars + kSFull + 16 * s + b, 1);
+                bar_init(bars + kPFull + 16 * s + b, 128);
+            }
+            bar_init(bars + kODone + 8 * s, 1);
         }
         bar_init(bars + kDone, 1);
         *abort = 0;
@@ -592,7 +619,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
         dequantise<L>(P, W, smem, bars, abort, warp - kSoftmaxWarps, lane);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegs));
-        if (warp == kSoftmaxWarps + kProducerWarps) issue(W, base, bars, tmem, abort, lane == 0 ? 1u : 0u);
+        if (warp == kSoftmaxWarps + kProducerWarps) issue(W, base, bars, tmem, abort);
     }
     __syncwarp();
     tc_fence_before();

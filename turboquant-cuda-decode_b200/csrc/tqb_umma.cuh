@@ -116,33 +116,30 @@ constexpr uint32_t umma_idesc(int m, int n, bool b_mn_major) {
     return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// Issued by the lane with `one` set while the whole warp runs the code around
-// it: with operands that the compiler can see to be uniform, an MMA costs its
-// issue and nothing else (from a branch that one lane takes, forming the
-// operands took 140 cycles of the 64 that a 128 x 128 x 16 product takes).
+// A converged warp calls these and one elected lane issues (the same one each
+// time), so that the operands stay warp-uniform.
 
 // D (TMEM) (+)= A B.
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t one) {
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
         " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(one)
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
 // A from TMEM (two f16 per column).
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t one) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
         " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(one)
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
-// `bar` completes one arrival when every MMA issued so far by this lane has.
-__device__ __forceinline__ void umma_commit(uint32_t bar, uint32_t one) {
+// `bar` completes one arrival when every MMA issued so far by that lane has.
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile(
-        "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
-        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
-        "r"(one)
+        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
         : "memory");
 }
 
