@@ -723,6 +723,7 @@ int tqb_prefix(const tqb_stage1_args* a, int32_t prefix_len, cudaStream_t stream
     p.B = s.B;
     p.Hk = s.Hk;
     p.G = s.G;
+    p.div_g = tqb::FastDiv((uint32_t)s.G);
     p.scale = s.attn_scale;
     return tqb::launch_prefix(p, stream);
 }

@@ -260,6 +260,7 @@ struct PrefixParams {
     int B, Hk, G;
     int chunks;  // of the prefix's 128-token tiles, a CTA each per KV head and 256 rows
     int split;   // two streams of the same <= 128 rows, a partial split each
+    FastDiv div_g;
     float scale;
 };
 

@@ -17,7 +17,7 @@
 //              tiles are always in flight;
 //   8-11       dequantise K and V tiles (fp16, 128-byte swizzle) into two
 //              stages of shared memory, the next tile's codes in registers;
-//   12         issues the MMAs (13-15 idle): S = Q K^T (operands in shared
+//   12, 13     issue the MMAs of a stream each (14, 15 idle): S = Q K^T (operands in shared
 //              memory), then O += P V with P in TMEM where S was.
 // A stream goes by half tiles of 64 tokens with two S buffers, so the next
 // half's scores are there when the softmax of this one ends (with one S per
@@ -68,9 +68,9 @@ constexpr float kSlack = 8.0f;
 
 // Barriers (8 bytes each) at kBarOff, then words.
 // Two of each: stages of K and V, S and P per stream m and buffer b (at 16 m +
-// 8 b), products of O per stream.
-enum : uint32_t { kKFull = 0, kVFull = 16, kKEmpty = 32, kVEmpty = 48, kSFull = 64, kPFull = 96, kODone = 128, kDone = 144,
-                  kMasks = 152, kTmem = 168, kAbort = 172 };
+// 8 b), the end of a stream's products.
+enum : uint32_t { kKFull = 0, kVFull = 16, kKEmpty = 32, kVEmpty = 48, kSFull = 64, kPFull = 96, kDone = 128,
+                  kQFull = 144, kMasks = 152, kTmem = 168, kAbort = 172 };
 constexpr int kHalfTile = kTile / 2;  // tokens of a softmax step
 
 
@@ -311,57 +311,59 @@ __device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W
     }
 }
 
-// The MMA warp.  All its MMAs execute in the order of issue,
-// so the scores of step u + 2 may follow P V of step u on the same columns.
-__device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t bars, uint32_t tmem, volatile uint32_t* abort) {
+// The MMA warp of stream m.  Its MMAs execute in the order of issue, so the
+// scores of step u + 2 may follow P V of step u on the same columns, and the
+// one commit behind both (event u + 2 of the stream, on s_full) also says that
+// the products up to step u are in O; events n and n + 1 say only that.  A warp
+// per stream, and few waits and commits: those cost 130 and 200 cycles each
+// where the 12 MMAs of a step take 300 to issue.
+__device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t bars, uint32_t tmem, volatile uint32_t* abort,
+                                      const int m) {
     constexpr uint32_t kQK = umma_idesc(kTile, kHalfTile, false), kPV = umma_idesc(kTile, kHeadDim, true);
-    const int last = W.split || W.rows <= kTile ? -1 : 1;  // the stream that releases a shared stage (-1: each its own)
-    const int steps[2] = {W.steps(0), W.steps(1)};
-    // the stream's last step on this step's tile, by the stream that releases it
-    auto releases = [&](int m, int u) { return (last < 0 || m == last) && ((u & 1) || u + 1 == steps[m]); };
-    auto qk = [&](int m, int u) {
+    const int n = W.steps(m);
+    if (n == 0) return;
+    const uint64_t q = umma_desc(smem + kQOff + (W.split ? 0 : m * kOperand), 16, 1024);
+    auto last_of_tile = [&](int u) { return (u & 1) || u + 1 == n; };
+    auto qk = [&](int u) {
         const int tile = W.tile(m, u), s = tile & 1;
-        if (!bar_wait_warp(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
-        tc_fence_after();
-        const uint64_t q = umma_desc(smem + kQOff + (W.split ? 0 : m * kOperand), 16, 1024);
+        if (!(u & 1)) {
+            if (!bar_wait_warp(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
+            tc_fence_after();
+        }
         const uint64_t k = umma_desc(smem + kKOff + s * kOperand + (u & 1) * (kHalfTile * 128), 16, 1024);
 #pragma unroll
         for (int e = 0; e < 8; e++) {  // 16 dims: 32 bytes of a swizzled row, the upper 64 dims a half further
             const uint64_t at = ((e >> 2) * kHalf + (e & 3) * 32) >> 4;
             umma_ss(tmem + m * kTile + (u & 1) * kHalfTile, q + at, k + at, kQK, e != 0);
         }
-        umma_commit(bars + kSFull + 16 * m + 8 * (u & 1));
-        if (releases(m, u)) umma_commit(bars + kKEmpty + 8 * s);
         return true;
     };
-    bool ok = true;
+    bool ok = bar_wait_warp(bars + kQFull, 0, abort);
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int u = 0; u < 2; u++) {
+        if (ok && u < n) ok = qk(u);
+        umma_commit(bars + kSFull + 16 * m + 8 * u);
+        if (u < n && last_of_tile(u)) umma_commit(bars + kKEmpty + 8 * (W.tile(m, u) & 1));
+    }
+    for (int u = 0; ok && u < n; u++) {
+        const int tile = W.tile(m, u), s = tile & 1;
+        ok = ((u & 1) || bar_wait_warp(bars + kVFull + 8 * s, (tile >> 1) & 1, abort)) &&
+             bar_wait_warp(bars + kPFull + 16 * m + 8 * (u & 1), (u >> 1) & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t v = umma_desc(smem + kVOff + s * kOperand + (u & 1) * (kHalfTile * 128), kHalf, 1024);
 #pragma unroll
-        for (int m = 0; m < 2; m++)
-            if (ok && u < steps[m]) ok = qk(m, u);
-    for (int u = 0; ok && u < steps[0]; u++) {
-#pragma unroll
-        for (int m = 0; m < 2; m++) {
-            if (!ok || u >= steps[m]) continue;
-            const int tile = W.tile(m, u), s = tile & 1;
-            ok = bar_wait_warp(bars + kVFull + 8 * s, (tile >> 1) & 1, abort) &&
-                 bar_wait_warp(bars + kPFull + 16 * m + 8 * (u & 1), (u >> 1) & 1, abort);
-            if (!ok) continue;
-            tc_fence_after();
-            const uint64_t v = umma_desc(smem + kVOff + s * kOperand + (u & 1) * (kHalfTile * 128), kHalf, 1024);
-#pragma unroll
-            for (int e = 0; e < 4; e++)  // 16 tokens: two 8-row groups
-                umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + (u & 1) * kHalfTile + 8 * e, v + e * (2048 >> 4), kPV,
-                        u != 0 || e != 0);
-            umma_commit(bars + kODone + 8 * m);
-            if (releases(m, u)) umma_commit(bars + kVEmpty + 8 * s);
-            if (u + 2 < steps[m]) ok = qk(m, u + 2);
-        }
+        for (int e = 0; e < 4; e++)  // 16 tokens: two 8-row groups
+            umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + (u & 1) * kHalfTile + 8 * e, v + e * (2048 >> 4), kPV,
+                    u != 0 || e != 0);
+        if (u + 2 < n) ok = qk(u + 2);
+        umma_commit(bars + kSFull + 16 * m + 8 * (u & 1));
+        if (last_of_tile(u)) umma_commit(bars + kVEmpty + 8 * s);
+        if (u + 2 < n && last_of_tile(u + 2)) umma_commit(bars + kKEmpty + 8 * (W.tile(m, u + 2) & 1));
     }
     // every product has ended before the CTA frees its TMEM
-    umma_commit(bars + kDone);
-    bar_wait_warp(bars + kDone, 0, abort);
+    umma_commit(bars + kDone + 8 * m);
+    bar_wait_warp(bars + kDone + 8 * m, 0, abort);
 }
 
 // Running reference, sum and products of a row.
@@ -371,11 +373,11 @@ struct RowState {
 
 // Moves the reference of the rows whose exponents exceed it by more than
 // kSlack (or that see their first token), and scales what they have summed so
-// far: l, O (once the products before this step are in it: phase u - 1 of
-// `o_done`, phase u - 2 being over since these scores were announced), and the first 32 weights of this step if they are written.
+// far: l, O (once the products before this step are in it: event u + 1 of the
+// stream, on `ready`), and the first 32 weights of this step if they are written.
 // Rare.
 __device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32_t ts, uint32_t to, bool second, int u,
-                                       uint32_t o_done, volatile uint32_t* abort) {
+                                       uint32_t ready, volatile uint32_t* abort) {
     const float f = over && st.ref != -INFINITY ? ex2_approx(-top) : 1.0f;
     if (over) st.ref = (st.ref == -INFINITY ? 0.0f : st.ref) + top;
     st.l *= f;
@@ -389,7 +391,7 @@ __device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32
         for (int j = 0; j < 16; j++) p[j] = h2_as_u32(__hmul2(u32_as_h2(p[j]), f2));
         tmem_st16(ts, p);
     }
-    if (u > 0 && bar_wait_warp(o_done, (u - 1) & 1, abort)) {
+    if (u > 0 && bar_wait_warp(ready + 8 * ((u + 1) & 1), ((u + 1) >> 1) & 1, abort)) {
         tc_fence_after();
         for (int i = 0; i < kHeadDim; i += 16) {
             uint32_t o[16];
@@ -404,53 +406,51 @@ __device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32
     return st;
 }
 
-// The weights of a step's 64 tokens for this thread's row: p = exp2(s kfac -
-// ref) in place of the scores (columns 0 .. 31, two fp16 each), 32 tokens at a
-// time; the second 32 scores are loaded under the first exponentials.
+// Exponents of 32 scores of this thread's row, x = s kfac - ref, with the
+// reference moved where a row needs it.
+struct StepAt {
+    uint32_t ts, to;  // TMEM: this step's scores, the stream's O
+    int u;
+    uint32_t ready;   // the stream's s_full barriers
+    volatile uint32_t* abort;
+};
 template <bool MASK>
-__device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, float kfac, int lim, uint32_t pages, int u,
-                                      uint32_t o_done, volatile uint32_t* abort) {
+__device__ __forceinline__ void exponents(RowState& st, uint64_t (&x)[16], const uint32_t (&s)[32], float kfac, int q, int lim,
+                                          uint32_t pages, uint64_t& acc, const StepAt& at) {
     const uint64_t k2 = pack2(kfac, kfac);
-    uint64_t acc = pack2(0.0f, 0.0f);
-    uint32_t s[2][32];
-    tmem_ld32(s[0], ts);
+    const float r = st.ref == -INFINITY ? 0.0f : st.ref;
+    uint64_t r2 = pack2(-r, -r);
+    float top = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-        tmem_wait_ld();
-        const float r = st.ref == -INFINITY ? 0.0f : st.ref;
-        uint64_t r2 = pack2(-r, -r), x[16];
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            x[j] = fma2((uint64_t)s[q][2 * j] | ((uint64_t)s[q][2 * j + 1] << 32), k2, r2);
-            if constexpr (MASK) {
-                const int t = 32 * q + 2 * j;
-                const bool page = (pages >> (t >> 4)) & 1u;
-                x[j] = pack2(page && t < lim ? lo2(x[j]) : -INFINITY, page && t + 1 < lim ? hi2(x[j]) : -INFINITY);
-            }
-            top = fmaxf(top, fmaxf(lo2(x[j]), hi2(x[j])));
+    for (int j = 0; j < 16; j++) {
+        x[j] = fma2((uint64_t)s[2 * j] | ((uint64_t)s[2 * j + 1] << 32), k2, r2);
+        if constexpr (MASK) {
+            const int t = 32 * q + 2 * j;
+            const bool page = (pages >> (t >> 4)) & 1u;
+            x[j] = pack2(page && t < lim ? lo2(x[j]) : -INFINITY, page && t + 1 < lim ? hi2(x[j]) : -INFINITY);
         }
-        const bool over = top < INFINITY && (top > kSlack || (st.ref == -INFINITY && top > -INFINITY));
-        if (__any_sync(0xffffffffu, over)) {
-            st.l += lo2(acc) + hi2(acc);
-            acc = pack2(0.0f, 0.0f);
-            st = raise(st, top, over, ts, to, q > 0, u, o_done, abort);
-            r2 = over ? pack2(-top, -top) : acc;
-#pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = add2(x[j], r2);
-        }
-        if (q == 0) tmem_ld32(s[1], ts + 32);
-        uint32_t p[16];
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float a = ex2_approx(lo2(x[j])), b = ex2_approx(hi2(x[j]));
-            acc = add2(acc, pack2(a, b));
-            p[j] = h2_as_u32(__floats2half2_rn(a, b));
-        }
-        tmem_st16(ts + 16 * q, p);
+        top = fmaxf(top, fmaxf(lo2(x[j]), hi2(x[j])));
     }
-    st.l += lo2(acc) + hi2(acc);
-    tmem_wait_st();
+    const bool over = top < INFINITY && (top > kSlack || (st.ref == -INFINITY && top > -INFINITY));
+    if (__any_sync(0xffffffffu, over)) {
+        st.l += lo2(acc) + hi2(acc);
+        acc = pack2(0.0f, 0.0f);
+        st = raise(st, top, over, at.ts, at.to, q > 0, at.u, at.ready, at.abort);
+        r2 = over ? pack2(-top, -top) : acc;
+#pragma unroll
+        for (int j = 0; j < 16; j++) x[j] = add2(x[j], r2);
+    }
+}
+// Their weights p = 2^x: fp16 pairs in place of the scores, and the sum.
+__device__ __forceinline__ void weights(const uint64_t (&x)[16], uint64_t& acc, uint32_t to) {
+    uint32_t p[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const float a = ex2_approx(lo2(x[j])), b = ex2_approx(hi2(x[j]));
+        acc = add2(acc, pack2(a, b));
+        p[j] = h2_as_u32(__floats2half2_rn(a, b));
+    }
+    tmem_st16(to, p);
 }
 
 __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, uint8_t* smem, uint32_t bars, uint32_t tmem,
@@ -461,38 +461,70 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     const int local = (W.split ? 0 : m * kTile) + 32 * wq + lane;  // row of the CTA
     const bool live = local < W.rows;
     const int row = W.row0 + min(local, W.rows - 1);
-    const int b = (int)((uint32_t)row / (uint32_t)P.G), g = row - b * P.G;
+    const int b = (int)P.div_g.div((uint32_t)row), g = row - b * P.G;
     const float kfac = *reinterpret_cast<const float*>(smem + kAuxOff + 4 * ((W.split ? 0 : m * kTile) + 32 * wq + lane));
     // tokens of the chunk this row sees, from the chunk's start
     const int lim = min(__ldg(P.seq_lens + b), P.n_pages * kBlockSize) - W.t0 * kTile;
     const bool any_row = __any_sync(0xffffffffu, live);
     RowState st{-INFINITY, 0.0f};
     const int n = W.steps(m);
+    // A step's 64 scores in two halves; the loads of each half run under the
+    // exponentials of the one before, the next step's first half under this
+    // step's second where its scores are there by then (they wait for no
+    // weights of this step).
+    uint32_t s0[32], s1[32];
+    auto arrived = [&](int u) {
+        if (!bar_wait_warp(bars + kSFull + 16 * m + 8 * (u & 1), (u >> 1) & 1, abort)) return false;
+        tc_fence_after();
+        return true;
+    };
+    if (n > 0) {
+        if (!arrived(0)) return;
+        tmem_ld32(s0, ts);
+        tmem_wait_ld();
+    }
     for (int u = 0; u < n; u++) {
         const int tile = W.tile(m, u), half = u & 1;
-        if (!bar_wait_warp(bars + kSFull + 16 * m + 8 * half, (u >> 1) & 1, abort)) return;
-        tc_fence_after();
+        const bool next = u + 1 < n;
+        bool early = false;
         if (any_row) {
             const uint32_t pages = (smem[kBarOff + kMasks + 4 * (tile & 3)] | smem[kBarOff + kMasks + 4 * (tile & 3) + 1]) >>
                                    (kTilePages / 2 * half) & 0xFu;
             const int left = lim - tile * kTile - half * kHalfTile;
-            const uint32_t at = ts + half * kHalfTile;
-            if (__any_sync(0xffffffffu, left < kHalfTile || pages != 0xFu))
-                weigh<true>(st, at, to, kfac, left, pages, u, bars + kODone + 8 * m, abort);
+            const bool mask = __any_sync(0xffffffffu, left < kHalfTile || pages != 0xFu);
+            const StepAt at{ts + half * kHalfTile, to, u, bars + kSFull + 16 * m, abort};
+            uint64_t x[16], acc = pack2(0.0f, 0.0f);
+            if (mask)
+                exponents<true>(st, x, s0, kfac, 0, left, pages, acc, at);
             else
-                weigh<false>(st, at, to, kfac, left, pages, u, bars + kODone + 8 * m, abort);
+                exponents<false>(st, x, s0, kfac, 0, left, pages, acc, at);
+            tmem_ld32(s1, at.ts + 32);
+            weights(x, acc, at.ts);
+            tmem_wait_ld();
+            if (mask)
+                exponents<true>(st, x, s1, kfac, 1, left, pages, acc, at);
+            else
+                exponents<false>(st, x, s1, kfac, 1, left, pages, acc, at);
+            early = next && __all_sync(0xffffffffu, bar_try(bars + kSFull + 16 * m + 8 * (half ^ 1), ((u + 1) >> 1) & 1));
+            if (early) {
+                tc_fence_after();
+                tmem_ld32(s0, ts + (half ^ 1) * kHalfTile);
+            }
+            weights(x, acc, at.ts + 16);
+            tmem_wait_ld();
+            st.l += lo2(acc) + hi2(acc);
+            tmem_wait_st();
         }
         tc_fence_before();
         bar_arrive(bars + kPFull + 16 * m + 8 * half);
+        if (next && !early) {
+            if (!arrived(u + 1)) return;
+            tmem_ld32(s0, ts + (half ^ 1) * kHalfTile);
+            tmem_wait_ld();
+        }
     }
     // ---- the partial rows ----
-    // (the last scores say that the products up to step n - 3 are done: the
-    // two phases after it are waited for one by one)
-    if (n > 0) {
-        if (n > 1 && !bar_wait_warp(bars + kODone + 8 * m, (n - 2) & 1, abort)) return;
-        if (!bar_wait_warp(bars + kODone + 8 * m, (n - 1) & 1, abort)) return;
-        tc_fence_after();
-    }
+    if (n > 0 && !arrived(n + 1)) return;
     if (!any_row) return;
     const int sp = W.split ? 2 * (int)blockIdx.x + m : (int)blockIdx.x;
     const bool seen = st.l > 0.0f || st.l != st.l;
@@ -501,8 +533,19 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
     if (live) dst[kHeadDim] = seen ? (st.ref + lg2_approx(st.l)) * kLn2 : -INFINITY;
     // 32 x 32 blocks turn through shared memory (this stream's query tile, or
-    // the unused second one), so that rows are written in runs of 128 bytes
-    float* turn = reinterpret_cast<float*>(smem + kQOff + (W.split ? kOperand + m * kHalf : m * kOperand) + wq * 4096);
+    // the unused second one; 16-byte chunk c of row r at chunk c ^ (r & 7)), so
+    // that rows are written in runs of 128 bytes: four rows per 16-byte store
+    // where the rows are aligned (the partials' pitch is the caller's), one per
+    // 4-byte store otherwise.
+    uint8_t* turn = smem + kQOff + (W.split ? kOperand + m * kHalf : m * kOperand) + wq * 4096;
+    const bool vec = ((reinterpret_cast<uintptr_t>(P.mid) & 15) | ((P.msb | P.msh | P.mss) & 3)) == 0;
+    const unsigned long long mine = reinterpret_cast<unsigned long long>(dst);
+    float* rows[8];
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            rows[i] = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, 4 * i + (lane >> 3))) + 4 * (lane & 7);
+    }
 #pragma unroll 1
     for (int q = 0; q < 4; q++) {
         uint32_t o[32];
@@ -511,24 +554,86 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
             tmem_wait_ld();
         }
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const int d = (j & ~7) | ((j & 1) << 2) | ((j & 7) >> 1);  // column j of O is dim d
-            turn[32 * lane + (d ^ lane)] = seen ? __uint_as_float(o[j]) * inv : 0.0f;
+        for (int c = 0; c < 8; c++) {  // dims 4c .. 4c + 3: every other column of the group of 8, from c & 1 on
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                v[j] = seen ? __uint_as_float(o[(c >> 1) * 8 + 2 * j + (c & 1)]) * inv : 0.0f;
+            *reinterpret_cast<float4*>(turn + 128 * lane + ((c ^ (lane & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
         }
         __syncwarp();
-#pragma unroll 8
-        for (int r = 0; r < 32; r++) {
-            float* to_row = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
-            const float v = turn[32 * r + (lane ^ r)];
-            if ((live_rows >> r) & 1u) to_row[32 * q + lane] = v;
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int r = 4 * i + (lane >> 3);
+                const float4 v = *reinterpret_cast<const float4*>(turn + 128 * r + (((lane & 7) ^ (r & 7)) << 4));
+                if ((live_rows >> r) & 1u) *reinterpret_cast<float4*>(rows[i] + 32 * q) = v;
+            }
+        } else {
+            for (int r = 0; r < 32; r++) {
+                float* to_row = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, r));
+                const float v = *reinterpret_cast<const float*>(turn + 128 * r + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
+                if ((live_rows >> r) & 1u) to_row[32 * q + lane] = v;
+            }
         }
         __syncwarp();
     }
 }
 
+// K table: entry = two codes, {c[low], c[high]} in fp16, a copy per lane.  A
+// producer warp makes 64 entries (16 for 3-bit codes), a lane each or two, and
+// spreads them over the copies.
+template <int L>
+__device__ __forceinline__ void build_table(const PrefixParams& P, uint8_t* smem, int pw, int lane) {
+    constexpr bool k3 = layout_3bit_keys(L);
+    constexpr int kPairs = k3 ? 64 : 256, kBits = k3 ? 3 : 4, kMask = k3 ? 7 : 15, kMine = kPairs / kProducerWarps;
+#pragma unroll
+    for (int e0 = 0; e0 < kMine; e0 += 16) {
+        const int pair = kMine * pw + e0 + (lane & 15);
+        const uint32_t v = h2_as_u32(__floats2half2_rn(__ldg(P.cents + (pair & kMask)), __ldg(P.cents + (pair >> kBits))));
+        uint32_t* lut = reinterpret_cast<uint32_t*>(smem + kLutOff) + (kMine * pw + e0) * 32 + lane;
+#pragma unroll
+        for (int i = 0; i < 16; i++) lut[32 * i] = __shfl_sync(0xffffffffu, v, i);
+    }
+}
+
+// Queries: fp16, scaled per row into [2^14, 2^15), 128-byte swizzle, and the
+// rows' score factors.  A softmax warp takes rows warp, warp + 8, ..., 16 of
+// them in flight.
+__device__ __forceinline__ void load_queries(const PrefixParams& P, const Place& W, uint8_t* smem, int warp, int lane) {
+    const int slots = W.split || W.rows <= kTile ? kTile : 2 * kTile;
+    for (int r0 = warp; r0 < slots; r0 += 16 * kSoftmaxWarps) {
+        float4 x[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int r = r0 + i * kSoftmaxWarps;
+            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r < W.rows) {
+                const int row = W.row0 + r, b = (int)P.div_g.div((uint32_t)row), g = row - b * P.G;
+                x[i] = __ldg(reinterpret_cast<const float4*>(P.q + (int64_t)b * P.qsb + (int64_t)(W.h * P.G + g) * P.qsh) + lane);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int r = r0 + i * kSoftmaxWarps;
+            // (bits of non-negative floats order as the floats do)
+            const float amax = __uint_as_float(__reduce_max_sync(
+                0xffffffffu,
+                __float_as_uint(fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))))));
+            const int e = fp16_scale_exp(amax);
+            const float f = exp2i(e);
+            if (lane == 0) reinterpret_cast<float*>(smem + kAuxOff)[r] = P.scale * kLog2e * exp2i(-e);
+            // dims 4 lane .. 4 lane + 3: half lane / 16, chunk (lane % 16) / 2
+            uint8_t* at = smem + kQOff + (r >> 7) * kOperand + (lane >> 4) * kHalf + (r & 127) * 128 +
+                          ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+            *reinterpret_cast<uint2*>(at) = make_uint2(h2_as_u32(__floats2half2_rn(x[i].x * f, x[i].y * f)),
+                                                       h2_as_u32(__floats2half2_rn(x[i].z * f, x[i].w * f)));
+        }
+    }
+}
+
 template <int L>
 __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixParams P) {
-    constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L);
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t base = smem_addr(smem), bars = base + kBarOff;
@@ -546,86 +651,57 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
     W.split = P.split != 0;
 
     if (tid == 0) {
+        const int readers = !W.split && W.rows > kTile ? 2 : 1;  // streams that read each stage
         for (int s = 0; s < 2; s++) {
             bar_init(bars + kKFull + 8 * s, kProducerWarps * 32);
             bar_init(bars + kVFull + 8 * s, kProducerWarps * 32);
-            bar_init(bars + kKEmpty + 8 * s, 1);
-            bar_init(bars + kVEmpty + 8 * s, 1);
+            bar_init(bars + kKEmpty + 8 * s, readers);
+            bar_init(bars + kVEmpty + 8 * s, readers);
             for (int b = 0; b < 16; b += 8) {
                 bar_init(bars + kSFull + 16 * s + b, 1);
                 bar_init(bars + kPFull + 16 * s + b, 128);
             }
-            bar_init(bars + kODone + 8 * s, 1);
+            bar_init(bars + kDone + 8 * s, 1);
         }
-        bar_init(bars + kDone, 1);
+        bar_init(bars + kQFull, kSoftmaxWarps * 32);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == kSoftmaxWarps + kProducerWarps) tmem_alloc<512>(bars + kTmem);
-    pdl_wait();  // the rotated queries, and the kernel before that reads mid_o
-
-    // ---- K table: entry = two codes, {c[low], c[high]} in fp16, a copy per lane
-    if constexpr (!k8) {
-        // a warp makes 16 entries, a lane each, and spreads them over the copies
-        constexpr int kPairs = k3 ? 64 : 256, kBits = k3 ? 3 : 4, kMask = k3 ? 7 : 15;
-        static_assert(kPrefixThreads / 32 * 16 >= kPairs, "one round of the warps");
-        if (warp < kPairs / 16) {
-            const int pair = 16 * warp + (lane & 15);
-            const uint32_t v = h2_as_u32(__floats2half2_rn(__ldg(P.cents + (pair & kMask)), __ldg(P.cents + (pair >> kBits))));
-            uint32_t* lut = reinterpret_cast<uint32_t*>(smem + kLutOff) + 16 * warp * 32 + lane;
-#pragma unroll
-            for (int i = 0; i < 16; i++) lut[32 * i] = __shfl_sync(0xffffffffu, v, i);
-        }
-    }
-    // ---- queries: fp16, scaled per row into [2^14, 2^15), 128-byte swizzle;
-    // a warp takes rows warp, warp + 16, ..., eight of them in flight
-    const int slots = W.split || W.rows <= kTile ? kTile : 2 * kTile;
-    for (int r0 = warp; r0 < slots; r0 += 8 * (kPrefixThreads / 32)) {
-        float4 x[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int r = r0 + i * (kPrefixThreads / 32);
-            x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (r < W.rows) {
-                const int row = W.row0 + r, b = (int)((uint32_t)row / (uint32_t)P.G), g = row - b * P.G;
-                x[i] = __ldg(reinterpret_cast<const float4*>(P.q + (int64_t)b * P.qsb + (int64_t)(W.h * P.G + g) * P.qsh) + lane);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int r = r0 + i * (kPrefixThreads / 32);
-            const float amax = warp_max_xor(fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))), 1, 16);
-            const int e = fp16_scale_exp(amax);
-            const float f = exp2i(e);
-            if (lane == 0) reinterpret_cast<float*>(smem + kAuxOff)[r] = P.scale * kLog2e * exp2i(-e);
-            // dims 4 lane .. 4 lane + 3: half lane / 16, chunk (lane % 16) / 2
-            uint8_t* at = smem + kQOff + (r >> 7) * kOperand + (lane >> 4) * kHalf + (r & 127) * 128 +
-                          ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
-            *reinterpret_cast<uint2*>(at) = make_uint2(h2_as_u32(__floats2half2_rn(x[i].x * f, x[i].y * f)),
-                                                       h2_as_u32(__floats2half2_rn(x[i].z * f, x[i].w * f)));
-        }
-    }
-    fence_async_smem();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kTmem), 0);
+    pdl_wait();  // the rotated queries, and the kernel before that reads mid_o
+
+    // All 512 columns start at column 0: a constant, so that the MMAs' TMEM
+    // operands need no register (checked, as an error that ends the waits).
+    constexpr uint32_t tmem = 0;
+    if (tid == 0 && *reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kTmem) != tmem) *abort = 1;
 
     if (warp < kSoftmaxWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
+        load_queries(P, W, smem, warp, lane);
+        fence_async_smem();
+        bar_arrive(bars + kQFull);
+        asm volatile("bar.sync 1, %0;\n" ::"n"(kSoftmaxWarps * 32) : "memory");  // the rows' score factors
         softmax(P, W, smem, bars, tmem, abort, warp >> 2, warp, lane);
     } else if (warp < kSoftmaxWarps + kProducerWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kProducerRegs));
+        if constexpr (!layout_fp8_keys(L)) {
+            build_table<L>(P, smem, warp - kSoftmaxWarps, lane);
+            asm volatile("bar.sync 2, %0;\n" ::"n"(kProducerWarps * 32) : "memory");
+        }
         dequantise<L>(P, W, smem, bars, abort, warp - kSoftmaxWarps, lane);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegs));
-        if (warp == kSoftmaxWarps + kProducerWarps) issue(W, base, bars, tmem, abort);
+        if (warp == kSoftmaxWarps + kProducerWarps) issue(W, base, bars, tmem, abort, 0);
+        if (warp == kSoftmaxWarps + kProducerWarps + 1) issue(W, base, bars, tmem, abort, 1);
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == kSoftmaxWarps + kProducerWarps) tmem_free<512>(tmem);
+    if (warp == kSoftmaxWarps + kProducerWarps) tmem_free<512>(*reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kTmem));
     if (tid == 0 && *abort != 0) atomicAdd(&g_prefix_timeouts, 1u);
 }
 

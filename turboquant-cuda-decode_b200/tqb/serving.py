@@ -29,6 +29,7 @@ from .ops import _DTYPE_ID, _SOA_FAMILY, _block_dense
 
 _F32, _U8, _I32, _I64 = torch.float32, torch.uint8, torch.int32, torch.int64
 _FOLDED = (LAYOUT_SOA, LAYOUT_SOA_K3, LAYOUT_SOA_K3V3)  # the stored norm may hold the norm correction
+_PITCH = HEAD_DIM + 4  # floats of a partial row in the calls' own workspace: 129, and rows of whole 16 bytes
 _SPLIT_TOKENS = 64    # shortest split worth its partial rows (516 bytes written and read per query head)
 _SPLIT_ITEMS = 2368   # (sequence, KV head, split) items of one round of the Stage1 grid: 148 CTAs x 2 groups x 8 warps
 
@@ -304,7 +305,7 @@ class _Step:
     def workspace(self, S: int) -> None:
         """Room for S splits; the query rows that Stage1 reads."""
         rows = self.B * self.Hq
-        need = 0 if self.mid_o is not None else rows * S * (HEAD_DIM + 1)
+        need = 0 if self.mid_o is not None else rows * S * _PITCH
         lse_at, need = need, need + (0 if self.lse else rows)
         q_at = need = (need + 31) // 32 * 32
         # queries that need no rotation are read as they are where Stage1 can (fp32, 16-byte aligned rows)
@@ -315,7 +316,7 @@ class _Step:
         self.keep = ws = torch.empty(max(need, 1), dtype=_F32, device=q.device)
         base = ws.data_ptr()
         if self.mid_o is None:
-            self.mid, self.ms = base, (self.Hq * S * (HEAD_DIM + 1), S * (HEAD_DIM + 1), HEAD_DIM + 1)
+            self.mid, self.ms = base, (self.Hq * S * _PITCH, S * _PITCH, _PITCH)
         else:
             m = self.mid_o
             if m.dim() != 4 or m.shape[0] < self.B or m.shape[1] < self.Hq or m.shape[2] < S or \
