@@ -11,18 +11,21 @@
 // dequantises a 128-token tile once for up to 256 rows.
 //
 // One CTA per SM, one (chunk, KV head, block of 256 rows); warps:
-//   0-3, 4-7   softmax of streams 0 and 1: thread = row (= TMEM lane).  A
-//              stream is 128 rows over every tile, or with at most 128 rows
-//              the same rows over the even or the odd tiles, so that two
-//              tiles are always in flight;
+//   0-3, 4-7   streams 0 and 1: thread = row (= TMEM lane).  A stream is 128
+//              rows over every tile, or with at most 128 rows the same rows
+//              over the even or the odd tiles, so that two tiles are always in
+//              flight.  Its four warps weigh a tile's scores, then its first
+//              warp issues the products of these weights and the next tile's
+//              scores;
 //   8-11       dequantise K and V tiles (fp16, 128-byte swizzle) into two
-//              stages of shared memory, the next tile's codes in registers;
-//   12, 13     issue the MMAs of a stream each (14, 15 idle): S = Q K^T (operands in shared
-//              memory), then O += P V with P in TMEM where S was.
-// A stream goes by half tiles of 64 tokens with two S buffers, so the next
-// half's scores are there when the softmax of this one ends (with one S per
-// stream of 128 tokens, softmax and MMAs took turns: 5300 cycles a tile for
-// 2800 of softmax).  TMEM: 2 x 2 S of 64 columns, 2 O of 128: all 512.
+//              stages of shared memory, the next tile's codes in registers.
+// S = Q K^T has its operands in shared memory; P overwrites S in TMEM and is
+// the A operand of O += P V there.  One stream's MMAs run under the other's
+// softmax.  TMEM: S0 S1 O0 O1 of 128 columns each, all 512, so there is one S
+// per stream.  (Measured at 256 rows x 32768 tokens x 8 heads, us: 57 with
+// warps of their own that issue, whose waits and commits cost 130 and 200
+// cycles each on the way from P to S; 52 with half tiles and two S per stream,
+// a 128 x 64 x 16 product taking the tensor core as long as 128 x 128 x 16.)
 //
 // Precision: Q (scaled per row by a power of two), K = c norm, V = code scale
 // + zero and P are rounded to fp16, each product accumulated in fp32; m, l, O
@@ -58,20 +61,19 @@ constexpr int kBarOff = kAuxOff + 2 * kTile * 4;
 constexpr int kPrefixSmem = kBarOff + 192;
 static_assert(kPrefixSmem <= 232448, "shared memory per CTA");
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 4;
-constexpr int kPrefixThreads = (kSoftmaxWarps + kProducerWarps + 4) * 32;  // whole warpgroups
-// Registers per thread: 128 at the launch, moved between the warpgroups by
-// setmaxnreg (the shares add up to the launch's).
-constexpr int kPrefixRegs = 128, kSoftmaxRegs = 168, kProducerRegs = 112, kIssueRegs = 64;
-static_assert(2 * kSoftmaxRegs + kProducerRegs + kIssueRegs <= 4 * kPrefixRegs && kPrefixRegs * kPrefixThreads <= 65536,
-              "register split");
+constexpr int kPrefixThreads = (kSoftmaxWarps + kProducerWarps) * 32;  // whole warpgroups
+// Registers per thread: 168 at the launch (the most that 384 threads can
+// have), moved between the warpgroups by setmaxnreg (the shares add up to the
+// launch's).
+constexpr int kPrefixRegs = 168, kSoftmaxRegs = 200, kProducerRegs = 104;
+static_assert(2 * kSoftmaxRegs + kProducerRegs <= 3 * kPrefixRegs && kPrefixRegs * kPrefixThreads <= 65536, "register split");
 constexpr float kSlack = 8.0f;
 
 // Barriers (8 bytes each) at kBarOff, then words.
-// Two of each: stages of K and V, S and P per stream m and buffer b (at 16 m +
-// 8 b), the end of a stream's products.
-enum : uint32_t { kKFull = 0, kVFull = 16, kKEmpty = 32, kVEmpty = 48, kSFull = 64, kPFull = 96, kDone = 128,
-                  kQFull = 144, kMasks = 152, kTmem = 168, kAbort = 172 };
-constexpr int kHalfTile = kTile / 2;  // tokens of a softmax step
+// Two of each: stages of K and V, S and the last products (after an error) per
+// stream.
+enum : uint32_t { kKFull = 0, kVFull = 16, kKEmpty = 32, kVEmpty = 48, kSFull = 64, kDone = 80, kMasks = 96, kTmem = 112,
+                  kAbort = 116 };
 
 
 __device__ __forceinline__ uint32_t dup16(uint32_t h) { return __byte_perm(h, 0u, 0x1010); }
@@ -239,19 +241,13 @@ __device__ __forceinline__ void put_v(uint8_t* smem, uint32_t tile, const RawV& 
     }
 }
 
-// Where a CTA works: its n tiles from t0 on (`tokens` of them tokens of the
-// prefix) and rows [row0, row0 + rows), and the half tiles of a stream (of
-// every tile, or with `split` of every other one).
+// Where a CTA works: its n tiles from t0 on and rows [row0, row0 + rows), and
+// the tiles of a stream (every tile, or with `split` every other one).
 struct Place {
-    int h, t0, n, tokens, row0, rows;
+    int h, t0, n, row0, rows;
     bool split;
-    __device__ __forceinline__ int tiles(int m) const { return split ? (n + 1 - m) / 2 : (m == 0 || rows > kTile ? n : 0); }
-    // half step u of stream m: tile (from t0 on), then the number of steps
-    __device__ __forceinline__ int tile(int m, int u) const { return split ? 2 * (u >> 1) + m : u >> 1; }
-    __device__ __forceinline__ int steps(int m) const {
-        const int t = tiles(m);  // the chunk's last tile may have one half only
-        return 2 * t - (t > 0 && tile(m, 2 * t - 2) == n - 1 && tokens <= (n - 1) * kTile + kHalfTile ? 1 : 0);
-    }
+    __device__ __forceinline__ int steps(int m) const { return split ? (n + 1 - m) / 2 : (m == 0 || rows > kTile ? n : 0); }
+    __device__ __forceinline__ int tile(int m, int u) const { return split ? 2 * u + m : u; }  // from t0 on
 };
 
 template <int L>
@@ -311,88 +307,67 @@ __device__ __forceinline__ void dequantise(const PrefixParams& P, const Place& W
     }
 }
 
-// The MMA warp of stream m.  Its MMAs execute in the order of issue, so the
-// scores of step u + 2 may follow P V of step u on the same columns, and the
-// one commit behind both (event u + 2 of the stream, on s_full) also says that
-// the products up to step u are in O; events n and n + 1 say only that.  A warp
-// per stream, and few waits and commits: those cost 130 and 200 cycles each
-// where the 12 MMAs of a step take 300 to issue.
-__device__ __forceinline__ void issue(const Place& W, uint32_t smem, uint32_t bars, uint32_t tmem, volatile uint32_t* abort,
-                                      const int m) {
-    constexpr uint32_t kQK = umma_idesc(kTile, kHalfTile, false), kPV = umma_idesc(kTile, kHeadDim, true);
-    const int n = W.steps(m);
-    if (n == 0) return;
-    const uint64_t q = umma_desc(smem + kQOff + (W.split ? 0 : m * kOperand), 16, 1024);
-    auto last_of_tile = [&](int u) { return (u & 1) || u + 1 == n; };
-    auto qk = [&](int u) {
+// The products of a stream, issued by its first warp (converged).  They execute
+// in the order of issue, so the scores of step u + 1 may follow P V of step u on
+// the same columns, and the one commit behind both (event u + 1 of the stream,
+// on s_full) also says that the products up to step u are in O; event n says
+// only that.
+struct Products {
+    uint32_t smem, bars, tmem, m;
+    volatile uint32_t* abort;
+    const Place& W;
+
+    __device__ __forceinline__ bool scores(int u) const {  // S = Q K^T of step u
+        constexpr uint32_t kQK = umma_idesc(kTile, kTile, false);
         const int tile = W.tile(m, u), s = tile & 1;
-        if (!(u & 1)) {
-            if (!bar_wait_warp(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
-            tc_fence_after();
-        }
-        const uint64_t k = umma_desc(smem + kKOff + s * kOperand + (u & 1) * (kHalfTile * 128), 16, 1024);
+        if (!bar_wait_warp(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
+        tc_fence_after();
+        const uint64_t q = umma_desc(smem + kQOff + (W.split ? 0 : m * kOperand), 16, 1024);
+        const uint64_t k = umma_desc(smem + kKOff + s * kOperand, 16, 1024);
 #pragma unroll
         for (int e = 0; e < 8; e++) {  // 16 dims: 32 bytes of a swizzled row, the upper 64 dims a half further
             const uint64_t at = ((e >> 2) * kHalf + (e & 3) * 32) >> 4;
-            umma_ss(tmem + m * kTile + (u & 1) * kHalfTile, q + at, k + at, kQK, e != 0);
+            umma_ss(tmem + m * kTile, q + at, k + at, kQK, e != 0);
         }
         return true;
-    };
-    bool ok = bar_wait_warp(bars + kQFull, 0, abort);
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-        if (ok && u < n) ok = qk(u);
-        umma_commit(bars + kSFull + 16 * m + 8 * u);
-        if (u < n && last_of_tile(u)) umma_commit(bars + kKEmpty + 8 * (W.tile(m, u) & 1));
     }
-    for (int u = 0; ok && u < n; u++) {
+    __device__ __forceinline__ bool begin() const {
+        if (!scores(0)) return false;
+        umma_commit(bars + kSFull + 8 * m);
+        umma_commit(bars + kKEmpty + 8 * (W.tile(m, 0) & 1));
+        return true;
+    }
+    __device__ __forceinline__ bool step(int u, int n) const {  // O += P V of step u, S of step u + 1
+        constexpr uint32_t kPV = umma_idesc(kTile, kHeadDim, true);
         const int tile = W.tile(m, u), s = tile & 1;
-        ok = ((u & 1) || bar_wait_warp(bars + kVFull + 8 * s, (tile >> 1) & 1, abort)) &&
-             bar_wait_warp(bars + kPFull + 16 * m + 8 * (u & 1), (u >> 1) & 1, abort);
-        if (!ok) break;
+        if (!bar_wait_warp(bars + kVFull + 8 * s, (tile >> 1) & 1, abort)) return false;
         tc_fence_after();
-        const uint64_t v = umma_desc(smem + kVOff + s * kOperand + (u & 1) * (kHalfTile * 128), kHalf, 1024);
+        const uint64_t v = umma_desc(smem + kVOff + s * kOperand, kHalf, 1024);
 #pragma unroll
-        for (int e = 0; e < 4; e++)  // 16 tokens: two 8-row groups
-            umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + (u & 1) * kHalfTile + 8 * e, v + e * (2048 >> 4), kPV,
-                    u != 0 || e != 0);
-        if (u + 2 < n) ok = qk(u + 2);
-        umma_commit(bars + kSFull + 16 * m + 8 * (u & 1));
-        if (last_of_tile(u)) umma_commit(bars + kVEmpty + 8 * s);
-        if (u + 2 < n && last_of_tile(u + 2)) umma_commit(bars + kKEmpty + 8 * (W.tile(m, u + 2) & 1));
+        for (int e = 0; e < 8; e++)  // 16 tokens: two 8-row groups
+            umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + 8 * e, v + e * (2048 >> 4), kPV, u != 0 || e != 0);
+        if (u + 1 < n && !scores(u + 1)) return false;
+        umma_commit(bars + kSFull + 8 * m);
+        umma_commit(bars + kVEmpty + 8 * s);
+        if (u + 1 < n) umma_commit(bars + kKEmpty + 8 * (W.tile(m, u + 1) & 1));
+        return true;
     }
-    // every product has ended before the CTA frees its TMEM
-    umma_commit(bars + kDone + 8 * m);
-    bar_wait_warp(bars + kDone + 8 * m, 0, abort);
-}
+};
 
-// Running reference, sum and products of a row.
+// Running reference and sum of a row.
 struct RowState {
     float ref, l;
 };
 
 // Moves the reference of the rows whose exponents exceed it by more than
 // kSlack (or that see their first token), and scales what they have summed so
-// far: l, O (once the products before this step are in it: event u + 1 of the
-// stream, on `ready`), and the first 32 weights of this step if they are written.
-// Rare.
-__device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32_t ts, uint32_t to, bool second, int u,
-                                       uint32_t ready, volatile uint32_t* abort) {
+// far: l and O (whose earlier products are in it since these scores were
+// announced).  Rare.
+__device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32_t to, bool has_o) {
     const float f = over && st.ref != -INFINITY ? ex2_approx(-top) : 1.0f;
     if (over) st.ref = (st.ref == -INFINITY ? 0.0f : st.ref) + top;
     st.l *= f;
-    if (second) {
-        tmem_wait_st();  // the weights just written
-        const __half2 f2 = __float2half2_rn(f);
-        uint32_t p[16];
-        tmem_ld16(p, ts);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; j++) p[j] = h2_as_u32(__hmul2(u32_as_h2(p[j]), f2));
-        tmem_st16(ts, p);
-    }
-    if (u > 0 && bar_wait_warp(ready + 8 * ((u + 1) & 1), ((u + 1) >> 1) & 1, abort)) {
-        tc_fence_after();
+    if (has_o) {
         for (int i = 0; i < kHeadDim; i += 16) {
             uint32_t o[16];
             tmem_ld16(o, to + i);
@@ -401,59 +376,66 @@ __device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32
             for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
             tmem_st16(to + i, o);
         }
+        tmem_wait_st();
     }
-    tmem_wait_st();
     return st;
 }
 
-// Exponents of 32 scores of this thread's row, x = s kfac - ref, with the
-// reference moved where a row needs it.
-struct StepAt {
-    uint32_t ts, to;  // TMEM: this step's scores, the stream's O
-    int u;
-    uint32_t ready;   // the stream's s_full barriers
-    volatile uint32_t* abort;
-};
+// A tile's scores of this thread's row turned into weights p = exp2(s kfac -
+// ref) in their place (columns 0 .. 63, two fp16 each).  The whole row is in
+// registers: one load, one vote on the reference, then the exponentials
+// without a break.
 template <bool MASK>
-__device__ __forceinline__ void exponents(RowState& st, uint64_t (&x)[16], const uint32_t (&s)[32], float kfac, int q, int lim,
-                                          uint32_t pages, uint64_t& acc, const StepAt& at) {
+__device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, bool has_o, float kfac, int lim,
+                                      uint32_t pages) {
     const uint64_t k2 = pack2(kfac, kfac);
     const float r = st.ref == -INFINITY ? 0.0f : st.ref;
-    uint64_t r2 = pack2(-r, -r);
-    float top = -INFINITY;
+    const uint64_t r2 = pack2(-r, -r);
+    uint32_t s[4][32];
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-        x[j] = fma2((uint64_t)s[2 * j] | ((uint64_t)s[2 * j + 1] << 32), k2, r2);
-        if constexpr (MASK) {
-            const int t = 32 * q + 2 * j;
-            const bool page = (pages >> (t >> 4)) & 1u;
-            x[j] = pack2(page && t < lim ? lo2(x[j]) : -INFINITY, page && t + 1 < lim ? hi2(x[j]) : -INFINITY);
+    for (int q = 0; q < 4; q++) tmem_ld32(s[q], ts + 32 * q);
+    tmem_wait_ld();
+    uint64_t x[4][16];
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            x[q][j] = fma2((uint64_t)s[q][2 * j] | ((uint64_t)s[q][2 * j + 1] << 32), k2, r2);
+            if constexpr (MASK) {
+                const int t = 32 * q + 2 * j;
+                const bool page = (pages >> (t >> 4)) & 1u;
+                x[q][j] = pack2(page && t < lim ? lo2(x[q][j]) : -INFINITY, page && t + 1 < lim ? hi2(x[q][j]) : -INFINITY);
+            }
+            tops[q] = fmaxf(tops[q], fmaxf(lo2(x[q][j]), hi2(x[q][j])));
         }
-        top = fmaxf(top, fmaxf(lo2(x[j]), hi2(x[j])));
-    }
+    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     const bool over = top < INFINITY && (top > kSlack || (st.ref == -INFINITY && top > -INFINITY));
     if (__any_sync(0xffffffffu, over)) {
-        st.l += lo2(acc) + hi2(acc);
-        acc = pack2(0.0f, 0.0f);
-        st = raise(st, top, over, at.ts, at.to, q > 0, at.u, at.ready, at.abort);
-        r2 = over ? pack2(-top, -top) : acc;
+        st = raise(st, top, over, to, has_o);
+        const uint64_t t2 = over ? pack2(-top, -top) : pack2(0.0f, 0.0f);
 #pragma unroll
-        for (int j = 0; j < 16; j++) x[j] = add2(x[j], r2);
-    }
-}
-// Their weights p = 2^x: fp16 pairs in place of the scores, and the sum.
-__device__ __forceinline__ void weights(const uint64_t (&x)[16], uint64_t& acc, uint32_t to) {
-    uint32_t p[16];
+        for (int q = 0; q < 4; q++)
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-        const float a = ex2_approx(lo2(x[j])), b = ex2_approx(hi2(x[j]));
-        acc = add2(acc, pack2(a, b));
-        p[j] = h2_as_u32(__floats2half2_rn(a, b));
+            for (int j = 0; j < 16; j++) x[q][j] = add2(x[q][j], t2);
     }
-    tmem_st16(to, p);
+    uint64_t acc = pack2(0.0f, 0.0f);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        uint32_t p[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float a = ex2_approx(lo2(x[q][j])), b = ex2_approx(hi2(x[q][j]));
+            acc = add2(acc, pack2(a, b));
+            p[j] = h2_as_u32(__floats2half2_rn(a, b));
+        }
+        tmem_st16(ts + 16 * q, p);
+    }
+    st.l += lo2(acc) + hi2(acc);
+    tmem_wait_st();
 }
 
-__device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, uint8_t* smem, uint32_t bars, uint32_t tmem,
+__device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, uint8_t* smem, uint32_t smem_base, uint32_t bars, uint32_t tmem,
                         volatile uint32_t* abort, int m, int warp, int lane) {
     const int wq = warp & 3;
     const uint32_t lanes = (uint32_t)(32 * wq) << 16;
@@ -468,63 +450,45 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     const bool any_row = __any_sync(0xffffffffu, live);
     RowState st{-INFINITY, 0.0f};
     const int n = W.steps(m);
-    // A step's 64 scores in two halves; the loads of each half run under the
-    // exponentials of the one before, the next step's first half under this
-    // step's second where its scores are there by then (they wait for no
-    // weights of this step).
-    uint32_t s0[32], s1[32];
-    auto arrived = [&](int u) {
-        if (!bar_wait_warp(bars + kSFull + 16 * m + 8 * (u & 1), (u >> 1) & 1, abort)) return false;
+    const Products mma{smem_base, bars, tmem, (uint32_t)m, abort, W};
+    bool ok = true;
+    if (n > 0 && wq == 0) ok = mma.begin();
+    // The streams take turns at weighing: on their own they fall into step,
+    // both weighing (sharing the exponential units) and then both waiting for
+    // their products; in turns one's products run under the other's weighing.
+    // Stream m's steps are its turns on barrier 5 + m, stream 0 first (its
+    // count of steps is stream 1's or one more).
+    const int other = W.steps(1 - m);
+    const bool turns = n > 0 && other > 0;
+    if (turns && m == 1) asm volatile("bar.arrive 5, 256;\n" ::: "memory");
+    for (int u = 0; u < n; u++) {  // every warp takes every turn at the barrier, also when a wait has given up
+        const int tile = W.tile(m, u);
+        ok = ok && bar_wait_warp(bars + kSFull + 8 * m, u & 1, abort);
         tc_fence_after();
-        return true;
-    };
-    if (n > 0) {
-        if (!arrived(0)) return;
-        tmem_ld32(s0, ts);
-        tmem_wait_ld();
-    }
-    for (int u = 0; u < n; u++) {
-        const int tile = W.tile(m, u), half = u & 1;
-        const bool next = u + 1 < n;
-        bool early = false;
-        if (any_row) {
-            const uint32_t pages = (smem[kBarOff + kMasks + 4 * (tile & 3)] | smem[kBarOff + kMasks + 4 * (tile & 3) + 1]) >>
-                                   (kTilePages / 2 * half) & 0xFu;
-            const int left = lim - tile * kTile - half * kHalfTile;
-            const bool mask = __any_sync(0xffffffffu, left < kHalfTile || pages != 0xFu);
-            const StepAt at{ts + half * kHalfTile, to, u, bars + kSFull + 16 * m, abort};
-            uint64_t x[16], acc = pack2(0.0f, 0.0f);
-            if (mask)
-                exponents<true>(st, x, s0, kfac, 0, left, pages, acc, at);
+        if (turns) asm volatile("bar.sync %0, 256;\n" ::"r"(5 + m) : "memory");
+        if (ok && any_row) {
+            const uint32_t pages = smem[kBarOff + kMasks + 4 * (tile & 3)] | smem[kBarOff + kMasks + 4 * (tile & 3) + 1];
+            const int left = lim - tile * kTile;
+            if (__any_sync(0xffffffffu, left < kTile || pages != 0xFFu))
+                weigh<true>(st, ts, to, u > 0, kfac, left, pages);
             else
-                exponents<false>(st, x, s0, kfac, 0, left, pages, acc, at);
-            tmem_ld32(s1, at.ts + 32);
-            weights(x, acc, at.ts);
-            tmem_wait_ld();
-            if (mask)
-                exponents<true>(st, x, s1, kfac, 1, left, pages, acc, at);
-            else
-                exponents<false>(st, x, s1, kfac, 1, left, pages, acc, at);
-            early = next && __all_sync(0xffffffffu, bar_try(bars + kSFull + 16 * m + 8 * (half ^ 1), ((u + 1) >> 1) & 1));
-            if (early) {
-                tc_fence_after();
-                tmem_ld32(s0, ts + (half ^ 1) * kHalfTile);
-            }
-            weights(x, acc, at.ts + 16);
-            tmem_wait_ld();
-            st.l += lo2(acc) + hi2(acc);
-            tmem_wait_st();
+                weigh<false>(st, ts, to, u > 0, kfac, left, pages);
         }
+        if (u + m < other) asm volatile("bar.arrive %0, 256;\n" ::"r"(6 - m) : "memory");
         tc_fence_before();
-        bar_arrive(bars + kPFull + 16 * m + 8 * half);
-        if (next && !early) {
-            if (!arrived(u + 1)) return;
-            tmem_ld32(s0, ts + (half ^ 1) * kHalfTile);
-            tmem_wait_ld();
-        }
+        asm volatile("bar.sync %0, 128;\n" ::"r"(3 + m) : "memory");  // the stream's weights are complete
+        if (wq == 0 && ok) ok = mma.step(u, n);
     }
     // ---- the partial rows ----
-    if (n > 0 && !arrived(n + 1)) return;
+    // (also: every product has ended before the CTA frees its TMEM)
+    if (n > 0 && !(ok && bar_wait_warp(bars + kSFull + 8 * m, n & 1, abort))) {
+        if (wq == 0) {  // what has been issued ends first, if it ends
+            umma_commit(bars + kDone + 8 * m);
+            bar_wait_warp(bars + kDone + 8 * m, 0, nullptr);
+        }
+        return;
+    }
+    tc_fence_after();
     if (!any_row) return;
     const int sp = W.split ? 2 * (int)blockIdx.x + m : (int)blockIdx.x;
     const bool seen = st.l > 0.0f || st.l != st.l;
@@ -645,7 +609,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
     W.h = blockIdx.y;
     W.t0 = (int)((int64_t)n_tiles * blockIdx.x / gridDim.x);
     W.n = (int)((int64_t)n_tiles * (blockIdx.x + 1) / gridDim.x) - W.t0;
-    W.tokens = min(P.n_pages * kBlockSize - W.t0 * kTile, W.n * kTile);
     W.row0 = blockIdx.z * 2 * kTile;
     W.rows = min(R - W.row0, 2 * kTile);
     W.split = P.split != 0;
@@ -657,17 +620,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
             bar_init(bars + kVFull + 8 * s, kProducerWarps * 32);
             bar_init(bars + kKEmpty + 8 * s, readers);
             bar_init(bars + kVEmpty + 8 * s, readers);
-            for (int b = 0; b < 16; b += 8) {
-                bar_init(bars + kSFull + 16 * s + b, 1);
-                bar_init(bars + kPFull + 16 * s + b, 128);
-            }
+            bar_init(bars + kSFull + 8 * s, 1);
             bar_init(bars + kDone + 8 * s, 1);
         }
-        bar_init(bars + kQFull, kSoftmaxWarps * 32);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == kSoftmaxWarps + kProducerWarps) tmem_alloc<512>(bars + kTmem);
+    if (warp == kSoftmaxWarps) tmem_alloc<512>(bars + kTmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -682,26 +641,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PrefixP
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
         load_queries(P, W, smem, warp, lane);
         fence_async_smem();
-        bar_arrive(bars + kQFull);
-        asm volatile("bar.sync 1, %0;\n" ::"n"(kSoftmaxWarps * 32) : "memory");  // the rows' score factors
-        softmax(P, W, smem, bars, tmem, abort, warp >> 2, warp, lane);
-    } else if (warp < kSoftmaxWarps + kProducerWarps) {
+        asm volatile("bar.sync 1, %0;\n" ::"n"(kSoftmaxWarps * 32) : "memory");  // queries and score factors
+        softmax(P, W, smem, base, bars, tmem, abort, warp >> 2, warp, lane);
+    } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kProducerRegs));
         if constexpr (!layout_fp8_keys(L)) {
             build_table<L>(P, smem, warp - kSoftmaxWarps, lane);
             asm volatile("bar.sync 2, %0;\n" ::"n"(kProducerWarps * 32) : "memory");
         }
         dequantise<L>(P, W, smem, bars, abort, warp - kSoftmaxWarps, lane);
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kIssueRegs));
-        if (warp == kSoftmaxWarps + kProducerWarps) issue(W, base, bars, tmem, abort, 0);
-        if (warp == kSoftmaxWarps + kProducerWarps + 1) issue(W, base, bars, tmem, abort, 1);
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == kSoftmaxWarps + kProducerWarps) tmem_free<512>(*reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kTmem));
+    if (warp == kSoftmaxWarps) tmem_free<512>(*reinterpret_cast<volatile uint32_t*>(smem + kBarOff + kTmem));
     if (tid == 0 && *abort != 0) atomicAdd(&g_prefix_timeouts, 1u);
 }
 

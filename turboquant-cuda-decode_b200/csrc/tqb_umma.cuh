@@ -30,14 +30,15 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 }
 // Waits, as a converged warp, for the phase of `bar` with the given parity.
 // False when about a second passes first, or when another warp of the CTA has
-// given up (`abort`, in shared memory, which this sets too).
+// given up (`abort`, in shared memory, which this sets too; null: neither).
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort) {
     if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
     const long long t0 = clock64();
     for (uint32_t i = 1;; i++) {
         if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
-        if ((i & 15u) == 0 && __any_sync(0xffffffffu, *abort != 0 || clock64() - t0 > kUmmaWaitCycles)) {
-            *abort = 1;
+        if ((i & 15u) == 0 &&
+            __any_sync(0xffffffffu, (abort != nullptr && *abort != 0) || clock64() - t0 > kUmmaWaitCycles)) {
+            if (abort != nullptr) *abort = 1;
             return false;
         }
     }
