@@ -33,8 +33,8 @@
 // terms whose errors average out: about 3e-4 of the output, a third of a
 // bf16 output's own rounding, which is why only 16-bit outputs come here.
 //
-// m is a lazy reference: it moves (and l and O are rescaled) only when a
-// score exceeds it by more than 2^8, so p <= 2^8 in fp16 and l stays in fp32.
+// m is a lazy reference: it moves (and l and O are rescaled) only when a weight
+// exceeds 2^8, far from the end of fp16.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -67,7 +67,7 @@ constexpr int kPrefixThreads = (kSoftmaxWarps + kProducerWarps) * 32;  // whole 
 // launch's).
 constexpr int kPrefixRegs = 168, kSoftmaxRegs = 200, kProducerRegs = 104;
 static_assert(2 * kSoftmaxRegs + kProducerRegs <= 3 * kPrefixRegs && kPrefixRegs * kPrefixThreads <= 65536, "register split");
-constexpr float kSlack = 8.0f;
+constexpr float kMost = 256.0f;  // the largest weight before the reference moves
 
 // Barriers (8 bytes each) at kBarOff, then words.
 // Two of each: stages of K and V, S and the last products (after an error) per
@@ -317,40 +317,44 @@ struct Products {
     volatile uint32_t* abort;
     const Place& W;
 
-    __device__ __forceinline__ bool scores(int u) const {  // S = Q K^T of step u
+    // The operands of step u's products: its values, the next step's keys.
+    // Waited for ahead of the scores, off the way from weights to scores.
+    __device__ __forceinline__ bool operands(int u, int n) const {
+        const int t = W.tile(m, u), t1 = W.tile(m, u + 1);
+        return bar_wait_warp(bars + kVFull + 8 * (t & 1), (t >> 1) & 1, abort) &&
+               (u + 1 == n || bar_wait_warp(bars + kKFull + 8 * (t1 & 1), (t1 >> 1) & 1, abort));
+    }
+    __device__ __forceinline__ void scores(int u) const {  // S = Q K^T of step u
         constexpr uint32_t kQK = umma_idesc(kTile, kTile, false);
-        const int tile = W.tile(m, u), s = tile & 1;
-        if (!bar_wait_warp(bars + kKFull + 8 * s, (tile >> 1) & 1, abort)) return false;
-        tc_fence_after();
         const uint64_t q = umma_desc(smem + kQOff + (W.split ? 0 : m * kOperand), 16, 1024);
-        const uint64_t k = umma_desc(smem + kKOff + s * kOperand, 16, 1024);
+        const uint64_t k = umma_desc(smem + kKOff + (W.tile(m, u) & 1) * kOperand, 16, 1024);
 #pragma unroll
         for (int e = 0; e < 8; e++) {  // 16 dims: 32 bytes of a swizzled row, the upper 64 dims a half further
             const uint64_t at = ((e >> 2) * kHalf + (e & 3) * 32) >> 4;
             umma_ss(tmem + m * kTile, q + at, k + at, kQK, e != 0);
         }
-        return true;
     }
     __device__ __forceinline__ bool begin() const {
-        if (!scores(0)) return false;
+        const int s = W.tile(m, 0) & 1;
+        if (!bar_wait_warp(bars + kKFull + 8 * s, 0, abort)) return false;
+        tc_fence_after();
+        scores(0);
         umma_commit(bars + kSFull + 8 * m);
-        umma_commit(bars + kKEmpty + 8 * (W.tile(m, 0) & 1));
+        umma_commit(bars + kKEmpty + 8 * s);
         return true;
     }
-    __device__ __forceinline__ bool step(int u, int n) const {  // O += P V of step u, S of step u + 1
+    __device__ __forceinline__ void step(int u, int n) const {  // O += P V of step u, S of step u + 1
         constexpr uint32_t kPV = umma_idesc(kTile, kHeadDim, true);
-        const int tile = W.tile(m, u), s = tile & 1;
-        if (!bar_wait_warp(bars + kVFull + 8 * s, (tile >> 1) & 1, abort)) return false;
+        const int s = W.tile(m, u) & 1;
         tc_fence_after();
         const uint64_t v = umma_desc(smem + kVOff + s * kOperand, kHalf, 1024);
 #pragma unroll
         for (int e = 0; e < 8; e++)  // 16 tokens: two 8-row groups
             umma_ts(tmem + 2 * kTile + m * kHeadDim, tmem + m * kTile + 8 * e, v + e * (2048 >> 4), kPV, u != 0 || e != 0);
-        if (u + 1 < n && !scores(u + 1)) return false;
+        if (u + 1 < n) scores(u + 1);
         umma_commit(bars + kSFull + 8 * m);
         umma_commit(bars + kVEmpty + 8 * s);
         if (u + 1 < n) umma_commit(bars + kKEmpty + 8 * (W.tile(m, u + 1) & 1));
-        return true;
     }
 };
 
@@ -359,13 +363,12 @@ struct RowState {
     float ref, l;
 };
 
-// Moves the reference of the rows whose exponents exceed it by more than
-// kSlack (or that see their first token), and scales what they have summed so
-// far: l and O (whose earlier products are in it since these scores were
-// announced).  Rare.
+// Moves the reference of the rows whose exponents exceed it by too much, and
+// scales what they have summed so far: l and O (whose earlier products are in
+// it since these scores were announced).  Rare.
 __device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32_t to, bool has_o) {
-    const float f = over && st.ref != -INFINITY ? ex2_approx(-top) : 1.0f;
-    if (over) st.ref = (st.ref == -INFINITY ? 0.0f : st.ref) + top;
+    const float f = over ? ex2_approx(-top) : 1.0f;
+    if (over) st.ref += top;
     st.l *= f;
     if (has_o) {
         for (int i = 0; i < kHeadDim; i += 16) {
@@ -381,58 +384,74 @@ __device__ __noinline__ RowState raise(RowState st, float top, bool over, uint32
     return st;
 }
 
+// The largest score of this thread's row (rare: from TMEM again).
+template <bool MASK>
+__device__ __noinline__ float largest(uint32_t ts, int lim, uint32_t pages) {
+    float top = -INFINITY;
+    for (int q = 0; q < kTile; q += 16) {
+        uint32_t s[16];
+        tmem_ld16(s, ts + q);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            if (!MASK || (q + j < lim && (pages >> (q >> 4)) & 1u)) top = fmaxf(top, __uint_as_float(s[j]));
+    }
+    return top;
+}
+
 // A tile's scores of this thread's row turned into weights p = exp2(s kfac -
 // ref) in their place (columns 0 .. 63, two fp16 each).  The whole row is in
-// registers: one load, one vote on the reference, then the exponentials
-// without a break.
+// registers, and nothing stands before the exponentials: whether the reference
+// still holds is read off the weights (their largest, infinite where fp16 ends),
+// and the scores are weighed again where it does not.
 template <bool MASK>
 __device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, bool has_o, float kfac, int lim,
                                       uint32_t pages) {
     const uint64_t k2 = pack2(kfac, kfac);
-    const float r = st.ref == -INFINITY ? 0.0f : st.ref;
-    const uint64_t r2 = pack2(-r, -r);
-    uint32_t s[4][32];
+    if (__any_sync(0xffffffffu, st.ref == -INFINITY)) {  // rows that see their first tokens
+        const float top = largest<MASK>(ts, lim, pages);
+        if (st.ref == -INFINITY && top < INFINITY) st.ref = top * kfac;
+    }
+    for (;;) {
+        uint32_t s[4][32], p[64];
 #pragma unroll
-    for (int q = 0; q < 4; q++) tmem_ld32(s[q], ts + 32 * q);
-    tmem_wait_ld();
-    uint64_t x[4][16];
-    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int q = 0; q < 4; q++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            x[q][j] = fma2((uint64_t)s[q][2 * j] | ((uint64_t)s[q][2 * j + 1] << 32), k2, r2);
-            if constexpr (MASK) {
-                const int t = 32 * q + 2 * j;
-                const bool page = (pages >> (t >> 4)) & 1u;
-                x[q][j] = pack2(page && t < lim ? lo2(x[q][j]) : -INFINITY, page && t + 1 < lim ? hi2(x[q][j]) : -INFINITY);
-            }
-            tops[q] = fmaxf(tops[q], fmaxf(lo2(x[q][j]), hi2(x[q][j])));
-        }
-    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    const bool over = top < INFINITY && (top > kSlack || (st.ref == -INFINITY && top > -INFINITY));
-    if (__any_sync(0xffffffffu, over)) {
-        st = raise(st, top, over, to, has_o);
-        const uint64_t t2 = over ? pack2(-top, -top) : pack2(0.0f, 0.0f);
+        for (int q = 0; q < 4; q++) tmem_ld32(s[q], ts + 32 * q);
+        tmem_wait_ld();
+        const float r = st.ref == -INFINITY ? 0.0f : st.ref;
+        const uint64_t r2 = pack2(-r, -r);
+        uint64_t acc = pack2(0.0f, 0.0f);
+        __half2 most = u32_as_h2(0u);
 #pragma unroll
         for (int q = 0; q < 4; q++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) x[q][j] = add2(x[q][j], t2);
-    }
-    uint64_t acc = pack2(0.0f, 0.0f);
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-        uint32_t p[16];
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float a = ex2_approx(lo2(x[q][j])), b = ex2_approx(hi2(x[q][j]));
-            acc = add2(acc, pack2(a, b));
-            p[j] = h2_as_u32(__floats2half2_rn(a, b));
+            for (int j = 0; j < 16; j++) {
+                uint64_t x = fma2((uint64_t)s[q][2 * j] | ((uint64_t)s[q][2 * j + 1] << 32), k2, r2);
+                if constexpr (MASK) {
+                    const int t = 32 * q + 2 * j;
+                    const bool page = (pages >> (t >> 4)) & 1u;
+                    x = pack2(page && t < lim ? lo2(x) : -INFINITY, page && t + 1 < lim ? hi2(x) : -INFINITY);
+                }
+                const float a = ex2_approx(lo2(x)), b = ex2_approx(hi2(x));
+                acc = add2(acc, pack2(a, b));
+                const __half2 h = __floats2half2_rn(a, b);
+                most = __hmax2(most, h);
+                p[16 * q + j] = h2_as_u32(h);
+            }
+        const bool over = fmaxf(__low2float(most), __high2float(most)) > kMost;
+        if (__any_sync(0xffffffffu, over)) {
+            const float x = largest<MASK>(ts, lim, pages) * kfac - r;
+            const bool move = over && x > 0.0f && x < INFINITY;  // infinite scores stay as they are
+            if (__any_sync(0xffffffffu, move)) {
+                st = raise(st, x, move, to, has_o);
+                continue;
+            }
         }
-        tmem_st16(ts + 16 * q, p);
+        st.l += lo2(acc) + hi2(acc);
+        tmem_st32(ts, p);
+        tmem_st32(ts + 32, p + 32);
+        tmem_wait_st();
+        return;
     }
-    st.l += lo2(acc) + hi2(acc);
-    tmem_wait_st();
 }
 
 __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, uint8_t* smem, uint32_t smem_base, uint32_t bars, uint32_t tmem,
@@ -448,7 +467,8 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     // tokens of the chunk this row sees, from the chunk's start
     const int lim = min(__ldg(P.seq_lens + b), P.n_pages * kBlockSize) - W.t0 * kTile;
     const bool any_row = __any_sync(0xffffffffu, live);
-    RowState st{-INFINITY, 0.0f};
+    // (a row that sees nothing of the chunk has weights of zero at any reference)
+    RowState st{lim > 0 ? -INFINITY : 0.0f, 0.0f};
     const int n = W.steps(m);
     const Products mma{smem_base, bars, tmem, (uint32_t)m, abort, W};
     bool ok = true;
@@ -463,6 +483,7 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     if (turns && m == 1) asm volatile("bar.arrive 5, 256;\n" ::: "memory");
     for (int u = 0; u < n; u++) {  // every warp takes every turn at the barrier, also when a wait has given up
         const int tile = W.tile(m, u);
+        if (wq == 0) ok = ok && mma.operands(u, n);
         ok = ok && bar_wait_warp(bars + kSFull + 8 * m, u & 1, abort);
         tc_fence_after();
         if (turns) asm volatile("bar.sync %0, 256;\n" ::"r"(5 + m) : "memory");
@@ -477,7 +498,7 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
         if (u + m < other) asm volatile("bar.arrive %0, 256;\n" ::"r"(6 - m) : "memory");
         tc_fence_before();
         asm volatile("bar.sync %0, 128;\n" ::"r"(3 + m) : "memory");  // the stream's weights are complete
-        if (wq == 0 && ok) ok = mma.step(u, n);
+        if (wq == 0 && ok) mma.step(u, n);
     }
     // ---- the partial rows ----
     // (also: every product has ended before the CTA frees its TMEM)
