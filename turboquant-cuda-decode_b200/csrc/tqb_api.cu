@@ -91,11 +91,12 @@ int tqb_version(void) { return TQB_VERSION; }
 int tqb_wait_timeouts(unsigned int* count, int reset) {
     g_detail[0] = '\0';
     TQB_REQUIRE(count != nullptr, TQB_ERR_INVALID_ARG, "count is NULL");
-    unsigned int ring = 0, p2p = 0, prefix = 0;
+    unsigned int ring = 0, p2p = 0, prefix = 0, append = 0;
     if (tqb::read_wait_timeouts(&ring, reset != 0) != TQB_OK) return TQB_ERR_CUDA;
     if (tqb::read_p2p_timeouts(&p2p, reset != 0) != TQB_OK) return TQB_ERR_CUDA;
     if (tqb::read_prefix_timeouts(&prefix, reset != 0) != TQB_OK) return TQB_ERR_CUDA;
-    *count = ring + p2p + prefix;
+    if (tqb::read_append_timeouts(&append, reset != 0) != TQB_OK) return TQB_ERR_CUDA;
+    *count = ring + p2p + prefix + append;
     return TQB_OK;
 }
 
@@ -800,6 +801,8 @@ int tqb_append(const tqb_append_args* a, cudaStream_t stream) {
     p.N = a->num_tokens;
     p.Hq = a->query ? a->num_q_heads : 0;
     p.Hk = a->num_kv_heads;
+    p.div_hk = tqb::FastDiv((uint32_t)p.Hk);
+    p.div_hq = tqb::FastDiv((uint32_t)(p.Hq > 0 ? p.Hq : 1));
     p.norm_correction = a->norm_correction;
     return tqb::launch_append(p, stream, nsm);
 }

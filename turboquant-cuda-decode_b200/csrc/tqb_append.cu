@@ -26,8 +26,12 @@
 #include "tqb_common.cuh"
 #include "tqb_internal.h"
 #include "tqb_quant_row.cuh"
+#include "tqb_umma.cuh"
 
 namespace tqb {
+
+// Kernels that gave up a wait (read by tqb_wait_timeouts).
+__device__ unsigned int g_append_timeouts = 0;
 
 namespace {
 
@@ -118,10 +122,12 @@ __device__ __noinline__ double exact_norm(const AppendParams& P, const T* row, c
     }
     return sqrt(warp_sum_f64(q));
 }
-// Code of coordinate e of a key row in 64 bits (whole warp).
+// Whether coordinate e of a key row is at border `mid` or above, in 64 bits
+// (whole warp): x R_e >= mid (|x| + 1e-8).
 template <typename T>
-__device__ __noinline__ int exact_code(const AppendParams& P, const T* row, const float* cs, int e, int nc, int lane) {
+__device__ __noinline__ bool exact_side(const AppendParams& P, const T* row, const float* cs, int e, float mid, int lane) {
     double q = 0.0, z = 0.0;
+#pragma unroll
     for (int i = 0; i < 4; i++) {
         const int d = lane + 32 * i;
         const double x = rope_f64<T>(P, row, cs, d);
@@ -130,10 +136,7 @@ __device__ __noinline__ int exact_code(const AppendParams& P, const T* row, cons
     }
     q = warp_sum_f64(q);
     z = warp_sum_f64(z);
-    const double y = z / (sqrt(q) + 1e-8);
-    int c = 0;
-    for (int k = 0; k < nc - 1; k++) c += y >= (double)__ldg(P.mids + k) ? 1 : 0;
-    return c;
+    return z >= (double)mid * (sqrt(q) + 1e-8);
 }
 
 template <typename T>
@@ -184,8 +187,14 @@ __device__ __forceinline__ void finish_row(const AppendParams& P, const float* s
             i += y >= smid[i + 1] ? 2 : 0;
             i += y >= smid[i] ? 1 : 0;
             code[j] = i;
-            // the borders on the two sides of the code (one side at the ends)
-            near |= (fabsf(y - smid[max(i - 1, 0)]) < kNear || fabsf(y - smid[min(i, nc - 2)]) < kNear) ? 1u << j : 0u;
+            // the borders on the two sides of the code (one side at the ends):
+            // next to one of them, the code is that border's for now, and goes
+            // up by one if the coordinate is on its upper side
+            const bool below = fabsf(y - smid[max(i - 1, 0)]) < kNear, above = fabsf(y - smid[min(i, nc - 2)]) < kNear;
+            if (below || above) {
+                near |= 1u << j;
+                code[j] = below ? max(i - 1, 0) : min(i, nc - 2);
+            }
         }
         if (!write) near = 0;
         uint32_t who;
@@ -194,11 +203,16 @@ __device__ __forceinline__ void finish_row(const AppendParams& P, const float* s
             const int sn = __shfl_sync(kFull, n, src), sh = __shfl_sync(kFull, h, src), sp = __shfl_sync(kFull, pos, src);
             const int j = __shfl_sync(kFull, __ffs(near) - 1, src);
             const T* row = static_cast<const T*>(P.key) + (int64_t)sn * P.ksn + (int64_t)sh * P.ksh;
-            const int c = exact_code<T>(P, row, table_row<T>(P, sp), 8 * (src & 15) + j, nc, lane);
+            int border = 0;
+#pragma unroll
+            for (int jj = 0; jj < 8; jj++)
+                if (jj == j) border = code[jj];
+            const float mid = smid[__shfl_sync(kFull, border, src)];
+            const bool up = exact_side<T>(P, row, table_row<T>(P, sp), 8 * (src & 15) + j, mid, lane);
             if (lane == src) {
 #pragma unroll
                 for (int jj = 0; jj < 8; jj++)
-                    if (jj == j) code[jj] = c;
+                    if (jj == j && up) code[jj]++;
                 near &= near - 1;
             }
         }
@@ -238,7 +252,7 @@ __device__ __forceinline__ void finish_row(const AppendParams& P, const float* s
     const ValueRow vr = quantise_values<v3>(vs);
     if (!write) return;
     write_row<L>(P.cache + (size_t)((uint32_t)slot / kBlockSize) * (size_t)P.block_bytes, (uint32_t)slot % kBlockSize,
-                 (uint32_t)h, P.Hk, P.pos_stride, P.head_stride, m, kbits, klo, khi, vr.bits, vn_h, vr.scale, vr.vmin);
+                 (uint32_t)h, P.Hk, P.pos_stride, P.head_stride, m, kbits, klo, khi, vr, vn_h);
 }
 
 // ---------------------------------------------------------------------------
@@ -251,7 +265,7 @@ constexpr int kAppThreads = 256;
 constexpr int kAppSmem = (kHeadDim * kHeadDim + kRows * kHeadDim) * 4;
 
 template <typename T, int L>
-__global__ void __launch_bounds__(kAppThreads) append_kernel(const AppendParams P, int key_ctas) {
+__global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_constant__ AppendParams P, int key_ctas) {
     constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L);
     constexpr int nc = k3 ? 8 : kNumCentroids;
     extern __shared__ __align__(16) float asm_[];
@@ -338,8 +352,558 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const AppendParams 
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows of aligned inputs (Lloyd-Max layouts): the rotation on the tensor
+// cores.  A persistent CTA walks tiles of 128 rows (of keys, then of queries):
+//   warps 0-3, 4-7  finish tiles by turns: thread = row (= TMEM lane), its 128
+//                   coordinates bucketised and packed, or written (queries);
+//   warps 8-11      turn the rows and split them: x 2^s = hi + lo in fp16 (22
+//                   bits), s from |x|; the first of them issues the products;
+//   warps 12-15     the values of the CTA's key rows, half a warp each.
+// x R = hi R_hi + lo R_hi + hi R_lo in fp32 (R 2^10 split the same way, kept in
+// shared memory): 24 MMAs of 128 x 128 x 16 a tile.  Errors against exact
+// arithmetic: 2^-23 from the fp32 turn, 3 * 2^-22 from the splits, and 24
+// accumulations of at most 2^-23 each, 2^-18 of |x| in all (kNearMma).
+// Bound by instruction issue: about 15 instructions per coordinate to
+// bucketise, 9 to turn and split, 10 per value.
+// ---------------------------------------------------------------------------
+constexpr float kNearMma = 0x1p-18f;
+constexpr int kATile = 128 * kHeadDim * 2;                                       // 32 KB
+constexpr int kAHiOff = 0, kALoOff = kATile, kBHiOff = 2 * kATile, kBLoOff = 3 * kATile;
+constexpr int kCells = 128;                                                      // of [-kCellSpan, kCellSpan)
+constexpr float kCellSpan = 0.25f;
+constexpr int kCellOff = 4 * kATile;                                             // [kCells][32 lanes]
+constexpr int kTurnOff = kCellOff + kCells * 32 * 4;                             // 8 warps x 4 KB
+constexpr int kInfoOff = kTurnOff + 8 * 4096;                                    // [2][128] RowInfo
+constexpr int kTabOff = kInfoOff + 2 * 128 * 16;                                 // mids, c^2
+constexpr int kUmmaBarOff = kTabOff + 2 * kNumCentroids * 4;
+constexpr int kUmmaSmem = kUmmaBarOff + 64;
+static_assert(kUmmaSmem <= 232448, "shared memory per CTA");
+constexpr int kUmmaThreads = 512;
+enum : uint32_t { kAEmpty = 0, kDFull = 8, kDEmpty = 24, kUTmem = 40, kUAbort = 44 };
+
+// What the finishing warps need of a row: the sum of squares, the factor that
+// undoes the scales, its token and KV head (or query head), and its slot (-1:
+// not stored; queries: -1 where the position is outside the table).
+struct __align__(16) RowInfo {
+    float nsq, unscale;
+    int n, slot;
+};
+
+// Two bf16 or fp16 numbers, or the first / second of two floats.
+template <typename T>
+struct Quad {  // four consecutive elements
+    float v[4];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(p));
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+            const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = to_f32<T>(h[i]);
+        }
+    }
+};
+
+struct UmmaTiles {
+    uint32_t key_rows, rows, key_tiles, tiles;
+};
+
+// A tile's rows turned, scaled, split and stored (128-byte swizzle, K-major),
+// half a warp per row: lane m of 16 takes pairs 4m .. 4m + 3 of the row's 64
+// (pairs that the rotary step turns together, and the rest two by two).
+template <typename T>
+__device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, const UmmaTiles& W, uint32_t tile, int buf,
+                                          int lw, int lane) {
+    const bool keys = tile < W.key_tiles;
+    const uint32_t first = (keys ? tile : tile - W.key_tiles) * 128u, total = keys ? W.key_rows : W.rows - W.key_rows;
+    const FastDiv& div = keys ? P.div_hk : P.div_hq;
+    const uint32_t H = (uint32_t)(keys ? P.Hk : P.Hq);
+    const T* base = static_cast<const T*>(keys ? P.key : P.query);
+    const int64_t sn = keys ? P.ksn : P.qsn, sh = keys ? P.ksh : P.qsh;
+    const int m = lane & 15, half = P.rotary >> 1, j0 = 4 * m;
+    const bool turned = j0 < half;
+    // dims of the lane's pairs: (a, b) = (da + i, db + i), or interleaved
+    // (2 j, 2 j + 1)
+    int da, db;
+    if (P.interleaved) {
+        da = 2 * j0;
+        db = da + 4;
+    } else {
+        da = turned ? j0 : P.rotary + (j0 - half);
+        db = turned ? j0 + half : P.rotary + (64 - half) + (j0 - half);
+    }
+    constexpr int kBatch = 4;
+    for (int r0 = 2 * lw + (lane >> 4); r0 < 128; r0 += 8 * kBatch) {
+        Quad<T> qa[kBatch], qb[kBatch];
+        int pos[kBatch], tok[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            const uint32_t row = min(first + r0 + 8 * i, total - 1);
+            const uint32_t n = div.div(row), h = row - n * H;
+            tok[i] = (int)n;
+            pos[i] = position_of(P, (int)n);
+            const T* p = base + (int64_t)n * sn + (int64_t)h * sh;
+            qa[i].load(p + da);
+            qb[i].load(p + db);
+        }
+        float4 c[kBatch], s[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            c[i] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+            s[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (turned) {
+                const float* cs = table_row<T>(P, pos[i]) + j0;
+                c[i] = __ldg(reinterpret_cast<const float4*>(cs));
+                s[i] = __ldg(reinterpret_cast<const float4*>(cs + half));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            const int r = r0 + 8 * i;
+            float x[8];  // dims da .. da + 3, db .. db + 3
+            if (P.interleaved) {
+                const float cc[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, ss[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
+                const float in[8] = {qa[i].v[0], qa[i].v[1], qa[i].v[2], qa[i].v[3],
+                                     qb[i].v[0], qb[i].v[1], qb[i].v[2], qb[i].v[3]};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    x[2 * k] = fmaf(in[2 * k], cc[k], -(in[2 * k + 1] * ss[k]));
+                    x[2 * k + 1] = fmaf(in[2 * k + 1], cc[k], in[2 * k] * ss[k]);
+                }
+            } else {
+                const float cc[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, ss[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    x[k] = fmaf(qa[i].v[k], cc[k], -(qb[i].v[k] * ss[k]));
+                    x[4 + k] = fmaf(qb[i].v[k], cc[k], qa[i].v[k] * ss[k]);
+                }
+            }
+            float nsq = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) nsq = fmaf(x[k], x[k], nsq);
+            nsq = warp_sum_xor(nsq, 1, 8);
+            // |x| 2^e in [2^13, 2^15): e from the exponent of |x|^2 (its half,
+            // rounded up); 0 for zero and non-finite rows, whose codes come
+            // from the exact path or are anything
+            const int be = (int)(__float_as_uint(nsq) >> 23);
+            const int e = be == 0 || be == 0xFF ? 0 : 14 - ((be - 126) >> 1);
+            const float f = exp2i(e);
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float u = x[2 * k] * f, v = x[2 * k + 1] * f;
+                const __half2 h = __floats2half2_rn(u, v);
+                hi[k] = h2_as_u32(h);
+                lo[k] = h2_as_u32(__floats2half2_rn(u - __low2float(h), v - __high2float(h)));
+            }
+            // four dims are 8 bytes of a 16-byte chunk
+            auto at = [&](int d) { return (d >> 6) * (kATile / 2) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2; };
+            *reinterpret_cast<uint2*>(smem + kAHiOff + at(da)) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(smem + kAHiOff + at(db)) = make_uint2(hi[2], hi[3]);
+            *reinterpret_cast<uint2*>(smem + kALoOff + at(da)) = make_uint2(lo[0], lo[1]);
+            *reinterpret_cast<uint2*>(smem + kALoOff + at(db)) = make_uint2(lo[2], lo[3]);
+            if (m == 0) {
+                RowInfo info;
+                info.nsq = nsq;
+                info.unscale = exp2i(-e) * 0x1p-10f;
+                info.n = tok[i];
+                int slot = -1;
+                if (first + r < total && pos[i] >= 0) {
+                    slot = keys ? __ldg(P.slots + tok[i]) : 0;
+                    if (keys && P.num_blocks > 0 && (int64_t)slot >= P.num_blocks * kBlockSize) slot = -1;
+                }
+                info.slot = max(slot, -1);
+                reinterpret_cast<RowInfo*>(smem + kInfoOff)[buf * 128 + r] = info;
+            }
+        }
+    }
+}
+
+// A key row: codes of its 128 coordinates, norm, slot.
 template <typename T, int L>
-int launch_append_t(const AppendParams& P, cudaStream_t stream) {
+__device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem, uint32_t tm, uint32_t row, const RowInfo& info,
+                                            bool fine, int lane) {
+    constexpr bool k3 = layout_3bit_keys(L);
+    constexpr int nc = k3 ? 8 : kNumCentroids, kBits = k3 ? 3 : 4, kWords = k3 ? 12 : 16;
+    constexpr unsigned kFull = 0xffffffffu;
+    const float* smid = reinterpret_cast<const float*>(smem + kTabOff);
+    const float* csq16 = smid + kNumCentroids;
+    const float norm = __fsqrt_rn(info.nsq);
+    const float f = info.unscale * __frcp_rn(norm + 1e-8f);
+    const uint32_t h = row - (uint32_t)info.n * (uint32_t)P.Hk;
+    const uint8_t* cells = smem + kCellOff + 4 * lane;
+    // coordinates next to a border, and those on its upper side as far as fp32 says
+    uint32_t words[kWords], near[4] = {0u, 0u, 0u, 0u}, upper[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kWords; i++) words[i] = 0u;
+    float csq = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        uint32_t z[32];
+        tmem_ld32(z, tm + 32 * q);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const float y = __uint_as_float(z[j]) * f;
+            int code;
+            bool close, up;
+            if (fine) {
+                // the nearest border of y's cell, its index in the low bits
+                const float t = fminf(fmaxf(fmaf(y, kCells / (2.0f * kCellSpan), 0x1p23f + kCells / 2), 0x1p23f),
+                                      0x1p23f + (kCells - 1));
+                const uint32_t e = *reinterpret_cast<const uint32_t*>(cells + ((__float_as_uint(t) & (kCells - 1)) << 7));
+                const float d = y - __uint_as_float(e);
+                up = d >= 0.0f;
+                code = (int)(e & 15u) + (up ? 1 : 0);
+                close = fabsf(d) < kNearMma;
+            } else {
+                code = 0;
+#pragma unroll 1
+                for (int k = 0; k < nc - 1; k++) code += y >= smid[k] ? 1 : 0;
+                up = code > 0 && y - smid[code - 1] < kNearMma;
+                close = up || (code < nc - 1 && smid[code] - y < kNearMma);
+            }
+            csq += csq16[code];
+            if (close) {
+                near[q] |= 1u << j;
+                if (up) upper[q] |= 1u << j;
+            }
+            const int bit = kBits * (32 * q + j);
+            words[bit >> 5] |= (uint32_t)code << (bit & 31);
+            if ((bit & 31) + kBits > 32) words[(bit >> 5) + 1] |= (uint32_t)code >> (32 - (bit & 31));
+        }
+    }
+    // coordinates next to a border, in 64 bits by the whole warp (a row with
+    // none stored needs none)
+    const bool stored = info.slot >= 0;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        if (!stored) near[q] = 0u;
+        uint32_t who;
+        while ((who = __ballot_sync(kFull, near[q] != 0u)) != 0u) {
+            const int src = __ffs(who) - 1;
+            const int sn = __shfl_sync(kFull, info.n, src), sh = __shfl_sync(kFull, (int)h, src);
+            const int j = __shfl_sync(kFull, __ffs(near[q]) - 1, src);
+            const int pos = position_of(P, sn);
+            const T* krow = static_cast<const T*>(P.key) + (int64_t)sn * P.ksn + (int64_t)sh * P.ksh;
+            // the border next to it: between the code and one of its neighbours
+            const int bit = kBits * (32 * q + j);
+            int code = 0;
+#pragma unroll
+            for (int w = 0; w < kWords; w++) {
+                if (w == (bit >> 5)) code |= (int)(words[w] >> (bit & 31));
+                if (w == (bit >> 5) + 1 && (bit & 31) + kBits > 32) code |= (int)(words[w] << (32 - (bit & 31)));
+            }
+            code &= (1 << kBits) - 1;
+            const int c0 = __shfl_sync(kFull, code, src);
+            const bool was_up = __shfl_sync(kFull, (int)(upper[q] >> j), src) & 1;
+            const int border = was_up ? c0 - 1 : c0;
+            const int c = border + (exact_side<T>(P, krow, table_row<T>(P, pos), 32 * q + j, smid[border], lane) ? 1 : 0);
+            if (lane == src) {
+                near[q] &= near[q] - 1;
+                if (c != c0) {
+                    csq += csq16[c] - csq16[c0];
+                    const uint64_t flip = (uint64_t)(uint32_t)(c ^ c0) << (bit & 31);
+#pragma unroll
+                    for (int w = 0; w < kWords; w++) {
+                        if (w == (bit >> 5)) words[w] ^= (uint32_t)flip;
+                        if (w == (bit >> 5) + 1) words[w] ^= (uint32_t)(flip >> 32);
+                    }
+                }
+            }
+        }
+    }
+    const bool fold = !layout_is_aos(L) && P.norm_correction;
+    const float kept = fold ? norm * rsqrtf(csq + 1e-16f) : norm;
+    unsigned short kept_h = __half_as_ushort(__float2half_rn(kept));
+    const bool split = stored && __half_as_ushort(__float2half_rn(kept * (1.0f - kNormNear))) !=
+                                     __half_as_ushort(__float2half_rn(kept * (1.0f + kNormNear)));
+    uint32_t ask = __ballot_sync(kFull, split);
+    while (ask != 0u) {
+        const int src = __ffs(ask) - 1;
+        ask &= ask - 1;
+        const int sn = __shfl_sync(kFull, info.n, src), sh = __shfl_sync(kFull, (int)h, src);
+        const T* krow = static_cast<const T*>(P.key) + (int64_t)sn * P.ksn + (int64_t)sh * P.ksh;
+        double v = exact_norm<T>(P, krow, table_row<T>(P, position_of(P, sn)), lane);
+        if (lane == src) {
+            if (fold) {
+                double cq = 0.0;
+#pragma unroll
+                for (int w = 0; w < kWords; w++) {
+                    if constexpr (!k3) {
+                        for (int i = 0; i < 8; i++) {
+                            const double cv = (double)__ldg(P.cents + ((words[w] >> (4 * i)) & 15u));
+                            cq += cv * cv;
+                        }
+                    } else if (w % 3 == 0) {
+                        const uint64_t a = (uint64_t)words[w] | ((uint64_t)words[w + 1] << 32);
+                        const uint64_t b = (uint64_t)words[w + 1] | ((uint64_t)words[w + 2] << 32);
+                        for (int i = 0; i < 32; i++) {
+                            const uint32_t c = (uint32_t)(3 * i < 60 ? a >> (3 * i) : b >> (3 * i - 32)) & 7u;
+                            const double cv = (double)__ldg(P.cents + c);
+                            cq += cv * cv;
+                        }
+                    }
+                }
+                v /= sqrt(cq + 1e-16);
+            }
+            kept_h = __half_as_ushort(__double2half(v));
+        }
+    }
+    if (!stored) return;
+    const SlotAt<L> at(P.cache + (size_t)((uint32_t)info.slot / kBlockSize) * (size_t)P.block_bytes,
+                       (uint32_t)info.slot % kBlockSize, h, P.Hk, P.pos_stride, P.head_stride);
+    if constexpr (layout_is_aos(L)) {  // 2-byte aligned slots
+#pragma unroll
+        for (int w = 0; w < kWords; w++) st_u16x2(at.key + 4 * w, words[w]);
+    } else {
+#pragma unroll
+        for (int w = 0; w < kWords; w += 4)
+            *reinterpret_cast<uint4*>(at.key + 4 * w) = make_uint4(words[w], words[w + 1], words[w + 2], words[w + 3]);
+    }
+    *reinterpret_cast<unsigned short*>(at.norm) = kept_h;
+}
+
+// Query rows: the product itself, turned through shared memory into runs of
+// 128 bytes.
+__device__ __forceinline__ void finish_queries(const AppendParams& P, uint8_t* turn, uint32_t tm, uint32_t row,
+                                               const RowInfo& info, bool live, int lane) {
+    const uint32_t h = row - (uint32_t)info.n * (uint32_t)P.Hq;
+    float* dst = P.q_rot + (int64_t)info.n * P.osn + (int64_t)h * P.osh;
+    const float f = info.slot < 0 ? __int_as_float(0x7fc00000) : info.unscale;
+    const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+    const unsigned long long mine = reinterpret_cast<unsigned long long>(dst);
+    float* rows[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        rows[i] = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, 4 * i + (lane >> 3))) + 4 * (lane & 7);
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        uint32_t z[32];
+        tmem_ld32(z, tm + 32 * q);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            *reinterpret_cast<float4*>(turn + 128 * lane + ((c ^ (lane & 7)) << 4)) =
+                make_float4(__uint_as_float(z[4 * c]) * f, __uint_as_float(z[4 * c + 1]) * f,
+                            __uint_as_float(z[4 * c + 2]) * f, __uint_as_float(z[4 * c + 3]) * f);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = 4 * i + (lane >> 3);
+            const float4 v = *reinterpret_cast<const float4*>(turn + 128 * r + (((lane & 7) ^ (r & 7)) << 4));
+            if ((live_rows >> r) & 1u) *reinterpret_cast<float4*>(rows[i] + 32 * q) = v;
+        }
+        __syncwarp();
+    }
+}
+
+// The values of a tile's rows, half a warp each, four in flight.
+template <typename T, int L>
+__device__ __forceinline__ void store_values(const AppendParams& P, const UmmaTiles& W, uint32_t tile, int vw, int lane) {
+    const int m = lane & 15;
+    constexpr int kBatch = 4;
+    for (int r0 = 2 * vw + (lane >> 4); r0 < 128; r0 += 8 * kBatch) {
+        Quad<T> a[kBatch], b[kBatch];
+        int slot[kBatch];
+        uint32_t hs[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            const uint32_t row0 = tile * 128u + r0 + 8 * i, row = min(row0, W.key_rows - 1);
+            const uint32_t n = P.div_hk.div(row), h = row - n * (uint32_t)P.Hk;
+            const T* v = static_cast<const T*>(P.value) + (int64_t)n * P.vsn + (int64_t)h * P.vsh + 8 * m;
+            a[i].load(v);
+            b[i].load(v + 4);
+            int s = row0 < W.key_rows ? __ldg(P.slots + n) : -1;
+            if ((P.num_blocks > 0 && (int64_t)s >= P.num_blocks * kBlockSize) || position_of(P, (int)n) < 0) s = -1;
+            slot[i] = s;
+            hs[i] = h;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; i++) {
+            const float v[8] = {a[i].v[0], a[i].v[1], a[i].v[2], a[i].v[3], b[i].v[0], b[i].v[1], b[i].v[2], b[i].v[3]};
+            const ValueRow q = quantise_values<layout_3bit_values(L)>(v);
+            if (slot[i] >= 0)
+                write_values<L>(SlotAt<L>(P.cache + (size_t)((uint32_t)slot[i] / kBlockSize) * (size_t)P.block_bytes,
+                                          (uint32_t)slot[i] % kBlockSize, hs[i], P.Hk, P.pos_stride, P.head_stride),
+                                m, q);
+        }
+    }
+}
+
+template <typename T, int L>
+__global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __grid_constant__ AppendParams P,
+                                                                      const UmmaTiles W) {
+    constexpr bool k3 = layout_3bit_keys(L);
+    constexpr int nc = k3 ? 8 : kNumCentroids;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const uint32_t base = smem_addr(smem), bars = base + kUmmaBarOff;
+    volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + kUmmaBarOff + kUAbort);
+    if (tid == 0) {
+        bar_init(bars + kAEmpty, 1);
+        for (int b = 0; b < 2; b++) {
+            bar_init(bars + kDFull + 8 * b, 1);
+            bar_init(bars + kDEmpty + 8 * b, 128);
+        }
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 8) tmem_alloc<256>(bars + kUTmem);
+    float* smid = reinterpret_cast<float*>(smem + kTabOff);
+    if (tid < kNumCentroids) {
+        smid[tid] = tid < nc - 1 ? __ldg(P.mids + tid) : INFINITY;
+        const float c = tid < nc ? __ldg(P.cents + tid) : 0.0f;
+        smid[kNumCentroids + tid] = c * c;
+    }
+    // R 2^10 = hi + lo, [64 columns][128 rows of 128 bytes], swizzled: the
+    // MN-major B operand
+    for (int i = tid; i < kHeadDim * kHeadDim / 8; i += kUmmaThreads) {
+        const int d = i >> 4, c = i & 15;  // row, group of 8 columns
+        const float4 u = __ldg(reinterpret_cast<const float4*>(P.rot + d * kHeadDim + 8 * c));
+        const float4 v = __ldg(reinterpret_cast<const float4*>(P.rot + d * kHeadDim + 8 * c + 4));
+        const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float a = x[2 * k] * 1024.0f, b = x[2 * k + 1] * 1024.0f;
+            const __half2 h = __floats2half2_rn(a, b);
+            hi[k] = h2_as_u32(h);
+            lo[k] = h2_as_u32(__floats2half2_rn(a - __low2float(h), b - __high2float(h)));
+        }
+        const int at = (c >> 3) * (kATile / 2) + d * 128 + (((c & 7) ^ (d & 7)) << 4);
+        *reinterpret_cast<uint4*>(smem + kBHiOff + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(smem + kBLoOff + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    fence_async_smem();
+    __syncthreads();
+    // Cells of the coordinate's range: the border nearest to the cell, its
+    // index in the four low bits (2^-22 of it, far below kNearMma).  A cell
+    // that two borders come near to leaves every row to the search.
+    bool fine = true;
+    if (tid < kCells) {
+        const float w = 2.0f * kCellSpan / kCells, mid = -kCellSpan + w * ((float)tid + 0.0f);
+        // cells are centred on mid (the index is rounded); the outer two reach on
+        int best = 0, inside = 0;
+        for (int k = 0; k < nc - 1; k++) {
+            if (fabsf(smid[k] - mid) < fabsf(smid[best] - mid)) best = k;
+            if (fabsf(smid[k] - mid) < 0.75f * w) inside++;
+        }
+        fine = inside <= 1 && smid[0] > -kCellSpan + w && smid[nc - 2] < kCellSpan - 2.0f * w;
+        uint32_t* cell = reinterpret_cast<uint32_t*>(smem + kCellOff) + 32 * tid;
+        const uint32_t e = (__float_as_uint(smid[best]) & ~15u) | (uint32_t)best;
+        for (int i = 0; i < 32; i++) cell[(i + lane) & 31] = e;
+    }
+    fine = __syncthreads_and(fine) != 0;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kUmmaBarOff + kUTmem);
+
+    if (warp < 8) {
+        const int g = warp >> 2, wq = warp & 3;
+        uint32_t i = (uint32_t)g;
+        for (uint32_t tile = blockIdx.x + g * gridDim.x; tile < W.tiles; tile += 2 * gridDim.x, i += 2) {
+            if (!bar_wait_warp(bars + kDFull + 8 * g, (i >> 1) & 1, abort)) break;
+            tc_fence_after();
+            const bool keys = tile < W.key_tiles;
+            const uint32_t row = (keys ? tile : tile - W.key_tiles) * 128u + 32u * wq + lane;
+            const bool live = row < (keys ? W.key_rows : W.rows - W.key_rows);
+            const RowInfo info = reinterpret_cast<const RowInfo*>(smem + kInfoOff)[g * 128 + 32 * wq + lane];
+            const uint32_t tm = tmem + ((uint32_t)(32 * wq) << 16) + 128u * g;
+            if (__any_sync(0xffffffffu, live)) {
+                if (keys)
+                    finish_keys<T, L>(P, smem, tm, min(row, W.key_rows - 1), info, fine, lane);
+                else
+                    finish_queries(P, smem + kTurnOff + 4096 * warp, tm, min(row, W.rows - W.key_rows - 1), info, live, lane);
+            }
+            tc_fence_before();
+            bar_arrive(bars + kDEmpty + 8 * g);
+        }
+    } else if (warp < 12) {
+        constexpr uint32_t kId = umma_idesc(128, kHeadDim, true);
+        const uint64_t a_hi = umma_desc(base + kAHiOff, 16, 1024), a_lo = umma_desc(base + kALoOff, 16, 1024);
+        const uint64_t b_hi = umma_desc(base + kBHiOff, kATile / 2, 1024), b_lo = umma_desc(base + kBLoOff, kATile / 2, 1024);
+        uint32_t i = 0;
+        bool ok = true;
+        for (uint32_t tile = blockIdx.x; tile < W.tiles; tile += gridDim.x, i++) {
+            const int buf = (int)(i & 1);
+            // the operands' last readers, and the rows' (their infos and sums)
+            ok = ok && bar_wait_warp(bars + kAEmpty, (i & 1) ^ 1, abort) &&
+                 bar_wait_warp(bars + kDEmpty + 8 * buf, ((i >> 1) & 1) ^ 1, abort);
+            if (ok) turn_rows<T>(P, smem, W, tile, buf, warp - 8, lane);
+            fence_async_smem();
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");  // every warp takes every turn, also after an error
+            if (ok && warp == 8) {
+                tc_fence_after();
+#pragma unroll
+                for (int p = 0; p < 3; p++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const uint64_t at = ((k >> 2) * (kATile / 2) + (k & 3) * 32) >> 4;
+                        umma_ss(tmem + 128u * buf, (p == 1 ? a_lo : a_hi) + at, (p == 2 ? b_lo : b_hi) + (k * 2048 >> 4), kId,
+                                p + k != 0);
+                    }
+                umma_commit(bars + kDFull + 8 * buf);
+                umma_commit(bars + kAEmpty);
+            }
+        }
+        // every product has ended before the CTA frees its TMEM
+        if (warp == 8 && i > 0) bar_wait_warp(bars + kAEmpty, (i - 1) & 1, nullptr);
+    } else {
+        for (uint32_t tile = blockIdx.x; tile < W.key_tiles; tile += gridDim.x) store_values<T, L>(P, W, tile, warp - 12, lane);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_free<256>(tmem);
+    if (tid == 0 && *abort != 0) atomicAdd(&g_append_timeouts, 1u);
+}
+
+// Inputs that the tensor-core form reads with 8- and 16-byte loads: elements in
+// fours, rotary halves in fours, SoA slots in 16 bytes.
+template <typename T, int L>
+bool umma_aligned(const AppendParams& P) {
+    const uintptr_t a = 4 * sizeof(T);
+    auto ok = [&](const void* p, int64_t sn, int64_t sh) {
+        return reinterpret_cast<uintptr_t>(p) % a == 0 && sn % 4 == 0 && sh % 4 == 0;
+    };
+    return ok(P.key, P.ksn, P.ksh) && ok(P.value, P.vsn, P.vsh) && (!P.query || ok(P.query, P.qsn, P.qsh)) &&
+           (!P.query || (reinterpret_cast<uintptr_t>(P.q_rot) % 16 == 0 && P.osn % 4 == 0 && P.osh % 4 == 0)) &&
+           P.rotary % 8 == 0 && (!P.pos || (reinterpret_cast<uintptr_t>(P.cos_sin) % 16 == 0 && P.cs_stride % 4 == 0)) &&
+           (layout_is_aos(L) || (reinterpret_cast<uintptr_t>(P.cache) % 16 == 0 && P.block_bytes % 16 == 0));
+}
+
+template <typename T, int L>
+int launch_append_umma(const AppendParams& P, cudaStream_t stream, int num_sms) {
+    auto kern = append_umma_kernel<T, L>;
+    static thread_local int configured_dev = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (configured_dev != dev) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kUmmaSmem) != cudaSuccess)
+            return report_launch(cudaGetLastError());
+        configured_dev = dev;
+    }
+    UmmaTiles W;
+    W.key_rows = (uint32_t)P.N * (uint32_t)P.Hk;
+    const uint32_t q_rows = P.query ? (uint32_t)P.N * (uint32_t)P.Hq : 0u;
+    W.rows = W.key_rows + q_rows;
+    W.key_tiles = (W.key_rows + 127) / 128;
+    W.tiles = W.key_tiles + (q_rows + 127) / 128;
+    const unsigned grid = W.tiles < (uint32_t)num_sms ? W.tiles : (unsigned)num_sms;
+    kern<<<grid, kUmmaThreads, kUmmaSmem, stream>>>(P, W);
+    return report_launch(cudaGetLastError());
+}
+
+template <typename T, int L>
+int launch_append_t(const AppendParams& P, cudaStream_t stream, int num_sms) {
+    if constexpr (!layout_fp8_keys(L))
+        if (umma_aligned<T, L>(P)) return launch_append_umma<T, L>(P, stream, num_sms);
     auto kern = append_kernel<T, L>;
     const int smem = layout_fp8_keys(L) ? kRows * kHeadDim * 4 : kAppSmem;
     static thread_local int configured_dev = -1;
@@ -357,16 +921,16 @@ int launch_append_t(const AppendParams& P, cudaStream_t stream) {
 }
 
 template <typename T>
-int launch_append_d(const AppendParams& P, cudaStream_t stream) {
+int launch_append_d(const AppendParams& P, cudaStream_t stream, int num_sms) {
     switch (P.layout) {
-        case TQB_LAYOUT_SOA: return launch_append_t<T, TQB_LAYOUT_SOA>(P, stream);
-        case TQB_LAYOUT_SOA_K8: return launch_append_t<T, TQB_LAYOUT_SOA_K8>(P, stream);
-        case TQB_LAYOUT_SOA_K3: return launch_append_t<T, TQB_LAYOUT_SOA_K3>(P, stream);
-        case TQB_LAYOUT_SOA_K3V3: return launch_append_t<T, TQB_LAYOUT_SOA_K3V3>(P, stream);
-        case TQB_LAYOUT_AOS: return launch_append_t<T, TQB_LAYOUT_AOS>(P, stream);
-        case TQB_LAYOUT_AOS_K8: return launch_append_t<T, TQB_LAYOUT_AOS_K8>(P, stream);
-        case TQB_LAYOUT_AOS_K3: return launch_append_t<T, TQB_LAYOUT_AOS_K3>(P, stream);
-        case TQB_LAYOUT_AOS_K3V3: return launch_append_t<T, TQB_LAYOUT_AOS_K3V3>(P, stream);
+        case TQB_LAYOUT_SOA: return launch_append_t<T, TQB_LAYOUT_SOA>(P, stream, num_sms);
+        case TQB_LAYOUT_SOA_K8: return launch_append_t<T, TQB_LAYOUT_SOA_K8>(P, stream, num_sms);
+        case TQB_LAYOUT_SOA_K3: return launch_append_t<T, TQB_LAYOUT_SOA_K3>(P, stream, num_sms);
+        case TQB_LAYOUT_SOA_K3V3: return launch_append_t<T, TQB_LAYOUT_SOA_K3V3>(P, stream, num_sms);
+        case TQB_LAYOUT_AOS: return launch_append_t<T, TQB_LAYOUT_AOS>(P, stream, num_sms);
+        case TQB_LAYOUT_AOS_K8: return launch_append_t<T, TQB_LAYOUT_AOS_K8>(P, stream, num_sms);
+        case TQB_LAYOUT_AOS_K3: return launch_append_t<T, TQB_LAYOUT_AOS_K3>(P, stream, num_sms);
+        case TQB_LAYOUT_AOS_K3V3: return launch_append_t<T, TQB_LAYOUT_AOS_K3V3>(P, stream, num_sms);
         default: return TQB_ERR_INVALID_ARG;
     }
 }
@@ -374,14 +938,22 @@ int launch_append_d(const AppendParams& P, cudaStream_t stream) {
 }  // namespace
 
 int launch_append(const AppendParams& P, cudaStream_t stream, int num_sms) {
-    (void)num_sms;
     if (P.N == 0) return TQB_OK;
     switch (P.dtype) {
-        case TQB_DTYPE_F32: return launch_append_d<float>(P, stream);
-        case TQB_DTYPE_F16: return launch_append_d<__half>(P, stream);
-        case TQB_DTYPE_BF16: return launch_append_d<__nv_bfloat16>(P, stream);
+        case TQB_DTYPE_F32: return launch_append_d<float>(P, stream, num_sms);
+        case TQB_DTYPE_F16: return launch_append_d<__half>(P, stream, num_sms);
+        case TQB_DTYPE_BF16: return launch_append_d<__nv_bfloat16>(P, stream, num_sms);
         default: return TQB_ERR_INVALID_ARG;
     }
+}
+
+int read_append_timeouts(unsigned int* count, bool reset) {
+    cudaError_t e = cudaMemcpyFromSymbol(count, g_append_timeouts, sizeof(unsigned int));
+    if (e == cudaSuccess && reset) {
+        const unsigned int zero = 0;
+        e = cudaMemcpyToSymbol(g_append_timeouts, &zero, sizeof(unsigned int));
+    }
+    return e == cudaSuccess ? TQB_OK : report_launch(e);
 }
 
 }  // namespace tqb

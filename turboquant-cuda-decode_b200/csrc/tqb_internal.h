@@ -229,6 +229,7 @@ struct AppendParams {
     float* q_rot;
     int64_t osn, osh;
     int N, Hq, Hk, norm_correction;
+    FastDiv div_hk, div_hq;
 };
 
 // Cached keys and values of chosen slots (tqb_gather.cu).
@@ -300,6 +301,7 @@ int launch_stage2_range(const Stage2Params& p, cudaStream_t stream);
 int launch_append(const AppendParams& p, cudaStream_t stream, int num_sms);
 int launch_prefix(const PrefixParams& p, cudaStream_t stream);
 int read_prefix_timeouts(unsigned int* count, bool reset);
+int read_append_timeouts(unsigned int* count, bool reset);
 int launch_gather(const GatherParams& p, cudaStream_t stream);
 
 }  // namespace tqb

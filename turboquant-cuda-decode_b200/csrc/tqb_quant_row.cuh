@@ -86,83 +86,70 @@ __device__ __forceinline__ ValueRow quantise_values(const float (&vs)[8]) {
     return ValueRow{vbits, scale, vmin};
 }
 
+// The slot of token-head (off, h) in the block at `base`: value codes, fp16
+// key norm, value scale and zero.
+template <int L>
+struct SlotAt {
+    uint8_t *key, *value, *norm, *scale, *zero;
+    __device__ __forceinline__ SlotAt(uint8_t* base, uint32_t off, uint32_t h, int H, int64_t pos_stride,
+                                      int64_t head_stride) {
+        if constexpr (layout_is_aos(L)) {
+            // [key codes | fp16 norm | value codes | fp16 scale | fp16 zero]
+            // (reference/aos_store.py:26-116, :183-203, :296-325)
+            key = base + (size_t)off * pos_stride + (size_t)h * head_stride;
+            value = key + aos_val_off(L);
+            norm = key + aos_norm_off(L);
+            scale = key + aos_scale_off(L);
+            zero = scale + 2;
+        } else {
+            constexpr int kKey = aos_key_bytes(L), kRow = kKey + val_code_bytes(L), kFields = layout_fp8_keys(L) ? 2 : 3;
+            key = base + (size_t)off * ((size_t)H * kRow) + (size_t)h * kRow;
+            value = key + kKey;
+            norm = base + (size_t)kBlockSize * H * kRow + ((size_t)h * kFields * kBlockSize + off) * 2;
+            scale = norm + (kFields - 2) * kBlockSize * 2;
+            zero = scale + kBlockSize * 2;
+        }
+    }
+};
+
+// Half a warp's value codes (lane m of 16: dims 8m .. 8m + 7) and their grid.
+template <int L>
+__device__ __forceinline__ void write_values(const SlotAt<L>& at, int m, const ValueRow& v) {
+    if constexpr (layout_3bit_values(L))
+        st_bytes3(at.value + 3 * m, v.bits);
+    else if constexpr (L == TQB_LAYOUT_SOA_K8)
+        reinterpret_cast<uint32_t*>(at.value)[m] = v.bits;  // 4-byte aligned rows (checked on the host)
+    else
+        st_u16x2(at.value + 4 * m, v.bits);
+    if (m == 0) {
+        *reinterpret_cast<unsigned short*>(at.scale) = __half_as_ushort(__float2half_rn(v.scale));
+        *reinterpret_cast<unsigned short*>(at.zero) = __half_as_ushort(__float2half_rn(v.vmin));
+    }
+}
+
 // Writes one token-head of layout L into token `off` of the block at `base`:
 // lane m of 16 holds dims 8m .. 8m + 7, their key codes in kbits (e4m3 keys:
-// the bytes in klo, khi) and value codes in vbits; vn_h is the fp16 key norm
-// as stored (SoA: with the norm correction folded in, AoS: the raw norm,
+// the bytes in klo, khi) and value codes in v; vn_h is the fp16 key norm as
+// stored (SoA: with the norm correction folded in, AoS: the raw norm,
 // reference/aos_store.py:317-325).  H KV heads, this one is h.
 template <int L>
 __device__ __forceinline__ void write_row(uint8_t* base, uint32_t off, uint32_t h, int H, int64_t pos_stride,
                                           int64_t head_stride, int m, uint32_t kbits, uint32_t klo, uint32_t khi,
-                                          uint32_t vbits, unsigned short vn_h, float scale, float vmin) {
-    constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), v3 = layout_3bit_values(L);
-    const unsigned short sc_h = __half_as_ushort(__float2half_rn(scale));
-    const unsigned short zr_h = __half_as_ushort(__float2half_rn(vmin));
+                                          const ValueRow& v, unsigned short vn_h) {
+    const SlotAt<L> at(base, off, h, H, pos_stride, head_stride);
     if constexpr (L == TQB_LAYOUT_SOA_K8) {
-        // 4-byte aligned rows (checked on the host): two words of e4m3 bytes
-        uint8_t* dp = base + (size_t)off * ((size_t)H * kK8DataBytes) + (size_t)h * kK8DataBytes;
-        reinterpret_cast<uint32_t*>(dp)[2 * m] = klo;
-        reinterpret_cast<uint32_t*>(dp)[2 * m + 1] = khi;
-        reinterpret_cast<uint32_t*>(dp + kK8KeyBytes)[m] = vbits;
-        if (m == 0) {
-            unsigned short* meta = reinterpret_cast<unsigned short*>(
-                base + (size_t)kBlockSize * H * kK8DataBytes) + (size_t)h * 2 * kBlockSize;
-            meta[off] = sc_h;
-            meta[kBlockSize + off] = zr_h;
-        }
-    } else if constexpr (L == TQB_LAYOUT_SOA_K3V3 || L == TQB_LAYOUT_SOA_K3) {
-        constexpr int row = v3 ? kK3V3DataBytes : kK3DataBytes;
-        uint8_t* dp = base + (size_t)off * ((size_t)H * row) + (size_t)h * row;
-        st_bytes3(dp + 3 * m, kbits);  // dims 8m .. 8m+7 = bits 24m .. 24m+23 of the stream
-        if constexpr (v3)
-            st_bytes3(dp + kK3KeyBytes + 3 * m, vbits);
-        else
-            st_u16x2(dp + kK3KeyBytes + 4 * m, vbits);
-        if (m == 0) {
-            unsigned short* meta = reinterpret_cast<unsigned short*>(
-                base + (size_t)kBlockSize * H * row) + (size_t)h * 3 * kBlockSize;
-            meta[off] = vn_h;
-            meta[kBlockSize + off] = sc_h;
-            meta[2 * kBlockSize + off] = zr_h;
-        }
-    } else if constexpr (L == TQB_LAYOUT_SOA) {
-        uint8_t* dp = base + (size_t)off * ((size_t)H * kDataBytes) + (size_t)h * kDataBytes;
-        st_u16x2(dp + 4 * m, kbits);
-        st_u16x2(dp + kKBytes + 4 * m, vbits);
-        if (m == 0) {
-            unsigned short* meta = reinterpret_cast<unsigned short*>(
-                base + (size_t)kBlockSize * H * kDataBytes) + (size_t)h * 3 * kBlockSize;
-            meta[off] = vn_h;
-            meta[kBlockSize + off] = sc_h;
-            meta[2 * kBlockSize + off] = zr_h;
-        }
+        reinterpret_cast<uint32_t*>(at.key)[2 * m] = klo;
+        reinterpret_cast<uint32_t*>(at.key)[2 * m + 1] = khi;
+    } else if constexpr (layout_fp8_keys(L)) {
+        st_u16x2(at.key + 8 * m, klo);
+        st_u16x2(at.key + 8 * m + 4, khi);
+    } else if constexpr (layout_3bit_keys(L)) {
+        st_bytes3(at.key + 3 * m, kbits);  // dims 8m .. 8m+7 = bits 24m .. 24m+23 of the stream
     } else {
-        // AoS slot (layout_is_aos): [key codes | fp16 norm | value codes |
-        // fp16 scale | fp16 zero], 2-byte aligned, so 16-bit and byte stores
-        // (reference/aos_store.py:26-116, :183-203, :296-325).
-        uint8_t* sp = base + (size_t)off * pos_stride + (size_t)h * head_stride;
-        if constexpr (k8) {  // e4m3 bytes of dims 8m .. 8m + 7
-            st_u16x2(sp + 8 * m, klo);
-            st_u16x2(sp + 8 * m + 4, khi);
-        } else if constexpr (k3) {
-            st_bytes3(sp + 3 * m, kbits);
-        } else {
-            st_u16x2(sp + 4 * m, kbits);
-        }
-        uint8_t* vq = sp + aos_val_off(L);
-        if constexpr (v3)
-            st_bytes3(vq + 3 * m, vbits);
-        else
-            st_u16x2(vq + 4 * m, vbits);
-        if (m == 0) {
-            // (e4m3 keys have no norm)
-            if constexpr (!k8) {
-                reinterpret_cast<unsigned short*>(sp + aos_norm_off(L))[0] = vn_h;
-            }
-            reinterpret_cast<unsigned short*>(sp + aos_scale_off(L))[0] = sc_h;
-            reinterpret_cast<unsigned short*>(sp + aos_scale_off(L) + 2)[0] = zr_h;
-        }
+        st_u16x2(at.key + 4 * m, kbits);
     }
+    if (!layout_fp8_keys(L) && m == 0) *reinterpret_cast<unsigned short*>(at.norm) = vn_h;
+    write_values<L>(at, m, v);
 }
 
 }  // namespace tqb

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kStoreWarps * 32) store_kernel(const StorePara
     // AoS stores the raw norm (its decoders apply the correction)
     if constexpr (layout_is_aos(L) && !k8) vn = __ldg(P.norms + pid);
     write_row<L>(P.cache + (size_t)blk * (size_t)P.block_bytes, off, h, P.H, P.pos_stride, P.head_stride, m, kbits, klo,
-                 khi, vr.bits, __half_as_ushort(__float2half_rn(vn)), vr.scale, vr.vmin);
+                 khi, vr, __half_as_ushort(__float2half_rn(vn)));
 }
 
 }  // namespace
