@@ -435,7 +435,10 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
         da = turned ? j0 : P.rotary + (j0 - half);
         db = turned ? j0 + half : P.rotary + (64 - half) + (j0 - half);
     }
-    constexpr int kBatch = 4;
+    // (two rows in flight, and one piece of code for both rotary rules: four
+    // roles run at once, and their instructions have to stay in the caches)
+    constexpr int kBatch = 2;
+#pragma unroll 1
     for (int r0 = 2 * lw + (lane >> 4); r0 < 128; r0 += 8 * kBatch) {
         Quad<T> qa[kBatch], qb[kBatch];
         int pos[kBatch], tok[kBatch];
@@ -463,27 +466,18 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
             const int r = r0 + 8 * i;
-            float x[8];  // dims da .. da + 3, db .. db + 3
-            if (P.interleaved) {
-                const float cc[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, ss[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
-                const float in[8] = {qa[i].v[0], qa[i].v[1], qa[i].v[2], qa[i].v[3],
-                                     qb[i].v[0], qb[i].v[1], qb[i].v[2], qb[i].v[3]};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    x[2 * k] = fmaf(in[2 * k], cc[k], -(in[2 * k + 1] * ss[k]));
-                    x[2 * k + 1] = fmaf(in[2 * k + 1], cc[k], in[2 * k] * ss[k]);
-                }
-            } else {
-                const float cc[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, ss[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    x[k] = fmaf(qa[i].v[k], cc[k], -(qb[i].v[k] * ss[k]));
-                    x[4 + k] = fmaf(qb[i].v[k], cc[k], qa[i].v[k] * ss[k]);
-                }
-            }
+            const float cc[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, ss[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
+            const float in[8] = {qa[i].v[0], qa[i].v[1], qa[i].v[2], qa[i].v[3],
+                                 qb[i].v[0], qb[i].v[1], qb[i].v[2], qb[i].v[3]};
+            float u[4], v[4], x[8];  // the pairs, then dims da .. da + 3, db .. db + 3
             float nsq = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; k++) nsq = fmaf(x[k], x[k], nsq);
+            for (int k = 0; k < 4; k++) {
+                const float ak = P.interleaved ? in[2 * k] : in[k], bk = P.interleaved ? in[2 * k + 1] : in[4 + k];
+                u[k] = fmaf(ak, cc[k], -(bk * ss[k]));
+                v[k] = fmaf(bk, cc[k], ak * ss[k]);
+                nsq = fmaf(u[k], u[k], fmaf(v[k], v[k], nsq));
+            }
             nsq = warp_sum_xor(nsq, 1, 8);
             // |x| 2^e in [2^13, 2^15): e from the exponent of |x|^2 (its half,
             // rounded up); 0 for zero and non-finite rows, whose codes come
@@ -491,13 +485,17 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
             const int be = (int)(__float_as_uint(nsq) >> 23);
             const int e = be == 0 || be == 0xFF ? 0 : 14 - ((be - 126) >> 1);
             const float f = exp2i(e);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                x[k] = (P.interleaved ? (k & 1 ? v[k >> 1] : u[k >> 1]) : u[k]) * f;
+                x[4 + k] = (P.interleaved ? (k & 1 ? v[2 + (k >> 1)] : u[2 + (k >> 1)]) : v[k]) * f;
+            }
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float u = x[2 * k] * f, v = x[2 * k + 1] * f;
-                const __half2 h = __floats2half2_rn(u, v);
+                const __half2 h = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
                 hi[k] = h2_as_u32(h);
-                lo[k] = h2_as_u32(__floats2half2_rn(u - __low2float(h), v - __high2float(h)));
+                lo[k] = h2_as_u32(__floats2half2_rn(x[2 * k] - __low2float(h), x[2 * k + 1] - __high2float(h)));
             }
             // four dims are 8 bytes of a 16-byte chunk
             auto at = [&](int d) { return (d >> 6) * (kATile / 2) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2; };
@@ -522,12 +520,35 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
     }
 }
 
+// Asks L2 for a tile's rows (t: 0 .. 127).
+template <typename T>
+__device__ __forceinline__ void prefetch_rows(const T* base, int64_t sn, int64_t sh, const FastDiv& div, uint32_t H, uint32_t first,
+                                              uint32_t total, int t) {
+    constexpr int kLines = sizeof(T);  // 128-byte lines of a row
+#pragma unroll
+    for (int i = 0; i < kLines; i++) {
+        const uint32_t line = (uint32_t)(t + 128 * i), row = first + line / kLines;
+        if (row < total) {
+            const uint32_t n = div.div(row), h = row - n * H;
+            asm volatile("prefetch.global.L2 [%0];\n" ::"l"(base + (int64_t)n * sn + (int64_t)h * sh + (line % kLines) * (128 / kLines)));
+        }
+    }
+}
+
+// Code of y by search (a codebook too fine for the cells).
+template <int NC>
+__device__ __noinline__ int search(const float* mids, float y) {
+    int code = 0;
+    for (int k = 0; k < NC - 1; k++) code += y >= mids[k] ? 1 : 0;
+    return code;
+}
+
 // A key row: codes of its 128 coordinates, norm, slot.
 template <typename T, int L>
 __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem, uint32_t tm, uint32_t row, const RowInfo& info,
                                             bool fine, int lane) {
     constexpr bool k3 = layout_3bit_keys(L);
-    constexpr int nc = k3 ? 8 : kNumCentroids, kBits = k3 ? 3 : 4, kWords = k3 ? 12 : 16;
+    constexpr int nc = k3 ? 8 : kNumCentroids, kBits = k3 ? 3 : 4;
     constexpr unsigned kFull = 0xffffffffu;
     const float* smid = reinterpret_cast<const float*>(smem + kTabOff);
     const float* csq16 = smid + kNumCentroids;
@@ -535,18 +556,22 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
     const float f = info.unscale * __frcp_rn(norm + 1e-8f);
     const uint32_t h = row - (uint32_t)info.n * (uint32_t)P.Hk;
     const uint8_t* cells = smem + kCellOff + 4 * lane;
-    // coordinates next to a border, and those on its upper side as far as fp32 says
-    uint32_t words[kWords], near[4] = {0u, 0u, 0u, 0u}, upper[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < kWords; i++) words[i] = 0u;
+    const bool stored = info.slot >= 0;
+    const uint32_t slot = stored ? (uint32_t)info.slot : 0u;
+    const SlotAt<L> at(P.cache + (size_t)(slot / kBlockSize) * (size_t)P.block_bytes, slot % kBlockSize, h, P.Hk, P.pos_stride,
+                       P.head_stride);
     float csq = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-        uint32_t z[32];
-        tmem_ld32(z, tm + 32 * q);
+#pragma unroll 1
+    for (int q = 0; q < 8; q++) {
+        uint32_t z[16];
+        tmem_ld16(z, tm + 16 * q);
         tmem_wait_ld();
+        // coordinates next to a border, and those on its upper side as far as
+        // fp32 says
+        uint32_t near = 0u, upper = 0u;
+        uint64_t codes = 0u;  // 16 of them
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
+        for (int j = 0; j < 16; j++) {
             const float y = __uint_as_float(z[j]) * f;
             int code;
             bool close, up;
@@ -560,59 +585,43 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
                 code = (int)(e & 15u) + (up ? 1 : 0);
                 close = fabsf(d) < kNearMma;
             } else {
-                code = 0;
-#pragma unroll 1
-                for (int k = 0; k < nc - 1; k++) code += y >= smid[k] ? 1 : 0;
-                up = code > 0 && y - smid[code - 1] < kNearMma;
+                code = search<nc>(smid, y);
+                up = code > 0 && y - smid[max(code - 1, 0)] < kNearMma;
                 close = up || (code < nc - 1 && smid[code] - y < kNearMma);
             }
             csq += csq16[code];
-            if (close) {
-                near[q] |= 1u << j;
-                if (up) upper[q] |= 1u << j;
-            }
-            const int bit = kBits * (32 * q + j);
-            words[bit >> 5] |= (uint32_t)code << (bit & 31);
-            if ((bit & 31) + kBits > 32) words[(bit >> 5) + 1] |= (uint32_t)code >> (32 - (bit & 31));
+            near |= close ? 1u << j : 0u;
+            upper |= up ? 1u << j : 0u;
+            codes |= (uint64_t)(uint32_t)code << (kBits * j);
         }
-    }
-    // coordinates next to a border, in 64 bits by the whole warp (a row with
-    // none stored needs none)
-    const bool stored = info.slot >= 0;
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-        if (!stored) near[q] = 0u;
+        // in 64 bits by the whole warp (a row that is not stored needs none)
+        if (!stored) near = 0u;
         uint32_t who;
-        while ((who = __ballot_sync(kFull, near[q] != 0u)) != 0u) {
+        while ((who = __ballot_sync(kFull, near != 0u)) != 0u) {
             const int src = __ffs(who) - 1;
             const int sn = __shfl_sync(kFull, info.n, src), sh = __shfl_sync(kFull, (int)h, src);
-            const int j = __shfl_sync(kFull, __ffs(near[q]) - 1, src);
-            const int pos = position_of(P, sn);
+            const int j = __shfl_sync(kFull, __ffs(near) - 1, src);
             const T* krow = static_cast<const T*>(P.key) + (int64_t)sn * P.ksn + (int64_t)sh * P.ksh;
-            // the border next to it: between the code and one of its neighbours
-            const int bit = kBits * (32 * q + j);
-            int code = 0;
-#pragma unroll
-            for (int w = 0; w < kWords; w++) {
-                if (w == (bit >> 5)) code |= (int)(words[w] >> (bit & 31));
-                if (w == (bit >> 5) + 1 && (bit & 31) + kBits > 32) code |= (int)(words[w] << (32 - (bit & 31)));
-            }
-            code &= (1 << kBits) - 1;
-            const int c0 = __shfl_sync(kFull, code, src);
-            const bool was_up = __shfl_sync(kFull, (int)(upper[q] >> j), src) & 1;
-            const int border = was_up ? c0 - 1 : c0;
-            const int c = border + (exact_side<T>(P, krow, table_row<T>(P, pos), 32 * q + j, smid[border], lane) ? 1 : 0);
+            const int c0 = (int)(codes >> (kBits * j)) & (nc - 1);
+            // the border next to it, below or above the code
+            const int border = __shfl_sync(kFull, c0 - (int)((upper >> j) & 1u), src);
+            const int c = border + (exact_side<T>(P, krow, table_row<T>(P, position_of(P, sn)), 16 * q + j, smid[border], lane) ? 1 : 0);
             if (lane == src) {
-                near[q] &= near[q] - 1;
-                if (c != c0) {
-                    csq += csq16[c] - csq16[c0];
-                    const uint64_t flip = (uint64_t)(uint32_t)(c ^ c0) << (bit & 31);
+                near &= near - 1;
+                csq += csq16[c] - csq16[c0];
+                codes ^= (uint64_t)(uint32_t)(c ^ c0) << (kBits * j);
+            }
+        }
+        if (stored) {
+            if constexpr (k3) {
 #pragma unroll
-                    for (int w = 0; w < kWords; w++) {
-                        if (w == (bit >> 5)) words[w] ^= (uint32_t)flip;
-                        if (w == (bit >> 5) + 1) words[w] ^= (uint32_t)(flip >> 32);
-                    }
-                }
+                for (int i = 0; i < 3; i++)
+                    reinterpret_cast<unsigned short*>(at.key)[3 * q + i] = (unsigned short)(codes >> (16 * i));
+            } else if constexpr (layout_is_aos(L)) {
+                st_u16x2(at.key + 8 * q, (uint32_t)codes);
+                st_u16x2(at.key + 8 * q + 4, (uint32_t)(codes >> 32));
+            } else {
+                reinterpret_cast<uint2*>(at.key)[q] = make_uint2((uint32_t)codes, (uint32_t)(codes >> 32));
             }
         }
     }
@@ -628,43 +637,23 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
         const int sn = __shfl_sync(kFull, info.n, src), sh = __shfl_sync(kFull, (int)h, src);
         const T* krow = static_cast<const T*>(P.key) + (int64_t)sn * P.ksn + (int64_t)sh * P.ksh;
         double v = exact_norm<T>(P, krow, table_row<T>(P, position_of(P, sn)), lane);
-        if (lane == src) {
-            if (fold) {
-                double cq = 0.0;
-#pragma unroll
-                for (int w = 0; w < kWords; w++) {
-                    if constexpr (!k3) {
-                        for (int i = 0; i < 8; i++) {
-                            const double cv = (double)__ldg(P.cents + ((words[w] >> (4 * i)) & 15u));
-                            cq += cv * cv;
-                        }
-                    } else if (w % 3 == 0) {
-                        const uint64_t a = (uint64_t)words[w] | ((uint64_t)words[w + 1] << 32);
-                        const uint64_t b = (uint64_t)words[w + 1] | ((uint64_t)words[w + 2] << 32);
-                        for (int i = 0; i < 32; i++) {
-                            const uint32_t c = (uint32_t)(3 * i < 60 ? a >> (3 * i) : b >> (3 * i - 32)) & 7u;
-                            const double cv = (double)__ldg(P.cents + c);
-                            cq += cv * cv;
-                        }
-                    }
-                }
-                v /= sqrt(cq + 1e-16);
+        if (fold) {
+            // the codes just written: four per lane, from the row's bytes
+            __syncwarp();
+            const uint8_t* codes = reinterpret_cast<const uint8_t*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(at.key), src));
+            double cq = 0.0;
+            for (int i = 0; i < 4; i++) {
+                const int bit = kBits * (4 * lane + i);
+                const volatile uint8_t* b = codes + (bit >> 3);
+                const uint32_t two = (uint32_t)b[0] | ((bit & 7) + kBits > 8 ? (uint32_t)b[1] << 8 : 0u);
+                const double cv = (double)__ldg(P.cents + ((two >> (bit & 7)) & (nc - 1)));
+                cq += cv * cv;
             }
-            kept_h = __half_as_ushort(__double2half(v));
+            v /= sqrt(warp_sum_f64(cq) + 1e-16);
         }
+        if (lane == src) kept_h = __half_as_ushort(__double2half(v));
     }
-    if (!stored) return;
-    const SlotAt<L> at(P.cache + (size_t)((uint32_t)info.slot / kBlockSize) * (size_t)P.block_bytes,
-                       (uint32_t)info.slot % kBlockSize, h, P.Hk, P.pos_stride, P.head_stride);
-    if constexpr (layout_is_aos(L)) {  // 2-byte aligned slots
-#pragma unroll
-        for (int w = 0; w < kWords; w++) st_u16x2(at.key + 4 * w, words[w]);
-    } else {
-#pragma unroll
-        for (int w = 0; w < kWords; w += 4)
-            *reinterpret_cast<uint4*>(at.key + 4 * w) = make_uint4(words[w], words[w + 1], words[w + 2], words[w + 3]);
-    }
-    *reinterpret_cast<unsigned short*>(at.norm) = kept_h;
+    if (stored) *reinterpret_cast<unsigned short*>(at.norm) = kept_h;
 }
 
 // Query rows: the product itself, turned through shared memory into runs of
@@ -701,11 +690,12 @@ __device__ __forceinline__ void finish_queries(const AppendParams& P, uint8_t* t
     }
 }
 
-// The values of a tile's rows, half a warp each, four in flight.
+// The values of a tile's rows, half a warp each, two in flight.
 template <typename T, int L>
 __device__ __forceinline__ void store_values(const AppendParams& P, const UmmaTiles& W, uint32_t tile, int vw, int lane) {
     const int m = lane & 15;
-    constexpr int kBatch = 4;
+    constexpr int kBatch = 2;
+#pragma unroll 1
     for (int r0 = 2 * vw + (lane >> 4); r0 < 128; r0 += 8 * kBatch) {
         Quad<T> a[kBatch], b[kBatch];
         int slot[kBatch];
@@ -834,6 +824,13 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
             // the operands' last readers, and the rows' (their infos and sums)
             ok = ok && bar_wait_warp(bars + kAEmpty, (i & 1) ^ 1, abort) &&
                  bar_wait_warp(bars + kDEmpty + 8 * buf, ((i >> 1) & 1) ^ 1, abort);
+            const uint32_t next = tile + gridDim.x;
+            if (next < W.key_tiles)
+                prefetch_rows<T>(static_cast<const T*>(P.key), P.ksn, P.ksh, P.div_hk, (uint32_t)P.Hk, next * 128u, W.key_rows,
+                                 tid & 127);
+            else if (next < W.tiles)
+                prefetch_rows<T>(static_cast<const T*>(P.query), P.qsn, P.qsh, P.div_hq, (uint32_t)P.Hq,
+                                 (next - W.key_tiles) * 128u, W.rows - W.key_rows, tid & 127);
             if (ok) turn_rows<T>(P, smem, W, tile, buf, warp - 8, lane);
             fence_async_smem();
             asm volatile("bar.sync 1, 128;\n" ::: "memory");  // every warp takes every turn, also after an error
@@ -854,7 +851,11 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
         // every product has ended before the CTA frees its TMEM
         if (warp == 8 && i > 0) bar_wait_warp(bars + kAEmpty, (i - 1) & 1, nullptr);
     } else {
-        for (uint32_t tile = blockIdx.x; tile < W.key_tiles; tile += gridDim.x) store_values<T, L>(P, W, tile, warp - 12, lane);
+        for (uint32_t tile = blockIdx.x; tile < W.key_tiles; tile += gridDim.x) {
+            prefetch_rows<T>(static_cast<const T*>(P.value), P.vsn, P.vsh, P.div_hk, (uint32_t)P.Hk, (tile + gridDim.x) * 128u,
+                             W.key_rows, tid & 127);
+            store_values<T, L>(P, W, tile, warp - 12, lane);
+        }
     }
     __syncwarp();
     tc_fence_before();
