@@ -390,19 +390,24 @@ struct __align__(16) RowInfo {
     int n, slot;
 };
 
-// Two bf16 or fp16 numbers, or the first / second of two floats.
 template <typename T>
-struct Quad {  // four consecutive elements
-    float v[4];
+struct Quad {  // four consecutive elements, as loaded
+    uint32_t w[sizeof(T)];
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (sizeof(T) == 4) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(p));
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
         } else {
             const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-            const T* h = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = to_f32<T>(h[i]);
+            w[0] = u.x; w[1] = u.y;
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[i]);
+        } else {
+            const unsigned short h = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
+            return to_f32<T>(*reinterpret_cast<const T*>(&h));
         }
     }
 };
@@ -435,40 +440,65 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
         da = turned ? j0 : P.rotary + (j0 - half);
         db = turned ? j0 + half : P.rotary + (64 - half) + (j0 - half);
     }
-    // (two rows in flight, and one piece of code for both rotary rules: four
-    // roles run at once, and their instructions have to stay in the caches)
+    // One piece of code for both rotary rules (four roles run at once, and their
+    // instructions have to stay in the caches), two rows at a time; the next
+    // two are loaded while these are turned, and the positions of the two after
+    // them, which their angles wait for.
+    struct Row {
+        Quad<T> a, b;
+        float4 c, s;
+        int n, pos;
+    };
     constexpr int kBatch = 2;
-#pragma unroll 1
-    for (int r0 = 2 * lw + (lane >> 4); r0 < 128; r0 += 8 * kBatch) {
-        Quad<T> qa[kBatch], qb[kBatch];
-        int pos[kBatch], tok[kBatch];
+    Row now[kBatch], then[kBatch];
+    const int r_first = 2 * lw + (lane >> 4);
+    auto token = [&](int r, int& n, uint32_t& h) {
+        const uint32_t row = min(first + (uint32_t)r, total - 1);
+        const uint32_t t = div.div(row);
+        n = (int)t;
+        h = row - t * H;
+    };
+    auto find = [&](Row (&x)[kBatch], int r0) {  // tokens and positions
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            const uint32_t row = min(first + r0 + 8 * i, total - 1);
-            const uint32_t n = div.div(row), h = row - n * H;
-            tok[i] = (int)n;
-            pos[i] = position_of(P, (int)n);
-            const T* p = base + (int64_t)n * sn + (int64_t)h * sh;
-            qa[i].load(p + da);
-            qb[i].load(p + db);
+            uint32_t h;
+            token(r0 + 8 * i, x[i].n, h);
+            x[i].pos = position_of(P, x[i].n);
         }
-        float4 c[kBatch], s[kBatch];
+    };
+    auto load = [&](Row (&x)[kBatch], int r0) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            c[i] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-            s[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            int n;
+            uint32_t h;
+            token(r0 + 8 * i, n, h);
+            const T* p = base + (int64_t)n * sn + (int64_t)h * sh;
+            x[i].a.load(p + da);
+            x[i].b.load(p + db);
+            x[i].c = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+            x[i].s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (turned) {
-                const float* cs = table_row<T>(P, pos[i]) + j0;
-                c[i] = __ldg(reinterpret_cast<const float4*>(cs));
-                s[i] = __ldg(reinterpret_cast<const float4*>(cs + half));
+                const float* cs = table_row<T>(P, x[i].pos) + j0;
+                x[i].c = __ldg(reinterpret_cast<const float4*>(cs));
+                x[i].s = __ldg(reinterpret_cast<const float4*>(cs + half));
             }
         }
+    };
+    find(now, r_first);
+    find(then, r_first + 8 * kBatch);
+    load(now, r_first);
+#pragma unroll 1
+    for (int r0 = r_first; r0 < 128; r0 += 8 * kBatch) {
+        load(then, r0 + 8 * kBatch);
+        Row after[kBatch];
+        find(after, r0 + 16 * kBatch);
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
             const int r = r0 + 8 * i;
-            const float cc[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, ss[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
-            const float in[8] = {qa[i].v[0], qa[i].v[1], qa[i].v[2], qa[i].v[3],
-                                 qb[i].v[0], qb[i].v[1], qb[i].v[2], qb[i].v[3]};
+            const float cc[4] = {now[i].c.x, now[i].c.y, now[i].c.z, now[i].c.w};
+            const float ss[4] = {now[i].s.x, now[i].s.y, now[i].s.z, now[i].s.w};
+            const float in[8] = {now[i].a[0], now[i].a[1], now[i].a[2], now[i].a[3],
+                                 now[i].b[0], now[i].b[1], now[i].b[2], now[i].b[3]};
             float u[4], v[4], x[8];  // the pairs, then dims da .. da + 3, db .. db + 3
             float nsq = 0.0f;
 #pragma unroll
@@ -507,15 +537,18 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
                 RowInfo info;
                 info.nsq = nsq;
                 info.unscale = exp2i(-e) * 0x1p-10f;
-                info.n = tok[i];
+                info.n = now[i].n;
                 int slot = -1;
-                if (first + r < total && pos[i] >= 0) {
-                    slot = keys ? __ldg(P.slots + tok[i]) : 0;
+                if (first + r < total && now[i].pos >= 0) {
+                    slot = keys ? __ldg(P.slots + now[i].n) : 0;
                     if (keys && P.num_blocks > 0 && (int64_t)slot >= P.num_blocks * kBlockSize) slot = -1;
                 }
                 info.slot = max(slot, -1);
                 reinterpret_cast<RowInfo*>(smem + kInfoOff)[buf * 128 + r] = info;
             }
+            now[i] = then[i];
+            then[i].n = after[i].n;
+            then[i].pos = after[i].pos;
         }
     }
 }
@@ -577,9 +610,10 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
             bool close, up;
             if (fine) {
                 // the nearest border of y's cell, its index in the low bits
-                const float t = fminf(fmaxf(fmaf(y, kCells / (2.0f * kCellSpan), 0x1p23f + kCells / 2), 0x1p23f),
-                                      0x1p23f + (kCells - 1));
-                const uint32_t e = *reinterpret_cast<const uint32_t*>(cells + ((__float_as_uint(t) & (kCells - 1)) << 7));
+                // (t counts 128ths of cells, so that its integer is the byte offset)
+                const float t = fminf(fmaxf(fmaf(y, 128.0f * kCells / (2.0f * kCellSpan), 0x1p23f + 64.0f * kCells + 64.0f), 0x1p23f),
+                                      0x1p23f + (128.0f * kCells - 1.0f));
+                const uint32_t e = *reinterpret_cast<const uint32_t*>(cells + (__float_as_uint(t) & (128u * (kCells - 1))));
                 const float d = y - __uint_as_float(e);
                 up = d >= 0.0f;
                 code = (int)(e & 15u) + (up ? 1 : 0);
@@ -690,36 +724,47 @@ __device__ __forceinline__ void finish_queries(const AppendParams& P, uint8_t* t
     }
 }
 
-// The values of a tile's rows, half a warp each, two in flight.
+// The values of a tile's rows, half a warp each, two at a time with the next
+// two in flight.
 template <typename T, int L>
 __device__ __forceinline__ void store_values(const AppendParams& P, const UmmaTiles& W, uint32_t tile, int vw, int lane) {
     const int m = lane & 15;
     constexpr int kBatch = 2;
-#pragma unroll 1
-    for (int r0 = 2 * vw + (lane >> 4); r0 < 128; r0 += 8 * kBatch) {
-        Quad<T> a[kBatch], b[kBatch];
-        int slot[kBatch];
-        uint32_t hs[kBatch];
+    struct Row {
+        Quad<T> a, b;
+        int slot, pos;
+        uint32_t h;
+    };
+    Row now[kBatch], then[kBatch];
+    auto load = [&](Row (&x)[kBatch], int r0) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
             const uint32_t row0 = tile * 128u + r0 + 8 * i, row = min(row0, W.key_rows - 1);
-            const uint32_t n = P.div_hk.div(row), h = row - n * (uint32_t)P.Hk;
-            const T* v = static_cast<const T*>(P.value) + (int64_t)n * P.vsn + (int64_t)h * P.vsh + 8 * m;
-            a[i].load(v);
-            b[i].load(v + 4);
-            int s = row0 < W.key_rows ? __ldg(P.slots + n) : -1;
-            if ((P.num_blocks > 0 && (int64_t)s >= P.num_blocks * kBlockSize) || position_of(P, (int)n) < 0) s = -1;
-            slot[i] = s;
-            hs[i] = h;
+            const uint32_t n = P.div_hk.div(row);
+            x[i].h = row - n * (uint32_t)P.Hk;
+            const T* v = static_cast<const T*>(P.value) + (int64_t)n * P.vsn + (int64_t)x[i].h * P.vsh + 8 * m;
+            x[i].a.load(v);
+            x[i].b.load(v + 4);
+            x[i].slot = row0 < W.key_rows ? __ldg(P.slots + n) : -1;
+            x[i].pos = position_of(P, (int)n);
         }
+    };
+    const int r_first = 2 * vw + (lane >> 4);
+    load(now, r_first);
+#pragma unroll 1
+    for (int r0 = r_first; r0 < 128; r0 += 8 * kBatch) {
+        load(then, r0 + 8 * kBatch);
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            const float v[8] = {a[i].v[0], a[i].v[1], a[i].v[2], a[i].v[3], b[i].v[0], b[i].v[1], b[i].v[2], b[i].v[3]};
+            const float v[8] = {now[i].a[0], now[i].a[1], now[i].a[2], now[i].a[3],
+                                now[i].b[0], now[i].b[1], now[i].b[2], now[i].b[3]};
             const ValueRow q = quantise_values<layout_3bit_values(L)>(v);
-            if (slot[i] >= 0)
-                write_values<L>(SlotAt<L>(P.cache + (size_t)((uint32_t)slot[i] / kBlockSize) * (size_t)P.block_bytes,
-                                          (uint32_t)slot[i] % kBlockSize, hs[i], P.Hk, P.pos_stride, P.head_stride),
+            const int slot = now[i].slot;
+            if (slot >= 0 && now[i].pos >= 0 && (P.num_blocks <= 0 || (int64_t)slot < P.num_blocks * kBlockSize))
+                write_values<L>(SlotAt<L>(P.cache + (size_t)((uint32_t)slot / kBlockSize) * (size_t)P.block_bytes,
+                                          (uint32_t)slot % kBlockSize, now[i].h, P.Hk, P.pos_stride, P.head_stride),
                                 m, q);
+            now[i] = then[i];
         }
     }
 }
