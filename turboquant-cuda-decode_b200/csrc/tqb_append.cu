@@ -355,39 +355,42 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
 // ---------------------------------------------------------------------------
 // Many rows of aligned inputs (Lloyd-Max layouts): the rotation on the tensor
 // cores.  A persistent CTA walks tiles of 128 rows (of keys, then of queries):
-//   warps 0-3, 4-7  finish tiles by turns: thread = row (= TMEM lane), its 128
-//                   coordinates bucketised and packed, or written (queries);
-//   warps 8-11      turn the rows and split them: x 2^s = hi + lo in fp16 (22
-//                   bits), s from |x|; the first of them issues the products;
-//   warps 12-15     the values of the CTA's key rows, half a warp each.
+//   warps 0-3    finish a tile: thread = row (= TMEM lane), its 128 coordinates
+//                bucketised and packed, or written (queries);
+//   warps 4-9    turn the next tile's rows and split them: x 2^s = hi + lo in
+//                fp16 (22 bits), s from |x|; the first of them issues the
+//                products;
+//   warps 10-15  the values of the CTA's key rows, half a warp each.
 // x R = hi R_hi + lo R_hi + hi R_lo in fp32 (R 2^10 split the same way, kept in
-// shared memory): 24 MMAs of 128 x 128 x 16 a tile.  Errors against exact
-// arithmetic: 2^-23 from the fp32 turn, 3 * 2^-22 from the splits, and 24
-// accumulations of at most 2^-23 each, 2^-18 of |x| in all (kNearMma).
+// shared memory): 24 MMAs of 128 x 128 x 16 a tile, the two small products
+// first.  Errors against exact arithmetic, of |x|: 2^-23 from the fp32 turn, 3 *
+// 2^-22 from the splits, 16 accumulations of 2^-23 at the size of the small
+// products (2^-10) and 8 of 2^-23 at full size: 2^-19 in all (kNearMma).
 // Bound by instruction issue: about 15 instructions per coordinate to
 // bucketise, 9 to turn and split, 10 per value.
 // ---------------------------------------------------------------------------
-constexpr float kNearMma = 0x1p-18f;
+constexpr float kNearMma = 0x1p-19f;
 constexpr int kATile = 128 * kHeadDim * 2;                                       // 32 KB
 constexpr int kAHiOff = 0, kALoOff = kATile, kBHiOff = 2 * kATile, kBLoOff = 3 * kATile;
 constexpr int kCells = 128;                                                      // of [-kCellSpan, kCellSpan)
 constexpr float kCellSpan = 0.25f;
 constexpr int kCellOff = 4 * kATile;                                             // [kCells][32 lanes]
-constexpr int kTurnOff = kCellOff + kCells * 32 * 4;                             // 8 warps x 4 KB
-constexpr int kInfoOff = kTurnOff + 8 * 4096;                                    // [2][128] RowInfo
-constexpr int kTabOff = kInfoOff + 2 * 128 * 16;                                 // mids, c^2
+constexpr int kTurnOff = kCellOff + kCells * 32 * 4;                             // 4 warps x 4 KB
+constexpr int kInfoOff = kTurnOff + 4 * 4096;                                    // [2][128] RowInfo
+constexpr int kTabOff = kInfoOff + 2 * 128 * 24;                                 // mids, c^2
 constexpr int kUmmaBarOff = kTabOff + 2 * kNumCentroids * 4;
 constexpr int kUmmaSmem = kUmmaBarOff + 64;
 static_assert(kUmmaSmem <= 232448, "shared memory per CTA");
-constexpr int kUmmaThreads = 512;
+constexpr int kFinishWarps = 4, kTurnWarps = 6, kValueWarps = 6;
+constexpr int kUmmaThreads = (kFinishWarps + kTurnWarps + kValueWarps) * 32;
 enum : uint32_t { kAEmpty = 0, kDFull = 8, kDEmpty = 24, kUTmem = 40, kUAbort = 44 };
 
 // What the finishing warps need of a row: the sum of squares, the factor that
 // undoes the scales, its token and KV head (or query head), and its slot (-1:
 // not stored; queries: -1 where the position is outside the table).
-struct __align__(16) RowInfo {
+struct __align__(8) RowInfo {
     float nsq, unscale;
-    int n, slot;
+    int n, slot, pos, pad;
 };
 
 template <typename T>
@@ -442,15 +445,14 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
     }
     // One piece of code for both rotary rules (four roles run at once, and their
     // instructions have to stay in the caches), two rows at a time; the next
-    // two are loaded while these are turned, and the positions of the two after
-    // them, which their angles wait for.
+    // two are loaded while these are turned.
     struct Row {
         Quad<T> a, b;
         float4 c, s;
         int n, pos;
     };
-    constexpr int kBatch = 2;
-    Row now[kBatch], then[kBatch];
+    constexpr int kBatch = 2, kStep = 2 * kTurnWarps;  // rows of the role's warps together
+    Row x0[kBatch], x1[kBatch];
     const int r_first = 2 * lw + (lane >> 4);
     auto token = [&](int r, int& n, uint32_t& h) {
         const uint32_t row = min(first + (uint32_t)r, total - 1);
@@ -462,7 +464,7 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
             uint32_t h;
-            token(r0 + 8 * i, x[i].n, h);
+            token(r0 + kStep * i, x[i].n, h);
             x[i].pos = position_of(P, x[i].n);
         }
     };
@@ -471,7 +473,7 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
         for (int i = 0; i < kBatch; i++) {
             int n;
             uint32_t h;
-            token(r0 + 8 * i, n, h);
+            token(r0 + kStep * i, n, h);
             const T* p = base + (int64_t)n * sn + (int64_t)h * sh;
             x[i].a.load(p + da);
             x[i].b.load(p + db);
@@ -484,17 +486,10 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
             }
         }
     };
-    find(now, r_first);
-    find(then, r_first + 8 * kBatch);
-    load(now, r_first);
-#pragma unroll 1
-    for (int r0 = r_first; r0 < 128; r0 += 8 * kBatch) {
-        load(then, r0 + 8 * kBatch);
-        Row after[kBatch];
-        find(after, r0 + 16 * kBatch);
+    auto turn = [&](const Row (&now)[kBatch], int r0) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            const int r = r0 + 8 * i;
+            const int r = r0 + kStep * i;
             const float cc[4] = {now[i].c.x, now[i].c.y, now[i].c.z, now[i].c.w};
             const float ss[4] = {now[i].s.x, now[i].s.y, now[i].s.z, now[i].s.w};
             const float in[8] = {now[i].a[0], now[i].a[1], now[i].a[2], now[i].a[3],
@@ -529,15 +524,18 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
             }
             // four dims are 8 bytes of a 16-byte chunk
             auto at = [&](int d) { return (d >> 6) * (kATile / 2) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2; };
-            *reinterpret_cast<uint2*>(smem + kAHiOff + at(da)) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(smem + kAHiOff + at(db)) = make_uint2(hi[2], hi[3]);
-            *reinterpret_cast<uint2*>(smem + kALoOff + at(da)) = make_uint2(lo[0], lo[1]);
-            *reinterpret_cast<uint2*>(smem + kALoOff + at(db)) = make_uint2(lo[2], lo[3]);
-            if (m == 0) {
+            if (r < 128) {
+                *reinterpret_cast<uint2*>(smem + kAHiOff + at(da)) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(smem + kAHiOff + at(db)) = make_uint2(hi[2], hi[3]);
+                *reinterpret_cast<uint2*>(smem + kALoOff + at(da)) = make_uint2(lo[0], lo[1]);
+                *reinterpret_cast<uint2*>(smem + kALoOff + at(db)) = make_uint2(lo[2], lo[3]);
+            }
+            if (m == 0 && r < 128) {
                 RowInfo info;
                 info.nsq = nsq;
                 info.unscale = exp2i(-e) * 0x1p-10f;
                 info.n = now[i].n;
+                info.pos = now[i].pos;
                 int slot = -1;
                 if (first + r < total && now[i].pos >= 0) {
                     slot = keys ? __ldg(P.slots + now[i].n) : 0;
@@ -546,34 +544,37 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
                 info.slot = max(slot, -1);
                 reinterpret_cast<RowInfo*>(smem + kInfoOff)[buf * 128 + r] = info;
             }
-            now[i] = then[i];
-            then[i].n = after[i].n;
-            then[i].pos = after[i].pos;
         }
+    };
+    // (two buffers by name: handing one's registers to the other would wait for
+    // its loads)
+    constexpr int kNext = kStep * kBatch;
+    find(x0, r_first);
+    find(x1, r_first + kNext);
+    load(x0, r_first);
+#pragma unroll 1
+    for (int r0 = r_first; r0 - (lane >> 4) < 128; r0 += 2 * kNext) {  // (the warp's halves stay together)
+        load(x1, r0 + kNext);
+        turn(x0, r0);
+        find(x0, r0 + 2 * kNext);
+        load(x0, r0 + 2 * kNext);
+        turn(x1, r0 + kNext);
+        find(x1, r0 + 3 * kNext);
     }
 }
 
-// Asks L2 for a tile's rows (t: 0 .. 127).
+// Asks L2 for a tile's rows (thread t of `threads`).
 template <typename T>
 __device__ __forceinline__ void prefetch_rows(const T* base, int64_t sn, int64_t sh, const FastDiv& div, uint32_t H, uint32_t first,
-                                              uint32_t total, int t) {
+                                              uint32_t total, int t, int threads) {
     constexpr int kLines = sizeof(T);  // 128-byte lines of a row
-#pragma unroll
-    for (int i = 0; i < kLines; i++) {
-        const uint32_t line = (uint32_t)(t + 128 * i), row = first + line / kLines;
+    for (uint32_t line = (uint32_t)t; line < 128u * kLines; line += (uint32_t)threads) {
+        const uint32_t row = first + line / kLines;
         if (row < total) {
             const uint32_t n = div.div(row), h = row - n * H;
             asm volatile("prefetch.global.L2 [%0];\n" ::"l"(base + (int64_t)n * sn + (int64_t)h * sh + (line % kLines) * (128 / kLines)));
         }
     }
-}
-
-// Code of y by search (a codebook too fine for the cells).
-template <int NC>
-__device__ __noinline__ int search(const float* mids, float y) {
-    int code = 0;
-    for (int k = 0; k < NC - 1; k++) code += y >= mids[k] ? 1 : 0;
-    return code;
 }
 
 // A key row: codes of its 128 coordinates, norm, slot.
@@ -603,30 +604,37 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
         // fp32 says
         uint32_t near = 0u, upper = 0u;
         uint64_t codes = 0u;  // 16 of them
+        if (fine) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float y = __uint_as_float(z[j]) * f;
-            int code;
-            bool close, up;
-            if (fine) {
+            for (int j = 0; j < 16; j++) {
+                const float y = __uint_as_float(z[j]) * f;
                 // the nearest border of y's cell, its index in the low bits
                 // (t counts 128ths of cells, so that its integer is the byte offset)
                 const float t = fminf(fmaxf(fmaf(y, 128.0f * kCells / (2.0f * kCellSpan), 0x1p23f + 64.0f * kCells + 64.0f), 0x1p23f),
                                       0x1p23f + (128.0f * kCells - 1.0f));
                 const uint32_t e = *reinterpret_cast<const uint32_t*>(cells + (__float_as_uint(t) & (128u * (kCells - 1))));
                 const float d = y - __uint_as_float(e);
-                up = d >= 0.0f;
-                code = (int)(e & 15u) + (up ? 1 : 0);
-                close = fabsf(d) < kNearMma;
-            } else {
-                code = search<nc>(smid, y);
-                up = code > 0 && y - smid[max(code - 1, 0)] < kNearMma;
-                close = up || (code < nc - 1 && smid[code] - y < kNearMma);
+                const bool up = d >= 0.0f;
+                const int code = (int)(e & 15u) + (up ? 1 : 0);
+                csq += csq16[code];
+                near |= fabsf(d) < kNearMma ? 1u << j : 0u;
+                upper |= up ? 1u << j : 0u;
+                codes |= (uint64_t)(uint32_t)code << (kBits * j);
             }
-            csq += csq16[code];
-            near |= close ? 1u << j : 0u;
-            upper |= up ? 1u << j : 0u;
-            codes |= (uint64_t)(uint32_t)code << (kBits * j);
+        } else {  // by search
+#pragma unroll 1
+            for (int j = 0; j < 16; j++) {
+                float y = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) y = i == j ? __uint_as_float(z[i]) * f : y;
+                int code = 0;
+                for (int k = 0; k < nc - 1; k++) code += y >= smid[k] ? 1 : 0;
+                const bool up = code > 0 && y - smid[max(code - 1, 0)] < kNearMma;
+                csq += csq16[code];
+                near |= up || (code < nc - 1 && smid[code] - y < kNearMma) ? 1u << j : 0u;
+                upper |= up ? 1u << j : 0u;
+                codes |= (uint64_t)(uint32_t)code << (kBits * j);
+            }
         }
         // in 64 bits by the whole warp (a row that is not stored needs none)
         if (!stored) near = 0u;
@@ -639,7 +647,7 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
             const int c0 = (int)(codes >> (kBits * j)) & (nc - 1);
             // the border next to it, below or above the code
             const int border = __shfl_sync(kFull, c0 - (int)((upper >> j) & 1u), src);
-            const int c = border + (exact_side<T>(P, krow, table_row<T>(P, position_of(P, sn)), 16 * q + j, smid[border], lane) ? 1 : 0);
+            const int c = border + (exact_side<T>(P, krow, table_row<T>(P, __shfl_sync(kFull, info.pos, src)), 16 * q + j, smid[border], lane) ? 1 : 0);
             if (lane == src) {
                 near &= near - 1;
                 csq += csq16[c] - csq16[c0];
@@ -670,7 +678,7 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
         ask &= ask - 1;
         const int sn = __shfl_sync(kFull, info.n, src), sh = __shfl_sync(kFull, (int)h, src);
         const T* krow = static_cast<const T*>(P.key) + (int64_t)sn * P.ksn + (int64_t)sh * P.ksh;
-        double v = exact_norm<T>(P, krow, table_row<T>(P, position_of(P, sn)), lane);
+        double v = exact_norm<T>(P, krow, table_row<T>(P, __shfl_sync(kFull, info.pos, src)), lane);
         if (fold) {
             // the codes just written: four per lane, from the row's bytes
             __syncwarp();
@@ -729,43 +737,48 @@ __device__ __forceinline__ void finish_queries(const AppendParams& P, uint8_t* t
 template <typename T, int L>
 __device__ __forceinline__ void store_values(const AppendParams& P, const UmmaTiles& W, uint32_t tile, int vw, int lane) {
     const int m = lane & 15;
-    constexpr int kBatch = 2;
+    constexpr int kBatch = 2, kStep = 2 * kValueWarps;
     struct Row {
         Quad<T> a, b;
         int slot, pos;
         uint32_t h;
     };
-    Row now[kBatch], then[kBatch];
+    Row x0[kBatch], x1[kBatch];
     auto load = [&](Row (&x)[kBatch], int r0) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            const uint32_t row0 = tile * 128u + r0 + 8 * i, row = min(row0, W.key_rows - 1);
+            const int r = r0 + kStep * i;
+            const uint32_t row0 = tile * 128u + r, row = min(row0, W.key_rows - 1);
             const uint32_t n = P.div_hk.div(row);
             x[i].h = row - n * (uint32_t)P.Hk;
             const T* v = static_cast<const T*>(P.value) + (int64_t)n * P.vsn + (int64_t)x[i].h * P.vsh + 8 * m;
             x[i].a.load(v);
             x[i].b.load(v + 4);
-            x[i].slot = row0 < W.key_rows ? __ldg(P.slots + n) : -1;
+            x[i].slot = r < 128 && row0 < W.key_rows ? __ldg(P.slots + n) : -1;
             x[i].pos = position_of(P, (int)n);
         }
     };
-    const int r_first = 2 * vw + (lane >> 4);
-    load(now, r_first);
-#pragma unroll 1
-    for (int r0 = r_first; r0 < 128; r0 += 8 * kBatch) {
-        load(then, r0 + 8 * kBatch);
+    auto store = [&](const Row (&x)[kBatch]) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            const float v[8] = {now[i].a[0], now[i].a[1], now[i].a[2], now[i].a[3],
-                                now[i].b[0], now[i].b[1], now[i].b[2], now[i].b[3]};
+            const float v[8] = {x[i].a[0], x[i].a[1], x[i].a[2], x[i].a[3], x[i].b[0], x[i].b[1], x[i].b[2], x[i].b[3]};
             const ValueRow q = quantise_values<layout_3bit_values(L)>(v);
-            const int slot = now[i].slot;
-            if (slot >= 0 && now[i].pos >= 0 && (P.num_blocks <= 0 || (int64_t)slot < P.num_blocks * kBlockSize))
+            const int slot = x[i].slot;
+            if (slot >= 0 && x[i].pos >= 0 && (P.num_blocks <= 0 || (int64_t)slot < P.num_blocks * kBlockSize))
                 write_values<L>(SlotAt<L>(P.cache + (size_t)((uint32_t)slot / kBlockSize) * (size_t)P.block_bytes,
-                                          (uint32_t)slot % kBlockSize, now[i].h, P.Hk, P.pos_stride, P.head_stride),
+                                          (uint32_t)slot % kBlockSize, x[i].h, P.Hk, P.pos_stride, P.head_stride),
                                 m, q);
-            now[i] = then[i];
         }
+    };
+    constexpr int kNext = kStep * kBatch;
+    const int r_first = 2 * vw + (lane >> 4);
+    load(x0, r_first);
+#pragma unroll 1
+    for (int r0 = r_first; r0 - (lane >> 4) < 128; r0 += 2 * kNext) {
+        load(x1, r0 + kNext);
+        store(x0);
+        load(x0, r0 + 2 * kNext);
+        store(x1);
     }
 }
 
@@ -787,7 +800,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == 8) tmem_alloc<256>(bars + kUTmem);
+    if (warp == kFinishWarps) tmem_alloc<256>(bars + kUTmem);
     float* smid = reinterpret_cast<float*>(smem + kTabOff);
     if (tid < kNumCentroids) {
         smid[tid] = tid < nc - 1 ? __ldg(P.mids + tid) : INFINITY;
@@ -838,10 +851,11 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + kUmmaBarOff + kUTmem);
 
-    if (warp < 8) {
-        const int g = warp >> 2, wq = warp & 3;
-        uint32_t i = (uint32_t)g;
-        for (uint32_t tile = blockIdx.x + g * gridDim.x; tile < W.tiles; tile += 2 * gridDim.x, i += 2) {
+    if (warp < kFinishWarps) {
+        const int wq = warp;
+        uint32_t i = 0;
+        for (uint32_t tile = blockIdx.x; tile < W.tiles; tile += gridDim.x, i++) {
+            const int g = (int)(i & 1);
             if (!bar_wait_warp(bars + kDFull + 8 * g, (i >> 1) & 1, abort)) break;
             tc_fence_after();
             const bool keys = tile < W.key_tiles;
@@ -858,7 +872,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
             tc_fence_before();
             bar_arrive(bars + kDEmpty + 8 * g);
         }
-    } else if (warp < 12) {
+    } else if (warp < kFinishWarps + kTurnWarps) {
         constexpr uint32_t kId = umma_idesc(128, kHeadDim, true);
         const uint64_t a_hi = umma_desc(base + kAHiOff, 16, 1024), a_lo = umma_desc(base + kALoOff, 16, 1024);
         const uint64_t b_hi = umma_desc(base + kBHiOff, kATile / 2, 1024), b_lo = umma_desc(base + kBLoOff, kATile / 2, 1024);
@@ -872,21 +886,22 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
             const uint32_t next = tile + gridDim.x;
             if (next < W.key_tiles)
                 prefetch_rows<T>(static_cast<const T*>(P.key), P.ksn, P.ksh, P.div_hk, (uint32_t)P.Hk, next * 128u, W.key_rows,
-                                 tid & 127);
+                                 tid - 32 * kFinishWarps, 32 * kTurnWarps);
             else if (next < W.tiles)
                 prefetch_rows<T>(static_cast<const T*>(P.query), P.qsn, P.qsh, P.div_hq, (uint32_t)P.Hq,
-                                 (next - W.key_tiles) * 128u, W.rows - W.key_rows, tid & 127);
-            if (ok) turn_rows<T>(P, smem, W, tile, buf, warp - 8, lane);
+                                 (next - W.key_tiles) * 128u, W.rows - W.key_rows,
+                                 tid - 32 * kFinishWarps, 32 * kTurnWarps);
+            if (ok) turn_rows<T>(P, smem, W, tile, buf, warp - kFinishWarps, lane);
             fence_async_smem();
-            asm volatile("bar.sync 1, 128;\n" ::: "memory");  // every warp takes every turn, also after an error
-            if (ok && warp == 8) {
+            asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kTurnWarps) : "memory");  // every warp takes every turn, also after an error
+            if (ok && warp == kFinishWarps) {
                 tc_fence_after();
 #pragma unroll
                 for (int p = 0; p < 3; p++)
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         const uint64_t at = ((k >> 2) * (kATile / 2) + (k & 3) * 32) >> 4;
-                        umma_ss(tmem + 128u * buf, (p == 1 ? a_lo : a_hi) + at, (p == 2 ? b_lo : b_hi) + (k * 2048 >> 4), kId,
+                        umma_ss(tmem + 128u * buf, (p == 0 ? a_lo : a_hi) + at, (p == 1 ? b_lo : b_hi) + (k * 2048 >> 4), kId,
                                 p + k != 0);
                     }
                 umma_commit(bars + kDFull + 8 * buf);
@@ -894,19 +909,19 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
             }
         }
         // every product has ended before the CTA frees its TMEM
-        if (warp == 8 && i > 0) bar_wait_warp(bars + kAEmpty, (i - 1) & 1, nullptr);
+        if (warp == kFinishWarps && i > 0) bar_wait_warp(bars + kAEmpty, (i - 1) & 1, nullptr);
     } else {
         for (uint32_t tile = blockIdx.x; tile < W.key_tiles; tile += gridDim.x) {
             prefetch_rows<T>(static_cast<const T*>(P.value), P.vsn, P.vsh, P.div_hk, (uint32_t)P.Hk, (tile + gridDim.x) * 128u,
-                             W.key_rows, tid & 127);
-            store_values<T, L>(P, W, tile, warp - 12, lane);
+                             W.key_rows, tid - 32 * (kFinishWarps + kTurnWarps), 32 * kValueWarps);
+            store_values<T, L>(P, W, tile, warp - kFinishWarps - kTurnWarps, lane);
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8) tmem_free<256>(tmem);
+    if (warp == kFinishWarps) tmem_free<256>(tmem);
     if (tid == 0 && *abort != 0) atomicAdd(&g_append_timeouts, 1u);
 }
 
