@@ -14,10 +14,12 @@
 // are those of exact arithmetic.  A coordinate whose fp32 value lies within
 // kNear of a border, and a norm whose fp32 value lies within kNormNear of a
 // border between two fp16 numbers, are computed again in 64 bits by the whole
-// warp (about one row in fifteen), so the bytes written do not depend on the
-// order of any sum.  kNear covers the fp32 sums: 128 products of a unit row
-// and a unit column, each partial sum off by at most 2^-24 of its magnitude
-// (<= 1 by Cauchy-Schwarz), 128 * 2^-24 = 2^-17 in all.
+// warp (about one row in sixty, and one in two hundred), so the bytes written do
+// not depend on the order of any sum.  kNear covers the fp32 sums, in units of
+// |x|: partial sums of a unit row times a unit column stay below 1
+// (Cauchy-Schwarz), and both forms below sum the full-size products in eight
+// accumulations of at most 2^-23 each, the rest at 2^-8 of that or less, with
+// operands good to 2^-20.4: 2^-19 in all.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -35,7 +37,7 @@ __device__ unsigned int g_append_timeouts = 0;
 
 namespace {
 
-constexpr float kNear = 0x1p-17f;
+constexpr float kNear = 0x1p-19f;
 constexpr float kNormNear = 0x1p-19f;
 
 template <typename T>
@@ -256,54 +258,88 @@ __device__ __forceinline__ void finish_row(const AppendParams& P, const float* s
 }
 
 // ---------------------------------------------------------------------------
-// Any alignment and strides: a CTA takes 32 rows (of keys, then of queries),
-// forms x in shared memory, multiplies by R (64 KB, staged) with fp32 FMAs,
-// and finishes key rows half a warp each.
+// Few rows, or inputs of any alignment, and the FP8-key layouts: a CTA of four
+// warps takes 16 rows (of keys, then of queries), turns them into shared
+// memory, multiplies by R on the register-operand tensor cores and finishes
+// key rows half a warp each.  Every operand is split into three bf16 parts (24
+// bits, fp32's range) and the six products down to 2^-16 are summed in fp32;
+// R's fragments come from L2, a k step's 16 loads at once, so that nothing has
+// to be staged before the first product: the latency of a decode step's call
+// counts here.
 // ---------------------------------------------------------------------------
-constexpr int kRows = 32;
-constexpr int kAppThreads = 256;
-constexpr int kAppSmem = (kHeadDim * kHeadDim + kRows * kHeadDim) * 4;
+constexpr int kRows = 16;
+constexpr int kAppThreads = 128;
+constexpr int kPitch = kHeadDim + 4;  // floats of a row in shared memory: rows four banks apart
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The next bf16 part of a pair of numbers, which keep the rest.
+__device__ __forceinline__ uint32_t take_bf16(float& x, float& y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    x -= __low2float(h);
+    y -= __high2float(h);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 
 template <typename T, int L>
 __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_constant__ AppendParams P, int key_ctas) {
     constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L);
     constexpr int nc = k3 ? 8 : kNumCentroids;
-    extern __shared__ __align__(16) float asm_[];
+    __shared__ __align__(16) float xs[kRows * kPitch];
     __shared__ float smid[kNumCentroids], scent[kNumCentroids];
-    float* xs = asm_;                        // [kRows][128]
-    float* Rs = asm_ + kRows * kHeadDim;     // [128][128] (not for FP8 keys)
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const bool keys = (int)blockIdx.x < key_ctas;
-    const int H = keys ? P.Hk : P.Hq;
-    const uint32_t total = (uint32_t)P.N * (uint32_t)H;
+    const uint32_t H = (uint32_t)(keys ? P.Hk : P.Hq);
+    const FastDiv& div = keys ? P.div_hk : P.div_hq;
+    const uint32_t total = (uint32_t)P.N * H;
     const uint32_t r0 = ((uint32_t)blockIdx.x - (keys ? 0u : (uint32_t)key_ctas)) * kRows;
+    const T* base = static_cast<const T*>(keys ? P.key : P.query);
+    const int64_t sn = keys ? P.ksn : P.qsn, sh = keys ? P.ksh : P.qsh;
+    // thread = dim; the rows' positions and elements, then their angles
+    const RopeDim rd = rope_dim(P, t);
+    const bool turned = t < P.rotary;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kRows && r0 + i0 < total; i0 += 8) {
+        float x[8], y[8], c[8], s[8];
+        int pos[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t row = min(r0 + i0 + i, total - 1), n = div.div(row), h = row - n * H;
+            pos[i] = position_of(P, (int)n);
+            const T* p = base + (int64_t)n * sn + (int64_t)h * sh;
+            x[i] = to_f32<T>(p[t]);
+            y[i] = turned ? to_f32<T>(p[rd.partner]) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float* cs = table_row<T>(P, pos[i]) + rd.j;
+            c[i] = turned ? __ldg(cs) : 1.0f;
+            s[i] = turned ? __ldg(cs + (P.rotary >> 1)) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            // (rounded once; a query whose position is outside the table has
+            // no value)
+            float v = turned ? pair_rn(x[i], c[i], y[i], rd.sign * s[i]) : x[i];
+            if (pos[i] < 0 && !keys) v = __int_as_float(0x7fc00000);
+            xs[(i0 + i) * kPitch + t] = v;
+        }
+    }
     if constexpr (!k8) {
         if (t < nc - 1) smid[t] = __ldg(P.mids + t);
         if (t < nc) scent[t] = __ldg(P.cents + t);
-        const float4* R4 = reinterpret_cast<const float4*>(P.rot);
-        for (int e = t; e < kHeadDim * kHeadDim / 4; e += kAppThreads) reinterpret_cast<float4*>(Rs)[e] = __ldg(R4 + e);
-    }
-    const T* base = static_cast<const T*>(keys ? P.key : P.query);
-    const int64_t sn = keys ? P.ksn : P.qsn, sh = keys ? P.ksh : P.qsh;
-    const int d = t % kHeadDim;
-    for (int i = t / kHeadDim; i < kRows; i += kAppThreads / kHeadDim) {
-        float x = 0.0f;
-        if (r0 + i < total) {
-            const uint32_t n = (r0 + i) / (uint32_t)H, h = (r0 + i) - n * (uint32_t)H;
-            const int pos = position_of(P, (int)n);
-            // a query whose position is outside the table has no value
-            x = pos < 0 && !keys ? __int_as_float(0x7fc00000)
-                                 : rope_f32<T>(P, base + (int64_t)n * sn + (int64_t)h * sh, table_row<T>(P, pos), d);
-        }
-        xs[i * kHeadDim + d] = x;
     }
     __syncthreads();
-    float nsq[2];  // sums of squares of this half-warp's two rows
-    const int m = lane & 15, half = (lane >> 4) + 2 * warp;
-    if (keys) {
+    const int m = lane & 15, half = (lane >> 4) + 2 * warp;  // rows half and half + 8 of this half-warp
+    float nsq[2] = {0.0f, 0.0f};
+    if (keys && !k8) {
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            const float* x = xs + (half + 16 * k) * kHeadDim + 8 * m;
+            const float* x = xs + (half + 8 * k) * kPitch + 8 * m;
             float q = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) q = fmaf(x[j], x[j], q);
@@ -311,44 +347,62 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
         }
     }
     if constexpr (!k8) {
-        constexpr int kPer = kRows / (kAppThreads / kHeadDim);  // rows per thread
-        const int i0 = (t / kHeadDim) * kPer;
-        float acc[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; i++) acc[i] = 0.0f;
+        const int g = lane >> 2, c = lane & 3, n0 = 32 * warp;
+        const float* R = P.rot + 2 * c * kHeadDim + n0 + g;
+        float acc[4][4] = {}, small[4][4] = {};  // the product of the first parts, and the others (2^-8 of it)
 #pragma unroll 2
-        for (int k = 0; k < kHeadDim; k += 4) {
-            const float a = Rs[k * kHeadDim + d], b = Rs[(k + 1) * kHeadDim + d], c = Rs[(k + 2) * kHeadDim + d],
-                        e = Rs[(k + 3) * kHeadDim + d];
+        for (int k = 0; k < kHeadDim; k += 16) {
+            float bv[4][4], av[8];
 #pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const float4 x = *reinterpret_cast<const float4*>(xs + (i0 + i) * kHeadDim + k);
-                acc[i] = fmaf(x.w, e, fmaf(x.z, c, fmaf(x.y, b, fmaf(x.x, a, acc[i]))));
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) bv[n][i] = __ldg(R + (k + (i & 1) + 8 * (i >> 1)) * kHeadDim + 8 * n);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {  // rows g, g + 8; dims 2c, 2c + 1 (+ 8)
+                const float2 v = *reinterpret_cast<const float2*>(xs + (g + 8 * (i & 1)) * kPitch + k + 2 * c + 8 * (i >> 1));
+                av[2 * i] = v.x;
+                av[2 * i + 1] = v.y;
             }
+            uint32_t a[3][4];
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) a[p][i] = take_bf16(av[2 * i], av[2 * i + 1]);
+#pragma unroll
+            for (int q = 0; q < 3; q++)
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const uint32_t b0 = take_bf16(bv[n][0], bv[n][1]), b1 = take_bf16(bv[n][2], bv[n][3]);
+#pragma unroll
+                    for (int p = 0; p + q < 3; p++) mma_bf16(p + q == 0 ? acc[n] : small[n], a[p], b0, b1);
+                }
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kPer; i++) xs[(i0 + i) * kHeadDim + d] = acc[i];
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                *reinterpret_cast<float2*>(xs + (g + 8 * i) * kPitch + n0 + 8 * n + 2 * c) =
+                    make_float2(acc[n][2 * i] + small[n][2 * i], acc[n][2 * i + 1] + small[n][2 * i + 1]);
         __syncthreads();
     }
     if (!keys) {
-        for (int i = t / kHeadDim; i < kRows; i += kAppThreads / kHeadDim) {
-            if (r0 + i >= total) break;
-            const uint32_t n = (r0 + i) / (uint32_t)H, h = (r0 + i) - n * (uint32_t)H;
-            P.q_rot[(int64_t)n * P.osn + (int64_t)h * P.osh + d] = xs[i * kHeadDim + d];
+        for (int i = 0; i < kRows && r0 + i < total; i++) {
+            const uint32_t n = div.div(r0 + i), h = (r0 + i) - n * H;
+            P.q_rot[(int64_t)n * P.osn + (int64_t)h * P.osh + t] = xs[i * kPitch + t];
         }
         return;
     }
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < 2; k++) {
-        const uint32_t row = r0 + half + 16 * k;
+        const uint32_t row = r0 + half + 8 * k;
         const bool live = row < total;
         const uint32_t rc = live ? row : total - 1;
-        const uint32_t n = rc / (uint32_t)H, h = rc - n * (uint32_t)H;
+        const uint32_t n = div.div(rc), h = rc - n * H;
         float z[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) z[j] = xs[(half + 16 * k) * kHeadDim + 8 * m + j];
-        finish_row<T, L>(P, smid, scent, (int)n, (int)h, live, lane, z, nsq[k]);
+        for (int j = 0; j < 8; j++) z[j] = xs[(half + 8 * k) * kPitch + 8 * m + j];
+        finish_row<T, L>(P, smid, scent, (int)n, (int)h, live, lane, z, k == 0 ? nsq[0] : nsq[1]);
     }
 }
 
@@ -365,11 +419,13 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
 // shared memory): 24 MMAs of 128 x 128 x 16 a tile, the two small products
 // first.  Errors against exact arithmetic, of |x|: 2^-23 from the fp32 turn, 3 *
 // 2^-22 from the splits, 16 accumulations of 2^-23 at the size of the small
-// products (2^-10) and 8 of 2^-23 at full size: 2^-19 in all (kNearMma).
+// products (2^-10) and 8 of 2^-23 at full size: below 2^-19 (kNear).
 // Bound by instruction issue: about 15 instructions per coordinate to
 // bucketise, 9 to turn and split, 10 per value.
 // ---------------------------------------------------------------------------
-constexpr float kNearMma = 0x1p-19f;
+// Up to here the form above is faster: 5120 rows of a 4-bit decode step take it
+// 16.2 us and this one 19.2 us, 20480 rows 34 and 25.
+constexpr int64_t kFewRows = 8192;
 constexpr int kATile = 128 * kHeadDim * 2;                                       // 32 KB
 constexpr int kAHiOff = 0, kALoOff = kATile, kBHiOff = 2 * kATile, kBLoOff = 3 * kATile;
 constexpr int kCells = 128;                                                      // of [-kCellSpan, kCellSpan)
@@ -617,7 +673,7 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
                 const bool up = d >= 0.0f;
                 const int code = (int)(e & 15u) + (up ? 1 : 0);
                 csq += csq16[code];
-                near |= fabsf(d) < kNearMma ? 1u << j : 0u;
+                near |= fabsf(d) < kNear ? 1u << j : 0u;
                 upper |= up ? 1u << j : 0u;
                 codes |= (uint64_t)(uint32_t)code << (kBits * j);
             }
@@ -629,9 +685,9 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
                 for (int i = 0; i < 16; i++) y = i == j ? __uint_as_float(z[i]) * f : y;
                 int code = 0;
                 for (int k = 0; k < nc - 1; k++) code += y >= smid[k] ? 1 : 0;
-                const bool up = code > 0 && y - smid[max(code - 1, 0)] < kNearMma;
+                const bool up = code > 0 && y - smid[max(code - 1, 0)] < kNear;
                 csq += csq16[code];
-                near |= up || (code < nc - 1 && smid[code] - y < kNearMma) ? 1u << j : 0u;
+                near |= up || (code < nc - 1 && smid[code] - y < kNear) ? 1u << j : 0u;
                 upper |= up ? 1u << j : 0u;
                 codes |= (uint64_t)(uint32_t)code << (kBits * j);
             }
@@ -829,7 +885,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
     fence_async_smem();
     __syncthreads();
     // Cells of the coordinate's range: the border nearest to the cell, its
-    // index in the four low bits (2^-22 of it, far below kNearMma).  A cell
+    // index in the four low bits (2^-22 of it, far below kNear).  A cell
     // that two borders come near to leaves every row to the search.
     bool fine = true;
     if (tid < kCells) {
@@ -963,21 +1019,11 @@ int launch_append_umma(const AppendParams& P, cudaStream_t stream, int num_sms) 
 
 template <typename T, int L>
 int launch_append_t(const AppendParams& P, cudaStream_t stream, int num_sms) {
+    const int64_t kr = (int64_t)P.N * P.Hk, qr = P.query ? (int64_t)P.N * P.Hq : 0;
     if constexpr (!layout_fp8_keys(L))
-        if (umma_aligned<T, L>(P)) return launch_append_umma<T, L>(P, stream, num_sms);
-    auto kern = append_kernel<T, L>;
-    const int smem = layout_fp8_keys(L) ? kRows * kHeadDim * 4 : kAppSmem;
-    static thread_local int configured_dev = -1;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (configured_dev != dev) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-            return report_launch(cudaGetLastError());
-        configured_dev = dev;
-    }
-    const int64_t kc = ((int64_t)P.N * P.Hk + kRows - 1) / kRows;
-    const int64_t qc = P.query ? ((int64_t)P.N * P.Hq + kRows - 1) / kRows : 0;
-    kern<<<(unsigned)(kc + qc), kAppThreads, smem, stream>>>(P, (int)kc);
+        if (kr + qr > kFewRows && umma_aligned<T, L>(P)) return launch_append_umma<T, L>(P, stream, num_sms);
+    const int64_t kc = (kr + kRows - 1) / kRows, qc = (qr + kRows - 1) / kRows;
+    append_kernel<T, L><<<(unsigned)(kc + qc), kAppThreads, 0, stream>>>(P, (int)kc);
     return report_launch(cudaGetLastError());
 }
 
