@@ -9,7 +9,10 @@ The shared pass over a prefix (16-bit outputs) rounds its operands to fp16, 2^-1
 mean A = sum p |v| of what is summed and not by |ref|, which may cancel.  V and P: 2 * 2^-11 A.  Scores: q_i k_i carries
 three roundings (q, c, c norm) of rms at most 2^-11 / sqrt(3), 2^-11 together; over 128 products that is sigma = 2^-11
 scale sqrt(sum q_i^2 k_i^2) = 2^-11 * 1.5 = 7.3e-4 for the rows here (|q| = 1.5 sqrt(128), |k| = sqrt(128)), and a score's
-error moves the output by at most that times A; 4 sigma A = 3e-3 A.  Together 4e-3 A in place of 2e-3 |ref|."""
+error moves the output by at most that times A; 4 sigma A = 3e-3 A.  Together 4e-3 A in place of 2e-3 |ref|; for rows of
+another size, |q| = u sqrt(128), (2^-10 + 4 * 2^-11 u) A.  That takes the roundings for independent, which the codebook's
+are not: a token has 16 different ones (8 of a symmetric codebook), so sum q_i k_i d(c_i) has the mean s * d, |d| <= 2^-11,
+besides its spread.  Scores far above a row's 4 sigma need that term, 2^-11 |s| A with |s| at most the row's LSE."""
 
 from __future__ import annotations
 
@@ -68,9 +71,11 @@ def projections(rng, n, hq, hk, dtype, pad=0):
 
 
 def run_append(layout, dtype, n, hq, hk, rotary, interleaved, *, seed=0, pad=0, pos64=True, pad_slots=0, norm_correction=True,
-               scale=1.0):
+               scale=1.0, codes=None, poison=False):
     rng = np.random.default_rng(seed)
     c, m, R = book(layout)
+    if codes is not None:
+        c, m = codes, tqb.get_midpoints(codes)
     nb = -(-n // 16) + 2
     cache0 = rng.integers(0, 256, (nb, 16, hk, SO.LAYOUTS[layout][2]), dtype=np.uint8)
     slots = rng.permutation(nb * 16)[:n].astype(np.int32)
@@ -78,6 +83,9 @@ def run_append(layout, dtype, n, hq, hk, rotary, interleaved, *, seed=0, pad=0, 
     q, k, v = projections(rng, n, hq, hk, dtype, pad)
     if scale != 1.0:
         k, v = k * scale, v * scale
+    if poison:  # what has no place may hold anything
+        for x, bad in ((q, np.nan), (k, np.nan), (v, np.inf)):
+            x[torch.from_numpy(np.flatnonzero(slots < 0)).cuda()] = bad
     table = cos_sin_table(500, rotary) if rotary else None
     pos = rng.integers(0, 500, n) if rotary else None
     cache = torch.from_numpy(cache0).cuda()
@@ -96,7 +104,8 @@ def run_append(layout, dtype, n, hq, hk, rotary, interleaved, *, seed=0, pad=0, 
             x = SO.rope(x, table[pos], interleaved)
         ref = x if R is None else x @ npy(R).astype(np.float64)
         tol = (2.0 ** -17 if R is not None else 2.0 ** -24) * np.linalg.norm(x, axis=-1, keepdims=True)
-        assert (np.abs(npy(got_q) - ref) <= tol).all()
+        live = np.flatnonzero(slots >= 0) if poison else slice(None)
+        assert (np.abs(npy(got_q) - ref) <= tol)[live].all()
 
 
 @pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
@@ -143,6 +152,65 @@ def test_append_skips_what_has_no_place():
                           cuda(m), cuda(c), query=q)
     assert torch.equal(cache, before)
     assert torch.isfinite(out[:2]).all() and torch.isnan(out[2:]).all()
+
+
+# More than 8192 rows, queries and keys together, whose rows are 16-byte aligned, take the tensor-core form.
+LLOYD_MAX = [x for x in sorted(SO.LAYOUTS) if not x.endswith("k8")]
+
+
+@pytest.mark.parametrize("layout", LLOYD_MAX)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_append_many_rows(layout, dtype):
+    run_append(layout, DT[dtype], 613, 12, 3, 128, False, seed=6, pad_slots=40, poison=True)
+
+
+@pytest.mark.parametrize("n,hq,hk,rotary,interleaved,pad,pos64", [
+    (8193, 0, 1, 128, True, 0, True), (2100, 0, 4, 64, True, 8, False), (1201, 5, 3, 96, False, 0, True),
+    (1100, 16, 2, 2, True, 0, False), (700, 12, 4, 34, False, 0, True), (1030, 8, 1, 0, False, 0, True),
+    (1100, 6, 2, 64, False, 3, True), (9000, 1, 1, 126, True, 0, True)])
+def test_append_many_rows_shapes(n, hq, hk, rotary, interleaved, pad, pos64):
+    """Few and many heads, partial and unaligned rotary dims, the last tile's ends, and rows that are not aligned."""
+    run_append("soa_k3", torch.bfloat16, n, hq, hk, rotary, interleaved, seed=n, pad=pad, pos64=pos64)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-6, 3000.0])
+def test_append_many_rows_of_extreme_norms(scale):
+    run_append("soa", torch.float32, 2100, 0, 4, 64, False, seed=3, scale=scale)
+
+
+@pytest.mark.parametrize("n", [40, 2100])
+def test_append_codebooks_of_any_spacing(n):
+    """Borders next to one another, equal ones and one far out, beside ordinary ones; no norm correction."""
+    codes = torch.tensor([-9.0, -0.2, -0.2, -0.1, -1e-3, -1e-4, -1e-5, 0, 1e-7, 1e-6, 2e-6, 0.05, 0.05003, 0.1, 0.3, 0.31])
+    run_append("soa", torch.bfloat16, n, 0, 4, 128, False, seed=n, codes=codes)
+    run_append("soa", torch.float32, n, 0, 4, 128, False, seed=n, codes=codes, norm_correction=False)
+
+
+@pytest.mark.parametrize("n", [17, 2100])
+def test_append_poisoned_rows(n):
+    for layout in ("aos", "soa_k8"):
+        run_append(layout, torch.bfloat16, n, 4, 4, 128, True, seed=n, pad_slots=n // 3, poison=True)
+
+
+def test_append_many_rows_without_a_place():
+    """Half the tokens without a slot or a position, spread over every tile."""
+    rng = np.random.default_rng(10)
+    c, m, R = book("soa")
+    n = 3000
+    cache0 = rng.integers(0, 256, (n // 16 + 1, 16, 2, 134), dtype=np.uint8)
+    slots = rng.permutation(n).astype(np.int32)
+    slots[::5] = rng.choice([-1, -2 ** 31, len(cache0) * 16, 2 ** 31 - 1], len(slots[::5]))
+    pos = rng.integers(0, 500, n)
+    pos[::3] = rng.choice([-1, 500, 2 ** 40, -2 ** 40], len(pos[::3]))
+    cs = cos_sin_table(500, 128)
+    q, k, v = projections(rng, n, 2, 2, torch.bfloat16)
+    cache = torch.from_numpy(cache0).cuda()
+    out = tqb.rope_append(k, v, cache, torch.from_numpy(slots).cuda(), torch.from_numpy(pos).cuda(),
+                          torch.from_numpy(cs).cuda(), cuda(R), cuda(m), cuda(c), query=q)
+    want = SO.append(cache0, "soa", npy(k), npy(v), slots, pos, cs, npy(R), npy(m), npy(c))
+    assert np.array_equal(cache.cpu().numpy(), want)
+    assert np.array_equal(np.isnan(npy(out)).all((1, 2)), (pos < 0) | (pos >= 500))
+    assert np.array_equal(np.isnan(npy(out)).any((1, 2)), (pos < 0) | (pos >= 500))
 
 
 def test_append_empty():
@@ -218,16 +286,16 @@ def batch(rng, lens, hk, layout, shared=0):
     return random_cache(rng, nb, hk, layout), table, np.asarray(lens, np.int32)
 
 
-def check_decode(got, lse, ref, ref_lse, dtype, size=None):
+def check_decode(got, lse, ref, ref_lse, dtype, size=None, rel=4e-3):
     """``size``: the mean |v| that the shared pass's bar goes by."""
     got, lse = got.double().cpu().numpy(), lse.double().cpu().numpy()
     dead = np.isnan(ref)
     assert np.array_equal(np.isnan(got), dead)
-    bar = 1e-4 + half_step(dtype) * np.abs(ref) + (2e-3 * np.abs(ref) if size is None else 4e-3 * size)
+    bar = 1e-4 + half_step(dtype) * np.abs(ref) + (2e-3 * np.abs(ref) if size is None else rel * size)
     assert (np.abs(got - ref)[~dead] <= bar[~dead]).all()
     assert np.array_equal(np.isneginf(lse), np.isneginf(ref_lse))
     live = np.isfinite(ref_lse)
-    assert (np.abs(lse - ref_lse)[live] <= 1e-4 + 2e-3 * np.abs(ref_lse[live])).all()
+    assert (np.abs(lse[live] - ref_lse[live]) <= 1e-4 + 2e-3 * np.abs(ref_lse[live])).all()
 
 
 def run_window(layout, dtype, lens, hq, hk, window, first, *, seed=0, sinks=False, raw=True, **kw):
@@ -328,12 +396,26 @@ def test_rotation_beside_stage1(dtype, rows):
     assert (np.abs(out.cpu().numpy() - x @ npy(R).astype(np.float64)) <= tol).all()
 
 
-def run_prefix(layout, dtype, own, prefix, hq, hk, *, seed=0, sinks=False, raw=True, short=(), scale_q=1.5, **kw):
+def run_prefix(layout, dtype, own, prefix, hq, hk, *, seed=0, sinks=False, raw=True, short=(), scale_q=1.5, shared=True,
+               chunks=None, bad=(), **kw):
+    """``shared`` None: as the call decides; else whether a prefix of 128 tokens or more takes the shared pass.
+    ``chunks``: its splits.  ``bad``: (entry, page id) pairs of the prefix in every row of the table."""
+    with pytest.MonkeyPatch.context() as mp:
+        if shared is not None:
+            mp.setattr(tqb.serving, "_shares", lambda batch, rows, heads, prefix_len: shared and prefix_len >= 128)
+        if chunks is not None:
+            mp.setattr(tqb.serving, "_prefix_splits", lambda rows, heads, prefix_len: chunks)
+        return run_prefix_as_set(layout, dtype, own, prefix, hq, hk, seed, sinks, raw, short, scale_q, bad, kw)
+
+
+def run_prefix_as_set(layout, dtype, own, prefix, hq, hk, seed, sinks, raw, short, scale_q, bad, kw):
     rng = np.random.default_rng(seed)
     c, _, R = book(layout)
     cache, table, lens = batch(rng, [prefix + n for n in own], hk, layout, prefix // 16)
     for b, n in short:
         lens[b] = n
+    for at, page in bad:
+        table[:, at] = page
     q = torch.from_numpy(rng.standard_normal((len(lens), hq, 128)).astype(np.float32) * scale_q).to(dtype).cuda()
     raw = raw and R is not None
     s = torch.from_numpy(rng.standard_normal(hq).astype(np.float32) * 2).cuda() if sinks else None
@@ -345,7 +427,9 @@ def run_prefix(layout, dtype, own, prefix, hq, hk, *, seed=0, sinks=False, raw=T
     x = x @ npy(R).astype(np.float64) if raw else x
     ref, ref_lse, size = SO.attention(x, cache, layout, table, lens, npy(c), lambda t, L: t >= 0, scale=kw.get("scale"),
                                       sinks=npy(s))
-    check_decode(got, lse, ref, ref_lse, got.dtype, size if got.dtype != torch.float32 and prefix >= 128 else None)
+    check_decode(got, lse, ref, ref_lse, got.dtype, size if got.dtype != torch.float32 and prefix >= 128 else None,
+                 2.0 ** -10 + 2.0 ** -9 * scale_q + (2.0 ** -11 * ref_lse[..., None] if scale_q > 4 else 0))
+    return got
 
 
 @pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
@@ -369,6 +453,125 @@ def test_prefix_lengths_and_batches(prefix, batch_size):
 def test_prefix_rows_shorter_than_the_prefix():
     """Padded rows of a batch (length 0) and rows that end inside the prefix, at a page's and a tile's edges."""
     run_prefix("soa", torch.bfloat16, [9] * 8, 320, 4, 1, seed=2, short=[(0, 0), (2, 1), (3, 128), (4, 129), (5, 320), (6, 255)])
+
+
+@pytest.mark.parametrize("rows,chunks", [(20, 1), (20, 2), (20, 4), (128, 2), (129, 1), (160, 2), (256, 1), (257, 3), (560, 1)])
+def test_prefix_of_many_tiles_to_a_block(rows, chunks):
+    """One stream, two streams of one row block, the same rows over even and odd tiles, several row blocks."""
+    hq = 8 if rows % 8 == 0 else 4 if rows % 4 == 0 else 1
+    run_prefix("soa", torch.bfloat16, [5] * (rows // hq), 1296, hq, 1, seed=rows, chunks=chunks, sinks=True)
+
+
+@pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
+def test_prefix_layouts_of_many_tiles(layout):
+    run_prefix(layout, torch.float16, [1, 9, 30] * 12, 720, 8, 2, seed=7, chunks=1)
+
+
+@pytest.mark.parametrize("own,chunks", [([5] * 8, 2), ([5] * 40, 1)])
+def test_prefix_scores_that_outgrow_their_reference(own, chunks):
+    """Scores of a standard deviation of 12: later tiles' maxima exceed the first ones' by far more than 2^8."""
+    run_prefix("soa", torch.bfloat16, own, 1280, 4, 1, seed=12, scale_q=12.0, chunks=chunks)
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_prefix_pages_that_do_not_exist(shared):
+    """Single ones, a tile of them, and a prefix of nothing else."""
+    bad = [(3, -1), (11, 10 ** 6), (19, -2 ** 31)] + [(i, 2 ** 31 - 1) for i in range(24, 32)]
+    run_prefix("soa", torch.bfloat16, [9] * 6, 640, 4, 1, seed=3, bad=bad, shared=shared)
+    run_prefix("soa", torch.bfloat16, [9] * 6, 256, 4, 1, seed=3, bad=[(i, -1) for i in range(16)], shared=shared)
+
+
+@pytest.mark.parametrize("batch_size,prefix", [(1, 640), (8, 128), (12, 16384), (64, 1024), (300, 512)])
+def test_prefix_as_the_call_decides(batch_size, prefix):
+    run_prefix("soa", torch.bfloat16, [3] * batch_size, prefix, 2, 2, seed=prefix, shared=None)
+
+
+def test_prefix_into_given_workspaces_and_outputs():
+    """Partials of 129 floats, a strided output, and the same numbers as with the call's own."""
+    a = run_prefix("aos_k3", torch.bfloat16, [20] * 5, 400, 6, 2, seed=5, num_splits=3)
+    buf = torch.zeros(5, 6, 130, dtype=torch.bfloat16, device="cuda")
+    mid = torch.full((6, 7, 11, 129), np.nan, device="cuda")
+    b = run_prefix("aos_k3", torch.bfloat16, [20] * 5, 400, 6, 2, seed=5, num_splits=3, output=buf[..., :128], mid_o=mid)
+    assert torch.equal(a, b) and (buf[..., 128:] == 0).all()
+    assert torch.isnan(mid[5:]).all() and torch.isnan(mid[:, 6:]).all()
+
+
+def test_prefix_empty_batch():
+    c, _, R = book("soa")
+    q = torch.empty(0, 4, 128, device="cuda")
+    cache = torch.zeros(9, 16, 2, 134, dtype=torch.uint8, device="cuda")
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    out = tqb.prefix_attention(q, cache, none.reshape(0, 9), none, cuda(R), cuda(c), prefix_len=128)
+    assert out.shape == (0, 4, 128)
+
+
+def serving_calls(seed):
+    """The four calls on inputs of their own, large enough for the tensor-core forms: a function and its results' names."""
+    rng = np.random.default_rng(seed)
+    c, m, R = (cuda(x) for x in book("soa"))
+    cache_np, table, lens = batch(rng, [640 + n for n in rng.integers(1, 60, 64)], 4, "soa", 40)
+    cache, table, lens = (torch.from_numpy(x).cuda() for x in (cache_np, table, lens))
+    n = 1100
+    store = torch.zeros(n // 16 + 1, 16, 4, 134, dtype=torch.uint8, device="cuda")
+    slots = torch.from_numpy(rng.permutation(n).astype(np.int32)).cuda()
+    q, k, v = projections(rng, n, 16, 4, torch.bfloat16)
+    cs, pos = torch.from_numpy(cos_sin_table(500, 128)).cuda(), torch.from_numpy(rng.integers(0, 500, n)).cuda()
+
+    def run(**kw):
+        qr = tqb.rope_append(k, v, store, slots, pos, cs, R, m, c, query=q, **kw)
+        gk, gv = tqb.gather_kv(store, slots, c, **kw)
+        w = tqb.window_attention(q[:64], cache, table, lens, R, c, window=200, first_tokens=4, **kw)
+        return qr, gk, gv, w, tqb.prefix_attention(q[:64], cache, table, lens, R, c, prefix_len=640, **kw), store
+
+    return run
+
+
+@pytest.fixture
+def shared_prefix(monkeypatch):
+    monkeypatch.setattr(tqb.serving, "_shares", lambda *a: True)
+
+
+def test_calls_on_two_streams_at_once(shared_prefix):
+    """Two threads' worth of calls in flight on two streams, by the current stream and by ``stream``: the same bits as
+    alone, every time."""
+    runs = [serving_calls(1), serving_calls(2)]
+    alone = [[x.clone() for x in run()] for run in runs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for i in range(6):
+        for run, st in zip(runs, streams):
+            if i % 2:
+                got.append(run(stream=st.cuda_stream))
+            else:
+                with torch.cuda.stream(st):
+                    got.append(run())
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        for a, b in zip(out, alone[i % 2]):
+            assert torch.equal(a, b)
+
+
+def test_calls_in_two_graphs_replayed_at_once(shared_prefix):
+    runs = [serving_calls(3), serving_calls(4)]
+    alone = [[x.clone() for x in run()] for run in runs]
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for run, g in zip(runs, graphs):
+        with torch.cuda.graph(g):
+            outs.append(run())
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for out in outs:
+            for x in out:
+                x.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, alone):
+            for a, b in zip(out, ref):
+                assert torch.equal(a, b)
 
 
 def test_step_append_then_attend_on_a_side_stream_and_in_a_graph():

@@ -7,14 +7,16 @@ A decode step of a model with rotary positions is two calls::
                                first_tokens=4, out_dtype=q.dtype)
 
 and a later chunk of a prefill reads its context back with ``gather_kv``.  All run on the tensors' device and its
-current stream (or ``stream``), launch asynchronously and can be captured into CUDA graphs; outputs and the split
-partials are allocated by torch unless they are given.  A workspace (``mid_o``) that two calls share serialises
+current stream, launch asynchronously and can be captured into CUDA graphs; outputs and the split partials are allocated
+by torch unless they are given.  ``stream``, a ``cuda_stream`` handle, makes a call one that is made inside
+``torch.cuda.stream`` of it: what it allocates belongs to that stream.  A workspace (``mid_o``) that two calls share serialises
 nothing: calls that may overlap need one each.  Errors raise ``TqbError``.
 """
 
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
 from typing import Optional
@@ -30,7 +32,9 @@ from .ops import _DTYPE_ID, _SOA_FAMILY, _block_dense
 _F32, _U8, _I32, _I64 = torch.float32, torch.uint8, torch.int32, torch.int64
 _FOLDED = (LAYOUT_SOA, LAYOUT_SOA_K3, LAYOUT_SOA_K3V3)  # the stored norm may hold the norm correction
 _PITCH = HEAD_DIM + 4  # floats of a partial row in the calls' own workspace: 129, and rows of whole 16 bytes
-_SPLIT_TOKENS = 64    # shortest split worth its partial rows (516 bytes written and read per query head)
+# Shortest split worth its partial rows (516 bytes written and read per query head).  1024 tokens of one sequence and 8
+# heads take 16.6, 16.0, 19.3 and 23.0 us with 16, 32, 64 and 128; 4096 take 22.3, 18.7, 19.7 and 24.9.
+_SPLIT_TOKENS = 32
 _SPLIT_ITEMS = 2368   # (sequence, KV head, split) items of one round of the Stage1 grid: 148 CTAs x 2 groups x 8 warps
 
 
@@ -126,6 +130,21 @@ def _stream(dev: int) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
+def _on_stream(call):
+    """``call`` with its ``stream`` made the current one, so that its workspaces are that stream's too."""
+    @functools.wraps(call)
+    def on(*args, stream: Optional[int] = None, **kw):
+        if stream is None:
+            return call(*args, **kw)
+        at = next((x.device for x in (*args, *kw.values()) if isinstance(x, torch.Tensor) and x.is_cuda), None)
+        if at is None or stream == _stream(at.index):
+            return call(*args, **kw)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, at) if stream else torch.cuda.default_stream(at)):
+            return call(*args, **kw)
+    return on
+
+
+@_on_stream
 def rope_append(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
                 positions: Optional[torch.Tensor], cos_sin: Optional[torch.Tensor],
                 rotation: Optional[torch.Tensor], midpoints: Optional[torch.Tensor],
@@ -195,10 +214,11 @@ def rope_append(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor, 
         key.data_ptr(), value.data_ptr(), q, kind, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], pos, bool(pos64), table,
         table_stride, max_pos, rotary, bool(interleaved), rot, mids, cents, slots, kv_cache.data_ptr(), lay, cs[0], cs[1],
         cs[2], cshape[0], out, os[0], os[1], N, Hq, Hk, HEAD_DIM, BLOCK_SIZE, n, bool(norm_correction) and lay in _FOLDED),
-        _stream(dev) if stream is None else stream)
+        _stream(dev))
     return q_rot
 
 
+@_on_stream
 def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, centroids: Optional[torch.Tensor], *, layout="soa",
               dtype: torch.dtype = torch.bfloat16, key: Optional[torch.Tensor] = None,
               value: Optional[torch.Tensor] = None, stream: Optional[int] = None):
@@ -228,7 +248,7 @@ def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, centroids: Opt
             _no(f"key and value must be [{N}, {Hk}, 128] tensors of one dtype")
     _call("tqb_gather", _GATHER.pack(
         kv_cache.data_ptr(), lay, cs[0], cs[1], cs[2], cshape[0], slots, cents, key.data_ptr(), value.data_ptr(), kind,
-        ks[0], ks[1], vs[0], vs[1], N, Hk, HEAD_DIM, BLOCK_SIZE, n), _stream(dev) if stream is None else stream)
+        ks[0], ks[1], vs[0], vs[1], N, Hk, HEAD_DIM, BLOCK_SIZE, n), _stream(dev))
     return key, value
 
 
@@ -244,7 +264,8 @@ def _splits(items: int, tokens: int) -> int:
         if s:
             used = -(-items * s // _SPLIT_ITEMS)
             best = min(best, (used * (-(-tokens // s) + 48), s))
-    return best[1]
+    pages = -(-tokens // BLOCK_SIZE)  # splits hold whole pages: no more of them than the longest needs
+    return -(-pages // -(-pages // best[1]))
 
 
 class _Step:
@@ -341,10 +362,10 @@ class _Step:
             self.table_stride, self.blocks, self.seq_lens, self.cents, self.n, 0, 0, self.mid + 4 * ms[2] * at, ms[0],
             ms[1], ms[2], self.B, self.Hq, self.Hk, HEAD_DIM, BLOCK_SIZE, S, self.scale)
 
-    def launch(self, rng: bytes, lead: int, S: int, stream, prefix_len: int = 0) -> torch.Tensor:
+    def launch(self, rng: bytes, lead: int, S: int, prefix_len: int = 0) -> torch.Tensor:
         """Stage1 of the range into the splits from ``lead`` on, the shared prefix into those before, the merge of all
         S."""
-        st = _stream(self.dev) if stream is None else stream
+        st = _stream(self.dev)
         ms, rs = self.ms, self.rs
         _call("tqb_stage1_range", self.stage1(lead, S - lead),
               None if not self.rot else _ROTATE.pack(self.query.data_ptr(), self.kind, self.qs[0], self.qs[1], self.rot,
@@ -370,6 +391,16 @@ def _prefix_splits(rows: int, heads: int, prefix_len: int) -> int:
     return best[1] * (2 if rows <= 128 else 1)
 
 
+def _shares(batch: int, rows: int, heads: int, prefix_len: int) -> bool:
+    """Whether one pass over the prefix for all rows is faster than Stage1 of every sequence.  The pass and its extra
+    merge cost about 8.5 us before the first tile and, per block of 256 rows, the time that Stage1 takes for the prefix
+    of five sequences.  Measured with 8 KV heads and 32 query heads, us, pass : Stage1 at (batch, prefix): (64, 512)
+    35.6 : 31.2, (64, 2048) 37.0 : 59.2, (32, 2048) 31.7 : 36.0, (16, 2048) 30.7 : 27.1, (16, 8192) 39.3 : 54.6, (8, 8192)
+    39.0 : 37.2, (8, 32768) 75 : 90, (4, 32768) 74 : 57, (64, 32768) 70 : 607."""
+    return (batch - 5 * -(-rows // 256)) * prefix_len * heads > 1 << 18 and rows <= 1 << 22
+
+
+@_on_stream
 def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                      rotation: Optional[torch.Tensor], centroids: Optional[torch.Tensor], *, window: int,
                      first_tokens: int = 0, scale: Optional[float] = None, layout="soa",
@@ -402,9 +433,10 @@ def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     window, first_tokens = min(window, most), min(first_tokens, most)
     S = num_splits or _splits(s.B * s.Hk, min(window + first_tokens, most))
     s.workspace(S)
-    return s.launch(_RANGE.pack(window, first_tokens, 0, most), 0, S, stream)
+    return s.launch(_RANGE.pack(window, first_tokens, 0, most), 0, S)
 
 
+@_on_stream
 def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                      rotation: Optional[torch.Tensor], centroids: Optional[torch.Tensor], *, prefix_len: int,
                      scale: Optional[float] = None, layout="soa", sinks: Optional[torch.Tensor] = None,
@@ -414,7 +446,12 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     """Decode attention ``[B, Hq, 128]`` of a batch whose sequences begin with the same ``prefix_len`` tokens, a
     multiple of 16: the first ``prefix_len / 16`` entries of every row of ``block_table`` are the same pages.
     ``seq_lens`` and ``block_table`` describe whole sequences, prefix included; a sequence shorter than the prefix sees
-    its own tokens only.  The other arguments are :func:`window_attention`'s."""
+    its own tokens only.  The other arguments are :func:`window_attention`'s.
+
+    With 16-bit outputs, a prefix that is long enough for the batch is read once for all rows, with fp16 operands (the
+    errors are a fraction of the output's own rounding); a short one, and fp32 outputs, go sequence by sequence.
+    ``mid_o`` holds the partials of the prefix too then: ``num_splits + 2 ceil(prefix_len / 128)`` splits are always
+    enough.  ``num_splits`` is the splits of each sequence's own tokens."""
     if not isinstance(prefix_len, int) or prefix_len < 0 or prefix_len % BLOCK_SIZE:
         _no("prefix_len must be a multiple of 16")
     if num_splits is not None and num_splits < 1:
@@ -426,12 +463,11 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
         _no("the block table's rows do not hold the prefix")
     if s.B == 0:
         return s.output
-    # Each sequence on its own: fp32 outputs, and prefixes too short for the shared pass.
-    lead = 0
-    if s.out_kind != _lib.TQB_DTYPE_F32 and s.B > 1 and prefix_len >= 128:
-        lead = _prefix_splits(s.B * (s.Hq // s.Hk), s.Hk, prefix_len)
+    lead, rows = 0, s.B * (s.Hq // s.Hk)
+    if s.out_kind != _lib.TQB_DTYPE_F32 and _shares(s.B, rows, s.Hk, prefix_len):
+        lead = _prefix_splits(rows, s.Hk, prefix_len)
     else:
         prefix_len = 0
     S = (num_splits or _splits(s.B * s.Hk, max(1, most - prefix_len))) + lead
     s.workspace(S)
-    return s.launch(_RANGE.pack(0, 0, prefix_len, most), lead, S, stream, prefix_len)
+    return s.launch(_RANGE.pack(0, 0, prefix_len, most), lead, S, prefix_len)
