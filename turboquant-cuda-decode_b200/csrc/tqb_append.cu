@@ -28,6 +28,7 @@
 #include "tqb_common.cuh"
 #include "tqb_internal.h"
 #include "tqb_quant_row.cuh"
+#include "tqb_rot_mma.cuh"
 #include "tqb_umma.cuh"
 
 namespace tqb {
@@ -260,30 +261,14 @@ __device__ __forceinline__ void finish_row(const AppendParams& P, const float* s
 // ---------------------------------------------------------------------------
 // Few rows, or inputs of any alignment, and the FP8-key layouts: a CTA of four
 // warps takes 16 rows (of keys, then of queries), turns them into shared
-// memory, multiplies by R on the register-operand tensor cores and finishes
-// key rows half a warp each.  Every operand is split into three bf16 parts (24
-// bits, fp32's range) and the six products down to 2^-16 are summed in fp32;
-// R's fragments come from L2, a k step's 16 loads at once, so that nothing has
-// to be staged before the first product: the latency of a decode step's call
-// counts here.
+// memory, multiplies by R on the register-operand tensor cores (rot_step: the
+// rows in three parts) and finishes key rows half a warp each.  R's fragments
+// come from L2, so that nothing has to be staged before the first product: the
+// latency of a decode step's call counts here.
 // ---------------------------------------------------------------------------
 constexpr int kRows = 16;
 constexpr int kAppThreads = 128;
-constexpr int kPitch = kHeadDim + 4;  // floats of a row in shared memory: rows four banks apart
-
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// The next bf16 part of a pair of numbers, which keep the rest.
-__device__ __forceinline__ uint32_t take_bf16(float& x, float& y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    x -= __low2float(h);
-    y -= __high2float(h);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
+constexpr int kPitch = kHeadDim + 16;  // floats of a row in shared memory: a pair of rows covers the 32 banks
 
 template <typename T, int L>
 __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_constant__ AppendParams P, int key_ctas) {
@@ -299,6 +284,7 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
     const uint32_t r0 = ((uint32_t)blockIdx.x - (keys ? 0u : (uint32_t)key_ctas)) * kRows;
     const T* base = static_cast<const T*>(keys ? P.key : P.query);
     const int64_t sn = keys ? P.ksn : P.qsn, sh = keys ? P.ksh : P.qsh;
+    if constexpr (!k8) rot_prefetch(P.rot, 32 * warp, lane);
     // thread = dim; the rows' positions and elements, then their angles
     const RopeDim rd = rope_dim(P, t);
     const bool turned = t < P.rotary;
@@ -348,42 +334,19 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
     }
     if constexpr (!k8) {
         const int g = lane >> 2, c = lane & 3, n0 = 32 * warp;
-        const float* R = P.rot + 2 * c * kHeadDim + n0 + g;
-        float acc[4][4] = {}, small[4][4] = {};  // the product of the first parts, and the others (2^-8 of it)
+        const float* R = P.rot + 4 * c * kHeadDim + n0 + 4 * g;
+        const float* x = xs + g * kPitch + 4 * c;
+        RotSums sums;
 #pragma unroll 2
-        for (int k = 0; k < kHeadDim; k += 16) {
-            float bv[4][4], av[8];
-#pragma unroll
-            for (int n = 0; n < 4; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) bv[n][i] = __ldg(R + (k + (i & 1) + 8 * (i >> 1)) * kHeadDim + 8 * n);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {  // rows g, g + 8; dims 2c, 2c + 1 (+ 8)
-                const float2 v = *reinterpret_cast<const float2*>(xs + (g + 8 * (i & 1)) * kPitch + k + 2 * c + 8 * (i >> 1));
-                av[2 * i] = v.x;
-                av[2 * i + 1] = v.y;
-            }
-            uint32_t a[3][4];
-#pragma unroll
-            for (int p = 0; p < 3; p++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) a[p][i] = take_bf16(av[2 * i], av[2 * i + 1]);
-#pragma unroll
-            for (int q = 0; q < 3; q++)
-#pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const uint32_t b0 = take_bf16(bv[n][0], bv[n][1]), b1 = take_bf16(bv[n][2], bv[n][3]);
-#pragma unroll
-                    for (int p = 0; p + q < 3; p++) mma_bf16(p + q == 0 ? acc[n] : small[n], a[p], b0, b1);
-                }
-        }
+        for (int k = 0; k < kHeadDim; k += 16)
+            rot_step<3, false>(sums, R, k, *reinterpret_cast<const float4*>(x + k),
+                               *reinterpret_cast<const float4*>(x + 8 * kPitch + k));
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < 4; n++)
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int i = 0; i < 2; i++)
-                *reinterpret_cast<float2*>(xs + (g + 8 * i) * kPitch + n0 + 8 * n + 2 * c) =
-                    make_float2(acc[n][2 * i] + small[n][2 * i], acc[n][2 * i + 1] + small[n][2 * i + 1]);
+            for (int j = 0; j < 2; j++)
+                *reinterpret_cast<float4*>(xs + (g + 8 * i) * kPitch + n0 + 8 * c + 4 * j) = sums.get(i, j);
         __syncthreads();
     }
     if (!keys) {

@@ -12,6 +12,7 @@
 
 #include "tqb_common.cuh"
 #include "tqb_internal.h"
+#include "tqb_rot_mma.cuh"
 
 namespace tqb {
 
@@ -88,26 +89,24 @@ __global__ void __launch_bounds__(kRotThreads) rotate_kernel(const RotateParams 
 
 // The same product on the tensor cores from registers alone (no shared
 // memory), so that a kernel that needs a whole SM's can start beside it.  A
-// warp takes 16 rows and 32 output dims; every operand is split into bf16
-// parts of 8 bits (R into three, the rows into as many as their type holds),
-// which keep fp32's range, and the products that matter are summed in fp32:
-// dropped terms are 2^-24 of the row and column lengths.  2048 rows are 512
-// warps; R's fragments are read from L2, 16 loads in flight each step.
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// warp takes 16 rows and 32 output dims; 2048 rows are 512 warps.  The
+// full-size products are added up outside the tensor core: an fp32 window of
+// 777 tokens has an LSE off by 0.5e-6 on average so, 2.3e-6 in one chain.
+// V: rows in vectors of four elements, which their address and strides allow;
+// the output is Stage1's input, whose rows are 16-byte aligned.
+template <typename T, bool V>
+__device__ __forceinline__ float4 load4(const T* p) {
+    if constexpr (!V)
+        return make_float4(to_f32<T>(p[0]), to_f32<T>(p[1]), to_f32<T>(p[2]), to_f32<T>(p[3]));
+    else if constexpr (sizeof(T) == 4)
+        return __ldg(reinterpret_cast<const float4*>(p));
+    else {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+        const T* e = reinterpret_cast<const T*>(&u);
+        return make_float4(to_f32<T>(e[0]), to_f32<T>(e[1]), to_f32<T>(e[2]), to_f32<T>(e[3]));
+    }
 }
-// Part p of a pair of numbers, which keep the rest.
-__device__ __forceinline__ uint32_t take_bf16(float& x, float& y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    x -= __low2float(h);
-    y -= __high2float(h);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-template <typename T>
+template <typename T, bool V>
 __global__ void __launch_bounds__(kHeadDim) rotate_beside_kernel(const RotateParams P) {
     constexpr int kParts = sizeof(T) == 4 ? 3 : __is_same(T, __half) ? 2 : 1;  // 24, 11 and 8 bits
     pdl_trigger();
@@ -117,54 +116,19 @@ __global__ void __launch_bounds__(kHeadDim) rotate_beside_kernel(const RotatePar
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const int64_t r = min(r0 + g + 8 * i, rows - 1), b = r / P.Hq, h = r - b * P.Hq;
-        x[i] = static_cast<const T*>(P.q) + b * P.qsb + h * P.qsh + 2 * c;
+        x[i] = static_cast<const T*>(P.q) + b * P.qsb + h * P.qsh + 4 * c;
     }
-    const float* R = P.rot + 2 * c * kHeadDim + n0 + g;
-    // The products of the first parts are added up in fp32 outside the tensor
-    // core, which truncates the sum it adds to (an LSE off by 2.3e-6 on average
-    // with one chain of products, 0.5e-6 so); the others are 2^-8 of them.
-    float acc[4][4] = {}, small[4][4] = {};
-#pragma unroll
-    for (int k = 0; k < kHeadDim; k += 16) {
-        float bv[4][4], av[8];
-#pragma unroll
-        for (int n = 0; n < 4; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                bv[n][i] = __ldg(R + (k + (i & 1) + 8 * (i >> 1)) * kHeadDim + 8 * n);
-#pragma unroll
-        for (int i = 0; i < 8; i++) av[i] = to_f32<T>(x[(i >> 1) & 1][k + (i & 1) + 8 * (i >> 2)]);
-        uint32_t a[kParts][4];
-#pragma unroll
-        for (int p = 0; p < kParts; p++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) a[p][i] = take_bf16(av[2 * i], av[2 * i + 1]);
-#pragma unroll
-        for (int q = 0; q < 3; q++)
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const uint32_t b0 = take_bf16(bv[n][0], bv[n][1]), b1 = take_bf16(bv[n][2], bv[n][3]);
-#pragma unroll
-                for (int p = 0; p < kParts; p++)
-                    if (p + q > 0 && (p + q < 3 || kParts == 2)) mma_bf16(small[n], a[p], b0, b1);
-                if (q == 0) {
-                    float first[4] = {};
-                    mma_bf16(first, a[0], b0, b1);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[n][i] += first[i];
-                }
-            }
-    }
+    const float* R = P.rot + 4 * c * kHeadDim + n0 + 4 * g;
+    RotSums sums;
+#pragma unroll 2
+    for (int k = 0; k < kHeadDim; k += 16) rot_step<kParts, true>(sums, R, k, load4<T, V>(x[0] + k), load4<T, V>(x[1] + k));
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         if (r0 + g + 8 * i >= rows) continue;
         const int64_t r = r0 + g + 8 * i, b = r / P.Hq, h = r - b * P.Hq;
-        float* out = P.out + b * P.osb + h * P.osh + n0 + 2 * c;
+        float* out = P.out + b * P.osb + h * P.osh + n0 + 8 * c;
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
-            out[8 * n] = acc[n][2 * i] + small[n][2 * i];
-            out[8 * n + 1] = acc[n][2 * i + 1] + small[n][2 * i + 1];
-        }
+        for (int j = 0; j < 2; j++) *reinterpret_cast<float4*>(out + 4 * j) = sums.get(i, j);
     }
 }
 
@@ -201,7 +165,9 @@ int launch_rotate(const RotateParams& P, cudaStream_t stream) {
 template <typename T>
 static int launch_rotate_beside_t(const RotateParams& P, cudaStream_t stream) {
     const int64_t rows = (int64_t)P.B * P.Hq;
-    rotate_beside_kernel<T><<<(unsigned)((rows + 15) / 16), kHeadDim, 0, stream>>>(P);
+    const bool vec = reinterpret_cast<uintptr_t>(P.q) % (4 * sizeof(T)) == 0 && P.qsb % 4 == 0 && P.qsh % 4 == 0;
+    auto kern = vec ? rotate_beside_kernel<T, true> : rotate_beside_kernel<T, false>;
+    kern<<<(unsigned)((rows + 15) / 16), kHeadDim, 0, stream>>>(P);
     return report_launch(cudaGetLastError());
 }
 

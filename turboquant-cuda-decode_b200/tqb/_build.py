@@ -24,7 +24,7 @@ LIB_PATH = PKG_DIR / "libtqb.so"
 SOURCES = ["tqb_api.cu", "tqb_stage1.cu", "tqb_stage1_ring.cu", "tqb_stage2.cu", "tqb_store.cu", "tqb_noalloc.cu",
            "tqb_rotate.cu", "tqb_p2p.cu", "tqb_append.cu", "tqb_gather.cu",
            "tqb_prefix.cu"]
-HEADERS = ["tqb_common.cuh", "tqb_internal.h", "tqb_merge_row.cuh", "tqb_quant_row.cuh", "tqb_umma.cuh"]
+HEADERS = ["tqb_common.cuh", "tqb_internal.h", "tqb_merge_row.cuh", "tqb_quant_row.cuh", "tqb_rot_mma.cuh", "tqb_umma.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
