@@ -849,6 +849,7 @@ int tqb_gather(const tqb_gather_args* a, cudaStream_t stream) {
     p.vsn = a->v_stride_n;
     p.vsh = a->v_stride_h;
     p.N = a->num_tokens;
+    p.div_hk = tqb::FastDiv((uint32_t)a->num_kv_heads);
     p.Hk = a->num_kv_heads;
     return tqb::launch_gather(p, stream);
 }

@@ -23,7 +23,7 @@ namespace tqb {
 
 namespace {
 
-constexpr int kGatherWarps = 8;
+constexpr int kGatherWarps = 8, kIn = 2;
 
 __device__ __forceinline__ uint32_t ldu16(const uint8_t* p) {
     return __ldg(reinterpret_cast<const unsigned short*>(p));
@@ -63,79 +63,110 @@ __device__ __forceinline__ void put8(T* p, const float (&v)[8]) {
     }
 }
 
-// Half a warp per token-head, lane m of 16 on dims 8m .. 8m + 7.
-template <typename T, int L, bool VEC>
-__global__ void __launch_bounds__(kGatherWarps * 32) gather_kernel(const GatherParams P) {
+// What half a warp reads of a token-head: lane m of 16 takes dims 8m .. 8m + 7.
+template <int L>
+struct Row {
+    uint32_t n, h, k[layout_fp8_keys(L) ? 2 : 1], v, norm, scale, zero;
+    bool ok;
+};
+
+// A4: codes at 4-byte aligned addresses.
+template <int L, bool A4>
+__device__ __forceinline__ uint32_t codes8(const uint8_t* p, int m, bool three) {
+    if (three) return ld_bytes3(p + 3 * m);
+    if constexpr (A4) return __ldg(reinterpret_cast<const uint32_t*>(p + 4 * m));
+    return ldu16(p + 4 * m) | (ldu16(p + 4 * m + 2) << 16);
+}
+
+template <int L, bool A4>
+__device__ __forceinline__ void load_row(Row<L>& r, const GatherParams& P, uint32_t pid, int m) {
     constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), v3 = layout_3bit_values(L), aos = layout_is_aos(L);
-    constexpr int nc = k3 ? 8 : kNumCentroids;
     constexpr int kKey = aos_key_bytes(L), kVal = val_code_bytes(L), kRow = kKey + kVal;  // SoA row
-    __shared__ float scent[kNumCentroids];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = lane & 15;
-    if constexpr (!k8) {
-        if (threadIdx.x < nc) scent[threadIdx.x] = __ldg(P.cents + threadIdx.x);
-        __syncthreads();
-    }
-    const uint32_t total = (uint32_t)P.N * (uint32_t)P.Hk;
-    const uint32_t w0 = (blockIdx.x * kGatherWarps + (uint32_t)warp) * 2u;
-    if (w0 >= total) return;
-    const uint32_t pid0 = w0 + (uint32_t)(lane >> 4);
-    const bool live = pid0 < total;
-    const uint32_t pid = live ? pid0 : total - 1;
-    const uint32_t n = pid / (uint32_t)P.Hk, h = pid - n * (uint32_t)P.Hk;
-    const int32_t slot = __ldg(P.slots + n);
-    const bool ok = slot >= 0 && (P.num_blocks <= 0 || (int64_t)slot < P.num_blocks * kBlockSize);
-    const uint32_t blk = ok ? (uint32_t)slot / kBlockSize : 0u, off = ok ? (uint32_t)slot % kBlockSize : 0u;
+    r.n = P.div_hk.div(pid);
+    r.h = pid - r.n * (uint32_t)P.Hk;
+    const int32_t slot = __ldg(P.slots + r.n);
+    r.ok = slot >= 0 && (P.num_blocks <= 0 || (int64_t)slot < P.num_blocks * kBlockSize);
+    const uint32_t blk = r.ok ? (uint32_t)slot / kBlockSize : 0u, off = r.ok ? (uint32_t)slot % kBlockSize : 0u;
     const uint8_t* base = P.cache + (size_t)blk * (size_t)P.block_bytes;
     const uint8_t *kp, *vp;
-    float norm = 1.0f, scale, zero;
     if constexpr (aos) {
-        const uint8_t* sp = base + (size_t)off * P.pos_stride + (size_t)h * P.head_stride;
-        kp = sp;
-        vp = sp + aos_val_off(L);
-        if constexpr (!k8) norm = half_bits_to_float(ldu16(sp + aos_norm_off(L)));
-        scale = half_bits_to_float(ldu16(sp + aos_scale_off(L)));
-        zero = half_bits_to_float(ldu16(sp + aos_scale_off(L) + 2));
+        kp = base + (size_t)off * P.pos_stride + (size_t)r.h * P.head_stride;
+        vp = kp + aos_val_off(L);
+        if constexpr (!k8) r.norm = ldu16(kp + aos_norm_off(L));
+        r.scale = ldu16(kp + aos_scale_off(L));
+        r.zero = ldu16(kp + aos_scale_off(L) + 2);
     } else {
-        kp = base + (size_t)off * ((size_t)P.Hk * kRow) + (size_t)h * kRow;
+        kp = base + (size_t)off * ((size_t)P.Hk * kRow) + (size_t)r.h * kRow;
         vp = kp + kKey;
         constexpr int kFields = k8 ? 2 : 3;
-        const uint8_t* meta = base + (size_t)kBlockSize * P.Hk * kRow + ((size_t)h * kFields * kBlockSize + off) * 2;
-        if constexpr (!k8) norm = half_bits_to_float(ldu16(meta));
-        scale = half_bits_to_float(ldu16(meta + (kFields - 2) * kBlockSize * 2));
-        zero = half_bits_to_float(ldu16(meta + (kFields - 1) * kBlockSize * 2));
+        const uint8_t* meta = base + (size_t)kBlockSize * P.Hk * kRow + ((size_t)r.h * kFields * kBlockSize + off) * 2;
+        if constexpr (!k8) r.norm = ldu16(meta);
+        r.scale = ldu16(meta + (kFields - 2) * kBlockSize * 2);
+        r.zero = ldu16(meta + (kFields - 1) * kBlockSize * 2);
     }
-    float k[8], v[8];
     if constexpr (k8) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t h2 = fp8x2_to_h2(ldu16(kp + 8 * m + 2 * j));
-            k[2 * j] = half_bits_to_float(h2);
-            k[2 * j + 1] = half_bits_to_float(h2 >> 16);
-        }
+        r.k[0] = codes8<L, A4>(kp, 2 * m, false);
+        r.k[1] = codes8<L, A4>(kp, 2 * m + 1, false);
     } else {
-        const uint32_t bits = k3 ? ld_bytes3(kp + 3 * m) : ldu16(kp + 4 * m) | (ldu16(kp + 4 * m + 2) << 16);
-        float csq = 0.0f;
+        r.k[0] = codes8<L, A4>(kp, m, k3);
+    }
+    r.v = codes8<L, A4>(vp, m, v3);
+}
+
+// kIn token-heads per half-warp, all their loads in flight together; the
+// codebook in shared memory as pairs, so that a table entry is two numbers.
+template <typename T, int L, bool VEC, bool A4>
+__global__ void __launch_bounds__(kGatherWarps * 32) gather_kernel(const __grid_constant__ GatherParams P) {
+    constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), v3 = layout_3bit_values(L), aos = layout_is_aos(L);
+    constexpr int kb = k3 ? 3 : 4, nc = 1 << kb;
+    __shared__ float2 pairs[nc * nc];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = lane & 15;
+    const uint32_t total = (uint32_t)P.N * (uint32_t)P.Hk;
+    const uint32_t w0 = (blockIdx.x * kGatherWarps + (uint32_t)warp) * (2u * kIn) + (uint32_t)(lane >> 4);
+    Row<L> row[kIn];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            k[j] = scent[(bits >> ((k3 ? 3 : 4) * j)) & (nc - 1)];
-            csq = fmaf(k[j], k[j], csq);
+    for (int i = 0; i < kIn; i++) load_row<L, A4>(row[i], P, min(w0 + 2u * i, total - 1), m);
+    if constexpr (!k8) {
+        if (threadIdx.x < nc * nc) pairs[threadIdx.x] = make_float2(__ldg(P.cents + threadIdx.x % nc), __ldg(P.cents + threadIdx.x / nc));
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < kIn; i++) {
+        const Row<L>& r = row[i];
+        float k[8], v[8];
+        if constexpr (k8) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t h2 = fp8x2_to_h2((r.k[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+                k[2 * j] = half_bits_to_float(h2);
+                k[2 * j + 1] = half_bits_to_float(h2 >> 16);
+            }
+        } else {
+            float norm = half_bits_to_float(r.norm), csq = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 c = pairs[(r.k[0] >> (2 * kb * j)) & (nc * nc - 1)];
+                k[2 * j] = c.x;
+                k[2 * j + 1] = c.y;
+                if constexpr (aos) csq = fmaf(c.y, c.y, fmaf(c.x, c.x, csq));
+            }
+            // AoS stores |k|: the centroids are scaled to unit length here
+            if constexpr (aos) norm = __fdiv_rn(norm, __fsqrt_rn(warp_sum_xor(csq, 1, 8) + 1e-16f));
+#pragma unroll
+            for (int j = 0; j < 8; j++) k[j] *= norm;
         }
-        // AoS stores |k|: the centroids are scaled to unit length here
-        if constexpr (aos) norm = __fdiv_rn(norm, __fsqrt_rn(warp_sum_xor(csq, 1, 8) + 1e-16f));
+        const float scale = half_bits_to_float(r.scale), zero = half_bits_to_float(r.zero);
 #pragma unroll
-        for (int j = 0; j < 8; j++) k[j] *= norm;
+        for (int j = 0; j < 8; j++)
+            v[j] = fmaf((float)((r.v >> ((v3 ? 3 : 4) * j)) & (v3 ? 7u : 15u)), scale, zero);
+        if (!r.ok) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) k[j] = v[j] = 0.0f;
+        }
+        if (w0 + 2u * i >= total) continue;
+        put8<T, VEC>(static_cast<T*>(P.key) + (int64_t)r.n * P.ksn + (int64_t)r.h * P.ksh + 8 * m, k);
+        put8<T, VEC>(static_cast<T*>(P.value) + (int64_t)r.n * P.vsn + (int64_t)r.h * P.vsh + 8 * m, v);
     }
-    const uint32_t bits = v3 ? ld_bytes3(vp + 3 * m) : ldu16(vp + 4 * m) | (ldu16(vp + 4 * m + 2) << 16);
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-        v[j] = fmaf((float)((bits >> ((v3 ? 3 : 4) * j)) & (v3 ? 7u : 15u)), scale, zero);
-    if (!live) return;
-    if (!ok) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) k[j] = v[j] = 0.0f;
-    }
-    put8<T, VEC>(static_cast<T*>(P.key) + (int64_t)n * P.ksn + (int64_t)h * P.ksh + 8 * m, k);
-    put8<T, VEC>(static_cast<T*>(P.value) + (int64_t)n * P.vsn + (int64_t)h * P.vsh + 8 * m, v);
 }
 
 template <typename T, int L>
@@ -143,11 +174,11 @@ int launch_gather_t(const GatherParams& P, cudaStream_t stream) {
     constexpr int a = 16 / (int)sizeof(T);
     const bool vec = ((reinterpret_cast<uintptr_t>(P.key) | reinterpret_cast<uintptr_t>(P.value)) & 15) == 0 &&
                      P.ksn % a == 0 && P.ksh % a == 0 && P.vsn % a == 0 && P.vsh % a == 0;
-    const unsigned grid = (unsigned)(((int64_t)P.N * P.Hk + 2 * kGatherWarps - 1) / (2 * kGatherWarps));
-    if (vec)
-        gather_kernel<T, L, true><<<grid, kGatherWarps * 32, 0, stream>>>(P);
-    else
-        gather_kernel<T, L, false><<<grid, kGatherWarps * 32, 0, stream>>>(P);
+    const bool a4 = ((reinterpret_cast<uintptr_t>(P.cache) | (uintptr_t)P.block_bytes) & 3) == 0 && !layout_is_aos(L);
+    constexpr int kRows = 2 * kIn * kGatherWarps;
+    const unsigned grid = (unsigned)(((int64_t)P.N * P.Hk + kRows - 1) / kRows);
+    auto kern = vec ? (a4 ? gather_kernel<T, L, true, true> : gather_kernel<T, L, true, false>) : gather_kernel<T, L, false, false>;
+    kern<<<grid, kGatherWarps * 32, 0, stream>>>(P);
     return report_launch(cudaGetLastError());
 }
 

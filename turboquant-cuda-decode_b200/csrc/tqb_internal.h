@@ -243,6 +243,7 @@ struct GatherParams {
     int dtype;
     int64_t ksn, ksh, vsn, vsh;
     int N, Hk;
+    FastDiv div_hk;
 };
 
 // A prefix shared by the whole batch (tqb_prefix.cu).
