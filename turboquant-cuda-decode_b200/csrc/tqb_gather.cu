@@ -10,7 +10,8 @@
 // per head and token rather than one per cached token.
 //
 // One pass: 134 bytes (or 196, 118, 102) read and 512 written per token-head
-// with 16-bit outputs, so HBM writes bound it.
+// with 16-bit outputs, so HBM writes bound it.  131072 tokens of 8 heads: 127 us,
+// 5.3 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -115,6 +116,8 @@ __device__ __forceinline__ void load_row(Row<L>& r, const GatherParams& P, uint3
 
 // kIn token-heads per half-warp, all their loads in flight together; the
 // codebook in shared memory as pairs, so that a table entry is two numbers.
+// (kIn = 1, with single numbers: 141 us; 2: 127; 4: 125, but 917 tokens of 2
+// heads take 3.1 us in place of 2.4; 8: 144.)
 template <typename T, int L, bool VEC, bool A4>
 __global__ void __launch_bounds__(kGatherWarps * 32) gather_kernel(const __grid_constant__ GatherParams P) {
     constexpr bool k8 = layout_fp8_keys(L), k3 = layout_3bit_keys(L), v3 = layout_3bit_values(L), aos = layout_is_aos(L);
