@@ -396,7 +396,8 @@ constexpr float kCellSpan = 0.25f;
 constexpr int kCellOff = 4 * kATile;                                             // [kCells][32 lanes]
 constexpr int kTurnOff = kCellOff + kCells * 32 * 4;                             // 4 warps x 4 KB
 constexpr int kInfoOff = kTurnOff + 4 * 4096;                                    // [2][128] RowInfo
-constexpr int kTabOff = kInfoOff + 2 * 128 * 24;                                 // mids, c^2
+constexpr int kRowOff = kInfoOff + 2 * 128 * 24;                                 // [128] element offsets of the rows
+constexpr int kTabOff = kRowOff + 128 * 8;                                       // mids, c^2
 constexpr int kUmmaBarOff = kTabOff + 2 * kNumCentroids * 4;
 constexpr int kUmmaSmem = kUmmaBarOff + 64;
 static_assert(kUmmaSmem <= 232448, "shared memory per CTA");
@@ -405,11 +406,11 @@ constexpr int kUmmaThreads = (kFinishWarps + kTurnWarps + kValueWarps) * 32;
 enum : uint32_t { kAEmpty = 0, kDFull = 8, kDEmpty = 24, kUTmem = 40, kUAbort = 44 };
 
 // What the finishing warps need of a row: the sum of squares, the factor that
-// undoes the scales, its token and KV head (or query head), and its slot (-1:
-// not stored; queries: -1 where the position is outside the table).
+// undoes the scales, its token, position and head, and its slot (-1: not
+// stored; queries: -1 where the position is outside the table).
 struct __align__(8) RowInfo {
     float nsq, unscale;
-    int n, slot, pos, pad;
+    int n, slot, pos, h;
 };
 
 template <typename T>
@@ -438,18 +439,32 @@ struct UmmaTiles {
     uint32_t key_rows, rows, key_tiles, tiles;
 };
 
+// Row r of a tile: its token, head, slot and position.  (One row per thread, a
+// tile ahead: these loads depend on one another.)
+__device__ __forceinline__ RowInfo find_row(const AppendParams& P, const UmmaTiles& W, uint32_t tile, uint32_t r) {
+    const bool keys = tile < W.key_tiles;
+    const uint32_t total = keys ? W.key_rows : W.rows - W.key_rows, row = (keys ? tile : tile - W.key_tiles) * 128u + r;
+    const FastDiv& div = keys ? P.div_hk : P.div_hq;
+    const uint32_t at = min(row, total - 1), n = div.div(at);
+    RowInfo x;
+    x.n = (int)n;
+    x.h = (int)(at - n * (uint32_t)(keys ? P.Hk : P.Hq));
+    x.pos = position_of(P, (int)n);
+    x.slot = row >= total ? -1 : keys ? __ldg(P.slots + n) : 0;
+    if (keys && P.num_blocks > 0 && (int64_t)x.slot >= P.num_blocks * kBlockSize) x.slot = -1;
+    x.slot = x.pos < 0 ? -1 : max(x.slot, -1);
+    x.nsq = x.unscale = 0.0f;
+    return x;
+}
+
 // A tile's rows turned, scaled, split and stored (128-byte swizzle, K-major),
 // half a warp per row: lane m of 16 takes pairs 4m .. 4m + 3 of the row's 64
 // (pairs that the rotary step turns together, and the rest two by two).
 template <typename T>
-__device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, const UmmaTiles& W, uint32_t tile, int buf,
-                                          int lw, int lane) {
-    const bool keys = tile < W.key_tiles;
-    const uint32_t first = (keys ? tile : tile - W.key_tiles) * 128u, total = keys ? W.key_rows : W.rows - W.key_rows;
-    const FastDiv& div = keys ? P.div_hk : P.div_hq;
-    const uint32_t H = (uint32_t)(keys ? P.Hk : P.Hq);
+__device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, bool keys, int buf, int lw, int lane) {
     const T* base = static_cast<const T*>(keys ? P.key : P.query);
-    const int64_t sn = keys ? P.ksn : P.qsn, sh = keys ? P.ksh : P.qsh;
+    RowInfo* infos = reinterpret_cast<RowInfo*>(smem + kInfoOff) + 128 * buf;
+    const int64_t* offs = reinterpret_cast<const int64_t*>(smem + kRowOff);
     const int m = lane & 15, half = P.rotary >> 1, j0 = 4 * m;
     const bool turned = j0 < half;
     // dims of the lane's pairs: (a, b) = (da + i, db + i), or interleaved
@@ -468,38 +483,21 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
     struct Row {
         Quad<T> a, b;
         float4 c, s;
-        int n, pos;
     };
     constexpr int kBatch = 2, kStep = 2 * kTurnWarps;  // rows of the role's warps together
     Row x0[kBatch], x1[kBatch];
-    const int r_first = 2 * lw + (lane >> 4);
-    auto token = [&](int r, int& n, uint32_t& h) {
-        const uint32_t row = min(first + (uint32_t)r, total - 1);
-        const uint32_t t = div.div(row);
-        n = (int)t;
-        h = row - t * H;
-    };
-    auto find = [&](Row (&x)[kBatch], int r0) {  // tokens and positions
-#pragma unroll
-        for (int i = 0; i < kBatch; i++) {
-            uint32_t h;
-            token(r0 + kStep * i, x[i].n, h);
-            x[i].pos = position_of(P, x[i].n);
-        }
-    };
+    const int hw = lane >> 4, r_first = 2 * lw + hw;
     auto load = [&](Row (&x)[kBatch], int r0) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
-            int n;
-            uint32_t h;
-            token(r0 + kStep * i, n, h);
-            const T* p = base + (int64_t)n * sn + (int64_t)h * sh;
+            const int r = min(r0 + kStep * i, 127);
+            const T* p = base + offs[r];
             x[i].a.load(p + da);
             x[i].b.load(p + db);
             x[i].c = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
             x[i].s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (turned) {
-                const float* cs = table_row<T>(P, x[i].pos) + j0;
+                const float* cs = table_row<T>(P, infos[r].pos) + j0;
                 x[i].c = __ldg(reinterpret_cast<const float4*>(cs));
                 x[i].s = __ldg(reinterpret_cast<const float4*>(cs + half));
             }
@@ -509,6 +507,7 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
             const int r = r0 + kStep * i;
+            if (r - hw >= 128) break;  // (the warp's halves stay together)
             const float cc[4] = {now[i].c.x, now[i].c.y, now[i].c.z, now[i].c.w};
             const float ss[4] = {now[i].s.x, now[i].s.y, now[i].s.z, now[i].s.w};
             const float in[8] = {now[i].a[0], now[i].a[1], now[i].a[2], now[i].a[3],
@@ -543,42 +542,23 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
             }
             // four dims are 8 bytes of a 16-byte chunk
             auto at = [&](int d) { return (d >> 6) * (kATile / 2) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 4) * 2; };
-            if (r < 128) {
-                *reinterpret_cast<uint2*>(smem + kAHiOff + at(da)) = make_uint2(hi[0], hi[1]);
-                *reinterpret_cast<uint2*>(smem + kAHiOff + at(db)) = make_uint2(hi[2], hi[3]);
-                *reinterpret_cast<uint2*>(smem + kALoOff + at(da)) = make_uint2(lo[0], lo[1]);
-                *reinterpret_cast<uint2*>(smem + kALoOff + at(db)) = make_uint2(lo[2], lo[3]);
-            }
-            if (m == 0 && r < 128) {
-                RowInfo info;
-                info.nsq = nsq;
-                info.unscale = exp2i(-e) * 0x1p-10f;
-                info.n = now[i].n;
-                info.pos = now[i].pos;
-                int slot = -1;
-                if (first + r < total && now[i].pos >= 0) {
-                    slot = keys ? __ldg(P.slots + now[i].n) : 0;
-                    if (keys && P.num_blocks > 0 && (int64_t)slot >= P.num_blocks * kBlockSize) slot = -1;
-                }
-                info.slot = max(slot, -1);
-                reinterpret_cast<RowInfo*>(smem + kInfoOff)[buf * 128 + r] = info;
-            }
+            *reinterpret_cast<uint2*>(smem + kAHiOff + at(da)) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(smem + kAHiOff + at(db)) = make_uint2(hi[2], hi[3]);
+            *reinterpret_cast<uint2*>(smem + kALoOff + at(da)) = make_uint2(lo[0], lo[1]);
+            *reinterpret_cast<uint2*>(smem + kALoOff + at(db)) = make_uint2(lo[2], lo[3]);
+            if (m == 0) *reinterpret_cast<float2*>(infos + r) = make_float2(nsq, exp2i(-e) * 0x1p-10f);
         }
     };
     // (two buffers by name: handing one's registers to the other would wait for
     // its loads)
     constexpr int kNext = kStep * kBatch;
-    find(x0, r_first);
-    find(x1, r_first + kNext);
     load(x0, r_first);
 #pragma unroll 1
-    for (int r0 = r_first; r0 - (lane >> 4) < 128; r0 += 2 * kNext) {  // (the warp's halves stay together)
+    for (int r0 = r_first; r0 - hw < 128; r0 += 2 * kNext) {
         load(x1, r0 + kNext);
         turn(x0, r0);
-        find(x0, r0 + 2 * kNext);
         load(x0, r0 + 2 * kNext);
         turn(x1, r0 + kNext);
-        find(x1, r0 + 3 * kNext);
     }
 }
 
@@ -598,7 +578,7 @@ __device__ __forceinline__ void prefetch_rows(const T* base, int64_t sn, int64_t
 
 // A key row: codes of its 128 coordinates, norm, slot.
 template <typename T, int L>
-__device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem, uint32_t tm, uint32_t row, const RowInfo& info,
+__device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem, uint32_t tm, const RowInfo& info,
                                             bool fine, int lane) {
     constexpr bool k3 = layout_3bit_keys(L);
     constexpr int nc = k3 ? 8 : kNumCentroids, kBits = k3 ? 3 : 4;
@@ -607,7 +587,7 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
     const float* csq16 = smid + kNumCentroids;
     const float norm = __fsqrt_rn(info.nsq);
     const float f = info.unscale * __frcp_rn(norm + 1e-8f);
-    const uint32_t h = row - (uint32_t)info.n * (uint32_t)P.Hk;
+    const uint32_t h = (uint32_t)info.h;
     const uint8_t* cells = smem + kCellOff + 4 * lane;
     const bool stored = info.slot >= 0;
     const uint32_t slot = stored ? (uint32_t)info.slot : 0u;
@@ -719,10 +699,9 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
 
 // Query rows: the product itself, turned through shared memory into runs of
 // 128 bytes.
-__device__ __forceinline__ void finish_queries(const AppendParams& P, uint8_t* turn, uint32_t tm, uint32_t row,
+__device__ __forceinline__ void finish_queries(const AppendParams& P, uint8_t* turn, uint32_t tm,
                                                const RowInfo& info, bool live, int lane) {
-    const uint32_t h = row - (uint32_t)info.n * (uint32_t)P.Hq;
-    float* dst = P.q_rot + (int64_t)info.n * P.osn + (int64_t)h * P.osh;
+    float* dst = P.q_rot + (int64_t)info.n * P.osn + (int64_t)info.h * P.osh;
     const float f = info.slot < 0 ? __int_as_float(0x7fc00000) : info.unscale;
     const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
     const unsigned long long mine = reinterpret_cast<unsigned long long>(dst);
@@ -777,9 +756,10 @@ __device__ __forceinline__ void store_values(const AppendParams& P, const UmmaTi
             x[i].pos = position_of(P, (int)n);
         }
     };
-    auto store = [&](const Row (&x)[kBatch]) {
+    auto store = [&](const Row (&x)[kBatch], int r0) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
+            if (r0 + kStep * i - (lane >> 4) >= 128) break;  // (the warp's halves stay together)
             const float v[8] = {x[i].a[0], x[i].a[1], x[i].a[2], x[i].a[3], x[i].b[0], x[i].b[1], x[i].b[2], x[i].b[3]};
             const ValueRow q = quantise_values<layout_3bit_values(L)>(v);
             const int slot = x[i].slot;
@@ -795,9 +775,9 @@ __device__ __forceinline__ void store_values(const AppendParams& P, const UmmaTi
 #pragma unroll 1
     for (int r0 = r_first; r0 - (lane >> 4) < 128; r0 += 2 * kNext) {
         load(x1, r0 + kNext);
-        store(x0);
+        store(x0, r0);
         load(x0, r0 + 2 * kNext);
-        store(x1);
+        store(x1, r0 + kNext);
     }
 }
 
@@ -884,9 +864,9 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
             const uint32_t tm = tmem + ((uint32_t)(32 * wq) << 16) + 128u * g;
             if (__any_sync(0xffffffffu, live)) {
                 if (keys)
-                    finish_keys<T, L>(P, smem, tm, min(row, W.key_rows - 1), info, fine, lane);
+                    finish_keys<T, L>(P, smem, tm, info, fine, lane);
                 else
-                    finish_queries(P, smem + kTurnOff + 4096 * warp, tm, min(row, W.rows - W.key_rows - 1), info, live, lane);
+                    finish_queries(P, smem + kTurnOff + 4096 * warp, tm, info, live, lane);
             }
             tc_fence_before();
             bar_arrive(bars + kDEmpty + 8 * g);
@@ -897,6 +877,9 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
         const uint64_t b_hi = umma_desc(base + kBHiOff, kATile / 2, 1024), b_lo = umma_desc(base + kBLoOff, kATile / 2, 1024);
         uint32_t i = 0;
         bool ok = true;
+        const int t = tid - 32 * kFinishWarps;
+        RowInfo mine{};  // row t of the next tile
+        if (t < 128 && blockIdx.x < W.tiles) mine = find_row(P, W, blockIdx.x, (uint32_t)t);
         for (uint32_t tile = blockIdx.x; tile < W.tiles; tile += gridDim.x, i++) {
             const int buf = (int)(i & 1);
             // the operands' last readers, and the rows' (their infos and sums)
@@ -905,12 +888,20 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
             const uint32_t next = tile + gridDim.x;
             if (next < W.key_tiles)
                 prefetch_rows<T>(static_cast<const T*>(P.key), P.ksn, P.ksh, P.div_hk, (uint32_t)P.Hk, next * 128u, W.key_rows,
-                                 tid - 32 * kFinishWarps, 32 * kTurnWarps);
+                                 t, 32 * kTurnWarps);
             else if (next < W.tiles)
                 prefetch_rows<T>(static_cast<const T*>(P.query), P.qsn, P.qsh, P.div_hq, (uint32_t)P.Hq,
                                  (next - W.key_tiles) * 128u, W.rows - W.key_rows,
-                                 tid - 32 * kFinishWarps, 32 * kTurnWarps);
-            if (ok) turn_rows<T>(P, smem, W, tile, buf, warp - kFinishWarps, lane);
+                                 t, 32 * kTurnWarps);
+            const bool keys = tile < W.key_tiles;
+            if (ok && t < 128) {
+                reinterpret_cast<RowInfo*>(smem + kInfoOff)[128 * buf + t] = mine;
+                reinterpret_cast<int64_t*>(smem + kRowOff)[t] =
+                    (int64_t)mine.n * (keys ? P.ksn : P.qsn) + (int64_t)mine.h * (keys ? P.ksh : P.qsh);
+            }
+            asm volatile("bar.sync 2, %0;\n" ::"n"(32 * kTurnWarps) : "memory");
+            if (t < 128 && next < W.tiles) mine = find_row(P, W, next, (uint32_t)t);
+            if (ok) turn_rows<T>(P, smem, keys, buf, warp - kFinishWarps, lane);
             fence_async_smem();
             asm volatile("bar.sync 1, %0;\n" ::"n"(32 * kTurnWarps) : "memory");  // every warp takes every turn, also after an error
             if (ok && warp == kFinishWarps) {
