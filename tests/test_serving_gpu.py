@@ -154,7 +154,7 @@ def test_append_skips_what_has_no_place():
     assert torch.isfinite(out[:2]).all() and torch.isnan(out[2:]).all()
 
 
-# More than 8192 rows, queries and keys together, whose rows are 16-byte aligned, take the tensor-core form.
+# Thousands of rows, queries and keys together, that are aligned to four elements take the tensor-core form.
 LLOYD_MAX = [x for x in sorted(SO.LAYOUTS) if not x.endswith("k8")]
 
 

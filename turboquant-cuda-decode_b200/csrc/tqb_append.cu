@@ -374,21 +374,23 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
 // cores.  A persistent CTA walks tiles of 128 rows (of keys, then of queries):
 //   warps 0-3    finish a tile: thread = row (= TMEM lane), its 128 coordinates
 //                bucketised and packed, or written (queries);
-//   warps 4-9    turn the next tile's rows and split them: x 2^s = hi + lo in
+//   warps 4-11   turn the next tile's rows and split them: x 2^s = hi + lo in
 //                fp16 (22 bits), s from |x|; the first of them issues the
 //                products;
-//   warps 10-15  the values of the CTA's key rows, half a warp each.
+//   warps 12-19  the values of the CTA's key rows, half a warp each.
 // x R = hi R_hi + lo R_hi + hi R_lo in fp32 (R 2^10 split the same way, kept in
 // shared memory): 24 MMAs of 128 x 128 x 16 a tile, the two small products
 // first.  Errors against exact arithmetic, of |x|: 2^-23 from the fp32 turn, 3 *
 // 2^-22 from the splits, 16 accumulations of 2^-23 at the size of the small
 // products (2^-10) and 8 of 2^-23 at full size: below 2^-19 (kNear).
-// Bound by instruction issue: about 15 instructions per coordinate to
-// bucketise, 9 to turn and split, 10 per value.
+// Bound by instruction issue and latency: about 15 instructions per coordinate
+// to bucketise, 9 to turn and split, 10 per value.  32768 tokens x 8 KV heads:
+// 152 us (4, 6, 6 warps: 177; a second group of finishing warps changes
+// nothing); 2037 tokens x 40 heads: 39 us.
 // ---------------------------------------------------------------------------
 // Up to here the form above is faster: 5120 rows of a 4-bit decode step take it
-// 16.2 us and this one 19.2 us, 20480 rows 34 and 25.
-constexpr int64_t kFewRows = 8192;
+// 15.8 us and this one 16.7, 10240 rows 21.5 and 17.5.
+constexpr int64_t kFewRows = 6144;
 constexpr int kATile = 128 * kHeadDim * 2;                                       // 32 KB
 constexpr int kAHiOff = 0, kALoOff = kATile, kBHiOff = 2 * kATile, kBLoOff = 3 * kATile;
 constexpr int kCells = 128;                                                      // of [-kCellSpan, kCellSpan)
@@ -401,7 +403,7 @@ constexpr int kTabOff = kRowOff + 128 * 8;                                      
 constexpr int kUmmaBarOff = kTabOff + 2 * kNumCentroids * 4;
 constexpr int kUmmaSmem = kUmmaBarOff + 64;
 static_assert(kUmmaSmem <= 232448, "shared memory per CTA");
-constexpr int kFinishWarps = 4, kTurnWarps = 6, kValueWarps = 6;
+constexpr int kFinishWarps = 4, kTurnWarps = 8, kValueWarps = 8;
 constexpr int kUmmaThreads = (kFinishWarps + kTurnWarps + kValueWarps) * 32;
 enum : uint32_t { kAEmpty = 0, kDFull = 8, kDEmpty = 24, kUTmem = 40, kUAbort = 44 };
 
