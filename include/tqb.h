@@ -3,8 +3,10 @@
  *
  * The library (libtqb.so) holds hand-written sm_100a kernels for the decode
  * Stage1 (split-KV partial attention over the 4-bit paged cache), the Stage2
- * log-sum-exp merge, the cross-GPU merge of partial results, and the cache
- * store.  Every entry point:
+ * log-sum-exp merge, the cross-GPU merge of partial results, the cache store,
+ * and the serving steps around the cache: the append of raw projections, the
+ * gather of cached keys and values, and decode over a window or a shared
+ * prefix.  Every entry point:
  *   - takes plain device pointers, sizes and byte/element strides (no torch
  *     types), and the CUDA stream to launch on;
  *   - launches asynchronously;
@@ -36,6 +38,10 @@
  *   tqb_merge_partials  (no counterpart: the reference is single-GPU; this
  *                   merges per-GPU (O, LSE) partials with the same algebra as
  *                   baseline/stage2.py:44-55)
+ *   tqb_gather   <- the dequantisation of a cached context
+ *                   (reference/soa_decode_v1.py:322-454)
+ *   tqb_append, tqb_stage1_range, tqb_stage2_range, tqb_prefix  (no
+ *                   counterpart)
  *   tqb_store    <- triton_turboquant_store kernel launch
  *                   (reference/soa_store.py:494-524, reference/aos_store.py:420-447)
  *   tqb_rotate_query <- the launcher's query cast + rotation GEMM + copy,

@@ -349,6 +349,12 @@ def test_window_in_the_caches_basis_and_other_arguments():
     run_window("soa", torch.float32, RAGGED, 8, 2, 50, 3, seed=3, raw=False, scale=0.05, out_dtype=torch.float16)
 
 
+def test_lengths_below_zero_are_empty():
+    run_window("soa", torch.bfloat16, [40, -1, 17, -2 ** 31], 4, 2, 20, 2, seed=1)
+    for shared in (True, False):
+        run_prefix("soa", torch.bfloat16, [4] * 3, 128, 4, 2, seed=1, short=[(1, -1), (2, -2 ** 31)], shared=shared)
+
+
 def test_window_many_sequences():
     """More items than one round of the grid, ragged lengths: the weight cut with a split of first tokens."""
     rng = np.random.default_rng(4)

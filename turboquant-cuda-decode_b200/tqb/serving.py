@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 import struct
 from typing import Optional
 
@@ -72,6 +73,13 @@ def _call(name: str, *args) -> None:
 
 def _no(msg: str):
     raise TqbError(_lib.TQB_ERR_INVALID_ARG, msg)
+
+
+def _int(x, name: str) -> int:
+    try:
+        return operator.index(x)
+    except TypeError:
+        _no(f"{name} must be an integer")
 
 
 def _on(t, name: str, dtype, dev: int = -1) -> int:
@@ -419,9 +427,10 @@ def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
 
     ``num_splits`` splits share the pages of a sequence's visible tokens; ``mid_o`` may hold their partials: float32
     ``[>= B, >= Hq, >= num_splits, 129]``."""
-    if not isinstance(window, int) or window < 1:
+    window, first_tokens = _int(window, "window"), _int(first_tokens, "first_tokens")
+    if window < 1:
         _no("window must be at least 1")
-    if not isinstance(first_tokens, int) or first_tokens < 0:
+    if first_tokens < 0:
         _no("first_tokens must not be negative")
     if num_splits is not None and num_splits < 1:
         _no("num_splits must be positive")
@@ -444,7 +453,8 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
                      out_dtype: Optional[torch.dtype] = None, lse: Optional[torch.Tensor] = None,
                      mid_o: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
     """Decode attention ``[B, Hq, 128]`` of a batch whose sequences begin with the same ``prefix_len`` tokens, a
-    multiple of 16: the first ``prefix_len / 16`` entries of every row of ``block_table`` are the same pages.
+    multiple of 16: the first ``prefix_len / 16`` entries of every row of ``block_table`` are the same pages, of short and
+    empty sequences too (the shared pass reads the first row's).
     ``seq_lens`` and ``block_table`` describe whole sequences, prefix included; a sequence shorter than the prefix sees
     its own tokens only.  The other arguments are :func:`window_attention`'s.
 
@@ -452,7 +462,8 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     errors are a fraction of the output's own rounding); a short one, and fp32 outputs, go sequence by sequence.
     ``mid_o`` holds the partials of the prefix too then: ``num_splits + 2 ceil(prefix_len / 128)`` splits are always
     enough.  ``num_splits`` is the splits of each sequence's own tokens."""
-    if not isinstance(prefix_len, int) or prefix_len < 0 or prefix_len % BLOCK_SIZE:
+    prefix_len = _int(prefix_len, "prefix_len")
+    if prefix_len < 0 or prefix_len % BLOCK_SIZE:
         _no("prefix_len must be a multiple of 16")
     if num_splits is not None and num_splits < 1:
         _no("num_splits must be positive")
