@@ -362,6 +362,9 @@ def test_window_many_sequences():
 
 
 def test_window_covering_everything_equals_the_decode_call():
+    """The same splits and products; only where P V is added up differs.  A split of 10 tokens lies in two pages at most,
+    so its sum of weights times codes times scales, at most 15 * 0.3 e^0.8 = 10 (the largest of 6000 scales lies below 4
+    sigma), is truncated twice at 2^-23 of it by the decode call: 2.4e-6, and a rounding or two of the merge beside it."""
     rng = np.random.default_rng(8)
     c, _, R = book("soa")
     cache, table, lens = batch(rng, [5, 300, 77], 2, "soa")
@@ -369,7 +372,7 @@ def test_window_covering_everything_equals_the_decode_call():
     args = (torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda())
     a = tqb.window_attention(tqb.rotate_query(q, cuda(R)), *args, None, cuda(c), window=10 ** 6, num_splits=32)
     b = tqb.triton_turboquant_decode_attention(q, *args, cuda(R).T.contiguous(), cuda(c), 128 ** -0.5, 4, 66, 4)
-    assert torch.equal(a, b)
+    assert (a - b).abs().max().item() <= 2.0 ** -18
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
