@@ -495,6 +495,27 @@ def test_prefix_as_the_call_decides(batch_size, prefix):
     run_prefix("soa", torch.bfloat16, [3] * batch_size, prefix, 2, 2, seed=prefix, shared=None)
 
 
+@pytest.mark.parametrize("layout", ["soa", "aos_k3"])
+def test_prefix_keys_that_are_not_finite_stay_where_they_are_seen(layout):
+    """Norms of inf and NaN behind two rows' ends: those rows have their own numbers, the others none."""
+    rng = np.random.default_rng(14)
+    c, _, R = book(layout)
+    cache, table, lens = batch(rng, [300] * 6, 1, layout, 16)
+    lens[1], lens[4] = 100, 200
+    for t, bad in ((200, np.nan), (230, np.inf), (255, -np.inf)):
+        _, _, norm, _, _ = SO.places(layout, 1, t % 16, 0)
+        cache.reshape(len(cache), -1)[table[0, t // 16], norm:norm + 2] = np.array([bad], np.float16).view(np.uint8)
+    q = torch.from_numpy(rng.standard_normal((6, 4, 128)).astype(np.float32)).to(torch.bfloat16).cuda()
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setattr(tqb.serving, "_shares", lambda *a: True)
+        got = tqb.prefix_attention(q, torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(),
+                                   torch.from_numpy(lens).cuda(), cuda(R), cuda(c), prefix_len=256, layout=layout)
+    x = npy(q).astype(np.float64) @ npy(R).astype(np.float64)
+    ref, _, size = SO.attention(x[[1, 4]], cache, layout, table[[1, 4]], lens[[1, 4]], npy(c), lambda t, L: t >= 0)
+    assert (np.abs(npy(got)[[1, 4]] - ref) <= 1e-4 + half_step(got.dtype) * np.abs(ref) + 4e-3 * size).all()
+    assert np.isnan(npy(got)[[0, 2, 3, 5]]).all()
+
+
 def test_prefix_into_given_workspaces_and_outputs():
     """Partials of 129 floats, a strided output, and the same numbers as with the call's own."""
     a = run_prefix("aos_k3", torch.bfloat16, [20] * 5, 400, 6, 2, seed=5, num_splits=3)

@@ -82,6 +82,15 @@ def _int(x, name: str) -> int:
         _no(f"{name} must be an integer")
 
 
+def _split_count(x) -> Optional[int]:
+    if x is None:
+        return None
+    x = _int(x, "num_splits")
+    if not 1 <= x <= 1 << 20:
+        _no("num_splits must be positive (and at most 2^20)")
+    return x
+
+
 def _on(t, name: str, dtype, dev: int = -1) -> int:
     """The CUDA device of tensor ``t`` of ``dtype``: device ``dev`` if that is given."""
     if not isinstance(t, torch.Tensor):
@@ -125,8 +134,8 @@ def _cache(kv_cache, lay: int, dev: int = -1):
     """(device, shape, strides in bytes) of the paged cache."""
     d = _on(kv_cache, "kv_cache", _U8, dev)
     shape, stride = kv_cache.shape, kv_cache.stride()
-    if len(shape) != 4 or shape[1] != BLOCK_SIZE or shape[2] < 1 or stride[3] != 1:
-        _no("kv_cache must be [num_blocks, 16, Hk, slot] bytes")
+    if len(shape) != 4 or shape[0] < 1 or shape[1] != BLOCK_SIZE or shape[2] < 1 or stride[3] != 1:
+        _no("kv_cache must be [num_blocks, 16, Hk, slot] bytes of at least one block")
     if shape[3] < SLOT_BYTES[lay]:
         _no(f"this layout has slots of {SLOT_BYTES[lay]} bytes, kv_cache has {shape[3]}")
     if lay in _SOA_FAMILY and not (stride[1] == shape[2] * shape[3] and stride[2] == shape[3]) and not _block_dense(kv_cache):
@@ -432,8 +441,7 @@ def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
         _no("window must be at least 1")
     if first_tokens < 0:
         _no("first_tokens must not be negative")
-    if num_splits is not None and num_splits < 1:
-        _no("num_splits must be positive")
+    num_splits = _split_count(num_splits)
     s = _Step(query, kv_cache, block_table, seq_lens, rotation, centroids, layout, scale, sinks, output, out_dtype, lse,
               mid_o)
     if s.B == 0:
@@ -454,7 +462,8 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
                      mid_o: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
     """Decode attention ``[B, Hq, 128]`` of a batch whose sequences begin with the same ``prefix_len`` tokens, a
     multiple of 16: the first ``prefix_len / 16`` entries of every row of ``block_table`` are the same pages, of short and
-    empty sequences too (the shared pass reads the first row's).
+    empty sequences too (the shared pass reads the first row's).  All its tokens are written: a value that is not finite
+    may reach every row there, also one that ends before it.
     ``seq_lens`` and ``block_table`` describe whole sequences, prefix included; a sequence shorter than the prefix sees
     its own tokens only.  The other arguments are :func:`window_attention`'s.
 
@@ -465,8 +474,7 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     prefix_len = _int(prefix_len, "prefix_len")
     if prefix_len < 0 or prefix_len % BLOCK_SIZE:
         _no("prefix_len must be a multiple of 16")
-    if num_splits is not None and num_splits < 1:
-        _no("num_splits must be positive")
+    num_splits = _split_count(num_splits)
     s = _Step(query, kv_cache, block_table, seq_lens, rotation, centroids, layout, scale, sinks, output, out_dtype, lse,
               mid_o)
     most = s.blocks * BLOCK_SIZE
