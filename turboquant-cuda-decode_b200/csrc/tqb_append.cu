@@ -20,8 +20,8 @@
 // (Cauchy-Schwarz), and both forms below sum the full-size products in eight
 // accumulations of at most 2^-23 each, the rest at 2^-8 of that or less, with
 // operands good to 2^-20.4: 2^-19 in all.  (Measured, largest of 65536 rows along
-// a column of R, where every partial sum is near 1: 2^-19.9 and 2^-21.4 here and
-// in the form for few rows; of random rows 2^-22.5 and 2^-23.4.)
+// a column of R, where every partial sum is near 1: 2^-19.9 with tcgen05, 2^-21.4
+// with mma.sync; of random rows 2^-22.5 and 2^-23.4.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
