@@ -331,6 +331,8 @@ int tqb_stage2_range(const tqb_stage2_args* args, const tqb_range* range, int32_
  * dequantised once for up to 256 queries of a KV head, and the products run
  * on the tensor cores with fp16 operands and fp32 accumulators: the partials
  * are good for 16-bit outputs (about 3e-4 relative), not for fp32 ones.
+ * Weights below 2^-32 of a split's largest count as zero in O (not in the
+ * LSE).
  * num_splits is at most ceil(prefix_len / 128); with batch * (Hq / Hk) <= 128
  * an even num_splits may be twice that.  tqb_stage1_range with the same
  * prefix_len adds each sequence's own tokens as further splits, and

@@ -1,0 +1,59 @@
+"""Serving operators where numbers, sizes or alignment are at their ends, against float64 forms."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import serving_oracle as SO
+import tqb
+from test_serving_gpu import batch, book, cos_sin_table, cuda, half_step, no_wait_timeouts, npy, random_cache  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def put_half(cache, layout, page, t, field, value):
+    """Sets a token's norm (field 2), scale (3) or zero (4), head 0."""
+    at = SO.places(layout, cache.shape[2], t, 0)[field]
+    cache.reshape(len(cache), -1)[page, at:at + 2] = np.array([value], np.float16).view(np.uint8)
+
+
+def share(monkeypatch, chunks=None):
+    monkeypatch.setattr(tqb.serving, "_shares", lambda *a: True)
+    if chunks is not None:
+        monkeypatch.setattr(tqb.serving, "_prefix_splits", lambda *a: chunks)
+
+
+@pytest.mark.parametrize("chunks", [1, 2])
+def test_prefix_of_one_token_that_outweighs_the_rest(monkeypatch, chunks):
+    """A first token of value 0 that takes nearly all of the weight, the others 2^-26 of it each: the output is theirs.
+
+    Every key is its norm times one vector c and every query a multiple of c, so the products q_i k_i are positive, and a
+    score is off by at most 3 * 2^-11 of itself (q, c and c norm rounded to fp16): 0.033 for the difference of the two
+    scores (20.3 and 2.25).  The small weights stand 2^-26 below the largest, which the reference keeps at 2^7 at least:
+    spacing 2^-24, half of it 2^-6 of a weight.  0.049 in all, 0.06 with what the values' rounding and the sums add."""
+    share(monkeypatch, chunks)
+    rng = np.random.default_rng(21)
+    c, _, _ = book("soa")
+    cache, table, lens = batch(rng, [2048 + 5] * 4, 1, "soa", 128)
+    codes = SO.pack(rng.integers(0, 16, 128), 4)
+    cache[:, :, :, :] = 0
+    flat = cache.reshape(len(cache), -1)
+    for t in range(16):
+        ka, va, _, _, _ = SO.places("soa", 1, t, 0)
+        flat[:, ka:ka + 64] = codes
+        flat[:, va:va + 64] = rng.integers(0, 256, (len(cache), 64))
+        for page in range(len(cache)):
+            put_half(cache, "soa", page, t, 2, 2.5 + 0.05 * rng.standard_normal())
+            put_half(cache, "soa", page, t, 3, 20.0)
+            put_half(cache, "soa", page, t, 4, 100.0)
+    put_half(cache, "soa", table[0, 0], 0, 2, 22.5)
+    put_half(cache, "soa", table[0, 0], 0, 3, 0.0)
+    put_half(cache, "soa", table[0, 0], 0, 4, 0.0)
+    d = npy(c)[SO.unpack(codes, 4)].astype(np.float64)
+    q = np.broadcast_to(d / (d @ d) * (26 * np.log(2) / 20 * np.sqrt(128)), (4, 4, 128)).astype(np.float32)
+    got = tqb.prefix_attention(torch.from_numpy(q.copy()).cuda(), torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(),
+                               torch.from_numpy(lens).cuda(), None, cuda(c), prefix_len=2048, out_dtype=torch.bfloat16)
+    ref, _, size = SO.attention(q, cache, "soa", table, lens, npy(c), lambda t, L: t >= 0)
+    assert (np.abs(npy(got) - ref) <= half_step(got.dtype) * np.abs(ref) + 0.06 * size).all()

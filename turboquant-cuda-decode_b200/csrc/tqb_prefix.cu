@@ -34,7 +34,7 @@
 // bf16 output's own rounding, which is why only 16-bit outputs come here.
 //
 // m is a lazy reference: it moves (and l and O are rescaled) only when a weight
-// exceeds 2^8, far from the end of fp16.
+// exceeds 2^15, half of what fp16 holds.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -67,7 +67,12 @@ constexpr int kPrefixThreads = (kSoftmaxWarps + kProducerWarps) * 32;  // whole 
 // launch's).
 constexpr int kPrefixRegs = 168, kSoftmaxRegs = 200, kProducerRegs = 104;
 static_assert(2 * kSoftmaxRegs + kProducerRegs <= 3 * kPrefixRegs && kPrefixRegs * kPrefixThreads <= 65536, "register split");
-constexpr float kMost = 256.0f;  // the largest weight before the reference moves
+// A row's largest weight stands at 2^7 where its reference is set and may grow
+// to 2^15 before it moves again (weighing a tile twice: 2^8 and 2^15 take 5 us
+// more at 64 x 32768).  fp16 ends at 2^-25, so weights down to 2^-32 of the
+// largest count, and those above 2^-21 of it have all their bits: a first
+// token that takes nearly all of the weight leaves the others theirs.
+constexpr float kStart = 7.0f, kMost = 32768.0f;
 
 // Barriers (8 bytes each) at kBarOff, then words.
 // Two of each: stages of K and V, S and the last products (after an error) per
@@ -410,7 +415,7 @@ __device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, bo
     const uint64_t k2 = pack2(kfac, kfac);
     if (__any_sync(0xffffffffu, st.ref == -INFINITY)) {  // rows that see their first tokens
         const float top = largest<MASK>(ts, lim, pages);
-        if (st.ref == -INFINITY && top < INFINITY) st.ref = top * kfac;
+        if (st.ref == -INFINITY && top < INFINITY) st.ref = top * kfac - kStart;
     }
     for (;;) {
         uint32_t s[4][32], p[64];
@@ -439,7 +444,7 @@ __device__ __forceinline__ void weigh(RowState& st, uint32_t ts, uint32_t to, bo
             }
         const bool over = fmaxf(__low2float(most), __high2float(most)) > kMost;
         if (__any_sync(0xffffffffu, over)) {
-            const float x = largest<MASK>(ts, lim, pages) * kfac - r;
+            const float x = largest<MASK>(ts, lim, pages) * kfac - r - kStart;
             const bool move = over && x > 0.0f && x < INFINITY;  // infinite scores stay as they are
             if (__any_sync(0xffffffffu, move)) {
                 st = raise(st, x, move, to, has_o);
