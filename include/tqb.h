@@ -330,7 +330,9 @@ int tqb_stage2_range(const tqb_stage2_args* args, const tqb_range* range, int32_
  * tqb_stage1's; prefix_len is a positive multiple of 16.  Each page is
  * dequantised once for up to 256 queries of a KV head, and the products run
  * on the tensor cores with fp16 operands and fp32 accumulators: the partials
- * are good for 16-bit outputs (about 3e-4 relative), not for fp32 ones.
+ * are off by about 1e-3 of their size for scores of a standard deviation of
+ * 2.5 (1.9e-3 for 10; FP8 keys half of that), good for bf16 outputs, whose own
+ * rounding is 1.65e-3, not for fp16 or fp32 ones.
  * Weights below 2^-32 of a split's largest count as zero in O (not in the
  * LSE).
  * num_splits is at most ceil(prefix_len / 128); with batch * (Hq / Hk) <= 128

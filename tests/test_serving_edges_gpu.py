@@ -57,3 +57,26 @@ def test_prefix_of_one_token_that_outweighs_the_rest(monkeypatch, chunks):
                                torch.from_numpy(lens).cuda(), None, cuda(c), prefix_len=2048, out_dtype=torch.bfloat16)
     ref, _, size = SO.attention(q, cache, "soa", table, lens, npy(c), lambda t, L: t >= 0)
     assert (np.abs(npy(got) - ref) <= half_step(got.dtype) * np.abs(ref) + 0.06 * size).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("spread", [0.7, 1.5, 2.5, 5.0])
+def test_prefix_error_against_the_outputs_own_rounding(monkeypatch, dtype, spread):
+    """The rms error of a batch behind a prefix, relative to the outputs' rms.
+
+    An output rounded once is off by at most half a step, 2^-11 (fp16) or 2^-8 (bf16) of it, spread evenly: rms 1 / sqrt(3)
+    of that.  fp16 outputs have no more than 1.2 times that.  bf16 ones add the shared pass: a score of standard deviation
+    u carries three roundings (q, c and c norm to fp16) of rms 2^-11 / sqrt(3) at most each, so 2^-11 u, which its weight
+    and with it the output follows; V and P one each, 2^-11 sqrt(2 / 3) together."""
+    share(monkeypatch)
+    rng = np.random.default_rng(int(10 * spread))
+    c, _, R = book("soa")
+    cache, table, lens = batch(rng, [1024 + n for n in (1, 9, 40, 17)], 2, "soa", 64)
+    q = torch.from_numpy((spread * rng.standard_normal((4, 8, 128))).astype(np.float32)).to(dtype).cuda()
+    got = tqb.prefix_attention(q, torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(),
+                               cuda(R), cuda(c), prefix_len=1024)
+    ref, _, _ = SO.attention(npy(q).astype(np.float64) @ npy(R).astype(np.float64), cache, "soa", table, lens, npy(c),
+                             lambda t, L: t >= 0)
+    error = np.sqrt(((got.double().cpu().numpy() - ref) ** 2).mean() / (ref ** 2).mean())
+    own = half_step(dtype) / np.sqrt(3)
+    assert error <= (1.2 * own if dtype == torch.float16 else np.sqrt(own ** 2 + 2.0 ** -22 * (spread ** 2 + 2 / 3)))
