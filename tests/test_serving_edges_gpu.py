@@ -80,3 +80,28 @@ def test_prefix_error_against_the_outputs_own_rounding(monkeypatch, dtype, sprea
     error = np.sqrt(((got.double().cpu().numpy() - ref) ** 2).mean() / (ref ** 2).mean())
     own = half_step(dtype) / np.sqrt(3)
     assert error <= (1.2 * own if dtype == torch.float16 else np.sqrt(own ** 2 + 2.0 ** -22 * (spread ** 2 + 2 / 3)))
+
+
+def run_append(key, R, mids, cents, layout="soa", **kw):
+    """Bytes of an append of ``key`` (float32 [n, hk, 128]) without rotary positions, and the definition's."""
+    rng = np.random.default_rng(len(key))
+    n, hk, _ = key.shape
+    cache0 = rng.integers(0, 256, (n // 16 + 1, 16, hk, SO.LAYOUTS[layout][2]), dtype=np.uint8)
+    slots = rng.permutation(n).astype(np.int32)
+    value = rng.standard_normal(key.shape).astype(np.float32)
+    cache = torch.from_numpy(cache0).cuda()
+    tqb.rope_append(torch.from_numpy(key).cuda(), torch.from_numpy(value).cuda(), cache, torch.from_numpy(slots).cuda(), None,
+                    None, cuda(R), cuda(mids), cuda(cents), layout=layout, **kw)
+    return cache.cpu().numpy(), SO.append(cache0, layout, key, value, slots, None, None, npy(R), npy(mids), npy(cents))
+
+
+@pytest.mark.parametrize("n", [300, 2600])
+def test_append_norm_of_codes_of_very_different_size(n):
+    """Rows along a column of R: one code of size 1 and 127 whose square, 5.9e-8, is less than half a unit of the sum's last
+    place.  The norms are spread, so that some lie next to a border between two fp16 numbers."""
+    _, _, R = book("soa")
+    cents = torch.tensor([-0.9, -0.8, -0.7, -0.6, -0.5, -0.4, -0.3, -0.2, 2.43e-4, 0.3, 0.4, 0.5, 0.6, 0.7, 0.8, 1.0])
+    rng = np.random.default_rng(n)
+    key = (npy(R)[:, 0] * rng.uniform(1, 64, (n, 4, 1))).astype(np.float32)
+    got, want = run_append(key, R, tqb.get_midpoints(cents), cents)
+    assert np.array_equal(got, want), f"{(got != want).sum()} bytes differ"

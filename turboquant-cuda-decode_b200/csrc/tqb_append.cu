@@ -9,19 +9,26 @@
 //     q_rot[n, h] = rope(query[n, h]) R in fp32.
 // FP8 keys store x itself as e4m3, and their queries are not rotated.
 //
-// Nothing is rounded to the inputs' 16 bits on the way: x is the exact pair
-// a c - b s rounded once to fp32 (error-free transformations), and the codes
-// are those of exact arithmetic.  A coordinate whose fp32 value lies within
-// kNear of a border, and a norm whose fp32 value lies within kNormNear of a
+// Nothing is rounded to the inputs' 16 bits on the way, and the codes are those
+// of exact arithmetic.  A coordinate whose fp32 value lies within kNear of a
+// border, and a norm whose fp32 value lies within kNormNear (relative) of a
 // border between two fp16 numbers, are computed again in 64 bits by the whole
-// warp (about one row in sixty, and one in two hundred), so the bytes written do
-// not depend on the order of any sum.  kNear covers the fp32 sums, in units of
-// |x|: partial sums of a unit row times a unit column stay below 1
-// (Cauchy-Schwarz), and both forms below sum the full-size products in eight
-// accumulations of at most 2^-23 each, the rest at 2^-8 of that or less, with
-// operands good to 2^-20.4: 2^-19 in all.  (Measured, largest of 65536 rows along
-// a column of R, where every partial sum is near 1: 2^-19.9 with tcgen05, 2^-21.4
-// with mma.sync; of random rows 2^-22.5 and 2^-23.4.)
+// warp (about one row in forty, and one in two hundred), so the bytes written do
+// not depend on the order of any sum.  Bounds, in units of 2^-23, the larger of
+// the two forms below:
+//   y (of |x|; partial sums of a unit row times a unit column stay below 1,
+//   Cauchy-Schwarz): the turned pairs 1; the splits of x and R 2 each and the
+//   product of the two rests 2; eight accumulations of the full-size products 8
+//   (the others are 2^-8 of them or less); the norm and its reciprocal, as
+//   below without c, 6; the border in the cell table, whose four low bits hold
+//   its index, 2 (15 units of 2^-26).  23 in all, kNear is 24.
+//   (Measured, largest of 65536 rows along a column of R, where every partial
+//   sum is near 1: 2^-19.9 with tcgen05, 2^-21.4 with mma.sync; of random rows
+//   2^-22.5 and 2^-23.4.)
+//   stored norm: the turned pairs 1; |x|^2 in a chain of 8 and 4 additions,
+//   halved by the root, 3; the root 0.5; sum c^2 in chains of 16 and 8
+//   additions, its squares rounded, halved, 6; rsqrtf 2, the product 0.5.  13
+//   in all, kNormNear is 16.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -40,8 +47,8 @@ __device__ unsigned int g_append_timeouts = 0;
 
 namespace {
 
-constexpr float kNear = 0x1p-19f;
-constexpr float kNormNear = 0x1p-19f;
+constexpr float kNear = 24 * 0x1p-23f;
+constexpr float kNormNear = 16 * 0x1p-23f;
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
 // shared memory): 24 MMAs of 128 x 128 x 16 a tile, the two small products
 // first.  Errors against exact arithmetic, of |x|: 2^-23 from the fp32 turn, 3 *
 // 2^-22 from the splits, 16 accumulations of 2^-23 at the size of the small
-// products (2^-10) and 8 of 2^-23 at full size: below 2^-19 (kNear).
+// products (2^-10) and 8 of 2^-23 at full size (kNear has the rest).
 // Bound by instruction issue and latency: about 15 instructions per coordinate
 // to bucketise, 9 to turn and split, 10 per value.  32768 tokens x 8 KV heads:
 // 152 us (4, 6, 6 warps: 177; a second group of finishing warps changes
@@ -600,6 +607,7 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
     float csq = 0.0f;
 #pragma unroll 1
     for (int q = 0; q < 8; q++) {
+        float part = 0.0f;  // of csq: one chain of 128 additions would be off by 2^-17
         uint32_t z[16];
         tmem_ld16(z, tm + 16 * q);
         tmem_wait_ld();
@@ -619,7 +627,7 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
                 const float d = y - __uint_as_float(e);
                 const bool up = d >= 0.0f;
                 const int code = (int)(e & 15u) + (up ? 1 : 0);
-                csq += csq16[code];
+                part += csq16[code];
                 near |= fabsf(d) < kNear ? 1u << j : 0u;
                 upper |= up ? 1u << j : 0u;
                 codes |= (uint64_t)(uint32_t)code << (kBits * j);
@@ -633,7 +641,7 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
                 int code = 0;
                 for (int k = 0; k < nc - 1; k++) code += y >= smid[k] ? 1 : 0;
                 const bool up = code > 0 && y - smid[max(code - 1, 0)] < kNear;
-                csq += csq16[code];
+                part += csq16[code];
                 near |= up || (code < nc - 1 && smid[code] - y < kNear) ? 1u << j : 0u;
                 upper |= up ? 1u << j : 0u;
                 codes |= (uint64_t)(uint32_t)code << (kBits * j);
@@ -653,10 +661,11 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
             const int c = border + (exact_side<T>(P, krow, table_row<T>(P, __shfl_sync(kFull, info.pos, src)), 16 * q + j, smid[border], lane) ? 1 : 0);
             if (lane == src) {
                 near &= near - 1;
-                csq += csq16[c] - csq16[c0];
+                part += csq16[c] - csq16[c0];
                 codes ^= (uint64_t)(uint32_t)(c ^ c0) << (kBits * j);
             }
         }
+        csq += part;
         if (stored) {
             if constexpr (k3) {
 #pragma unroll
@@ -832,7 +841,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
     fence_async_smem();
     __syncthreads();
     // Cells of the coordinate's range: the border nearest to the cell, its
-    // index in the four low bits (2^-22 of it, far below kNear).  A cell
+    // index in the four low bits (at most 15 units of 2^-26, see kNear).  A cell
     // that two borders come near to leaves every row to the search.
     bool fine = true;
     if (tid < kCells) {
