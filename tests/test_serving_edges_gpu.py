@@ -105,3 +105,21 @@ def test_append_norm_of_codes_of_very_different_size(n):
     key = (npy(R)[:, 0] * rng.uniform(1, 64, (n, 4, 1))).astype(np.float32)
     got, want = run_append(key, R, tqb.get_midpoints(cents), cents)
     assert np.array_equal(got, want), f"{(got != want).sum()} bytes differ"
+
+
+@pytest.mark.parametrize("n", [20, 2100])
+@pytest.mark.parametrize("layout", ["soa", "aos_k3"])
+def test_append_borders_closer_than_fp32_can_tell(n, layout):
+    """Neighbouring fp32 numbers as borders, and keys whose coordinates all lie among them."""
+    _, _, R = book(layout)
+    at = np.float32(1 / np.sqrt(128))
+    close = [at]
+    for _ in range(3):
+        close = [np.nextafter(close[0], np.float32(0)), *close, np.nextafter(close[-1], np.float32(1))]
+    rest = [-0.2, -0.1, -0.05, 0.02, 0.12, 0.15, 0.18, 0.2] if layout == "soa" else []
+    mids = torch.from_numpy(np.sort(np.array([*close, *rest], np.float32)))
+    cents = torch.linspace(-0.2, 0.2, len(mids) + 1)
+    t = np.full((n, 4, 128), 1.0) * np.random.default_rng(n).uniform(0.5, 2, (n, 4, 1))
+    key = (t @ npy(R).astype(np.float64).T).astype(np.float32)
+    got, want = run_append(key, R, mids, cents, layout)
+    assert np.array_equal(got, want), f"{(got != want).sum()} bytes differ"

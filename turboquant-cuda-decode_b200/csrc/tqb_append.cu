@@ -134,10 +134,12 @@ __device__ __noinline__ double exact_norm(const AppendParams& P, const T* row, c
     }
     return sqrt(warp_sum_f64(q));
 }
-// Whether coordinate e of a key row is at border `mid` or above, in 64 bits
-// (whole warp): x R_e >= mid (|x| + 1e-8).
+// Code of coordinate e of a key row in 64 bits (whole warp): the borders with
+// x R_e >= mid (|x| + 1e-8), a lane each (borders may lie closer to one another
+// than fp32 can tell).
 template <typename T>
-__device__ __noinline__ bool exact_side(const AppendParams& P, const T* row, const float* cs, int e, float mid, int lane) {
+__device__ __noinline__ int exact_code(const AppendParams& P, const T* row, const float* cs, int e, const float* smid, int borders,
+                                       int lane) {
     double q = 0.0, z = 0.0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -148,7 +150,7 @@ __device__ __noinline__ bool exact_side(const AppendParams& P, const T* row, con
     }
     q = warp_sum_f64(q);
     z = warp_sum_f64(z);
-    return z >= (double)mid * (sqrt(q) + 1e-8);
+    return __popc(__ballot_sync(0xffffffffu, lane < borders && z >= (double)smid[min(lane, borders - 1)] * (sqrt(q) + 1e-8)));
 }
 
 template <typename T>
@@ -199,14 +201,9 @@ __device__ __forceinline__ void finish_row(const AppendParams& P, const float* s
             i += y >= smid[i + 1] ? 2 : 0;
             i += y >= smid[i] ? 1 : 0;
             code[j] = i;
-            // the borders on the two sides of the code (one side at the ends):
-            // next to one of them, the code is that border's for now, and goes
-            // up by one if the coordinate is on its upper side
-            const bool below = fabsf(y - smid[max(i - 1, 0)]) < kNear, above = fabsf(y - smid[min(i, nc - 2)]) < kNear;
-            if (below || above) {
-                near |= 1u << j;
-                code[j] = below ? max(i - 1, 0) : min(i, nc - 2);
-            }
+            // the borders on the two sides of the code (one side at the ends)
+            const float below = fabsf(y - smid[max(i - 1, 0)]), above = fabsf(y - smid[min(i, nc - 2)]);
+            near |= fminf(below, above) < kNear ? 1u << j : 0u;
         }
         if (!write) near = 0;
         uint32_t who;
@@ -215,16 +212,11 @@ __device__ __forceinline__ void finish_row(const AppendParams& P, const float* s
             const int sn = __shfl_sync(kFull, n, src), sh = __shfl_sync(kFull, h, src), sp = __shfl_sync(kFull, pos, src);
             const int j = __shfl_sync(kFull, __ffs(near) - 1, src);
             const T* row = static_cast<const T*>(P.key) + (int64_t)sn * P.ksn + (int64_t)sh * P.ksh;
-            int border = 0;
-#pragma unroll
-            for (int jj = 0; jj < 8; jj++)
-                if (jj == j) border = code[jj];
-            const float mid = smid[__shfl_sync(kFull, border, src)];
-            const bool up = exact_side<T>(P, row, table_row<T>(P, sp), 8 * (src & 15) + j, mid, lane);
+            const int c = exact_code<T>(P, row, table_row<T>(P, sp), 8 * (src & 15) + j, smid, nc - 1, lane);
             if (lane == src) {
 #pragma unroll
                 for (int jj = 0; jj < 8; jj++)
-                    if (jj == j && up) code[jj]++;
+                    if (jj == j) code[jj] = c;
                 near &= near - 1;
             }
         }
@@ -611,9 +603,7 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
         uint32_t z[16];
         tmem_ld16(z, tm + 16 * q);
         tmem_wait_ld();
-        // coordinates next to a border, and those on its upper side as far as
-        // fp32 says
-        uint32_t near = 0u, upper = 0u;
+        uint32_t near = 0u;   // coordinates next to a border
         uint64_t codes = 0u;  // 16 of them
         if (fine) {
 #pragma unroll
@@ -625,11 +615,9 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
                                       0x1p23f + (128.0f * kCells - 1.0f));
                 const uint32_t e = *reinterpret_cast<const uint32_t*>(cells + (__float_as_uint(t) & (128u * (kCells - 1))));
                 const float d = y - __uint_as_float(e);
-                const bool up = d >= 0.0f;
-                const int code = (int)(e & 15u) + (up ? 1 : 0);
+                const int code = (int)(e & 15u) + (d >= 0.0f ? 1 : 0);
                 part += csq16[code];
                 near |= fabsf(d) < kNear ? 1u << j : 0u;
-                upper |= up ? 1u << j : 0u;
                 codes |= (uint64_t)(uint32_t)code << (kBits * j);
             }
         } else {  // by search
@@ -640,10 +628,8 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
                 for (int i = 0; i < 16; i++) y = i == j ? __uint_as_float(z[i]) * f : y;
                 int code = 0;
                 for (int k = 0; k < nc - 1; k++) code += y >= smid[k] ? 1 : 0;
-                const bool up = code > 0 && y - smid[max(code - 1, 0)] < kNear;
                 part += csq16[code];
-                near |= up || (code < nc - 1 && smid[code] - y < kNear) ? 1u << j : 0u;
-                upper |= up ? 1u << j : 0u;
+                near |= (code > 0 && y - smid[max(code - 1, 0)] < kNear) || (code < nc - 1 && smid[code] - y < kNear) ? 1u << j : 0u;
                 codes |= (uint64_t)(uint32_t)code << (kBits * j);
             }
         }
@@ -655,11 +641,9 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
             const int sn = __shfl_sync(kFull, info.n, src), sh = __shfl_sync(kFull, (int)h, src);
             const int j = __shfl_sync(kFull, __ffs(near) - 1, src);
             const T* krow = static_cast<const T*>(P.key) + (int64_t)sn * P.ksn + (int64_t)sh * P.ksh;
-            const int c0 = (int)(codes >> (kBits * j)) & (nc - 1);
-            // the border next to it, below or above the code
-            const int border = __shfl_sync(kFull, c0 - (int)((upper >> j) & 1u), src);
-            const int c = border + (exact_side<T>(P, krow, table_row<T>(P, __shfl_sync(kFull, info.pos, src)), 16 * q + j, smid[border], lane) ? 1 : 0);
+            const int c = exact_code<T>(P, krow, table_row<T>(P, __shfl_sync(kFull, info.pos, src)), 16 * q + j, smid, nc - 1, lane);
             if (lane == src) {
+                const int c0 = (int)(codes >> (kBits * j)) & (nc - 1);
                 near &= near - 1;
                 part += csq16[c] - csq16[c0];
                 codes ^= (uint64_t)(uint32_t)(c ^ c0) << (kBits * j);
