@@ -123,3 +123,46 @@ def test_append_borders_closer_than_fp32_can_tell(n, layout):
     key = (t @ npy(R).astype(np.float64).T).astype(np.float32)
     got, want = run_append(key, R, mids, cents, layout)
     assert np.array_equal(got, want), f"{(got != want).sum()} bytes differ"
+
+
+@pytest.mark.parametrize("n", [40, 2600])
+@pytest.mark.parametrize("layout", ["soa", "aos", "soa_k3"])
+@pytest.mark.parametrize("border", ["at zero", "beside zero", "none near"])
+def test_append_rows_of_zeros(n, layout, border):
+    """Zeros of both signs, rows of one tiny number (their squares vanish, the sides of zero do not), among ordinary ones."""
+    c, m, R = book(layout)
+    if border != "at zero":
+        c = c + (1e-9 if border == "beside zero" else 0.01)
+        m = tqb.get_midpoints(c)
+    rng = np.random.default_rng(n)
+    key = rng.standard_normal((n, 3, 128)).astype(np.float32)
+    key[rng.random((n, 3)) < 0.3] = 0.0
+    key[rng.random((n, 3)) < 0.1] = -0.0
+    tiny = rng.random((n, 3)) < 0.02
+    key[tiny] = 0.0
+    key[tiny, rng.integers(0, 128)] = rng.choice(np.array([1e-45, -1e-45, 3e-39, -1e-30, 1e-22], np.float32), tiny.sum())
+    got, want = run_append(key, R, m, c, layout)
+    assert np.array_equal(got, want), f"{(got != want).sum()} bytes differ"
+
+
+@pytest.mark.parametrize("n", [64, 2048])
+def test_append_of_zeros_takes_no_longer(n):
+    """Dummy inputs: at most three times as long as random ones (a hundredfold where each coordinate takes 64 bits)."""
+    c, m, R = (cuda(x) for x in book("soa"))
+    cache = torch.zeros(n // 16, 16, 8, 134, dtype=torch.uint8, device="cuda")
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    value = torch.randn(n, 8, 128, device="cuda")
+    took = []
+    for key in (torch.randn_like(value), torch.zeros_like(value)):
+        best = []
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            tqb.rope_append(key, value, cache, slots, None, None, R, m, c)
+            a.record()
+            for _ in range(10):
+                tqb.rope_append(key, value, cache, slots, None, None, R, m, c)
+            b.record()
+            b.synchronize()
+            best.append(a.elapsed_time(b))
+        took.append(min(best))
+    assert took[1] <= 3 * took[0], took
