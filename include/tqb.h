@@ -355,7 +355,8 @@ int tqb_prefix(const tqb_stage1_args* args, int32_t prefix_len, cudaStream_t str
  * given.  Rotary rule: cos_sin[p] = [cos of rotary_dim / 2 angles | their
  * sines]; pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved;
  * dims from rotary_dim on are not turned.  positions NULL: no rotary step.
- * rotation is orthogonal.  A token with a negative or out-of-range slot is
+ * rotation is orthogonal.  A key whose |x|^2 is beyond fp32 has a norm of inf
+ * and codes of 0.  A token with a negative or out-of-range slot is
  * not stored; nor is one whose position is outside [0, max_pos), and its
  * q_rot rows are NaN.  Slots must be distinct: a slot named twice holds a
  * mixture of its tokens.  key, value and query have unit inner stride and any

@@ -166,3 +166,46 @@ def test_append_of_zeros_takes_no_longer(n):
             best.append(a.elapsed_time(b))
         took.append(min(best))
     assert took[1] <= 3 * took[0], took
+
+
+@pytest.mark.parametrize("n", [20, 700])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_append_queries_of_any_size(n, dtype):
+    """Rows whose squares leave fp32's range, beside ordinary ones and rows of zeros: 2^-17 |q|, as for every query."""
+    c, m, R = book("soa")
+    rng = np.random.default_rng(n)
+    q = rng.standard_normal((n, 8, 128)) * np.exp2(rng.choice([-110, -80, -62, -55, 0, 0, 0, 55, 62, 63, 64, 80, 110], (n, 8, 1)))
+    q[rng.random((n, 8)) < 0.1] = 0
+    q = torch.from_numpy(q.astype(np.float32)).to(dtype).cuda()
+    k = torch.from_numpy(rng.standard_normal((n, 4, 128)).astype(np.float32)).to(dtype).cuda()
+    cache = torch.zeros(n // 16 + 1, 16, 4, 134, dtype=torch.uint8, device="cuda")
+    cs, pos = cos_sin_table(500, 64), rng.integers(0, 500, n)
+    got = tqb.rope_append(k, k, cache, torch.arange(n, dtype=torch.int32, device="cuda"), torch.from_numpy(pos).cuda(),
+                          torch.from_numpy(cs).cuda(), cuda(R), cuda(m), cuda(c), query=q)
+    x = SO.rope(npy(q).astype(np.float64), cs[pos], False)
+    off = np.abs(got.double().cpu().numpy() - x @ npy(R).astype(np.float64))
+    assert (off <= 2.0 ** -17 * np.linalg.norm(x, axis=-1, keepdims=True)).all()
+
+
+def test_append_keys_beyond_fp32_write_the_same_in_both_forms():
+    """|x|^2 above fp32's range, infinities and NaN: a norm of inf or NaN and codes of 0, however many rows there are."""
+    c, m, R = (cuda(x) for x in book("soa"))
+    rng = np.random.default_rng(5)
+    n = 1700
+    key = rng.standard_normal((n, 4, 128)).astype(np.float32)
+    bad = rng.random((n, 4)) < 0.2
+    key[bad] *= np.float32(2.0 ** 80)
+    key[rng.random(key.shape) < 1e-4] = np.inf
+    key[rng.random(key.shape) < 1e-4] = np.nan
+    key = torch.from_numpy(key).cuda()
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    caches = [torch.zeros(n // 16 + 1, 16, 4, 134, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    value = torch.randn(n, 4, 128, device="cuda")
+    tqb.rope_append(key, value, caches[0], slots, None, None, R, m, c)
+    for i in range(0, n, 100):
+        tqb.rope_append(key[i:i + 100], value[i:i + 100], caches[1], slots[i:i + 100], None, None, R, m, c)
+    assert torch.equal(*caches)
+    flat = caches[0].cpu().numpy().reshape(len(caches[0]), -1)
+    for t, h in zip(*np.nonzero(bad)):
+        ka, _, norm, _, _ = SO.places("soa", 4, t % 16, h)
+        assert not np.isfinite(flat[t // 16, norm:norm + 2].view(np.float16)[0]) and (flat[t // 16, ka:ka + 64] == 0).all()

@@ -215,6 +215,11 @@ __device__ __forceinline__ void finish_row(const AppendParams& P, const float* s
             const uint32_t rows = __ballot_sync(kFull, some);
             if (nsq == 0.0f && ((rows >> (lane & 16)) & 0xFFFFu) == 0) near = 0;
         }
+        if (!(norm < INFINITY)) {  // a stored norm of inf or NaN: no codes
+            near = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) code[j] = 0;
+        }
         if (!write) near = 0;
         uint32_t who;
         while ((who = __ballot_sync(kFull, near != 0)) != 0) {
@@ -536,8 +541,8 @@ __device__ __forceinline__ void turn_rows(const AppendParams& P, uint8_t* smem, 
             }
             nsq = warp_sum_xor(nsq, 1, 8);
             // |x| 2^e in [2^13, 2^15): e from the exponent of |x|^2 (its half,
-            // rounded up); 0 for zero and non-finite rows, whose codes come
-            // from the exact path or are anything
+            // rounded up); 0 where |x|^2 is 0 or not finite (keys: the exact path
+            // or no codes; queries: exact_queries)
             const int be = (int)(__float_as_uint(nsq) >> 23);
             const int e = be == 0 || be == 0xFF ? 0 : 14 - ((be - 126) >> 1);
             const float f = exp2i(e);
@@ -589,19 +594,25 @@ __device__ __forceinline__ void prefetch_rows(const T* base, int64_t sn, int64_t
     }
 }
 
-// Whether a row's elements are all zero (a sum of squares of 0 may be that of
-// small numbers), and the codes of such a row.
+// A row's elements: all zero (a sum of squares of 0 may also be that of small
+// numbers), all finite, or not.
+enum Elements : int { kZeros, kFinite, kNonFinite };
 template <typename T>
-__device__ __noinline__ bool zero_row(const T* row) {
-    bool some = false;
+__device__ __noinline__ Elements elements(const T* row) {
+    bool some = false, finite = true;
 #pragma unroll 4
     for (int d = 0; d < kHeadDim; d += 4) {
         Quad<T> x;
         x.load(row + d);
-        some |= x[0] != 0.0f || x[1] != 0.0f || x[2] != 0.0f || x[3] != 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            some |= x[i] != 0.0f;
+            finite &= isfinite(x[i]);
+        }
     }
-    return !some;
+    return !some ? kZeros : finite ? kFinite : kNonFinite;
 }
+// The codes of a row of zeros.
 template <int L>
 __device__ __noinline__ void zero_codes(uint8_t* key, const float* smid) {
     constexpr bool k3 = layout_3bit_keys(L);
@@ -632,7 +643,8 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
     // A row of zeros (dummy inputs): every coordinate is 0 exactly, and next to
     // a middle border all 128 would go through 64 bits (4096 tokens x 8 heads:
     // 5.8 ms, 25 us for random ones).  Its codes are written again below.
-    const bool zeros = stored && info.nsq == 0.0f && zero_row<T>(static_cast<const T*>(P.key) + (int64_t)info.n * P.ksn + (int64_t)info.h * P.ksh);
+    const bool zeros = stored && info.nsq == 0.0f &&
+                       elements<T>(static_cast<const T*>(P.key) + (int64_t)info.n * P.ksn + (int64_t)info.h * P.ksh) == kZeros;
     float csq = 0.0f;
 #pragma unroll 1
     for (int q = 0; q < 8; q++) {
@@ -704,8 +716,8 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
     const bool fold = !layout_is_aos(L) && P.norm_correction;
     const float kept = fold ? norm * rsqrtf(csq + 1e-16f) : norm;
     unsigned short kept_h = __half_as_ushort(__float2half_rn(kept));
-    const bool split = stored && __half_as_ushort(__float2half_rn(kept * (1.0f - kNormNear))) !=
-                                     __half_as_ushort(__float2half_rn(kept * (1.0f + kNormNear)));
+    // (NaN too: turn_rows makes it of infinite elements that it does not turn)
+    const bool split = stored && !__heq(__float2half_rn(kept * (1.0f - kNormNear)), __float2half_rn(kept * (1.0f + kNormNear)));
     uint32_t ask = __ballot_sync(kFull, split);
     while (ask != 0u) {
         const int src = __ffs(ask) - 1;
@@ -727,13 +739,43 @@ __device__ __forceinline__ void finish_keys(const AppendParams& P, uint8_t* smem
             }
             v /= sqrt(warp_sum_f64(cq) + 1e-16);
         }
-        if (lane == src) kept_h = __half_as_ushort(__double2half(v));
+        // (one NaN for both forms: the float conversion's)
+        if (lane == src) kept_h = __half_as_ushort(v != v ? __float2half_rn((float)v) : __double2half(v));
     }
     if (stored) *reinterpret_cast<unsigned short*>(at.norm) = kept_h;
 }
 
+// The lanes' query rows (token n, head h) that are `odd`, in 64 bits (whole
+// warp); rows of zeros and rows that are not finite are left as they are.
+template <typename T>
+__device__ __noinline__ void exact_queries(const AppendParams& P, int n, int h, int pos, bool odd, int lane) {
+    constexpr unsigned kFull = 0xffffffffu;
+    uint32_t who = __ballot_sync(
+        kFull, odd && elements<T>(static_cast<const T*>(P.query) + (int64_t)n * P.qsn + (int64_t)h * P.qsh) == kFinite);
+    while (who != 0u) {
+        const int src = __ffs(who) - 1;
+        who &= who - 1;
+        const int64_t sn = __shfl_sync(kFull, n, src), sh = __shfl_sync(kFull, h, src);
+        const T* row = static_cast<const T*>(P.query) + sn * P.qsn + sh * P.qsh;
+        const float* cs = table_row<T>(P, __shfl_sync(kFull, pos, src));
+        double z[4] = {};
+#pragma unroll 1
+        for (int d = 0; d < kHeadDim; d++) {
+            const double x = rope_f64<T>(P, row, cs, d);
+            const float4 r = __ldg(reinterpret_cast<const float4*>(P.rot + d * kHeadDim) + lane);
+            z[0] += x * (double)r.x;
+            z[1] += x * (double)r.y;
+            z[2] += x * (double)r.z;
+            z[3] += x * (double)r.w;
+        }
+        reinterpret_cast<float4*>(P.q_rot + sn * P.osn + sh * P.osh)[lane] =
+            make_float4((float)z[0], (float)z[1], (float)z[2], (float)z[3]);
+    }
+}
+
 // Query rows: the product itself, turned through shared memory into runs of
 // 128 bytes.
+template <typename T>
 __device__ __forceinline__ void finish_queries(const AppendParams& P, uint8_t* turn, uint32_t tm,
                                                const RowInfo& info, bool live, int lane) {
     float* dst = P.q_rot + (int64_t)info.n * P.osn + (int64_t)info.h * P.osh;
@@ -763,6 +805,9 @@ __device__ __forceinline__ void finish_queries(const AppendParams& P, uint8_t* t
         }
         __syncwarp();
     }
+    // rows whose squares leave fp32's range, and with them the split's scale
+    const bool odd = live && info.slot >= 0 && (info.nsq < 0x1p-120f || info.nsq == INFINITY);
+    if (__any_sync(0xffffffffu, odd)) exact_queries<T>(P, info.n, info.h, info.pos, odd, lane);
 }
 
 // The values of a tile's rows, half a warp each, two at a time with the next
@@ -901,7 +946,7 @@ __global__ void __launch_bounds__(kUmmaThreads, 1) append_umma_kernel(const __gr
                 if (keys)
                     finish_keys<T, L>(P, smem, tm, info, fine, lane);
                 else
-                    finish_queries(P, smem + kTurnOff + 4096 * warp, tm, info, live, lane);
+                    finish_queries<T>(P, smem + kTurnOff + 4096 * warp, tm, info, live, lane);
             }
             tc_fence_before();
             bar_arrive(bars + kDEmpty + 8 * g);
