@@ -209,3 +209,20 @@ def test_append_keys_beyond_fp32_write_the_same_in_both_forms():
     for t, h in zip(*np.nonzero(bad)):
         ka, _, norm, _, _ = SO.places("soa", 4, t % 16, h)
         assert not np.isfinite(flat[t // 16, norm:norm + 2].view(np.float16)[0]) and (flat[t // 16, ka:ka + 64] == 0).all()
+
+
+@pytest.mark.parametrize("rows,chunks", [(4, 4), (160, 2)])
+def test_prefix_partials_of_empty_sequences(monkeypatch, rows, chunks):
+    """Lengths of 0 and below: every split of the prefix is written with O 0 and an LSE of -inf."""
+    share(monkeypatch, chunks)
+    rng = np.random.default_rng(31)
+    c, _, _ = book("soa")
+    cache, table, lens = batch(rng, [512 + 3] * (rows // 4), 1, "soa", 32)
+    lens[:] = rng.choice([0, -1, -2 ** 31, -2 ** 31 + 200], len(lens))
+    lens[0] = -2 ** 31
+    q = torch.from_numpy(rng.standard_normal((rows // 4, 4, 128)).astype(np.float32)).cuda()
+    mid = torch.full((rows // 4, 4, chunks + 1, 129), 7.0, device="cuda")
+    out = tqb.prefix_attention(q, torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(),
+                               None, cuda(c), prefix_len=512, out_dtype=torch.bfloat16, mid_o=mid, num_splits=1)
+    assert torch.isnan(out).all()
+    assert (mid[:, :, :chunks, :128] == 0).all() and torch.isneginf(mid[:, :, :chunks, 128]).all()

@@ -475,7 +475,7 @@ __device__ __forceinline__ void softmax(const PrefixParams& P, const Place& W, u
     const int b = (int)P.div_g.div((uint32_t)row), g = row - b * P.G;
     const float kfac = *reinterpret_cast<const float*>(smem + kAuxOff + 4 * ((W.split ? 0 : m * kTile) + 32 * wq + lane));
     // tokens of the chunk this row sees, from the chunk's start
-    const int lim = min(__ldg(P.seq_lens + b), P.n_pages * kBlockSize) - W.t0 * kTile;
+    const int lim = max(min(__ldg(P.seq_lens + b), P.n_pages * kBlockSize), 0) - W.t0 * kTile;
     const bool any_row = __any_sync(0xffffffffu, live);
     // (a row that sees nothing of the chunk has weights of zero at any reference)
     RowState st{lim > 0 ? -INFINITY : 0.0f, 0.0f};
