@@ -226,3 +226,17 @@ def test_prefix_partials_of_empty_sequences(monkeypatch, rows, chunks):
                                None, cuda(c), prefix_len=512, out_dtype=torch.bfloat16, mid_o=mid, num_splits=1)
     assert torch.isnan(out).all()
     assert (mid[:, :, :chunks, :128] == 0).all() and torch.isneginf(mid[:, :, :chunks, 128]).all()
+
+
+@pytest.mark.parametrize("layout", ["soa", "soa_k8"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_queries_of_any_alignment(layout, dtype):
+    """Contiguous queries that begin one element into a buffer, in the cache's basis: the numbers of an aligned copy."""
+    rng = np.random.default_rng(41)
+    c, _, _ = book(layout)
+    cache, table, lens = (torch.from_numpy(x).cuda() for x in batch(rng, [200, 77, 150], 2, layout, 4))
+    q = torch.randn(1 + 3 * 8 * 128, device="cuda").to(dtype)[1:].view(3, 8, 128)
+    for query in (q, q.transpose(0, 1).contiguous().transpose(0, 1), q[..., :].expand(3, 8, 128)):
+        for call in (lambda x: tqb.window_attention(x, cache, table, lens, None, cuda(c), window=64, layout=layout),
+                     lambda x: tqb.prefix_attention(x, cache, table, lens, None, cuda(c), prefix_len=64, layout=layout)):
+            assert torch.equal(call(query), call(query.clone()))

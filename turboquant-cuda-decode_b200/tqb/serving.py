@@ -368,7 +368,7 @@ class _Step:
         elif self.rot:
             self.rows, self.rs = base + 4 * q_at, (self.Hq * HEAD_DIM, HEAD_DIM)
         else:
-            self.query = q = q.to(_F32).contiguous()
+            self.query = q = torch.empty(q.shape, dtype=_F32, device=q.device).copy_(q)  # fp32 ones too: they are not aligned
             self.rows, self.rs = q.data_ptr(), q.stride()
 
     def stage1(self, at: int, S: int) -> bytes:
