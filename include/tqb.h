@@ -292,8 +292,9 @@ int tqb_store(const tqb_store_args* args, cudaStream_t stream);
  * and the tokens [0, min(first_tokens, lo)), which stay visible before the
  * window (first_tokens > 0 needs prefix_len 0).  Tokens [0, prefix_len), a
  * multiple of 16, are left out: another call supplies their partials
- * (tqb_prefix).  The splits share the pages that hold these tokens equally;
- * pages without any are not read, and splits without a page are left
+ * (tqb_prefix).  Pages without a visible token are not read.  The pages with
+ * one, up to the last token, hold n tokens (masked ones count); a split takes
+ * ceil(n / num_splits) of them in turn, and splits behind the last are left
  * unwritten.
  */
 typedef struct tqb_range {

@@ -36,7 +36,7 @@ _PITCH = HEAD_DIM + 4  # floats of a partial row in the calls' own workspace: 12
 # Shortest split worth its partial rows (516 bytes written and read per query head).  1024 tokens of one sequence and 8
 # heads take 16.6, 16.0, 19.3 and 23.0 us with 16, 32, 64 and 128; 4096 take 22.3, 18.7, 19.7 and 24.9.
 _SPLIT_TOKENS = 32
-_SPLIT_ITEMS = 2368   # (sequence, KV head, split) items of one round of the Stage1 grid: 148 CTAs x 2 groups x 8 warps
+_SMS = 148  # of a B200, the only GPU that the library is built for
 
 
 # The step's calls are launches of a few microseconds, so their arguments are packed into the C structs' bytes at once
@@ -269,19 +269,25 @@ def gather_kv(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, centroids: Opt
     return key, value
 
 
-def _splits(items: int, tokens: int) -> int:
-    """Splits of ``tokens`` for ``items`` (sequence, KV head) pairs.  Stage1 walks tiles of 8 items with 296 groups of
-    warps, so a split count that just exceeds a whole round of the groups costs another round: of the counts that fill
-    one to four rounds, the one with the least time, a round taking its split's tokens and the start and end of a tile
-    (about 48 tokens' time); splits stay above ``_SPLIT_TOKENS`` tokens."""
+def _splits(items: int, tokens: int, group: int) -> int:
+    """Splits of ``tokens`` for ``items`` (sequence, KV head) pairs of ``group`` query heads each.  Stage1 walks tiles of 8
+    (item, split) pairs with a group of warps each, two groups to an SM with up to 4 query heads and one with more, so a
+    split count that just exceeds a whole round of the groups costs another round: of the counts that fill one to four
+    rounds, the one with the least time, a round taking its split's tokens and the start and end of a tile (about 48
+    tokens' time).  Splits of the longest sequence that ``tokens`` allows stay above ``_SPLIT_TOKENS`` tokens.
+
+    Measured, us by splits (one round's in brackets): 4 heads, 64 sequences x 8, 1024 tokens: 2 63, [4 44], 5 54, 9 45;
+    8 heads, the same: 1 88, [2 57], 3 72, 4 62; 8 heads, 37 x 8, 777 tokens: 3 39, [4 36], 5 46, 8 39; 5 heads, 8 x 8,
+    2048 tokens: 14 25, [16 23, 18 26], 20 34, 32 29; 8 heads, 16 x 8, 3000 tokens: 8 36, [9 34], 10 52, 18 38."""
     most = max(1, -(-tokens // _SPLIT_TOKENS))
+    round_ = _SMS * (16 if group <= 4 else 8)
     best = (float("inf"), 1)
     for rounds in (1, 2, 3, 4):
-        s = min(most, _SPLIT_ITEMS * rounds // items)
+        s = min(most, round_ * rounds // items)
         if s:
-            used = -(-items * s // _SPLIT_ITEMS)
+            used = -(-items * s // round_)
             best = min(best, (used * (-(-tokens // s) + 48), s))
-    pages = -(-tokens // BLOCK_SIZE)  # splits hold whole pages: no more of them than the longest needs
+    pages = -(-tokens // BLOCK_SIZE)  # the fewest splits of as many whole pages
     return -(-pages // -(-pages // best[1]))
 
 
@@ -398,11 +404,11 @@ class _Step:
 
 def _prefix_splits(rows: int, heads: int, prefix_len: int) -> int:
     """Splits of the shared prefix for ``rows`` queries of each of ``heads`` KV heads: chunks of 128-token tiles that
-    fill the 148 SMs in as few rounds as pay (a CTA starts and ends in about the time of three tiles)."""
+    fill the SMs in as few rounds as pay (a CTA starts and ends in about the time of three tiles)."""
     tiles, units = -(-prefix_len // 128), heads * -(-rows // 256)
     best = (float("inf"), 1)
     for rounds in (1, 2, 3):
-        chunks = min(tiles, 148 * rounds // units)
+        chunks = min(tiles, _SMS * rounds // units)
         if chunks:
             best = min(best, (rounds * (-(-tiles // chunks) + 3), chunks))
     return best[1] * (2 if rows <= 128 else 1)
@@ -434,7 +440,7 @@ def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     visible tokens are read.  A sequence of length 0 gets NaN and an LSE of -inf, as in ``stage2``.  Sequences longer
     than the block table's rows are cut there.
 
-    ``num_splits`` splits share the pages of a sequence's visible tokens; ``mid_o`` may hold their partials: float32
+    ``num_splits`` splits share the tokens of the pages that hold a sequence's visible ones; ``mid_o`` may hold their partials: float32
     ``[>= B, >= Hq, >= num_splits, 129]``."""
     window, first_tokens = _int(window, "window"), _int(first_tokens, "first_tokens")
     if window < 1:
@@ -448,7 +454,7 @@ def window_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
         return s.output
     most = s.blocks * BLOCK_SIZE
     window, first_tokens = min(window, most), min(first_tokens, most)
-    S = num_splits or _splits(s.B * s.Hk, min(window + first_tokens, most))
+    S = num_splits or _splits(s.B * s.Hk, min(window + first_tokens, most), s.Hq // s.Hk)
     s.workspace(S)
     return s.launch(_RANGE.pack(window, first_tokens, 0, most), 0, S)
 
@@ -488,6 +494,6 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
         lead = _prefix_splits(rows, s.Hk, prefix_len)
     else:
         prefix_len = 0
-    S = (num_splits or _splits(s.B * s.Hk, max(1, most - prefix_len))) + lead
+    S = (num_splits or _splits(s.B * s.Hk, max(1, most - prefix_len), s.Hq // s.Hk)) + lead
     s.workspace(S)
     return s.launch(_RANGE.pack(0, 0, prefix_len, most), lead, S, prefix_len)
