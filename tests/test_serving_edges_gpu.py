@@ -240,3 +240,15 @@ def test_queries_of_any_alignment(layout, dtype):
         for call in (lambda x: tqb.window_attention(x, cache, table, lens, None, cuda(c), window=64, layout=layout),
                      lambda x: tqb.prefix_attention(x, cache, table, lens, None, cuda(c), prefix_len=64, layout=layout)):
             assert torch.equal(call(query), call(query.clone()))
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("nan"), float("inf"), 1e39, 10 ** 400, "x"])
+def test_scales_that_are_refused(scale):
+    rng = np.random.default_rng(1)
+    c, _, _ = book("soa")
+    cache, table, lens = (torch.from_numpy(x).cuda() for x in batch(rng, [40], 1, "soa", 1))
+    q = torch.zeros(1, 4, 128, device="cuda")
+    for call in (lambda: tqb.window_attention(q, cache, table, lens, None, cuda(c), window=9, scale=scale),
+                 lambda: tqb.prefix_attention(q, cache, table, lens, None, cuda(c), prefix_len=16, scale=scale)):
+        with pytest.raises(tqb.TqbError, match="scale"):
+            call()

@@ -322,9 +322,12 @@ class _Step:
                 _no("rotation must be a contiguous [128, 128] matrix")
             self.rot = rotation.data_ptr()
         self.sinks = None if sinks is None else _vector(sinks, "sinks", self.Hq, _F32, dev)
-        self.scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-        if not self.scale > 0:
-            _no("scale must be positive")
+        try:
+            self.scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+        except (TypeError, ValueError, OverflowError):
+            _no("scale must be a number")
+        if not 0 < self.scale < 2.0 ** 127:
+            _no("scale must be positive and an fp32 number")
         if output is None:
             output = torch.empty((self.B, self.Hq, HEAD_DIM), dtype=out_dtype or query.dtype, device=query.device)
             self.os = (self.Hq * HEAD_DIM, HEAD_DIM)
