@@ -252,3 +252,27 @@ def test_scales_that_are_refused(scale):
                  lambda: tqb.prefix_attention(q, cache, table, lens, None, cuda(c), prefix_len=16, scale=scale)):
         with pytest.raises(tqb.TqbError, match="scale"):
             call()
+
+
+@pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
+@pytest.mark.parametrize("hq", [4, 8])
+def test_window_values_that_cancel(layout, hq):
+    """Every value is the middle code times its scale less as much, 0 exactly, whatever the scales: errors go by the mean
+    |v|, so the output is 0."""
+    rng = np.random.default_rng(hq)
+    c, _, _ = book(layout)
+    kb, vb, _ = SO.LAYOUTS[layout]
+    cache, table, lens = batch(rng, [300, 41, 17], 1, layout)
+    middle = SO.pack(np.full(128, 1 << (vb - 1)), vb)
+    flat = cache.reshape(len(cache), -1)
+    for t in range(16):
+        va = SO.places(layout, 1, t, 0)[1]
+        flat[:, va:va + len(middle)] = middle
+        for page in range(len(cache)):
+            scale = np.float16(0.3 * np.exp(0.2 * rng.standard_normal()))
+            put_half(cache, layout, page, t, 3, scale)
+            put_half(cache, layout, page, t, 4, -scale * np.float16(1 << (vb - 1)))
+    q = torch.from_numpy(1.5 * rng.standard_normal((3, hq, 128)).astype(np.float32)).cuda()
+    got = tqb.window_attention(q, torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(),
+                               None, cuda(c), window=200, layout=layout)
+    assert (got == 0).all()
