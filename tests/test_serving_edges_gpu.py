@@ -276,3 +276,75 @@ def test_window_values_that_cancel(layout, hq):
     got = tqb.window_attention(q, torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(),
                                None, cuda(c), window=200, layout=layout)
     assert (got == 0).all()
+
+
+@pytest.mark.parametrize("layout", ["soa", "soa_k3v3", "aos_k8"])
+@pytest.mark.parametrize("above", [20, 30])
+@pytest.mark.parametrize("kernel", ["ring", "regs"])
+def test_window_behind_a_first_token_that_outweighs_it(monkeypatch, layout, above, kernel):
+    """A first token of value 0 with 2^above times the weight of each of the others: the output is theirs.  The bar is the
+    decode calls' 2e-3, of the mean |v| here."""
+    if kernel == "regs":
+        monkeypatch.setenv("TQB_STAGE1_KERNEL", "regs")
+    rng = np.random.default_rng(above)
+    c, _, _ = book(layout)
+    kb, vb, _ = SO.LAYOUTS[layout]
+    cache, table, lens = batch(rng, [500, 260], 1, layout)
+    flat = cache.reshape(len(cache), -1)
+    if kb == 8:
+        d = rng.standard_normal(128)
+        raw = torch.from_numpy(d.astype(np.float32)).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+        d = SO.f8(raw)
+        grow = 8  # exact in e4m3: three exponents up
+        big = torch.from_numpy((d * grow).astype(np.float32)).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    else:
+        raw = big = SO.pack(rng.integers(0, 1 << kb, 128), kb)
+        d = npy(c)[SO.unpack(raw, kb)].astype(np.float64)
+        grow = 8
+    for t in range(16):
+        ka = SO.places(layout, 1, t, 0)[0]
+        flat[:, ka:ka + len(raw)] = raw
+        for page in range(len(cache)):
+            if kb != 8:
+                put_half(cache, layout, page, t, 2, 3.0)
+    for row in table:
+        ka = SO.places(layout, 1, 0, 0)[0]
+        flat[row[0], ka:ka + len(big)] = big
+        if kb != 8:
+            put_half(cache, layout, row[0], 0, 2, 3.0 * grow)
+        put_half(cache, layout, row[0], 0, 3, 0.0)
+        put_half(cache, layout, row[0], 0, 4, 0.0)
+    size = (1.0 if kb == 8 else 3.0) * (d @ d)
+    if layout.startswith("aos") and kb != 8:
+        size /= np.sqrt(d @ d)
+    q = np.broadcast_to(d * (above * np.log(2) * np.sqrt(128) / (size * (grow - 1))), (2, 4, 128)).astype(np.float32)
+    args = (torch.from_numpy(cache).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(), None, cuda(c))
+    for dtype in (torch.float32, torch.bfloat16):
+        got = tqb.window_attention(torch.from_numpy(q.copy()).cuda(), *args, window=200, first_tokens=1, layout=layout,
+                                   out_dtype=dtype, num_splits=1)
+        ref, _, mean = SO.attention(q, cache, layout, table, lens, npy(c), lambda t, L: (t < 1) | (t >= L - 200))
+        assert (np.abs(got.double().cpu().numpy() - ref) <= half_step(dtype) * np.abs(ref) + 2e-3 * mean).all()
+
+
+@pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
+@pytest.mark.parametrize("kernel", ["ring", "regs"])
+def test_window_values_of_any_size(monkeypatch, layout, kernel):
+    """Scales and zeros times 2^-8, exactly: outputs times 2^-8.  Both are fp32 sums of the same products, of weights good to
+    2^-22: 2^-20 of the mean |v|, 2 here."""
+    if kernel == "regs":
+        monkeypatch.setenv("TQB_STAGE1_KERNEL", "regs")
+    rng = np.random.default_rng(3)
+    c, _, _ = book(layout)
+    cache, table, lens = batch(rng, [300, 41, 999], 1, layout)
+    q = torch.from_numpy(1.5 * rng.standard_normal((3, 5, 128)).astype(np.float32)).cuda()
+    outs = []
+    for f in (1.0, 2.0 ** -8):
+        now = cache.copy()
+        flat = now.reshape(len(now), -1)
+        for t in range(16):
+            for at in SO.places(layout, 1, t, 0)[3:]:
+                flat[:, at:at + 2] = (np.ascontiguousarray(flat[:, at:at + 2]).view(np.float16) * np.float16(f)).view(np.uint8)
+        out = tqb.window_attention(q, torch.from_numpy(now).cuda(), torch.from_numpy(table).cuda(), torch.from_numpy(lens).cuda(),
+                                   None, cuda(c), window=400, layout=layout)
+        outs.append(out.double() / f)
+    assert (outs[0] - outs[1]).abs().max().item() <= 2.0 ** -20 * 2

@@ -153,6 +153,28 @@ __device__ __forceinline__ float ex2_approx(float x) {
     return y;
 }
 
+// ---------------------------------------------------------------------------
+// Stage1 over a range of tokens (both Stage1 kernels)
+// ---------------------------------------------------------------------------
+// Ranged calls take their reference from what has to fit fp16, p scale: the
+// largest of the page's 16 tokens comes to 2^7 (fp16's precision ends 2^-32
+// below that), wherever the scales and scores lie.  A first token that takes
+// nearly all of the weight and has a value near 0, as attention sinks do, has a
+// small scale, and leaves the others their precision.  The weights p themselves
+// are only summed in fp32 and may reach 2^kFar.  Whole numbers, so that moving
+// the reference scales the sums exactly.
+constexpr float kFar = 64.0f, kFarStart = 32.0f, kWeightStart = 7.0f;
+__device__ __forceinline__ float weight_reference(float s0, float s1, float vs0, float vs1) {
+    const float far = warp_max_xor(fmaxf(s0, s1), 4, 16) - kFarStart;
+    const float big = warp_max_xor(fmaxf(s0 + lg2_approx(vs0), s1 + lg2_approx(vs1)), 4, 16) - kWeightStart;
+    return ceilf(fmaxf(far, big));
+}
+
+// Codes * 2^-20 (a pair of fp16 subnormals) less the middle code, exactly.
+template <bool V3>
+__device__ __forceinline__ uint32_t mid_code(uint32_t a) {
+    return h2_as_u32(__hadd2(u32_as_h2(a), u32_as_h2(V3 ? 0x80408040u : 0x80808080u)));
+}
 
 // Eight 3-bit fields (bits 3i .. 3i+2 of h, 24 bits) to eight nibbles
 // (bits 4i .. 4i+2): halves, then quarters, then pairs move apart.

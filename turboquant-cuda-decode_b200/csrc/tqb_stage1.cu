@@ -393,6 +393,11 @@ __device__ __forceinline__ void process_page(ItemState<NT>& st, const PageRegs& 
     const float vz0 = va ? half_bits_to_float(cur.vz) : 0.0f;
     const float vz1 = vb ? half_bits_to_float(cur.vz >> 16) : 0.0f;
 
+    // ranged calls: the value of the middle code, which the products count from
+    constexpr bool kVal3 = layout_3bit_values(LAYOUT);
+    constexpr float kMidCode = kVal3 ? 4.0f : 8.0f;
+    const float vc0 = fmaf(kMidCode, vs0, vz0), vc1 = fmaf(kMidCode, vs1, vz1);
+
     // -- online softmax (exp2 domain), exact rescale --
     uint32_t bw0[NT], bw1[NT];
     float alpha[NT];
@@ -413,16 +418,19 @@ __device__ __forceinline__ void process_page(ItemState<NT>& st, const PageRegs& 
         float s1 = d1 * kn1 * st.kfac[nt];
         s0 = va ? s0 : -INFINITY;
         s1 = vb ? s1 : -INFINITY;
-        const float tmax = warp_max_xor(fmaxf(s0, s1), 4, 16);
         const float mold = st.m_run[nt];
+        float tmax = 0.0f;
+        if constexpr (!RG) tmax = warp_max_xor(fmaxf(s0, s1), 4, 16);
         // Lazy reference max: it only moves when a score exceeds it by more
         // than kLazy (log2 units), so most pages need no rescale; p <= 2^kLazy.
-        float mref = tmax > mold + kLazy ? tmax : mold;
+        float mref = !RG && tmax > mold + kLazy ? tmax : mold;
         float mref_e = mref == -INFINITY ? 0.0f : mref;  // page with no valid token
         float p0 = ex2(s0 - mref_e), p1 = ex2(s1 - mref_e);
         float w0 = p0 * vs0, w1 = p1 * vs1;
-        // W must stay inside fp16: a huge V scale falls back to the exact max.
-        if (__any_sync(0xffffffffu, fmaxf(w0, w1) > kWMax)) {
+        // W must stay inside fp16: a huge V scale falls back to the exact max
+        // (ranged calls: weight_reference).
+        if (__any_sync(0xffffffffu, (RG && fmaxf(s0, s1) > mold + kFar) || fmaxf(w0, w1) > kWMax)) {
+            if constexpr (RG) tmax = weight_reference(s0, s1, vs0, vs1);
             mref = fmaxf(mold, tmax);
             mref_e = mref == -INFINITY ? 0.0f : mref;
             p0 = ex2(s0 - mref_e);
@@ -434,7 +442,7 @@ __device__ __forceinline__ void process_page(ItemState<NT>& st, const PageRegs& 
         alpha[nt] = (mold == -INFINITY || mref == mold) ? 1.0f : ex2(mold - mref);
         rescale |= alpha[nt] != 1.0f;
         st.l_part[nt] = st.l_part[nt] * alpha[nt] + (p0 + p1);
-        st.z_part[nt] = st.z_part[nt] * alpha[nt] + (p0 * vz0 + p1 * vz1);
+        st.z_part[nt] = st.z_part[nt] * alpha[nt] + (RG ? p0 * vc0 + p1 * vc1 : p0 * vz0 + p1 * vz1);
         st.m_run[nt] = mref;
         const __half2 wh = __floats2half2_rn(w0, w1);
         const __half2 wl = __floats2half2_rn(w0 - __low2float(wh), w1 - __high2float(wh));
@@ -476,7 +484,17 @@ __device__ __forceinline__ void process_page(ItemState<NT>& st, const PageRegs& 
         const uint32_t a2 = (p23 << 4) & 0x00F000F0u;
         const uint32_t a3 = p23 & 0x00F000F0u;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) mma_16816(st.acc[nt][i], a0, a1, a2, a3, bw0[nt], bw1[nt]);
+        for (int nt = 0; nt < NT; nt++) {
+            if constexpr (RG) {  // as in the page ring's kernel: codes from the middle one, sums outside the tensor core
+                float d[4] = {};
+                mma_16816(d, mid_code<kVal3>(a0), mid_code<kVal3>(a1), mid_code<kVal3>(a2), mid_code<kVal3>(a3), bw0[nt],
+                          bw1[nt]);
+#pragma unroll
+                for (int k = 0; k < 4; k++) st.acc[nt][i][k] += d[k];
+            } else {
+                mma_16816(st.acc[nt][i], a0, a1, a2, a3, bw0[nt], bw1[nt]);
+            }
+        }
     }
 }
 

@@ -810,12 +810,6 @@ struct LaneSmem {
     uint32_t row;     // AoS: bytes between consecutive tokens of a page
 };
 
-// Codes * 2^-20 (a pair of fp16 subnormals) less the middle code, exactly.
-template <bool V3>
-__device__ __forceinline__ uint32_t mid_code(uint32_t a) {
-    return h2_as_u32(__hadd2(u32_as_h2(a), u32_as_h2(V3 ? 0x80408040u : 0x80808080u)));
-}
-
 template <int NT, int LAYOUT, bool RG>
 __device__ __forceinline__ void page_math(ItemState<NT>& st, const uint32_t sb, const LaneSmem& o, bool page_ok,
                                           int tok0, int start, int end, int hole0, uint32_t hole, uint32_t lut_sel_src, int g,
@@ -1013,7 +1007,8 @@ __device__ __forceinline__ void page_math(ItemState<NT>& st, const uint32_t sb, 
     // -- online softmax (exp2 domain), lazy reference max: a page is weighted
     //    against the running reference m_run while no score exceeds it by
     //    more than kLazy (log2 units) and no weight leaves fp16; only then is
-    //    the exact row max formed (three shuffles) and the state rescaled.
+    //    the exact row max formed (three shuffles) and the state rescaled
+    //    (ranged calls: weight_reference).
     uint32_t bw0[NT], bw1[NT];
     float alpha[NT];
     bool rescale = false;
@@ -1035,9 +1030,9 @@ __device__ __forceinline__ void page_math(ItemState<NT>& st, const uint32_t sb, 
         float p0 = ex2(s0 - mold_e), p1 = ex2(s1 - mold_e);
         float w0 = p0 * vs0, w1 = p1 * vs1;
         float mref = mold;
-        const bool over = fmaxf(s0, s1) > mold + kLazy || fmaxf(w0, w1) > kWMax;
+        const bool over = fmaxf(s0, s1) > mold + (RG ? kFar : kLazy) || fmaxf(w0, w1) > kWMax;
         if (__any_sync(0xffffffffu, over)) {
-            mref = fmaxf(mold, warp_max_xor(fmaxf(s0, s1), 4, 16));
+            mref = fmaxf(mold, RG ? weight_reference(s0, s1, vs0, vs1) : warp_max_xor(fmaxf(s0, s1), 4, 16));
             const float mref_e = mref == -INFINITY ? 0.0f : mref;
             p0 = ex2(s0 - mref_e);
             p1 = ex2(s1 - mref_e);
