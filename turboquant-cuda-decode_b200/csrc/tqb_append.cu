@@ -399,10 +399,10 @@ __global__ void __launch_bounds__(kAppThreads) append_kernel(const __grid_consta
 // first.  Errors against exact arithmetic, of |x|: 2^-23 from the fp32 turn, 3 *
 // 2^-22 from the splits, 16 accumulations of 2^-23 at the size of the small
 // products (2^-10) and 8 of 2^-23 at full size (kNear has the rest).
-// Bound by instruction issue and latency: about 15 instructions per coordinate
+// Bound by instruction issue and latency: about 14 instructions per coordinate
 // to bucketise, 9 to turn and split, 10 per value.  32768 tokens x 8 KV heads:
 // 152 us (4, 6, 6 warps: 177; a second group of finishing warps changes
-// nothing); 2037 tokens x 40 heads: 39 us.
+// nothing); 2037 tokens x 40 heads, 3-bit AoS: 35 us.
 // ---------------------------------------------------------------------------
 // Up to here the form above is faster: 5120 rows of a 4-bit decode step take it
 // 15.8 us and this one 16.7, 10240 rows 21.5 and 17.5.

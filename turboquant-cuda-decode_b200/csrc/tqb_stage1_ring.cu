@@ -1089,9 +1089,9 @@ __device__ __forceinline__ void page_math(ItemState<NT>& st, const uint32_t sb, 
                 // The tensor core truncates its sums.  Ranged calls add them up
                 // outside it, and count codes from the middle one, so that the
                 // sums have the size of what they stand for and no one sign:
-                // an fp32 window of 777 tokens is off by 0.8e-6 of its size so
+                // an fp32 window of 777 tokens is off by 0.75e-6 of its size so
                 // (torch in fp32: 1.0e-6), by 1.7e-6 with codes from 0, and by
-                // 2.2e-6 in one chain (36.3, 35.6 and 35.6 us).
+                // 2.2e-6 in one chain (36.9, 35.6 and 35.6 us).
                 float d[4] = {};
                 mma_16816(d, mid_code<kVal3>(a0), mid_code<kVal3>(a1), mid_code<kVal3>(a2), mid_code<kVal3>(a3), bw0[nt],
                           bw1[nt]);

@@ -480,7 +480,8 @@ def prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor, block_table: t
     0.4e-3 to 1.1e-3 of the outputs' rms for scores of a standard deviation of 0.7 to 2.5, 1.9e-3 for 10, beside a bf16
     output's own rounding of 1.65e-3.  A short prefix, and fp16 and fp32 outputs, go sequence by sequence, in fp32.
     ``mid_o`` holds the partials of the prefix too then: ``num_splits + 2 ceil(prefix_len / 128)`` splits are always
-    enough.  ``num_splits`` is the splits of each sequence's own tokens."""
+    enough.  ``num_splits`` is the splits of each sequence's own tokens; without it their count goes by the block table's
+    width, which suits tables of about the longest sequence's length."""
     prefix_len = _int(prefix_len, "prefix_len")
     if prefix_len < 0 or prefix_len % BLOCK_SIZE:
         _no("prefix_len must be a multiple of 16")
