@@ -335,7 +335,7 @@ int tqb_stage2_range(const tqb_stage2_args* args, const tqb_range* range, int32_
  * 2.5 (1.9e-3 for 10; FP8 keys half of that), good for bf16 outputs, whose own
  * rounding is 1.65e-3, not for fp16 or fp32 ones.
  * Weights below 2^-32 of a split's largest count as zero in O (not in the
- * LSE).
+ * LSE), and values below 2^-14 are held to 2^-25.
  * num_splits is at most ceil(prefix_len / 128); with batch * (Hq / Hk) <= 128
  * an even num_splits may be twice that.  tqb_stage1_range with the same
  * prefix_len adds each sequence's own tokens as further splits, and

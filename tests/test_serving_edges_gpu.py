@@ -8,7 +8,7 @@ import torch
 
 import serving_oracle as SO
 import tqb
-from test_serving_gpu import batch, book, cos_sin_table, cuda, half_step, no_wait_timeouts, npy, random_cache  # noqa: F401
+from test_serving_gpu import batch, book, cos_sin_table, cuda, half_step, no_wait_timeouts, npy, run_prefix  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -348,3 +348,10 @@ def test_window_values_of_any_size(monkeypatch, layout, kernel):
                                    None, cuda(c), window=400, layout=layout)
         outs.append(out.double() / f)
     assert (outs[0] - outs[1]).abs().max().item() <= 2.0 ** -20 * 2
+
+
+@pytest.mark.parametrize("layout", sorted(SO.LAYOUTS))
+@pytest.mark.parametrize("own,hq,chunks", [([1, 9, 30] * 12, 8, 1), ([4, 60], 16, 2)])
+def test_prefix_pass_of_many_tiles_on_every_layout(layout, own, hq, chunks):
+    """bf16 outputs, one stream over every tile and two over every other one."""
+    run_prefix(layout, torch.bfloat16, own, 720, hq, 2, seed=chunks, chunks=chunks)
